@@ -325,6 +325,78 @@ int tt_fc_forward(int dtype, int64_t batch, int64_t fin, int64_t fout, const voi
  * a GEMM with a row of ones).  dtype TT_F32 or TT_BF16; rows = 0 gives 0. */
 int tt_col_sum(int dtype, const void* x, void* y, int64_t rows, int64_t cols, void* stream);
 
+/* ---------------------------------------------------------------- microscaled 4-bit floating point */
+
+/* Values held in 4 bits (no counterpart in the reference, which has no type
+ * below 32 bits): a row of n values is ceil(n / 32) blocks of 32, the last one
+ * padded with zeros; a block is 16 bytes of codes (element 2 i in the low half
+ * of byte i; sign, two exponent bits, one fraction bit: +-{0, 0.5, 1, 1.5, 2,
+ * 3, 4, 6}) and one scale byte that stands for 2^(byte - 127).  codes are
+ * row-major [rows][blocks][16] and 16-byte aligned (TT_ERR_ARG otherwise),
+ * scales row-major [rows][blocks].
+ *
+ * Quantising takes a block's scale as 2^(floor(log2 max|x|) - 2), at least
+ * 2^-127, and rounds x / scale to nearest, halves to even, values beyond 6 to
+ * 6.  A block that holds an infinity or a NaN gets scale byte 255 and codes of
+ * zero, and every value of such a block reads as NaN.  Only the rounding to
+ * the element grid is inexact, so the result is the same everywhere, bit for
+ * bit.  A signed zero keeps its sign. */
+
+/* x [rows][cols] (trans = 0) to codes and scales; with trans = 1, x is stored
+ * [cols][rows] and row r of the result takes its column r (a layer's weight
+ * [fin][fout] to the [fout][fin] that the product takes).  dtype TT_F32 or
+ * TT_BF16, x at any element alignment. */
+int tt_mxfp4_quantize(int dtype, int trans, const void* x, uint8_t* codes, uint8_t* scales, int64_t rows,
+                      int64_t cols, void* stream);
+/* The values y [rows][cols] that codes and scales stand for, exact in
+ * either dtype; those from 2^128 on are infinite. */
+int tt_mxfp4_dequantize(int dtype, const uint8_t* codes, const uint8_t* scales, void* y, int64_t rows, int64_t cols,
+                        void* stream);
+
+/* C = alpha A B^T + beta C: A [m][k] and B [n][k] both in 4 bits, quantised
+ * along k, C [m][n] row-major of `dtype` (TT_F32 or TT_BF16), sums in fp32.
+ * beta = 0 does not read C; k = 0 gives beta C.  Allocates nothing. */
+int tt_gemm_mxfp4(int dtype, int64_t m, int64_t n, int64_t k, float alpha, const uint8_t* a_codes,
+                  const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales, float beta, void* C,
+                  void* stream);
+/* The fully connected layer with such a weight: out [batch][fout] =
+ * quantised(in [batch][fin]) W^T + bias, W [fout][fin] in 4 bits, the bias
+ * (fout values, or one where bias_scalar != 0) added to the fp32 sum.  in,
+ * bias and out of `dtype`.  More than 16 rows are quantised into a 32 MiB
+ * per-stream library workspace (allocated on first use) and multiplied from
+ * there; without it (refused, or under graph capture before a call has left it
+ * on the stream) the product quantises them as it reads them, which is slower
+ * and gives the same result. */
+int tt_fc_forward_mxfp4(int dtype, int64_t batch, int64_t fin, int64_t fout, const void* in, const uint8_t* w_codes,
+                        const uint8_t* w_scales, const void* bias, int bias_scalar, void* out, void* stream);
+
+/* A K/V cache in 4 bits: codes [B][Hkv][cap][d / 2], scales [B][Hkv][cap][d / 32]
+ * for K and the same for V, d in {32, 64, 128}.  lengths (int, on the device)
+ * holds each sequence's number of keys, the T newest tokens included: token t
+ * of them is key lengths[b] - T + t and sees the keys up to itself.
+ *
+ * Append: quantises the new rows k, v [B][Hkv][T][d] into the cache.  A token
+ * whose key would lie outside [0, cap) is not written, so a batch of prompts
+ * padded on the left needs no other mask, and a slot of length 0 stays as it
+ * is, as does every row that no token goes to. */
+int tt_kv_append_mxfp4(int dtype, const void* k, const void* v, uint8_t* k_codes, uint8_t* k_scales, uint8_t* v_codes,
+                       uint8_t* v_scales, const int* lengths, int64_t B, int64_t Hkv, int64_t T, int64_t cap,
+                       int64_t d, void* stream);
+/* Attention of those tokens over the cache: q, o [B][H][T][d] of `dtype`, H a
+ * multiple of Hkv (query head h reads K/V head h / (H / Hkv)), lse [B][H][T]
+ * (float, natural log, may be NULL).  Token t sees key j where j < lengths[b] -
+ * (T - 1 - t) and j < cap; one that sees none gets o = 0 and lse = -inf.  Rows
+ * of the cache that no token sees are not used, whatever they hold.  K and V
+ * enter with their 4-bit values, scores, weights and sums in fp32 precision.
+ * Few heads split the keys over workgroups and merge their sums through a
+ * fixed 24 MiB per-stream library workspace (allocated on first use); without
+ * it (refused, or under graph capture before a call has left it on the stream)
+ * they run unsplit. */
+int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_codes, const uint8_t* k_scales,
+                         const uint8_t* v_codes, const uint8_t* v_scales, const int* lengths, void* o, float* lse,
+                         int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t cap, int64_t d, float scale,
+                         void* stream);
+
 /* ---------------------------------------------------------------- convolution data movement */
 
 /* im[N][C][H][W] -> col[N][OH*OW][C][kh][kw] with OH = (H + 2 pad_h - kh) /

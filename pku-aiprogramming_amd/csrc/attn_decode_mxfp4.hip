@@ -1,0 +1,430 @@
+// Attention of the newest tokens over a K / V cache held in the microscaled
+// 4-bit format (mxfp4.h): o = softmax(s q K^T) V for T tokens of H query heads
+// over Hkv cached heads.
+//
+// The bytes of the cache bound it (17/32 a value, K and V each read once), and
+// with few bytes a value the arithmetic must stay small beside them, so both
+// products run on the matrix unit for every group size: the R = H / Hkv * T
+// query rows that share one K / V head are a tile of 16 columns (rows past R
+// are zeros: the unit has the time, a memory access has not).  A wave owns 32
+// keys at a time with a running maximum and sum of its own:
+//   S^T [32 keys x 16 rows] = K Q^T: a lane's piece of a K row (D / 8 bytes of
+//     codes, one scale) becomes the bf16 operand by v_cvt_scalef32_pk_bf16_fp4,
+//     exactly, with no LDS: the k order of the contraction is free, and q is
+//     laid out to match.  Result: a lane owns one query row and 8 keys.
+//   O^T [D x 16 rows] += V^T P^T: P comes out of S^T in the operand's layout
+//     (the order of the keys is free as well); V's rows are converted to bf16 into the wave's LDS
+//     tile and read back transposed (ds_read_b64_tr_b16).  P is split into bf16
+//     terms (two for bf16 tensors, 2^-17 off; three for fp32, whose q is split
+//     into three exact terms too), so that no rounding of the weights shows in
+//     the result.
+// The next 32 keys' codes are in flight meanwhile (they are only 4 to 16
+// registers).  The waves of a workgroup meet in LDS at the end, and splits of the
+// keys over workgroups in a second launch.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <optional>
+#include <string>
+
+#include "attn_tiles.h"
+#include "mxfp4.h"
+#include "tt_internal.h"
+
+namespace tt {
+namespace {
+
+constexpr int kMdThreads = 256, kMdWaves = kMdThreads / 64;
+constexpr int kMdRows = 16;  // query rows of a workgroup
+constexpr int kMdKeys = 32;  // keys of a wave's step
+
+__device__ __forceinline__ f32x4 mfma_bf16_16x16x32(const bf16x8& a, const bf16x8& b, const f32x4& c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+// max and sum over lanes l, l ^ 16, l ^ 32, l ^ 48, in every one of them
+__device__ __forceinline__ float max_rows(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return max_xor32(vmax(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+__device__ __forceinline__ float sum_rows(float x) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
+}
+
+// A lane's piece of a K or V row: W dwords of codes (8 values each) under one scale.
+template <int W>
+struct MdPiece {
+  uint32_t c[W], s;
+};
+template <int W>
+__device__ __forceinline__ void md_load(MdPiece<W>& p, const uint32_t* codes, const uint8_t* scales, int64_t row,
+                                        int g) {
+  __builtin_memcpy(p.c, codes + row * (4 * W) + g * W, 4 * W);
+  p.s = scales[W == 4 ? row * 4 + g : (W == 2 ? row * 2 + (g >> 1) : row)];
+}
+__device__ __forceinline__ bf16x8 md_bf16(uint32_t codes, float scale) {
+  MxEight<u16> v;
+  v.from(codes, scale);
+  return __builtin_bit_cast(bf16x8, v.w);
+}
+
+// x as a sum of N bf16 terms, each what the earlier ones leave, rounded, or
+// (CUT) cut off: three cut terms hold any fp32 value exactly.
+template <int N, bool CUT>
+__device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
+  float left[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) left[e] = x[e];
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const __bf16 b = CUT ? __builtin_bit_cast(__bf16, (u16)(__float_as_uint(left[e]) >> 16)) : (__bf16)left[e];
+      t[n][e] = b;
+      left[e] -= (float)b;
+    }
+}
+
+__device__ __forceinline__ void md_load8(const u16* p, float (&f)[8]) {
+  u16 x[8];
+  __builtin_memcpy(x, p, 16);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = bf16_to_f32(x[e]);
+}
+__device__ __forceinline__ void md_load8(const float* p, float (&f)[8]) { __builtin_memcpy(f, p, 32); }
+__device__ __forceinline__ void md_put(u16* p, float v) { *p = f32_to_bf16(v); }
+__device__ __forceinline__ void md_put(float* p, float v) { *p = v; }
+
+// o and lse of a row from its sums (den = 0: no key, or only scores of -inf).
+template <typename T>
+__device__ __forceinline__ float md_quotient(float num, float den) {
+  return den == 0.f ? 0.f : num / den;
+}
+__device__ __forceinline__ float md_lse(float m, float den) {
+  return den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
+}
+
+// Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv,
+// tile = 16 of the head's R query rows.  Each sequence's own length is cut into
+// nsplit spans, so that sequences of any length keep every workgroup busy.
+template <typename T, int D>
+__global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
+    const T* __restrict__ q, const uint32_t* __restrict__ kc, const uint8_t* __restrict__ ks,
+    const uint32_t* __restrict__ vc, const uint8_t* __restrict__ vs, const int* __restrict__ lengths,
+    float* __restrict__ part_o, float2* __restrict__ part_ml, T* __restrict__ o, float* __restrict__ lse, int Hkv,
+    int64_t R, int tokens, int64_t tiles, int cap, int nsplit, float sl2) {
+  constexpr int W = D / 32;                                  // dwords of a lane's piece, and k steps of a key tile
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;  // terms of q and of the weights
+  constexpr int ND = D / 16;                                 // 16-row tiles of O^T
+  using Tile = SwzTile<D>;
+  __shared__ __align__(16) u16 s_v[kMdWaves][Tile::kElems(kMdKeys)];
+  __shared__ float s_m[kMdWaves][kMdRows], s_l[kMdWaves][kMdRows];
+  static_assert(sizeof(s_v[0]) == kMdRows * D * sizeof(float), "the waves' sums reuse their tiles");
+
+  const int l = threadIdx.x & 63, r = l & 15, g = l >> 4;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int split = blockIdx.x % nsplit;
+  const int64_t unit = blockIdx.x / nsplit, head = unit / tiles, row0 = (unit - head * tiles) * kMdRows;
+  const int64_t qrow = head * R + row0;  // the tile's first row of q and o
+  const int nrows = (int)min((int64_t)kMdRows, R - row0);
+
+  // Keys that the newest token sees, and that this lane's row sees.
+  const int full = lengths[head / Hkv];
+  const int len = min(full, cap);
+  const int t = r < nrows ? (int)((row0 + r) % tokens) : 0;
+  const int seen = r < nrows ? (int)min((int64_t)len, (int64_t)full - (tokens - 1 - t)) : 0;
+  const int all_see = (int)min((int64_t)len, (int64_t)full - (tokens - 1));  // keys that every row sees
+  int kbeg = 0, kend = 0;
+  if (len > 0) {
+    const int span = ((len + nsplit - 1) / nsplit + kMdKeys - 1) / kMdKeys * kMdKeys;
+    kbeg = (int)min((int64_t)split * span, (int64_t)len);
+    kend = min(kbeg + span, len);
+  }
+
+  bf16x8 qf[W][NQ];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    if (r < nrows) md_load8(q + (qrow + r) * D + g * (8 * W) + 8 * j, x);
+    md_terms<NQ, true>(x, qf[j]);
+  }
+
+  f32x4 acc[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  float m = -INFINITY, lsum = 0.f;
+  u16* tile = s_v[w];
+  const int64_t base = head * cap;
+
+  MdPiece<W> k[2], v[2];
+  auto fetch = [&](int j0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int64_t row = base + min(j0 + 16 * u + r, len - 1);  // keys past the end: the last one, masked below
+      md_load(k[u], kc, ks, row, g);
+      md_load(v[u], vc, vs, row, g);
+    }
+  };
+  int j0 = kbeg + w * kMdKeys;
+  if (j0 < kend) fetch(j0);
+  for (; j0 < kend; j0 += kMdWaves * kMdKeys) {
+    MdPiece<W> kx[2] = {k[0], k[1]}, vx[2] = {v[0], v[1]};
+    const int next = j0 + kMdWaves * kMdKeys;
+    if (next < kend) fetch(next);
+
+    f32x4 s[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      const float f = mx_scale(kx[u].s);
+#pragma unroll
+      for (int j = 0; j < W; ++j) {
+        const bf16x8 a = md_bf16(kx[u].c[j], f);
+#pragma unroll
+        for (int n = NQ - 1; n >= 0; --n) s[u] = mfma_bf16_16x16x32(a, qf[j][n], s[u]);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) s[u] *= sl2;
+    uint64_t odd[2] = {0, 0};  // lanes whose V block reads as NaN, in a step that some row does not see whole
+    const bool edge = j0 + kMdKeys > min(kend, all_see);
+    if (edge) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = j0 + 16 * u + 4 * g + i;
+          s[u][i] = key < min(seen, kend) ? s[u][i] : -INFINITY;
+        }
+        // A weight of zero must not meet a NaN: V rows that no row sees become
+        // zeros, and a block of NaN that only some see is added below.
+        const bool out = j0 + 16 * u + r >= kend;
+        odd[u] = __ballot(!out && vx[u].s == 255u);
+        if (out || vx[u].s == 255u) {
+          vx[u].s = 127u;
+#pragma unroll
+          for (int j = 0; j < W; ++j) vx[u].c[j] = 0u;
+        }
+      }
+    }
+
+    float top = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) top = vmax(top, s[u][i]);
+    top = max_rows(top);
+    const float mn = vmax(m, top);
+    const float mb = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every weight 0
+    if (wave_any(mn != m)) {
+      const float a = fast_exp2(m - mb);
+      lsum *= a;
+#pragma unroll
+      for (int i = 0; i < ND; ++i) acc[i] *= a;
+      m = mn;
+    }
+    float p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      p[e] = fast_exp2(s[e >> 2][e & 3] - mb);
+      lsum += p[e];
+    }
+    bf16x8 pf[NP];
+    md_terms<NP, false>(p, pf);
+
+    // V rows to the wave's tile, 8 values a 16-byte chunk
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const float f = mx_scale(vx[u].s);
+#pragma unroll
+      for (int j = 0; j < W; ++j)
+        *reinterpret_cast<bf16x8*>(&tile[Tile::chunk(16 * u + r, g * W + j)]) = md_bf16(vx[u].c[j], f);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+    for (int i = 0; i < ND; ++i) {
+      const int col = 16 * i + 4 * (r & 3), krow = 4 * g + (r >> 2);
+      const bf16x8 a = lds_read_tr16x2(&tile[Tile::at4(krow, col)], &tile[Tile::at4(krow + 16, col)]);
+#pragma unroll
+      for (int n = NP - 1; n >= 0; --n) acc[i] = mfma_bf16_16x16x32(a, pf[n], acc[i]);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      for (uint64_t left = odd[u]; left; left &= left - 1) {  // rare: NaN blocks at the border of the mask
+        const int at = __builtin_ctzll(left), blk = W == 4 ? at >> 4 : (W == 2 ? at >> 5 : 0);
+        const bool hit = j0 + 16 * u + (at & 15) < seen;
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          if (hit && i / 2 == blk) acc[i] += f32x4{NAN, NAN, NAN, NAN};
+      }
+  }
+
+  // The waves' sums meet in LDS: [row][D] fp32 over each wave's own tile, chunks
+  // of four swizzled by the row.
+  lsum = sum_rows(lsum);
+  float* mine = reinterpret_cast<float*>(tile);
+#pragma unroll
+  for (int i = 0; i < ND; ++i)
+    *reinterpret_cast<f32x4*>(&mine[r * D + 4 * ((4 * i + g) ^ (r & (D / 4 - 1)))]) = acc[i];
+  if (g == 0) {
+    s_m[w][r] = m;
+    s_l[w][r] = lsum;
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < nrows * (D / 4); c += kMdThreads) {
+    const int row = c / (D / 4), d4 = c - row * (D / 4);
+    float top = s_m[0][row];
+#pragma unroll
+    for (int i = 1; i < kMdWaves; ++i) top = vmax(top, s_m[i][row]);
+    const float mb = top == -INFINITY ? 0.f : top;
+    float den = 0.f;
+    f32x4 num = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < kMdWaves; ++i) {
+      const float wgt = fast_exp2(s_m[i][row] - mb);
+      const float* theirs = reinterpret_cast<const float*>(s_v[i]);
+      den += wgt * s_l[i][row];
+      num += wgt * *reinterpret_cast<const f32x4*>(&theirs[row * D + 4 * (d4 ^ (row & (D / 4 - 1)))]);
+    }
+    if (nsplit > 1) {
+      const int64_t at = (qrow + row) * nsplit + split;
+      *reinterpret_cast<f32x4*>(part_o + at * D + 4 * d4) = num;
+      if (d4 == 0) part_ml[at] = float2{top, den};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) md_put(o + (qrow + row) * D + 4 * d4 + e, md_quotient<T>(num[e], den));
+      if (d4 == 0 && lse) lse[qrow + row] = md_lse(top, den);
+    }
+  }
+}
+
+// Merges the splits of a row: 256 threads, D / 4 to a partial and 1024 / D
+// partials side by side, which meet in LDS.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_decode_mxfp4_merge_kernel(const float* __restrict__ part_o,
+                                                                      const float2* __restrict__ part_ml,
+                                                                      T* __restrict__ o, float* __restrict__ lse,
+                                                                      int nsplit) {
+  constexpr int TPR = D / 4, G = 256 / TPR;
+  __shared__ __align__(16) float s_acc[G][D];
+  __shared__ float s_w[G];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, c = tid % TPR, g = tid / TPR;
+  const float2* pl = part_ml + row * nsplit;
+  const float* po = part_o + row * nsplit * D + 4 * c;
+  float mx = -INFINITY;  // every wave forms the maximum by itself
+  for (int s = tid & 63; s < nsplit; s += 64) mx = vmax(mx, pl[s].x);
+#pragma unroll
+  for (int off = 32; off > 0; off >>= 1) mx = vmax(mx, __shfl_xor(mx, off, 64));
+  const float mb = mx == -INFINITY ? 0.f : mx;
+  float sw = 0.f;
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = g; s < nsplit; s += G) {
+    const float2 ml = pl[s];
+    const float wgt = fast_exp2(ml.x - mb);
+    sw += wgt * ml.y;
+    acc += wgt * *reinterpret_cast<const f32x4*>(po + (int64_t)s * D);
+  }
+  *reinterpret_cast<f32x4*>(&s_acc[g][4 * c]) = acc;
+  if (c == 0) s_w[g] = sw;
+  __syncthreads();
+  if (tid >= D) return;
+  float num = 0.f, den = 0.f;
+#pragma unroll
+  for (int i = 0; i < G; ++i) {
+    num += s_acc[i][tid];
+    den += s_w[i];
+  }
+  md_put(o + row * D + tid, md_quotient<T>(num, den));
+  if (tid == 0 && lse) lse[row] = md_lse(mx, den);
+}
+
+constexpr size_t kMdWork = size_t(24) << 20;  // the partials' scratch, of one size so that graphs may keep its address
+constexpr int64_t kMdFill = 1024;             // workgroups that fill the chip
+
+template <typename T, int D>
+int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
+           const int* lengths, T* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t tokens, int64_t cap,
+           float scale, hipStream_t st) {
+  const int64_t R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
+  const int64_t rows = B * H * tokens;
+  // Splits: enough workgroups to fill the chip, each with 256 keys or more.
+  int64_t nsplit = (kMdFill + units - 1) / units;
+  nsplit = std::min(nsplit, (cap + 255) / 256);
+  nsplit = std::min(nsplit, (int64_t)(kMdWork / ((size_t)rows * (D + 2) * sizeof(float))));
+  void* ws = nullptr;
+  std::optional<WorkspaceLease> lease;  // held until both kernels are queued
+  if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsMxfp4Decode, kMdWork, &ws)) nsplit = 1;
+  if (!grid_fits(units * nsplit, kMdThreads) || !grid_fits(rows, 256))
+    return fail(TT_ERR_ARG, std::string(fn) + ": grid too large");
+  float* part_o = (float*)ws;
+  float2* part_ml = (float2*)(part_o + rows * nsplit * D);
+  hipLaunchKernelGGL((attn_decode_mxfp4_kernel<T, D>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, st, q,
+                     (const uint32_t*)kc, ks, (const uint32_t*)vc, vs, lengths, part_o, part_ml, o, lse, (int)Hkv, R,
+                     (int)tokens, tiles, (int)cap, (int)nsplit, scale * kLog2e);
+  TT_LAUNCHED(fn, st);
+  if (nsplit > 1) {
+    hipLaunchKernelGGL((attn_decode_mxfp4_merge_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, part_o, part_ml,
+                       o, lse, (int)nsplit);
+    TT_LAUNCHED(fn, st);
+  }
+  return ok();
+}
+
+template <typename T>
+int launch_d(const char* fn, const void* q, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
+             const int* lengths, void* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t tokens, int64_t cap,
+             int64_t d, float scale, hipStream_t st) {
+#define TT_MD(D) \
+  return launch<T, D>(fn, (const T*)q, kc, ks, vc, vs, lengths, (T*)o, lse, B, H, Hkv, tokens, cap, scale, st)
+  switch (d) {
+    case 32: TT_MD(32);
+    case 64: TT_MD(64);
+    default: TT_MD(128);
+  }
+#undef TT_MD
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_codes, const uint8_t* k_scales,
+                                    const uint8_t* v_codes, const uint8_t* v_scales, const int* lengths, void* o,
+                                    float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t cap, int64_t d,
+                                    float scale, void* stream) {
+  const char* fn = "tt_attn_decode_mxfp4";
+  int rc = check_cache_mxfp4(fn, dtype, B, Hkv, T, cap, d);
+  if (rc) return rc;
+  if (H < 0 || (Hkv == 0 ? H != 0 : H % Hkv != 0))
+    return fail(TT_ERR_ARG, std::string(fn) + ": H must be a multiple of Hkv");
+  if (B == 0 || H == 0 || T == 0) return ok();
+  if (H > (int64_t(1) << 24) || B * H > (int64_t(1) << 24)) return fail(TT_ERR_ARG, std::string(fn) + ": too many heads");
+  if (!q || !o || !lengths || (cap > 0 && (!k_codes || !k_scales || !v_codes || !v_scales)))
+    return fail(TT_ERR_ARG, std::string(fn) + ": null pointer");
+  if (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15)
+    return fail(TT_ERR_ARG, std::string(fn) + ": codes must be 16-byte aligned");
+  const size_t qb = (size_t)(B * H * T * d) * (dtype == TT_F32 ? 4 : 2);
+  const size_t cb = (size_t)(B * Hkv * cap * d / 2), sb = (size_t)(B * Hkv * cap * d / kMxBlock);
+  if ((rc = check_no_overlap(fn,
+                             {{q, qb, "q"}, {k_codes, cb, "k_codes"}, {k_scales, sb, "k_scales"},
+                              {v_codes, cb, "v_codes"}, {v_scales, sb, "v_scales"},
+                              {lengths, (size_t)B * sizeof(int), "lengths"}},
+                             {{o, qb, "o"}, {lse, (size_t)(B * H * T) * sizeof(float), "lse"}})))
+    return rc;
+  if ((rc = ensure_init())) return rc;
+  hipStream_t st = stream_or_default(stream);
+  return dtype == TT_F32 ? launch_d<float>(fn, q, k_codes, k_scales, v_codes, v_scales, lengths, o, lse, B, H, Hkv, T,
+                                           cap, d, scale, st)
+                         : launch_d<u16>(fn, q, k_codes, k_scales, v_codes, v_scales, lengths, o, lse, B, H, Hkv, T,
+                                         cap, d, scale, st);
+}

@@ -1,0 +1,260 @@
+// Products of matrices held in the microscaled 4-bit format (mxfp4.h), and the
+// fully connected layer with such weights.
+//
+//   C[m][n] = alpha sum_k A[m][k] B[n][k] + beta C[m][n] + bias[n]
+//
+// A [M][K] and B [N][K] are both quantised along k, so a block of 32 k values
+// of either has one scale and v_mfma_scale_f32_*_f8f6f4 multiplies them as they
+// are stored: codes in a lane's four registers, the scale byte beside them,
+// fp32 sums.  The products of two elements are multiples of 1/4 and the scales
+// powers of two, so only the sums round.
+#include <hip/hip_runtime.h>
+
+#include <optional>
+#include <string>
+
+#include "attn_tiles.h"
+#include "mxfp4.h"
+#include "tt_internal.h"
+
+namespace tt {
+namespace {
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+constexpr int kFp4 = 4;  // the instruction's format code of e2m1
+__device__ __forceinline__ i32x8 fp4_operand(const uint4& c) {
+  return i32x8{(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
+}
+// 16 x 16 x 128: lane l holds row l % 16, k block l / 16 of both operands, and
+// its scale in byte 0; result register i is C[4 (l / 16) + i][l % 16].
+__device__ __forceinline__ f32x4 mfma_fp4_16(const uint4& a, const uint4& b, const f32x4& c, uint32_t sa, uint32_t sb) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fp4_operand(a), fp4_operand(b), c, kFp4, kFp4, 0, (int)sa, 0,
+                                                          (int)sb);
+}
+
+// alpha acc + bias + beta C and the store, for element (row, col) inside C.
+template <typename O>
+struct MxEpilogue {
+  O* C;
+  const O* bias;  // null: none
+  int64_t bias_step;
+  float alpha, beta;
+  int64_t N;
+  __device__ __forceinline__ static float get(const float* p) { return *p; }
+  __device__ __forceinline__ static float get(const u16* p) { return bf16_to_f32(*p); }
+  __device__ __forceinline__ static void put(float* p, float v) { *p = v; }
+  __device__ __forceinline__ static void put(u16* p, float v) { *p = f32_to_bf16(v); }
+  __device__ __forceinline__ float value(int64_t row, int64_t col, float acc) const {
+    float v = alpha * acc;
+    if (bias) v += get(bias + col * bias_step);
+    if (beta != 0.f) v += beta * get(C + row * N + col);
+    return v;
+  }
+  __device__ __forceinline__ void store(int64_t row, int64_t col, float acc) const {
+    put(C + row * N + col, value(row, col, acc));
+  }
+};
+
+// The 32 values of one block, quantised in registers: its codes, *s its scale.
+template <typename T>
+__device__ __forceinline__ uint4 quantize_block(const MxEight<T> (&v)[4], uint32_t* s) {
+  uint32_t e = 0;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) e = max(e, v[j].top());
+  *s = mx_scale_byte(e);
+  const float f = mx_scale(*s);
+  if (*s == 255u) return uint4{0, 0, 0, 0};
+  return uint4{v[0].codes(f), v[1].codes(f), v[2].codes(f), v[3].codes(f)};
+}
+
+// Strips: a workgroup makes 16 columns of C for 16 MS rows, its eight waves
+// taking every eighth k step of 128 and meeting in LDS.  Operands go from
+// global memory to the matrix unit's registers directly.  For few rows, where
+// B's codes are the bytes that count: each is read once, four steps in flight
+// a wave.  QA: A is not quantised yet (x, rows of K values), and each lane
+// quantises the block that it would have loaded; one launch for a token's
+// layer.
+constexpr int kStripWaves = 8;
+
+template <typename O, int MS, bool QA>
+__global__ __launch_bounds__(64 * kStripWaves) void k_mxfp4_strip(const uint4* __restrict__ A,
+                                                                  const uint8_t* __restrict__ As,
+                                                                  const O* __restrict__ X,
+                                                                  const uint4* __restrict__ B,
+                                                                  const uint8_t* __restrict__ Bs, int64_t M, int64_t N,
+                                                                  int64_t K, int nb, uint32_t strips,
+                                                                  MxEpilogue<O> ep) {
+  constexpr int UN = QA && sizeof(O) == 4 ? 2 : 4;
+  __shared__ __align__(16) f32x4 red[kStripWaves][MS][64];
+  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, r = l & 15, g = l >> 4;
+  const int64_t n0 = (int64_t)(blockIdx.x % strips) * 16, m0 = (int64_t)(blockIdx.x / strips) * (16 * MS);
+  const int64_t brow = min(n0 + r, N - 1) * nb;  // rows past the end repeat the last one and are not stored
+  int64_t arow[MS];
+#pragma unroll
+  for (int i = 0; i < MS; ++i) arow[i] = min(m0 + 16 * i + r, M - 1);
+  f32x4 acc[MS];
+#pragma unroll
+  for (int i = 0; i < MS; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (nb + 3) / 4;
+  for (int i0 = w; i0 < steps; i0 += kStripWaves * UN) {
+    uint4 b[UN], a[UN][MS];
+    uint32_t sb[UN], sa[UN][MS];
+    MxEight<O> v[QA ? UN : 1][4];
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      // blocks past the row's end: some block of the row, made zero below
+      const int blk = 4 * (i0 + kStripWaves * u) + g, at = min(blk, nb - 1);
+      b[u] = B[brow + at];
+      sb[u] = Bs[brow + at];
+      if constexpr (QA) {
+        const O* p = X + arow[0] * K + (int64_t)at * kMxBlock;
+        const int n = (int)min((int64_t)kMxBlock, K - (int64_t)at * kMxBlock);
+        if (n == kMxBlock) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][j].load(p + 8 * j);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[u][j].load_part(p + 8 * j, n - 8 * j);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < MS; ++i) {
+          a[u][i] = A[arow[i] * nb + at];
+          sa[u][i] = As[arow[i] * nb + at];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if constexpr (QA) a[u][0] = quantize_block(v[u], &sa[u][0]);
+      const bool in = 4 * (i0 + kStripWaves * u) + g < nb;
+      const uint4 bu = in ? b[u] : uint4{0, 0, 0, 0};
+      const uint32_t sbu = in ? sb[u] : 127u;
+#pragma unroll
+      for (int i = 0; i < MS; ++i) {
+        const uint4 au = in ? a[u][i] : uint4{0, 0, 0, 0};
+        acc[i] = mfma_fp4_16(bu, au, acc[i], sbu, in ? sa[u][i] : 127u);
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < MS; ++i) red[w][i][l] = acc[i];
+  __syncthreads();
+  for (int i = w; i < MS; i += kStripWaves) {
+    f32x4 s = red[0][i][l];
+#pragma unroll
+    for (int q = 1; q < kStripWaves; ++q) s += red[q][i][l];
+    const int64_t row = m0 + 16 * i + r, col = n0 + 4 * g;
+    if (row >= M) continue;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (col + e < N) ep.store(row, col + e, s[e]);
+  }
+}
+
+template <typename O, int MS, bool QA>
+int strip_launch(const char* fn, const uint8_t* A, const uint8_t* As, const O* X, const uint8_t* B, const uint8_t* Bs,
+                 int64_t M, int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
+  const int64_t strips = (N + 15) / 16, tiles = strips * ((M + 16 * MS - 1) / (16 * MS));
+  if (!grid_fits(tiles, 64 * kStripWaves)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
+  hipLaunchKernelGGL((k_mxfp4_strip<O, MS, QA>), dim3((unsigned)tiles), dim3(64 * kStripWaves), 0, s, (const uint4*)A,
+                     As, X, (const uint4*)B, Bs, M, N, K, (int)mx_blocks(K), (uint32_t)strips, ep);
+  TT_LAUNCHED(fn, s);
+  return ok();
+}
+
+template <typename O>
+int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, int64_t M,
+            int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
+  return strip_launch<O, 4, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+}
+
+// Rows of x quantised at a time; the scratch is of one size, so that graphs may keep its address.
+constexpr size_t kMxRowsWork = size_t(32) << 20;
+
+template <typename O>
+int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O* bias, int64_t bias_step, int64_t M,
+       int64_t N, int64_t K, O* out, hipStream_t s) {
+  const MxEpilogue<O> all{out, bias, bias_step, 1.f, 0.f, N};
+  const int64_t nb = mx_blocks(K), row_bytes = nb * (kMxBlockBytes + 1);
+  const int64_t fit = row_bytes > 0 ? (int64_t)(kMxRowsWork / row_bytes) / 16 * 16 : 0;
+  void* ws = nullptr;
+  std::optional<WorkspaceLease> lease;  // held until the last kernel that reads the buffer is queued
+  if (M <= 16 || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
+    return strip_launch<O, 1, true>(fn, nullptr, nullptr, x, W, Ws, M, N, K, all, s);
+  for (int64_t r0 = 0; r0 < M; r0 += fit) {
+    const int64_t rows = M - r0 < fit ? M - r0 : fit;
+    uint8_t* codes = (uint8_t*)ws;
+    uint8_t* scales = codes + (size_t)(rows * nb) * kMxBlockBytes;
+    int rc = tt_mxfp4_quantize(sizeof(O) == 4 ? TT_F32 : TT_BF16, 0, x + r0 * K, codes, scales, rows, K, s);
+    if (rc) return rc;
+    MxEpilogue<O> ep = all;
+    ep.C = out + r0 * N;
+    if ((rc = product<O>(fn, codes, scales, W, Ws, rows, N, K, ep, s))) return rc;
+  }
+  return ok();
+}
+
+int check_product(const char* fn, int dtype, int64_t m, int64_t n, int64_t k) {
+  const std::string f(fn);
+  if (dtype != TT_F32 && dtype != TT_BF16) return fail(TT_ERR_ARG, f + ": dtype must be TT_F32 or TT_BF16");
+  if (m < 0 || n < 0 || k < 0) return fail(TT_ERR_ARG, f + ": negative size");
+  if (m > 0x7fffffff || n > 0x7fffffff || k > 0x7fffffff)
+    return fail(TT_ERR_ARG, f + ": dimension above 2^31 - 1");
+  return TT_OK;
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" int tt_gemm_mxfp4(int dtype, int64_t m, int64_t n, int64_t k, float alpha, const uint8_t* a_codes,
+                             const uint8_t* a_scales, const uint8_t* b_codes, const uint8_t* b_scales, float beta,
+                             void* C, void* stream) {
+  const char* fn = "tt_gemm_mxfp4";
+  int rc = check_product(fn, dtype, m, n, k);
+  if (rc) return rc;
+  if (m == 0 || n == 0) return ok();
+  if (!C || (k > 0 && (!a_codes || !a_scales || !b_codes || !b_scales)))
+    return fail(TT_ERR_ARG, std::string(fn) + ": null pointer");
+  if (k > 0 && (((uintptr_t)a_codes | (uintptr_t)b_codes) & 15))
+    return fail(TT_ERR_ARG, std::string(fn) + ": codes must be 16-byte aligned");
+  const size_t na = (size_t)(m * mx_blocks(k)), nb = (size_t)(n * mx_blocks(k));
+  if ((rc = check_no_overlap(fn, {{a_codes, na * kMxBlockBytes, "a_codes"}, {a_scales, na, "a_scales"},
+                                  {b_codes, nb * kMxBlockBytes, "b_codes"}, {b_scales, nb, "b_scales"}},
+                             {{C, (size_t)(m * n) * (dtype == TT_F32 ? 4 : 2), "C"}})))
+    return rc;
+  if ((rc = ensure_init())) return rc;
+  hipStream_t s = stream_or_default(stream);
+  if (dtype == TT_F32)
+    return product<float>(fn, a_codes, a_scales, b_codes, b_scales, m, n, k,
+                          MxEpilogue<float>{(float*)C, nullptr, 0, alpha, beta, n}, s);
+  return product<u16>(fn, a_codes, a_scales, b_codes, b_scales, m, n, k,
+                      MxEpilogue<u16>{(u16*)C, nullptr, 0, alpha, beta, n}, s);
+}
+
+extern "C" int tt_fc_forward_mxfp4(int dtype, int64_t batch, int64_t fin, int64_t fout, const void* in,
+                                   const uint8_t* w_codes, const uint8_t* w_scales, const void* bias, int bias_scalar,
+                                   void* out, void* stream) {
+  const char* fn = "tt_fc_forward_mxfp4";
+  int rc = check_product(fn, dtype, batch, fout, fin);
+  if (rc) return rc;
+  if (batch == 0 || fout == 0) return ok();
+  if (!bias || !out || (fin > 0 && (!in || !w_codes || !w_scales)))
+    return fail(TT_ERR_ARG, std::string(fn) + ": null pointer");
+  if (fin > 0 && ((uintptr_t)w_codes & 15)) return fail(TT_ERR_ARG, std::string(fn) + ": codes must be 16-byte aligned");
+  const size_t e = dtype == TT_F32 ? 4 : 2, nw = (size_t)(fout * mx_blocks(fin));
+  if ((rc = check_no_overlap(fn, {{in, (size_t)(batch * fin) * e, "in"}, {w_codes, nw * kMxBlockBytes, "w_codes"},
+                                  {w_scales, nw, "w_scales"}, {bias, (size_t)(bias_scalar ? 1 : fout) * e, "bias"}},
+                             {{out, (size_t)(batch * fout) * e, "out"}})))
+    return rc;
+  if ((rc = ensure_init())) return rc;
+  hipStream_t s = stream_or_default(stream);
+  const int64_t step = bias_scalar ? 0 : 1;
+  if (dtype == TT_F32)
+    return fc<float>(fn, (const float*)in, w_codes, w_scales, (const float*)bias, step, batch, fout, fin, (float*)out, s);
+  return fc<u16>(fn, (const u16*)in, w_codes, w_scales, (const u16*)bias, step, batch, fout, fin, (u16*)out, s);
+}

@@ -48,7 +48,7 @@ void* noalloc_scratch(size_t* bytes);
 // the buffer has been launched on that stream.  A user that also runs under
 // capture (the fp32 forward, the backward, the long decode splits) shares its
 // buffer with no other: their requests would replace the one a graph keeps.
-enum { kWsBackwardRows = 0, kWsDecodePartials = 1, kWsForwardSplits = 2, kWsSoftmaxPartials = 3, kWsGemmSplits = 4, kWsDecodeShort = 5, kWsForwardSplitsBf16 = 6 };
+enum { kWsBackwardRows = 0, kWsDecodePartials = 1, kWsForwardSplits = 2, kWsSoftmaxPartials = 3, kWsGemmSplits = 4, kWsDecodeShort = 5, kWsForwardSplitsBf16 = 6, kWsMxfp4Rows = 7, kWsMxfp4Decode = 8 };
 class WorkspaceLease {
  public:
   WorkspaceLease();

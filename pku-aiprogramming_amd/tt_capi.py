@@ -82,6 +82,12 @@ _SIGS = {
     "tt_conv_forward": (C.c_int, [C.c_int, _p, _p, _p, _i64] + [C.c_int] * 10 + [_p]),
     "tt_conv_backward": (C.c_int, [C.c_int, _p, _p, _p, _p, _p, _i64] + [C.c_int] * 10 + [_p]),
     "tt_fc_forward": (C.c_int, [C.c_int, _i64, _i64, _i64, _p, _p, _p, C.c_int, _p, _p]),
+    "tt_mxfp4_quantize": (C.c_int, [C.c_int, C.c_int, _p, _p, _p, _i64, _i64, _p]),
+    "tt_mxfp4_dequantize": (C.c_int, [C.c_int, _p, _p, _p, _i64, _i64, _p]),
+    "tt_gemm_mxfp4": (C.c_int, [C.c_int, _i64, _i64, _i64, C.c_float, _p, _p, _p, _p, C.c_float, _p, _p]),
+    "tt_fc_forward_mxfp4": (C.c_int, [C.c_int, _i64, _i64, _i64, _p, _p, _p, _p, C.c_int, _p, _p]),
+    "tt_kv_append_mxfp4": (C.c_int, [C.c_int] + [_p] * 7 + [_i64] * 5 + [_p]),
+    "tt_attn_decode_mxfp4": (C.c_int, [C.c_int] + [_p] * 8 + [_i64] * 6 + [C.c_float, _p]),
     "tt_col_sum": (C.c_int, [C.c_int, _p, _p, _i64, _i64, _p]),
 }
 
@@ -158,9 +164,10 @@ def bf16_to_f32(bits: np.ndarray) -> np.ndarray:
 
 class DeviceBuffer:
     """A tt_malloc'd device block holding a tensor of ``shape`` and ``dtype``
-    ("f32", "bf16" or "i32"), freed with tt_free when collected."""
+    ("f32", "bf16", "i32", "f64" or "u8"), freed with tt_free when collected."""
 
-    ITEM = {"f32": 4, "bf16": 2, "i32": 4, "f64": 8}
+    ITEM = {"f32": 4, "bf16": 2, "i32": 4, "f64": 8, "u8": 1}
+    HOST = {"f32": np.float32, "bf16": np.uint16, "i32": np.int32, "f64": np.float64, "u8": np.uint8}
 
     def __init__(self, shape: Sequence[int], dtype: str = "f32"):
         self.L = lib()
@@ -185,14 +192,7 @@ class DeviceBuffer:
             assert 2 * host.size == self.nbytes, (host.shape, self.shape)
             self.L.call("tt_upload_bf16_from_f32", self.ptr, host.ctypes.data, host.size)
             return
-        if self.dtype == "bf16":
-            host = np.ascontiguousarray(a)
-        elif self.dtype == "f32":
-            host = np.ascontiguousarray(a, dtype=np.float32)
-        elif self.dtype == "i32":
-            host = np.ascontiguousarray(a, dtype=np.int32)
-        else:
-            host = np.ascontiguousarray(a, dtype=np.float64)
+        host = np.ascontiguousarray(a, dtype=self.HOST[self.dtype])
         assert host.nbytes == self.nbytes, (host.shape, self.shape)
         self.L.call("tt_memcpy_h2d", self.ptr, host.ctypes.data, self.nbytes)
 
@@ -202,13 +202,13 @@ class DeviceBuffer:
             out = np.empty(self.shape, np.float32)
             self.L.call("tt_download_bf16_to_f32", out.ctypes.data, self.ptr, out.size)
             return out
-        raw = np.empty(self.shape, {"f32": np.float32, "i32": np.int32, "f64": np.float64}[self.dtype])
+        raw = np.empty(self.shape, self.HOST[self.dtype])
         self.L.call("tt_memcpy_d2h", raw.ctypes.data, self.ptr, self.nbytes)
         return raw
 
     def download_bytes(self) -> np.ndarray:
         """The stored bytes as is (bf16 as uint16 bit patterns)."""
-        raw = np.empty(self.shape, {"f32": np.float32, "i32": np.int32, "f64": np.float64, "bf16": np.uint16}[self.dtype])
+        raw = np.empty(self.shape, self.HOST[self.dtype])
         self.L.call("tt_memcpy_d2h", raw.ctypes.data, self.ptr, self.nbytes)
         return raw
 
@@ -266,6 +266,108 @@ def gemm(transa: bool, transb: bool, m: int, n: int, k: int, alpha: float, A: De
         raise ValueError("gemm: A, B and C must share one dtype")
     name = "tt_gemm_bf16" if C.dtype == "bf16" else "tt_gemm_f32"
     lib().call(name, int(transa), int(transb), m, n, k, alpha, A.ptr, B.ptr, beta, C.ptr, stream)
+
+
+# ------------------------------------------------------------------ microscaled 4-bit
+
+MX_BLOCK = 32  # values under one scale; their codes are 16 bytes
+
+
+def _mx_dtype(what: str, *bufs: DeviceBuffer) -> int:
+    """The dtype code that the float buffers share."""
+    if any(b.dtype != bufs[0].dtype for b in bufs) or bufs[0].dtype not in ("f32", "bf16"):
+        raise ValueError(f"{what}: float buffers of one dtype, f32 or bf16")
+    return TT_BF16 if bufs[0].dtype == "bf16" else TT_F32
+
+
+def _mx_bytes(what: str, codes: DeviceBuffer, scales: DeviceBuffer, shape: Sequence[int]):
+    """codes and scales ("u8") must hold rows of ``shape`` [.., n]."""
+    if codes.dtype != "u8" or scales.dtype != "u8":
+        raise ValueError(f"{what}: codes and scales are u8 buffers")
+    nb = -(-int(shape[-1]) // MX_BLOCK)
+    rows = int(np.prod(shape[:-1], dtype=np.int64))
+    if codes.nbytes != rows * nb * 16 or scales.nbytes != rows * nb:
+        raise ValueError(f"{what}: codes and scales of {tuple(shape)} hold {rows * nb * 16} and {rows * nb} bytes")
+
+
+def mxfp4_buffers(shape: Sequence[int]):
+    """New codes [.., 16 nb] and scales [.., nb] buffers for values of ``shape`` [.., n]."""
+    nb = -(-int(shape[-1]) // MX_BLOCK)
+    return DeviceBuffer((*shape[:-1], 16 * nb), "u8"), DeviceBuffer((*shape[:-1], nb), "u8")
+
+
+def mxfp4_quantize(x: DeviceBuffer, codes: DeviceBuffer, scales: DeviceBuffer, trans: bool = False, stream=None):
+    """x [.., cols] to codes and scales; with trans, the columns of a matrix x [cols, rows]."""
+    if trans:
+        cols, rows = x.shape
+    else:
+        cols, rows = x.shape[-1], int(np.prod(x.shape[:-1], dtype=np.int64))
+    _mx_bytes("mxfp4_quantize", codes, scales, (rows, cols))
+    lib().call("tt_mxfp4_quantize", _mx_dtype("mxfp4_quantize", x), int(trans), x.ptr, codes.ptr, scales.ptr, rows, cols,
+               stream)
+
+
+def mxfp4_dequantize(codes: DeviceBuffer, scales: DeviceBuffer, y: DeviceBuffer, stream=None):
+    """The values y [.., cols] that codes and scales stand for."""
+    _mx_bytes("mxfp4_dequantize", codes, scales, y.shape)
+    lib().call("tt_mxfp4_dequantize", _mx_dtype("mxfp4_dequantize", y), codes.ptr, scales.ptr, y.ptr,
+               int(np.prod(y.shape[:-1], dtype=np.int64)), y.shape[-1], stream)
+
+
+def gemm_mxfp4(k: int, alpha: float, a_codes: DeviceBuffer, a_scales: DeviceBuffer, b_codes: DeviceBuffer,
+               b_scales: DeviceBuffer, beta: float, C: DeviceBuffer, stream=None):
+    """C [m, n] = alpha A B^T + beta C of A [m, k] and B [n, k] in 4 bits."""
+    m, n = C.shape
+    _mx_bytes("gemm_mxfp4", a_codes, a_scales, (m, k))
+    _mx_bytes("gemm_mxfp4", b_codes, b_scales, (n, k))
+    lib().call("tt_gemm_mxfp4", _mx_dtype("gemm_mxfp4", C), m, n, k, alpha, a_codes.ptr, a_scales.ptr, b_codes.ptr,
+               b_scales.ptr, beta, C.ptr, stream)
+
+
+def fc_forward_mxfp4(x: DeviceBuffer, w_codes: DeviceBuffer, w_scales: DeviceBuffer, bias: DeviceBuffer,
+                     out: DeviceBuffer, stream=None):
+    """out [batch, fout] = quantised(x [batch, fin]) W^T + bias, W [fout, fin] in 4 bits."""
+    (batch, fin), fout = x.shape, out.shape[-1]
+    _mx_bytes("fc_forward_mxfp4", w_codes, w_scales, (fout, fin))
+    scalar = bias.shape == (1,)
+    if tuple(out.shape) != (batch, fout) or (not scalar and bias.shape != (fout,)):
+        raise ValueError("fc_forward_mxfp4: out is [batch, fout], bias [fout] or [1]")
+    lib().call("tt_fc_forward_mxfp4", _mx_dtype("fc_forward_mxfp4", x, bias, out), batch, fin, fout, x.ptr, w_codes.ptr,
+               w_scales.ptr, bias.ptr, int(scalar), out.ptr, stream)
+
+
+def _mx_cache(what: str, k_codes, k_scales, v_codes, v_scales, lengths):
+    B, Hkv, cap, half = k_codes.shape
+    d = 2 * half
+    for codes, scales in ((k_codes, k_scales), (v_codes, v_scales)):
+        _mx_bytes(what, codes, scales, (B, Hkv, cap, d))
+    if lengths.dtype != "i32" or lengths.shape != (B,):
+        raise ValueError(f"{what}: lengths is an i32 buffer [B]")
+    return B, Hkv, cap, d
+
+
+def kv_append_mxfp4(k: DeviceBuffer, v: DeviceBuffer, k_codes: DeviceBuffer, k_scales: DeviceBuffer,
+                    v_codes: DeviceBuffer, v_scales: DeviceBuffer, lengths: DeviceBuffer, stream=None):
+    """New rows k, v [B, Hkv, T, d] into the cache; lengths count them already."""
+    B, Hkv, cap, d = _mx_cache("kv_append_mxfp4", k_codes, k_scales, v_codes, v_scales, lengths)
+    T = k.shape[2]
+    if k.shape != (B, Hkv, T, d) or v.shape != k.shape:
+        raise ValueError("kv_append_mxfp4: k and v are [B, Hkv, T, d] of the cache")
+    lib().call("tt_kv_append_mxfp4", _mx_dtype("kv_append_mxfp4", k, v), k.ptr, v.ptr, k_codes.ptr, k_scales.ptr,
+               v_codes.ptr, v_scales.ptr, lengths.ptr, B, Hkv, T, cap, d, stream)
+
+
+def attn_decode_mxfp4(q: DeviceBuffer, k_codes: DeviceBuffer, k_scales: DeviceBuffer, v_codes: DeviceBuffer,
+                      v_scales: DeviceBuffer, lengths: DeviceBuffer, o: DeviceBuffer, lse: Optional[DeviceBuffer],
+                      scale: float, stream=None):
+    """Attention of the T newest tokens q [B, H, T, d] over the cache."""
+    B, Hkv, cap, d = _mx_cache("attn_decode_mxfp4", k_codes, k_scales, v_codes, v_scales, lengths)
+    H, T = q.shape[1], q.shape[2]
+    if q.shape != (B, H, T, d) or o.shape != q.shape or (lse and (lse.dtype != "f32" or lse.shape != (B, H, T))):
+        raise ValueError("attn_decode_mxfp4: q and o are [B, H, T, d], lse f32 [B, H, T]")
+    lib().call("tt_attn_decode_mxfp4", _mx_dtype("attn_decode_mxfp4", q, o), q.ptr, k_codes.ptr, k_scales.ptr,
+               v_codes.ptr, v_scales.ptr, lengths.ptr, o.ptr, lse.ptr if lse else None, B, H, Hkv, T, cap, d, scale,
+               stream)
 
 
 # ------------------------------------------------------------------ softmax
