@@ -165,9 +165,201 @@ int strip_launch(const char* fn, const uint8_t* A, const uint8_t* As, const O* X
   return ok();
 }
 
+// p, which every lane holds alike, in scalar registers.
+__device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
+  const uint64_t x = (uint64_t)(uintptr_t)p;
+  const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)x), hi = __builtin_amdgcn_readfirstlane((uint32_t)(x >> 32));
+  return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
+}
+
+// Tiles: BM x BN of C a workgroup of WM x WN waves, k in stages of 256 (8
+// blocks, 128 bytes of codes a row).  A stage's codes of both operands come
+// straight into LDS (global_load_lds, 16 bytes a lane) a stage ahead, chunk c of
+// row r at chunk c ^ (r / 2 % 8), so that the 32 rows that an operand read takes
+// one chunk of lie in all banks.  The scales of two stages (16 bytes a row) go
+// through registers into LDS two stages ahead.  Rows past M or N repeat the last
+// one and are not stored.  The matrix unit takes B's rows first, so a lane ends
+// with four consecutive columns of one row of C.
+constexpr int kStageBlocks = 8, kStageBytes = kStageBlocks * kMxBlockBytes;
+
+template <typename O, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* __restrict__ A,
+                                                                const uint8_t* __restrict__ As,
+                                                                const uint8_t* __restrict__ B,
+                                                                const uint8_t* __restrict__ Bs, int64_t M, int64_t N,
+                                                                int nb, int mtiles, int ntiles, MxEpilogue<O> ep) {
+  constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
+  constexpr int MT = BM / WM / 32, NTL = BN / WN / 32;         // 32-row operand tiles of a wave
+  constexpr int LOADS = ROWS * kStageBlocks / NT;              // 16-byte loads a lane and stage
+  static_assert(NT == ROWS && LOADS == kStageBlocks && BM % 64 == 0 && BN % 64 == 0, "one row's scales a thread");
+  __shared__ __align__(16) uint8_t s_c[2][ROWS * kStageBytes];
+  __shared__ __align__(16) uint4 s_s[2][ROWS];
+
+  // Workgroups go round the eight XCDs in turn: each gets one run of tiles, four
+  // rows of them high, so that what its workgroups share lies in its own L2.
+  const int tiles = mtiles * ntiles, per = (tiles + 7) / 8;
+  const int tl = (int)(blockIdx.x % 8) * per + (int)(blockIdx.x / 8);
+  if ((int)(blockIdx.x / 8) >= per || tl >= tiles) return;
+  const int band = tl / (4 * ntiles), high = min(4, mtiles - 4 * band), in = tl - band * 4 * ntiles;
+  const int64_t m0 = (int64_t)(4 * band + in % high) * BM, n0 = (int64_t)(in / high) * BN;
+
+  const int tid = threadIdx.x, l = tid & 63, r32 = l & 31, g = l >> 5;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w % WN;
+  const int64_t row_bytes = (int64_t)nb * kMxBlockBytes;
+  const uint8_t* Ab = A + m0 * row_bytes;
+  const uint8_t* Bb = B + n0 * row_bytes;
+  const int amax = (int)min((int64_t)BM, M - m0) - 1, bmax = (int)min((int64_t)BN, N - n0) - 1;
+
+  // Load i of wave w fills chunk slots 64 (w LOADS + i) + l: 8 rows of one
+  // operand (BM is a multiple of 64, a wave's 64 rows belong to one).
+  const bool is_a = w * 64 < BM;
+  const uint8_t* src = uniform_ptr(is_a ? Ab : Bb);
+  const int wrow = is_a ? w * 64 : w * 64 - BM, rmax = is_a ? amax : bmax;
+  const uint32_t lds0 = lds_addr(&s_c[0][0]) + (uint32_t)w * (64 * kStageBytes);
+  uint32_t voff[LOADS];
+#pragma unroll
+  for (int i = 0; i < LOADS; ++i) {
+    const int row = wrow + 8 * i + (l >> 3);
+    voff[i] = (uint32_t)min(row, rmax) * (uint32_t)row_bytes + 16u * (uint32_t)((l & 7) ^ ((row >> 1) & 7));
+  }
+  const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
+  auto issue = [&](int st, int i) {
+    const uint32_t lds = lds0 + (uint32_t)(st & 1) * (ROWS * kStageBytes) + 1024u * (uint32_t)i;
+    const uint8_t* from = src + (int64_t)st * kStageBytes;
+    const int left = nb - st * kStageBlocks;
+    if (left >= kStageBlocks) {
+      glds16(from, voff[i], lds);
+    } else {  // the row's last blocks: chunks past them repeat the last one, and are not used
+      const int row = wrow + 8 * i + (l >> 3), c = (l & 7) ^ ((row >> 1) & 7);
+      glds16(from, voff[i] - 16u * (uint32_t)(c - min(c, left - 1)), lds);
+    }
+  };
+  // This thread's row of scales, blocks [16 bt, 16 bt + 16).
+  const int srow = tid < BM ? min(tid, amax) : min(tid - BM, bmax);
+  const uint8_t* sp = (tid < BM ? As + (m0 + srow) * nb : Bs + (n0 + srow) * nb);
+  auto load_scales = [&](int bt) {
+    uint4 v{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
+    const int left = nb - 16 * bt;
+    if (left >= 16) {
+      __builtin_memcpy(&v, sp + 16 * bt, 16);
+    } else if (left > 0) {
+      uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i < left) x[i / 4] = (x[i / 4] & ~(0xffu << (8 * (i % 4)))) | ((uint32_t)sp[16 * bt + i] << (8 * (i % 4)));
+      v = uint4{x[0], x[1], x[2], x[3]};
+    }
+    return v;
+  };
+
+  f32x16 acc[NTL][MT];
+#pragma unroll
+  for (int i = 0; i < NTL; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
+
+  if (stages > 0) {
+    s_s[0][tid] = load_scales(0);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) issue(0, i);
+  }
+  // Operand reads: this lane's row of tile 0, chunk 2 s + g.
+  uint32_t coff[4];
+#pragma unroll
+  for (int s = 0; s < 4; ++s) coff[s] = (uint32_t)r32 * kStageBytes + 16u * (uint32_t)((2 * s + g) ^ ((r32 >> 1) & 7));
+  const uint8_t* abase = &s_c[0][0] + wm * (MT * 32 * kStageBytes);
+  const uint8_t* bbase = &s_c[0][0] + (BM + wn * (NTL * 32)) * kStageBytes;
+  uint4 next_scales{0, 0, 0, 0};
+  uint4 sa[MT], sb[NTL];
+
+  for (int st = 0; st < stages; ++st) {
+    wait_vmem_le<0>();
+    __syncthreads();  // stage st is in LDS, and nobody reads the other buffers any more
+    if ((st & 1) == 0) {
+      const uint4* ss = s_s[(st >> 1) & 1];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) sa[j] = ss[(wm * MT + j) * 32 + r32];
+#pragma unroll
+      for (int i = 0; i < NTL; ++i) sb[i] = ss[BM + (wn * NTL + i) * 32 + r32];
+      if (st + 2 < stages) next_scales = load_scales((st >> 1) + 1);
+    } else if (st + 1 < stages) {
+      s_s[((st + 1) >> 1) & 1][tid] = next_scales;
+    }
+    const uint8_t* ab = abase + (st & 1) * (ROWS * kStageBytes);
+    const uint8_t* bb = bbase + (st & 1) * (ROWS * kStageBytes);
+    const int left = nb - st * kStageBlocks;
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (st + 1 < stages) {
+        issue(st + 1, 2 * s);
+        issue(st + 1, 2 * s + 1);
+      }
+      if (2 * s >= left) continue;
+      i32x8 av[MT], bv[NTL];
+#pragma unroll
+      for (int i = 0; i < NTL; ++i) bv[i] = fp4_operand(*reinterpret_cast<const uint4*>(bb + i * (32 * kStageBytes) + coff[s]));
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        uint4 a = *reinterpret_cast<const uint4*>(ab + j * (32 * kStageBytes) + coff[s]);
+        if (2 * s + 1 >= left && g == 1) a = uint4{0, 0, 0, 0};  // an odd last block: no partner
+        av[j] = fp4_operand(a);
+      }
+#pragma unroll
+      for (int i = 0; i < NTL; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const bool odd = st & 1;
+          const uint32_t wa = s < 2 ? (odd ? sa[j].z : sa[j].x) : (odd ? sa[j].w : sa[j].y);
+          const uint32_t wb = s < 2 ? (odd ? sb[i].z : sb[i].x) : (odd ? sb[i].w : sb[i].y);
+          if (s % 2 == 0)
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv[i], av[j], acc[i][j], kFp4, kFp4, 0,
+                                                                        (int)(wb >> (8 * g)), 0, (int)(wa >> (8 * g)));
+          else
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv[i], av[j], acc[i][j], kFp4, kFp4, 2,
+                                                                        (int)(wb >> (8 * g)), 2, (int)(wa >> (8 * g)));
+        }
+    }
+  }
+
+#pragma unroll
+  for (int j = 0; j < MT; ++j) {
+    const int64_t row = m0 + (wm * MT + j) * 32 + r32;
+#pragma unroll
+    for (int i = 0; i < NTL; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t col = n0 + (wn * NTL + i) * 32 + 8 * q + 4 * g;
+        if (row < M)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (col + e < N) ep.store(row, col + e, acc[i][j][4 * q + e]);
+      }
+  }
+}
+
+template <typename O, int BM, int BN, int WM, int WN>
+int tile_launch(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, int64_t M,
+                int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
+  const int64_t mt = (M + BM - 1) / BM, nt = (N + BN - 1) / BN, grid = (mt * nt + 7) / 8 * 8;
+  if (!grid_fits(grid, 64 * WM * WN)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
+  hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As, B, Bs, M,
+                     N, (int)mx_blocks(K), (int)mt, (int)nt, ep);
+  TT_LAUNCHED(fn, s);
+  return ok();
+}
+
 template <typename O>
 int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, int64_t M,
             int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
+  // 32-bit offsets of a tile's rows
+  const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
+  auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
+  if (!wide && M > 64 && tiles(256) >= 128) return tile_launch<O, 256, 256, 2, 4>(fn, A, As, B, Bs, M, N, K, ep, s);
+  if (!wide && M > 64) return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
+  if (M <= 16) return strip_launch<O, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  if (M <= 32) return strip_launch<O, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
   return strip_launch<O, 4, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
 }
 
