@@ -52,6 +52,57 @@ struct MxEpilogue {
     if (beta != 0.f) v += beta * get(C + row * N + col);
     return v;
   }
+  // bias of columns [col, col + 4), 0 past the last one
+  __device__ __forceinline__ void load_bias(int64_t col, float (&b)[4]) const {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = bias && col + e < N ? get(bias + (col + e) * bias_step) : 0.f;
+  }
+  // What half g (l / 32) of a wave holds of a row: v[h], columns [col + 8 h + 4 g, + 4)
+  // without beta C, for both halves' lanes of the same row (every lane calls;
+  // `in`: the row is inside C).  fp32 stores four columns at a time; bf16
+  // changes halves first, so that each lane stores eight.
+  __device__ __forceinline__ void store_pair(bool in, int64_t row, int64_t col, int g, float (&v)[2][4]) const {
+    O* c = C + row * N;
+    if (beta != 0.f && in) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + 8 * h + 4 * g + e < N) v[h][e] += beta * get(c + col + 8 * h + 4 * g + e);
+    }
+    if constexpr (sizeof(O) == 4) {
+      if (!in) return;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int64_t at = col + 8 * h + 4 * g;
+        if (at + 4 <= N) {
+          __builtin_memcpy(c + at, v[h], 16);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (at + e < N) put(c + at + e, v[h][e]);
+        }
+      }
+    } else {
+      uint32_t x[4];
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        const auto t = __builtin_amdgcn_permlane32_swap(pack_bf16x2(v[0][2 * p], v[0][2 * p + 1]),
+                                                        pack_bf16x2(v[1][2 * p], v[1][2 * p + 1]), false, false);
+        x[p] = t[0];
+        x[2 + p] = t[1];
+      }
+      if (!in) return;
+      const int64_t at = col + 8 * g;
+      if (at + 8 <= N) {
+        __builtin_memcpy(c + at, x, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (at + e < N) c[at + e] = (u16)(x[e / 2] >> (16 * (e & 1)));
+      }
+    }
+  }
   __device__ __forceinline__ void store(int64_t row, int64_t col, float acc) const {
     put(C + row * N + col, value(row, col, acc));
   }
@@ -193,7 +244,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   constexpr int LOADS = ROWS * kStageBlocks / NT;              // 16-byte loads a lane and stage
   static_assert(NT == ROWS && LOADS == kStageBlocks && BM % 64 == 0 && BN % 64 == 0, "one row's scales a thread");
   __shared__ __align__(16) uint8_t s_c[2][ROWS * kStageBytes];
-  __shared__ __align__(16) uint4 s_s[2][ROWS];
+  __shared__ __align__(16) ulonglong2 s_s[2][ROWS];
 
   // Workgroups go round the eight XCDs in turn: each gets one run of tiles, four
   // rows of them high, so that what its workgroups share lies in its own L2.
@@ -211,45 +262,38 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   const int amax = (int)min((int64_t)BM, M - m0) - 1, bmax = (int)min((int64_t)BN, N - n0) - 1;
 
   // Load i of wave w fills chunk slots 64 (w LOADS + i) + l: 8 rows of one
-  // operand (BM is a multiple of 64, a wave's 64 rows belong to one).
+  // operand (BM is a multiple of 64, a wave's 64 rows belong to one).  The
+  // chunk that belongs there goes by the parity of i; chunks past the row's end
+  // repeat its last one and are not used.
   const bool is_a = w * 64 < BM;
   const uint8_t* src = uniform_ptr(is_a ? Ab : Bb);
   const int wrow = is_a ? w * 64 : w * 64 - BM, rmax = is_a ? amax : bmax;
   const uint32_t lds0 = lds_addr(&s_c[0][0]) + (uint32_t)w * (64 * kStageBytes);
-  uint32_t voff[LOADS];
+  uint32_t roff[LOADS];
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) {
-    const int row = wrow + 8 * i + (l >> 3);
-    voff[i] = (uint32_t)min(row, rmax) * (uint32_t)row_bytes + 16u * (uint32_t)((l & 7) ^ ((row >> 1) & 7));
-  }
+  for (int i = 0; i < LOADS; ++i) roff[i] = (uint32_t)min(wrow + 8 * i + (l >> 3), rmax) * (uint32_t)row_bytes;
+  const int chunk0 = (l & 7) ^ (l >> 4), chunk1 = chunk0 ^ 4;
   const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
   auto issue = [&](int st, int i) {
-    const uint32_t lds = lds0 + (uint32_t)(st & 1) * (ROWS * kStageBytes) + 1024u * (uint32_t)i;
-    const uint8_t* from = src + (int64_t)st * kStageBytes;
-    const int left = nb - st * kStageBlocks;
-    if (left >= kStageBlocks) {
-      glds16(from, voff[i], lds);
-    } else {  // the row's last blocks: chunks past them repeat the last one, and are not used
-      const int row = wrow + 8 * i + (l >> 3), c = (l & 7) ^ ((row >> 1) & 7);
-      glds16(from, voff[i] - 16u * (uint32_t)(c - min(c, left - 1)), lds);
-    }
+    const int last = nb - st * kStageBlocks - 1;
+    glds16(src + (int64_t)st * kStageBytes, roff[i] + 16u * (uint32_t)min(i & 1 ? chunk1 : chunk0, last),
+           lds0 + (uint32_t)(st & 1) * (ROWS * kStageBytes) + 1024u * (uint32_t)i);
   };
-  // This thread's row of scales, blocks [16 bt, 16 bt + 16).
+  // This thread's row of scales, blocks [16 bt, 16 bt + 16): zeros past the row's end.
   const int srow = tid < BM ? min(tid, amax) : min(tid - BM, bmax);
   const uint8_t* sp = (tid < BM ? As + (m0 + srow) * nb : Bs + (n0 + srow) * nb);
-  auto load_scales = [&](int bt) {
-    uint4 v{0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu, 0x7f7f7f7fu};
-    const int left = nb - 16 * bt;
-    if (left >= 16) {
-      __builtin_memcpy(&v, sp + 16 * bt, 16);
-    } else if (left > 0) {
-      uint32_t x[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-      for (int i = 0; i < 16; ++i)
-        if (i < left) x[i / 4] = (x[i / 4] & ~(0xffu << (8 * (i % 4)))) | ((uint32_t)sp[16 * bt + i] << (8 * (i % 4)));
-      v = uint4{x[0], x[1], x[2], x[3]};
+  auto load_scales = [&](int bt) {  // nb >= 16
+    uint64_t x[2];
+    const int at = min(16 * bt, nb - 16), past = 8 * (16 * bt - at);
+    __builtin_memcpy(x, sp + at, 16);
+    if (past >= 64) {
+      x[0] = x[1] >> (past - 64);
+      x[1] = 0;
+    } else if (past > 0) {
+      x[0] = (x[0] >> past) | (x[1] << (64 - past));
+      x[1] >>= past;
     }
-    return v;
+    return ulonglong2{x[0], x[1]};
   };
 
   f32x16 acc[NTL][MT];
@@ -261,9 +305,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
   if (stages > 0) {
-    s_s[0][tid] = load_scales(0);
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) issue(0, i);
+    if (nb >= 16) {
+      s_s[0][tid] = load_scales(0);
+    } else {
+      uint8_t* to = reinterpret_cast<uint8_t*>(&s_s[0][tid]);
+      for (int i = 0; i < 16; ++i) to[i] = i < nb ? sp[i] : (uint8_t)0;
+    }
   }
   // Operand reads: this lane's row of tile 0, chunk 2 s + g.
   uint32_t coff[4];
@@ -271,72 +320,97 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   for (int s = 0; s < 4; ++s) coff[s] = (uint32_t)r32 * kStageBytes + 16u * (uint32_t)((2 * s + g) ^ ((r32 >> 1) & 7));
   const uint8_t* abase = &s_c[0][0] + wm * (MT * 32 * kStageBytes);
   const uint8_t* bbase = &s_c[0][0] + (BM + wn * (NTL * 32)) * kStageBytes;
-  uint4 next_scales{0, 0, 0, 0};
-  uint4 sa[MT], sb[NTL];
-
-  for (int st = 0; st < stages; ++st) {
-    wait_vmem_le<0>();
-    __syncthreads();  // stage st is in LDS, and nobody reads the other buffers any more
-    if ((st & 1) == 0) {
-      const uint4* ss = s_s[(st >> 1) & 1];
-#pragma unroll
-      for (int j = 0; j < MT; ++j) sa[j] = ss[(wm * MT + j) * 32 + r32];
-#pragma unroll
-      for (int i = 0; i < NTL; ++i) sb[i] = ss[BM + (wn * NTL + i) * 32 + r32];
-      if (st + 2 < stages) next_scales = load_scales((st >> 1) + 1);
-    } else if (st + 1 < stages) {
-      s_s[((st + 1) >> 1) & 1][tid] = next_scales;
-    }
+  ulonglong2 next_scales{0, 0};
+  uint4 av[2][MT], bv[2][NTL];
+  uint32_t sa[MT][2], sb[NTL][2];  // a stage's scales, this half's bytes at 0 and 2
+  auto read = [&](int st, int s) {
     const uint8_t* ab = abase + (st & 1) * (ROWS * kStageBytes);
     const uint8_t* bb = bbase + (st & 1) * (ROWS * kStageBytes);
-    const int left = nb - st * kStageBlocks;
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (st + 1 < stages) {
-        issue(st + 1, 2 * s);
-        issue(st + 1, 2 * s + 1);
-      }
-      if (2 * s >= left) continue;
-      i32x8 av[MT], bv[NTL];
+    for (int i = 0; i < NTL; ++i) bv[s & 1][i] = *reinterpret_cast<const uint4*>(bb + i * (32 * kStageBytes) + coff[s]);
 #pragma unroll
-      for (int i = 0; i < NTL; ++i) bv[i] = fp4_operand(*reinterpret_cast<const uint4*>(bb + i * (32 * kStageBytes) + coff[s]));
-#pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        uint4 a = *reinterpret_cast<const uint4*>(ab + j * (32 * kStageBytes) + coff[s]);
-        if (2 * s + 1 >= left && g == 1) a = uint4{0, 0, 0, 0};  // an odd last block: no partner
-        av[j] = fp4_operand(a);
-      }
-#pragma unroll
-      for (int i = 0; i < NTL; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const bool odd = st & 1;
-          const uint32_t wa = s < 2 ? (odd ? sa[j].z : sa[j].x) : (odd ? sa[j].w : sa[j].y);
-          const uint32_t wb = s < 2 ? (odd ? sb[i].z : sb[i].x) : (odd ? sb[i].w : sb[i].y);
-          if (s % 2 == 0)
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv[i], av[j], acc[i][j], kFp4, kFp4, 0,
-                                                                        (int)(wb >> (8 * g)), 0, (int)(wa >> (8 * g)));
-          else
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bv[i], av[j], acc[i][j], kFp4, kFp4, 2,
-                                                                        (int)(wb >> (8 * g)), 2, (int)(wa >> (8 * g)));
-        }
-    }
-  }
-
-#pragma unroll
-  for (int j = 0; j < MT; ++j) {
-    const int64_t row = m0 + (wm * MT + j) * 32 + r32;
+    for (int j = 0; j < MT; ++j) av[s & 1][j] = *reinterpret_cast<const uint4*>(ab + j * (32 * kStageBytes) + coff[s]);
+  };
+  auto multiply = [&](int s) {
 #pragma unroll
     for (int i = 0; i < NTL; ++i)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int64_t col = n0 + (wn * NTL + i) * 32 + 8 * q + 4 * g;
-        if (row < M)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (col + e < N) ep.store(row, col + e, acc[i][j][4 * q + e]);
+      for (int j = 0; j < MT; ++j) {
+        const i32x8 x = fp4_operand(bv[s & 1][i]), y = fp4_operand(av[s & 1][j]);
+        const int wb = (int)sb[i][s >> 1], wa = (int)sa[j][s >> 1];
+        acc[i][j] = s % 2 == 0
+                        ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 0, wb, 0, wa)
+                        : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 2, wb, 2, wa);
       }
+  };
+  auto begin = [&](int st) {  // stage st is in LDS, and nobody reads the other buffers any more
+    wait_vmem_le<0>();
+    __syncthreads();
+    const uint64_t* ss = reinterpret_cast<const uint64_t*>(s_s[(st >> 1) & 1]) + (st & 1);
+    read(st, 0);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+      const uint64_t x = ss[2 * ((wm * MT + j) * 32 + r32)] >> (8 * g);
+      sa[j][0] = (uint32_t)x;
+      sa[j][1] = (uint32_t)(x >> 32);
+    }
+#pragma unroll
+    for (int i = 0; i < NTL; ++i) {
+      const uint64_t x = ss[2 * (BM + (wn * NTL + i) * 32 + r32)] >> (8 * g);
+      sb[i][0] = (uint32_t)x;
+      sb[i][1] = (uint32_t)(x >> 32);
+    }
+  };
+  // Stages that another one follows are whole.
+  for (int st = 0; st + 1 < stages; ++st) {
+    begin(st);
+    if ((st & 1) == 0) {
+      if (st + 2 < stages) next_scales = load_scales((st >> 1) + 1);
+    } else {
+      s_s[((st + 1) >> 1) & 1][tid] = next_scales;
+    }
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      issue(st + 1, 2 * s);
+      issue(st + 1, 2 * s + 1);
+      if (s < 3) read(st, s + 1);
+      multiply(s);
+    }
   }
+  if (stages > 0) {
+    const int st = stages - 1, left = nb - st * kStageBlocks;
+    begin(st);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      if (2 * s >= left) break;
+      if (s > 0) read(st, s);
+      if (2 * s + 1 >= left && g == 1) {  // an odd last block: no partner
+#pragma unroll
+        for (int j = 0; j < MT; ++j) av[s & 1][j] = uint4{0, 0, 0, 0};
+      }
+      multiply(s);
+    }
+  }
+
+#pragma unroll
+  for (int i = 0; i < NTL; ++i)
+#pragma unroll
+    for (int q = 0; q < 4; q += 2) {
+      const int64_t col = n0 + (wn * NTL + i) * 32 + 8 * q;
+      float bias[2][4];
+      ep.load_bias(col + 4 * g, bias[0]);
+      ep.load_bias(col + 8 + 4 * g, bias[1]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const int64_t row = m0 + (wm * MT + j) * 32 + r32;
+        float v[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[h][e] = ep.alpha * acc[i][j][4 * (q + h) + e] + bias[h][e];
+        ep.store_pair(row < M, row, col, g, v);
+      }
+    }
 }
 
 template <typename O, int BM, int BN, int WM, int WN>
