@@ -223,27 +223,31 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
   return (const uint8_t*)(uintptr_t)(((uint64_t)hi << 32) | lo);
 }
 
-// Tiles: BM x BN of C a workgroup of WM x WN waves, k in stages of 256 (8
-// blocks, 128 bytes of codes a row).  A stage's codes of both operands come
-// straight into LDS (global_load_lds, 16 bytes a lane) a stage ahead, chunk c of
-// row r at chunk c ^ (r / 2 % 8), so that the 32 rows that an operand read takes
-// one chunk of lie in all banks.  The scales of two stages (16 bytes a row) go
-// through registers into LDS two stages ahead.  Rows past M or N repeat the last
-// one and are not stored.  The matrix unit takes B's rows first, so a lane ends
-// with four consecutive columns of one row of C.
-constexpr int kStageBlocks = 8, kStageBytes = kStageBlocks * kMxBlockBytes;
+// Tiles: BM x BN of C a workgroup of WM x WN waves, k in stages of 128 (4
+// blocks, 64 bytes of codes a row).  A stage's codes of both operands come
+// straight into LDS (global_load_lds, 16 bytes a lane) three stages ahead
+// through a ring of four; chunk c of row r lies at chunk c ^ (r / 4 % 4), so that
+// the 32 rows of which an operand read takes one chunk spread over all banks.
+// The scales of four stages (16 bytes a row) come with them where rows of
+// scales are 16-byte aligned (DMA), else through registers, whose wait drains
+// the ring once in four stages.  A wave reads the operands of a k step of 64
+// while it multiplies the one before, also across the barrier of the next
+// stage.  Rows past M or N repeat the last one and are not stored.  The matrix
+// unit takes B's rows first, so a lane ends with runs of four consecutive
+// columns of one row of C.
+constexpr int kStageBlocks = 4, kStageBytes = kStageBlocks * kMxBlockBytes, kStages = 4;
 
-template <typename O, int BM, int BN, int WM, int WN>
+template <typename O, int BM, int BN, int WM, int WN, bool DMA>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* __restrict__ A,
                                                                 const uint8_t* __restrict__ As,
                                                                 const uint8_t* __restrict__ B,
                                                                 const uint8_t* __restrict__ Bs, int64_t M, int64_t N,
                                                                 int nb, int mtiles, int ntiles, MxEpilogue<O> ep) {
   constexpr int NT = 64 * WM * WN, ROWS = BM + BN;
-  constexpr int MT = BM / WM / 32, NTL = BN / WN / 32;         // 32-row operand tiles of a wave
-  constexpr int LOADS = ROWS * kStageBlocks / NT;              // 16-byte loads a lane and stage
+  constexpr int MT = BM / WM / 32, NTL = BN / WN / 32;  // 32-row operand tiles of a wave
+  constexpr int LOADS = ROWS * kStageBlocks / NT;       // 16-byte loads a lane and stage
   static_assert(NT == ROWS && LOADS == kStageBlocks && BM % 64 == 0 && BN % 64 == 0, "one row's scales a thread");
-  __shared__ __align__(16) uint8_t s_c[2][ROWS * kStageBytes];
+  __shared__ __align__(16) uint8_t s_c[kStages][ROWS * kStageBytes];
   __shared__ __align__(16) ulonglong2 s_s[2][ROWS];
 
   // Workgroups go round the eight XCDs in turn: each gets one run of tiles, four
@@ -257,35 +261,35 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   const int tid = threadIdx.x, l = tid & 63, r32 = l & 31, g = l >> 5;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6), wm = w / WN, wn = w % WN;
   const int64_t row_bytes = (int64_t)nb * kMxBlockBytes;
-  const uint8_t* Ab = A + m0 * row_bytes;
-  const uint8_t* Bb = B + n0 * row_bytes;
   const int amax = (int)min((int64_t)BM, M - m0) - 1, bmax = (int)min((int64_t)BN, N - n0) - 1;
+  const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
 
-  // Load i of wave w fills chunk slots 64 (w LOADS + i) + l: 8 rows of one
-  // operand (BM is a multiple of 64, a wave's 64 rows belong to one).  The
-  // chunk that belongs there goes by the parity of i; chunks past the row's end
-  // repeat its last one and are not used.
+  // Load i of wave w fills chunk slots 64 (w LOADS + i) + l: 16 rows of one
+  // operand (BM is a multiple of 64, a wave's 64 rows belong to one).  Chunks
+  // past the row's end repeat its last one and are not used.
   const bool is_a = w * 64 < BM;
-  const uint8_t* src = uniform_ptr(is_a ? Ab : Bb);
+  const uint8_t* src = uniform_ptr(is_a ? A + m0 * row_bytes : B + n0 * row_bytes);
   const int wrow = is_a ? w * 64 : w * 64 - BM, rmax = is_a ? amax : bmax;
   const uint32_t lds0 = lds_addr(&s_c[0][0]) + (uint32_t)w * (64 * kStageBytes);
   uint32_t roff[LOADS];
 #pragma unroll
-  for (int i = 0; i < LOADS; ++i) roff[i] = (uint32_t)min(wrow + 8 * i + (l >> 3), rmax) * (uint32_t)row_bytes;
-  const int chunk0 = (l & 7) ^ (l >> 4), chunk1 = chunk0 ^ 4;
-  const int stages = (nb + kStageBlocks - 1) / kStageBlocks;
+  for (int i = 0; i < LOADS; ++i) roff[i] = (uint32_t)min(wrow + 16 * i + (l >> 2), rmax) * (uint32_t)row_bytes;
+  const int chunk = (l & 3) ^ (l >> 4);
   auto issue = [&](int st, int i) {
-    const int last = nb - st * kStageBlocks - 1;
-    glds16(src + (int64_t)st * kStageBytes, roff[i] + 16u * (uint32_t)min(i & 1 ? chunk1 : chunk0, last),
-           lds0 + (uint32_t)(st & 1) * (ROWS * kStageBytes) + 1024u * (uint32_t)i);
+    const uint32_t c = 16u * (uint32_t)min(chunk, nb - st * kStageBlocks - 1);
+    glds16(src + (int64_t)st * kStageBytes, roff[i] + c,
+           lds0 + (uint32_t)(st % kStages) * (ROWS * kStageBytes) + 1024u * (uint32_t)i);
   };
-  // This thread's row of scales, blocks [16 bt, 16 bt + 16): zeros past the row's end.
-  const int srow = tid < BM ? min(tid, amax) : min(tid - BM, bmax);
-  const uint8_t* sp = (tid < BM ? As + (m0 + srow) * nb : Bs + (n0 + srow) * nb);
-  auto load_scales = [&](int bt) {  // nb >= 16
+  // Scales: blocks [16 bt, 16 bt + 16) of this thread's row.
+  const uint8_t* ssrc = uniform_ptr(is_a ? As + m0 * nb : Bs + n0 * nb);
+  const uint32_t soff = (uint32_t)min(wrow + l, rmax) * (uint32_t)nb;
+  auto issue_scales = [&](int bt) {
+    glds16(ssrc + 16 * bt, soff, lds_addr(&s_s[bt & 1][0]) + (uint32_t)w * 1024u);
+  };
+  auto load_scales = [&](int bt) {  // nb >= 16; zeros past the row's end
     uint64_t x[2];
     const int at = min(16 * bt, nb - 16), past = 8 * (16 * bt - at);
-    __builtin_memcpy(x, sp + at, 16);
+    __builtin_memcpy(x, ssrc + soff + at, 16);
     if (past >= 64) {
       x[0] = x[1] >> (past - 64);
       x[1] = 0;
@@ -304,91 +308,101 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
 #pragma unroll
       for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.f;
 
-  if (stages > 0) {
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) issue(0, i);
-    if (nb >= 16) {
-      s_s[0][tid] = load_scales(0);
-    } else {
-      uint8_t* to = reinterpret_cast<uint8_t*>(&s_s[0][tid]);
-      for (int i = 0; i < 16; ++i) to[i] = i < nb ? sp[i] : (uint8_t)0;
-    }
-  }
   // Operand reads: this lane's row of tile 0, chunk 2 s + g.
-  uint32_t coff[4];
-#pragma unroll
-  for (int s = 0; s < 4; ++s) coff[s] = (uint32_t)r32 * kStageBytes + 16u * (uint32_t)((2 * s + g) ^ ((r32 >> 1) & 7));
+  const uint32_t coff[2] = {(uint32_t)r32 * kStageBytes + 16u * (uint32_t)(g ^ ((r32 >> 2) & 3)),
+                            (uint32_t)r32 * kStageBytes + 16u * (uint32_t)((2 + g) ^ ((r32 >> 2) & 3))};
   const uint8_t* abase = &s_c[0][0] + wm * (MT * 32 * kStageBytes);
   const uint8_t* bbase = &s_c[0][0] + (BM + wn * (NTL * 32)) * kStageBytes;
-  ulonglong2 next_scales{0, 0};
   uint4 av[2][MT], bv[2][NTL];
-  uint32_t sa[MT][2], sb[NTL][2];  // a stage's scales, this half's bytes at 0 and 2
+  uint32_t sa[2][MT], sb[2][NTL];  // a stage's scales, this half's bytes at 0 and 2
   auto read = [&](int st, int s) {
-    const uint8_t* ab = abase + (st & 1) * (ROWS * kStageBytes);
-    const uint8_t* bb = bbase + (st & 1) * (ROWS * kStageBytes);
+    const uint32_t at = (uint32_t)(st % kStages) * (ROWS * kStageBytes) + coff[s];
 #pragma unroll
-    for (int i = 0; i < NTL; ++i) bv[s & 1][i] = *reinterpret_cast<const uint4*>(bb + i * (32 * kStageBytes) + coff[s]);
+    for (int i = 0; i < NTL; ++i) bv[s][i] = *reinterpret_cast<const uint4*>(bbase + i * (32 * kStageBytes) + at);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) av[s & 1][j] = *reinterpret_cast<const uint4*>(ab + j * (32 * kStageBytes) + coff[s]);
+    for (int j = 0; j < MT; ++j) av[s][j] = *reinterpret_cast<const uint4*>(abase + j * (32 * kStageBytes) + at);
+  };
+  auto read_scales = [&](int st, int p) {
+    const uint32_t* ss = reinterpret_cast<const uint32_t*>(s_s[(st >> 2) & 1]) + (st & 3);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sa[p][j] = ss[4 * ((wm * MT + j) * 32 + r32)];
+#pragma unroll
+    for (int i = 0; i < NTL; ++i) sb[p][i] = ss[4 * (BM + (wn * NTL + i) * 32 + r32)];
   };
   auto multiply = [&](int s) {
 #pragma unroll
     for (int i = 0; i < NTL; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        const i32x8 x = fp4_operand(bv[s & 1][i]), y = fp4_operand(av[s & 1][j]);
-        const int wb = (int)sb[i][s >> 1], wa = (int)sa[j][s >> 1];
-        acc[i][j] = s % 2 == 0
-                        ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 0, wb, 0, wa)
-                        : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 2, wb, 2, wa);
+        const i32x8 x = fp4_operand(bv[s][i]), y = fp4_operand(av[s][j]);
+        acc[i][j] = s == 0 ? __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 0,
+                                                                             (int)sb[0][i], 0, (int)sa[0][j])
+                           : __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(x, y, acc[i][j], kFp4, kFp4, 2,
+                                                                             (int)sb[0][i], 2, (int)sa[0][j]);
       }
   };
-  auto begin = [&](int st) {  // stage st is in LDS, and nobody reads the other buffers any more
-    wait_vmem_le<0>();
+  auto shift_scales = [&](int p) {
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sa[0][j] = sa[p][j] >> (8 * g);
+#pragma unroll
+    for (int i = 0; i < NTL; ++i) sb[0][i] = sb[p][i] >> (8 * g);
+  };
+  // Stage st has landed for every wave, and nobody reads the stage before any more.
+  auto meet = [&](int st) {
+    wait_vmem_tiles<LOADS, 2>(min(2, stages - 1 - st));
     __syncthreads();
-    const uint64_t* ss = reinterpret_cast<const uint64_t*>(s_s[(st >> 1) & 1]) + (st & 1);
-    read(st, 0);
-#pragma unroll
-    for (int j = 0; j < MT; ++j) {
-      const uint64_t x = ss[2 * ((wm * MT + j) * 32 + r32)] >> (8 * g);
-      sa[j][0] = (uint32_t)x;
-      sa[j][1] = (uint32_t)(x >> 32);
-    }
-#pragma unroll
-    for (int i = 0; i < NTL; ++i) {
-      const uint64_t x = ss[2 * (BM + (wn * NTL + i) * 32 + r32)] >> (8 * g);
-      sb[i][0] = (uint32_t)x;
-      sb[i][1] = (uint32_t)(x >> 32);
-    }
   };
-  // Stages that another one follows are whole.
-  for (int st = 0; st + 1 < stages; ++st) {
-    begin(st);
-    if ((st & 1) == 0) {
-      if (st + 2 < stages) next_scales = load_scales((st >> 1) + 1);
-    } else {
-      s_s[((st + 1) >> 1) & 1][tid] = next_scales;
-    }
+  auto zero_odd = [&](int s, int left) {  // an odd last block: no partner
+    if (2 * s + 1 >= left && g == 1)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      issue(st + 1, 2 * s);
-      issue(st + 1, 2 * s + 1);
-      if (s < 3) read(st, s + 1);
-      multiply(s);
-    }
-  }
+      for (int j = 0; j < MT; ++j) av[s][j] = uint4{0, 0, 0, 0};
+  };
+
   if (stages > 0) {
-    const int st = stages - 1, left = nb - st * kStageBlocks;
-    begin(st);
+    if constexpr (DMA) {
+      issue_scales(0);
+    } else if (nb >= 16) {
+      s_s[0][tid] = load_scales(0);
+    } else {
+      uint8_t* to = reinterpret_cast<uint8_t*>(&s_s[0][tid]);
+      for (int i = 0; i < 16; ++i) to[i] = i < nb ? ssrc[soff + i] : (uint8_t)0;
+    }
+    for (int st = 0; st < min(stages, 3); ++st)
 #pragma unroll
-    for (int s = 0; s < 4; ++s) {
-      if (2 * s >= left) break;
-      if (s > 0) read(st, s);
-      if (2 * s + 1 >= left && g == 1) {  // an odd last block: no partner
-#pragma unroll
-        for (int j = 0; j < MT; ++j) av[s & 1][j] = uint4{0, 0, 0, 0};
+      for (int i = 0; i < LOADS; ++i) issue(st, i);
+    meet(0);
+    read(0, 0);
+    read_scales(0, 1);
+    ulonglong2 next_scales{0, 0};
+    // Stages that another one follows are whole.
+    for (int st = 0; st + 1 < stages; ++st) {
+      shift_scales(1);
+      read(st, 1);
+      const bool more = (st & 3) == 1 && st + 3 < stages;  // the batch of stage st + 3
+      if constexpr (DMA) {
+        if (more) issue_scales((st + 3) >> 2);
+      } else {
+        if (more) next_scales = load_scales((st + 3) >> 2);
       }
-      multiply(s);
+      if (st + 3 < stages)
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) issue(st + 3, i);
+      multiply(0);
+      if constexpr (!DMA)
+        if ((st & 3) == 3) s_s[((st + 1) >> 2) & 1][tid] = next_scales;
+      meet(st + 1);
+      read(st + 1, 0);
+      read_scales(st + 1, 1);
+      multiply(1);
+    }
+    const int left = nb - (stages - 1) * kStageBlocks;
+    shift_scales(1);
+    zero_odd(0, left);
+    multiply(0);
+    if (left > 2) {
+      read(stages - 1, 1);
+      zero_odd(1, left);
+      multiply(1);
     }
   }
 
@@ -418,8 +432,13 @@ int tile_launch(const char* fn, const uint8_t* A, const uint8_t* As, const uint8
                 int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
   const int64_t mt = (M + BM - 1) / BM, nt = (N + BN - 1) / BN, grid = (mt * nt + 7) / 8 * 8;
   if (!grid_fits(grid, 64 * WM * WN)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
-  hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As, B, Bs, M,
-                     N, (int)mx_blocks(K), (int)mt, (int)nt, ep);
+  const int64_t nb = mx_blocks(K);
+  if (nb % 16 == 0 && (((uintptr_t)As | (uintptr_t)Bs) & 15) == 0)
+    hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN, true>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As, B,
+                       Bs, M, N, (int)nb, (int)mt, (int)nt, ep);
+  else
+    hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN, false>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As,
+                       B, Bs, M, N, (int)nb, (int)mt, (int)nt, ep);
   TT_LAUNCHED(fn, s);
   return ok();
 }
