@@ -228,16 +228,17 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
 // straight into LDS (global_load_lds, 16 bytes a lane) three stages ahead
 // through a ring of four; chunk c of row r lies at chunk c ^ (r / 4 % 4), so that
 // the 32 rows of which an operand read takes one chunk spread over all banks.
-// The scales of four stages (16 bytes a row) come with them where rows of
-// scales are 16-byte aligned (DMA), else through registers, whose wait drains
-// the ring once in four stages.  A wave reads the operands of a k step of 64
+// The scales of four stages (16 bytes a row) come the same way, at any
+// alignment: as the two aligned 16-byte words that hold them (a load through
+// registers would wait for every load of the ring, 477 us for 348 at 8192 x 8192
+// x 8224), which the wave that loaded them then lays out by stage.  A wave reads the operands of a k step of 64
 // while it multiplies the one before, also across the barrier of the next
 // stage.  Rows past M or N repeat the last one and are not stored.  The matrix
 // unit takes B's rows first, so a lane ends with runs of four consecutive
 // columns of one row of C.
 constexpr int kStageBlocks = 4, kStageBytes = kStageBlocks * kMxBlockBytes, kStages = 4;
 
-template <typename O, int BM, int BN, int WM, int WN, bool DMA>
+template <typename O, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* __restrict__ A,
                                                                 const uint8_t* __restrict__ As,
                                                                 const uint8_t* __restrict__ B,
@@ -248,7 +249,8 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   constexpr int LOADS = ROWS * kStageBlocks / NT;       // 16-byte loads a lane and stage
   static_assert(NT == ROWS && LOADS == kStageBlocks && BM % 64 == 0 && BN % 64 == 0, "one row's scales a thread");
   __shared__ __align__(16) uint8_t s_c[kStages][ROWS * kStageBytes];
-  __shared__ __align__(16) ulonglong2 s_s[2][ROWS];
+  __shared__ __align__(16) uint4 s_w[2 * ROWS];        // a batch of scales as loaded
+  __shared__ __align__(16) uint32_t s_s[2][4][ROWS];  // and as used: a stage's four bytes of each row
 
   // Workgroups go round the eight XCDs in turn: each gets one run of tiles, four
   // rows of them high, so that what its workgroups share lies in its own L2.
@@ -280,24 +282,27 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
     glds16(src + (int64_t)st * kStageBytes, roff[i] + c,
            lds0 + (uint32_t)(st % kStages) * (ROWS * kStageBytes) + 1024u * (uint32_t)i);
   };
-  // Scales: blocks [16 bt, 16 bt + 16) of this thread's row.
-  const uint8_t* ssrc = uniform_ptr(is_a ? As + m0 * nb : Bs + n0 * nb);
-  const uint32_t soff = (uint32_t)min(wrow + l, rmax) * (uint32_t)nb;
+  // Scales: the 16 bytes of blocks [16 bt, 16 bt + 16) of row r lie in words 2 r
+  // and 2 r + 1; bytes past the row's end are some other ones, of words that
+  // hold a scale of the operand at least.
+  const uint8_t* sall = is_a ? As : Bs;
+  const uintptr_t send = ((uintptr_t)sall + (uint64_t)(is_a ? M : N) * nb - 1) & ~(uintptr_t)15;  // the last such word
   auto issue_scales = [&](int bt) {
-    glds16(ssrc + 16 * bt, soff, lds_addr(&s_s[bt & 1][0]) + (uint32_t)w * 1024u);
-  };
-  auto load_scales = [&](int bt) {  // nb >= 16; zeros past the row's end
-    uint64_t x[2];
-    const int at = min(16 * bt, nb - 16), past = 8 * (16 * bt - at);
-    __builtin_memcpy(x, ssrc + soff + at, 16);
-    if (past >= 64) {
-      x[0] = x[1] >> (past - 64);
-      x[1] = 0;
-    } else if (past > 0) {
-      x[0] = (x[0] >> past) | (x[1] << (64 - past));
-      x[1] >>= past;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint8_t* row = sall + ((is_a ? m0 : n0) + min(wrow + 32 * i + (l >> 1), rmax)) * nb + 16 * bt;
+      const uintptr_t at = ((uintptr_t)row & ~(uintptr_t)15) + 16u * (l & 1);
+      glds16_at((const void*)(at < send ? at : send), lds_addr(s_w) + (uint32_t)(2 * w + i) * 1024u);
     }
-    return ulonglong2{x[0], x[1]};
+  };
+  const uint32_t first = (uint32_t)((uintptr_t)sall + (uint64_t)((is_a ? m0 : n0) + min(wrow + l, rmax)) * nb) & 15u;
+  auto lay_out_scales = [&](int bt) {  // this thread's row
+    const uint32_t* x = reinterpret_cast<const uint32_t*>(s_w + 2 * (w * 64 + l)) + (first >> 2);
+    uint32_t d[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) d[i] = x[i];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s_s[bt & 1][i][w * 64 + l] = __builtin_amdgcn_alignbyte(d[i + 1], d[i], first);
   };
 
   f32x16 acc[NTL][MT];
@@ -314,7 +319,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
   const uint8_t* abase = &s_c[0][0] + wm * (MT * 32 * kStageBytes);
   const uint8_t* bbase = &s_c[0][0] + (BM + wn * (NTL * 32)) * kStageBytes;
   uint4 av[2][MT], bv[2][NTL];
-  uint32_t sa[2][MT], sb[2][NTL];  // a stage's scales, this half's bytes at 0 and 2
+  uint32_t sa[2][MT], sb[2][NTL];  // [0]: a stage's scales, this half's bytes at 0 and 2; [1]: the next stage's, as read
   auto read = [&](int st, int s) {
     const uint32_t at = (uint32_t)(st % kStages) * (ROWS * kStageBytes) + coff[s];
 #pragma unroll
@@ -322,12 +327,12 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
 #pragma unroll
     for (int j = 0; j < MT; ++j) av[s][j] = *reinterpret_cast<const uint4*>(abase + j * (32 * kStageBytes) + at);
   };
-  auto read_scales = [&](int st, int p) {
-    const uint32_t* ss = reinterpret_cast<const uint32_t*>(s_s[(st >> 2) & 1]) + (st & 3);
+  auto read_scales = [&](int st) {
+    const uint32_t* ss = s_s[(st >> 2) & 1][st & 3];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sa[p][j] = ss[4 * ((wm * MT + j) * 32 + r32)];
+    for (int j = 0; j < MT; ++j) sa[1][j] = ss[(wm * MT + j) * 32 + r32];
 #pragma unroll
-    for (int i = 0; i < NTL; ++i) sb[p][i] = ss[4 * (BM + (wn * NTL + i) * 32 + r32)];
+    for (int i = 0; i < NTL; ++i) sb[1][i] = ss[BM + (wn * NTL + i) * 32 + r32];
   };
   auto multiply = [&](int s) {
 #pragma unroll
@@ -341,62 +346,56 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
                                                                              (int)sb[0][i], 2, (int)sa[0][j]);
       }
   };
-  auto shift_scales = [&](int p) {
+  auto shift_scales = [&]() {
 #pragma unroll
-    for (int j = 0; j < MT; ++j) sa[0][j] = sa[p][j] >> (8 * g);
+    for (int j = 0; j < MT; ++j) sa[0][j] = sa[1][j] >> (8 * g);
 #pragma unroll
-    for (int i = 0; i < NTL; ++i) sb[0][i] = sb[p][i] >> (8 * g);
+    for (int i = 0; i < NTL; ++i) sb[0][i] = sb[1][i] >> (8 * g);
   };
   // Stage st has landed for every wave, and nobody reads the stage before any more.
   auto meet = [&](int st) {
     wait_vmem_tiles<LOADS, 2>(min(2, stages - 1 - st));
     __syncthreads();
   };
-  auto zero_odd = [&](int s, int left) {  // an odd last block: no partner
-    if (2 * s + 1 >= left && g == 1)
+  auto zero_odd = [&](int s, int left) {  // an odd last block: no partner, whatever lies in its place
+    if (2 * s + 1 >= left && g == 1) {
 #pragma unroll
-      for (int j = 0; j < MT; ++j) av[s][j] = uint4{0, 0, 0, 0};
+      for (int j = 0; j < MT; ++j) {
+        av[s][j] = uint4{0, 0, 0, 0};
+        sa[0][j] = 0;
+      }
+#pragma unroll
+      for (int i = 0; i < NTL; ++i) sb[0][i] = 0;
+    }
   };
 
   if (stages > 0) {
-    if constexpr (DMA) {
-      issue_scales(0);
-    } else if (nb >= 16) {
-      s_s[0][tid] = load_scales(0);
-    } else {
-      uint8_t* to = reinterpret_cast<uint8_t*>(&s_s[0][tid]);
-      for (int i = 0; i < 16; ++i) to[i] = i < nb ? ssrc[soff + i] : (uint8_t)0;
-    }
+    issue_scales(0);
     for (int st = 0; st < min(stages, 3); ++st)
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) issue(st, i);
     meet(0);
+    lay_out_scales(0);
+    __syncthreads();
     read(0, 0);
-    read_scales(0, 1);
-    ulonglong2 next_scales{0, 0};
+    read_scales(0);
     // Stages that another one follows are whole.
     for (int st = 0; st + 1 < stages; ++st) {
-      shift_scales(1);
+      shift_scales();
       read(st, 1);
-      const bool more = (st & 3) == 1 && st + 3 < stages;  // the batch of stage st + 3
-      if constexpr (DMA) {
-        if (more) issue_scales((st + 3) >> 2);
-      } else {
-        if (more) next_scales = load_scales((st + 3) >> 2);
-      }
+      if ((st & 3) == 0 && st + 4 < stages) issue_scales((st + 4) >> 2);  // landed with stage st + 3
+      if ((st & 3) == 3) lay_out_scales((st + 1) >> 2);
       if (st + 3 < stages)
 #pragma unroll
         for (int i = 0; i < LOADS; ++i) issue(st + 3, i);
       multiply(0);
-      if constexpr (!DMA)
-        if ((st & 3) == 3) s_s[((st + 1) >> 2) & 1][tid] = next_scales;
       meet(st + 1);
       read(st + 1, 0);
-      read_scales(st + 1, 1);
+      read_scales(st + 1);
       multiply(1);
     }
     const int left = nb - (stages - 1) * kStageBlocks;
-    shift_scales(1);
+    shift_scales();
     zero_odd(0, left);
     multiply(0);
     if (left > 2) {
@@ -432,13 +431,8 @@ int tile_launch(const char* fn, const uint8_t* A, const uint8_t* As, const uint8
                 int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
   const int64_t mt = (M + BM - 1) / BM, nt = (N + BN - 1) / BN, grid = (mt * nt + 7) / 8 * 8;
   if (!grid_fits(grid, 64 * WM * WN)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
-  const int64_t nb = mx_blocks(K);
-  if (nb % 16 == 0 && (((uintptr_t)As | (uintptr_t)Bs) & 15) == 0)
-    hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN, true>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As, B,
-                       Bs, M, N, (int)nb, (int)mt, (int)nt, ep);
-  else
-    hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN, false>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As,
-                       B, Bs, M, N, (int)nb, (int)mt, (int)nt, ep);
+  hipLaunchKernelGGL((k_mxfp4_tile<O, BM, BN, WM, WN>), dim3((unsigned)grid), dim3(64 * WM * WN), 0, s, A, As, B, Bs, M,
+                     N, (int)mx_blocks(K), (int)mt, (int)nt, ep);
   TT_LAUNCHED(fn, s);
   return ok();
 }
