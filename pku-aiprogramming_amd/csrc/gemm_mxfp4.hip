@@ -46,12 +46,6 @@ struct MxEpilogue {
   __device__ __forceinline__ static float get(const u16* p) { return bf16_to_f32(*p); }
   __device__ __forceinline__ static void put(float* p, float v) { *p = v; }
   __device__ __forceinline__ static void put(u16* p, float v) { *p = f32_to_bf16(v); }
-  __device__ __forceinline__ float value(int64_t row, int64_t col, float acc) const {
-    float v = alpha * acc;
-    if (bias) v += get(bias + col * bias_step);
-    if (beta != 0.f) v += beta * get(C + row * N + col);
-    return v;
-  }
   // bias of columns [col, col + 4), 0 past the last one
   __device__ __forceinline__ void load_bias(int64_t col, float (&b)[4]) const {
 #pragma unroll
@@ -103,8 +97,25 @@ struct MxEpilogue {
       }
     }
   }
-  __device__ __forceinline__ void store(int64_t row, int64_t col, float acc) const {
-    put(C + row * N + col, value(row, col, acc));
+  // The sums of columns [col, col + 4) of a row inside C, stored at once where all are.
+  __device__ __forceinline__ void store_four(int64_t row, int64_t col, const f32x4& acc) const {
+    O* c = C + row * N + col;
+    float b[4];
+    load_bias(col, b);
+    O o[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float v = alpha * acc[e] + b[e];
+      if (beta != 0.f && col + e < N) v += beta * get(c + e);
+      put(&o[e], v);
+    }
+    if (col + 4 <= N) {
+      __builtin_memcpy(c, o, sizeof(o));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < N) c[e] = o[e];
+    }
   }
 };
 
@@ -120,98 +131,143 @@ __device__ __forceinline__ uint4 quantize_block(const MxEight<T> (&v)[4], uint32
   return uint4{v[0].codes(f), v[1].codes(f), v[2].codes(f), v[3].codes(f)};
 }
 
-// Strips: a workgroup makes 16 columns of C for 16 MS rows, its eight waves
-// taking every eighth k step of 128 and meeting in LDS.  Operands go from
-// global memory to the matrix unit's registers directly.  For few rows, where
-// B's codes are the bytes that count: each is read once, four steps in flight
-// a wave.  QA: A is not quantised yet (x, rows of K values), and each lane
-// quantises the block that it would have loaded; one launch for a token's
-// layer.
-constexpr int kStripWaves = 8;
+// Blocks: a workgroup makes 16 MT rows by 16 NT columns of C, its eight waves
+// taking an eighth of the k steps of 128 each and meeting in LDS: for products
+// of few tiles, whose time is the serial chain of one workgroup.  Operands go
+// from global memory to the matrix unit's registers directly, four steps in
+// flight a wave (their scales as one 16-byte load a row), with no barrier before
+// the end.  QA: A is not quantised yet (X, rows of K values), and each lane
+// quantises the blocks that it would have loaded: one launch for a layer of few
+// rows.
+constexpr int kBlockWaves = 8;
 
-template <typename O, int MS, bool QA>
-__global__ __launch_bounds__(64 * kStripWaves) void k_mxfp4_strip(const uint4* __restrict__ A,
-                                                                  const uint8_t* __restrict__ As,
-                                                                  const O* __restrict__ X,
-                                                                  const uint4* __restrict__ B,
-                                                                  const uint8_t* __restrict__ Bs, int64_t M, int64_t N,
-                                                                  int64_t K, int nb, uint32_t strips,
-                                                                  MxEpilogue<O> ep) {
-  constexpr int UN = QA && sizeof(O) == 4 ? 2 : 4;
-  __shared__ __align__(16) f32x4 red[kStripWaves][MS][64];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, r = l & 15, g = l >> 4;
-  const int64_t n0 = (int64_t)(blockIdx.x % strips) * 16, m0 = (int64_t)(blockIdx.x / strips) * (16 * MS);
-  const int64_t brow = min(n0 + r, N - 1) * nb;  // rows past the end repeat the last one and are not stored
-  int64_t arow[MS];
+// The scales of k steps [st, st + U) of a row, as this lane's half-filled words:
+// block 4 u + g in byte g of w[u] at least, 0 past the row's nb blocks.
+template <int U>
+__device__ __forceinline__ void load_step_scales(uint32_t (&w)[U], const uint8_t* row, int st, int nb, int g) {
+  if (4 * (st + U) <= nb) {
+    __builtin_memcpy(w, row + 4 * st, 4 * U);
+  } else {
 #pragma unroll
-  for (int i = 0; i < MS; ++i) arow[i] = min(m0 + 16 * i + r, M - 1);
-  f32x4 acc[MS];
-#pragma unroll
-  for (int i = 0; i < MS; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  const int steps = (nb + 3) / 4;
-  for (int i0 = w; i0 < steps; i0 += kStripWaves * UN) {
-    uint4 b[UN], a[UN][MS];
-    uint32_t sb[UN], sa[UN][MS];
-    MxEight<O> v[QA ? UN : 1][4];
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      // blocks past the row's end: some block of the row, made zero below
-      const int blk = 4 * (i0 + kStripWaves * u) + g, at = min(blk, nb - 1);
-      b[u] = B[brow + at];
-      sb[u] = Bs[brow + at];
-      if constexpr (QA) {
-        const O* p = X + arow[0] * K + (int64_t)at * kMxBlock;
-        const int n = (int)min((int64_t)kMxBlock, K - (int64_t)at * kMxBlock);
-        if (n == kMxBlock) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[u][j].load(p + 8 * j);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) v[u][j].load_part(p + 8 * j, n - 8 * j);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < MS; ++i) {
-          a[u][i] = A[arow[i] * nb + at];
-          sa[u][i] = As[arow[i] * nb + at];
-        }
-      }
+    for (int u = 0; u < U; ++u) {
+      const int at = 4 * (st + u);
+      w[u] = 0;
+      if (at + 4 <= nb)
+        __builtin_memcpy(&w[u], row + at, 4);
+      else if (at + g < nb)
+        w[u] = (uint32_t)row[at + g] << (8 * g);
     }
-#pragma unroll
-    for (int u = 0; u < UN; ++u) {
-      if constexpr (QA) a[u][0] = quantize_block(v[u], &sa[u][0]);
-      const bool in = 4 * (i0 + kStripWaves * u) + g < nb;
-      const uint4 bu = in ? b[u] : uint4{0, 0, 0, 0};
-      const uint32_t sbu = in ? sb[u] : 127u;
-#pragma unroll
-      for (int i = 0; i < MS; ++i) {
-        const uint4 au = in ? a[u][i] : uint4{0, 0, 0, 0};
-        acc[i] = mfma_fp4_16(bu, au, acc[i], sbu, in ? sa[u][i] : 127u);
-      }
-    }
-  }
-#pragma unroll
-  for (int i = 0; i < MS; ++i) red[w][i][l] = acc[i];
-  __syncthreads();
-  for (int i = w; i < MS; i += kStripWaves) {
-    f32x4 s = red[0][i][l];
-#pragma unroll
-    for (int q = 1; q < kStripWaves; ++q) s += red[q][i][l];
-    const int64_t row = m0 + 16 * i + r, col = n0 + 4 * g;
-    if (row >= M) continue;
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (col + e < N) ep.store(row, col + e, s[e]);
   }
 }
 
-template <typename O, int MS, bool QA>
-int strip_launch(const char* fn, const uint8_t* A, const uint8_t* As, const O* X, const uint8_t* B, const uint8_t* Bs,
+template <typename O, int MT, int NT, bool QA>
+__global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
+    const uint4* __restrict__ A, const uint8_t* __restrict__ As, const O* __restrict__ X, const uint4* __restrict__ B,
+    const uint8_t* __restrict__ Bs, int64_t M, int64_t N, int64_t K, int nb, uint32_t ntiles, MxEpilogue<O> ep) {
+  constexpr int TILES = MT * NT, HALF = kBlockWaves / 2, UN = QA && sizeof(O) == 4 ? 2 : 4;
+  __shared__ __align__(16) f32x4 red[HALF][TILES][64];
+  const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = l & 15, g = l >> 4;
+  const int64_t n0 = (int64_t)(blockIdx.x % ntiles) * (16 * NT), m0 = (int64_t)(blockIdx.x / ntiles) * (16 * MT);
+  int64_t brow[NT], arow[MT];  // rows past the end repeat the last one and are not stored
+#pragma unroll
+  for (int i = 0; i < NT; ++i) brow[i] = min(n0 + 16 * i + r, N - 1) * nb;
+#pragma unroll
+  for (int j = 0; j < MT; ++j) arow[j] = min(m0 + 16 * j + r, M - 1) * (QA ? K : (int64_t)nb);
+  f32x4 acc[NT][MT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+  const int steps = (nb + 3) / 4, share = (steps + kBlockWaves - 1) / kBlockWaves, end = min((w + 1) * share, steps);
+  for (int st = w * share; st < end; st += UN) {
+    uint4 b[UN][NT], a[UN][MT];
+    uint32_t sb[NT][UN], sa[MT][UN];
+    MxEight<O> v[QA ? UN : 1][MT][4];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) load_step_scales<UN>(sb[i], Bs + brow[i], st, nb, g);
+    if constexpr (!QA) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) load_step_scales<UN>(sa[j], As + arow[j], st, nb, g);
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (u > 0 && st + u >= end) break;
+      // blocks past the row's end: its last one, made zero below
+      const int at = min(4 * (st + u) + g, nb - 1);
+#pragma unroll
+      for (int i = 0; i < NT; ++i) b[u][i] = B[brow[i] + at];
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if constexpr (QA) {
+          const O* p = X + arow[j] + (int64_t)at * kMxBlock;
+          const int n = (int)min((int64_t)kMxBlock, K - (int64_t)at * kMxBlock);
+          if (n == kMxBlock) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[u][j][q].load(p + 8 * q);
+          } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[u][j][q].load_part(p + 8 * q, n - 8 * q);
+          }
+        } else {
+          a[u][j] = A[arow[j] + at];
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < UN; ++u) {
+      if (u > 0 && st + u >= end) break;
+      const bool in = 4 * (st + u) + g < nb;
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if constexpr (QA)
+          a[u][j] = quantize_block(v[u][j], &sa[j][u]);
+        else
+          sa[j][u] >>= 8 * g;
+        if (!in) {
+          a[u][j] = uint4{0, 0, 0, 0};
+          sa[j][u] = 0u;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < NT; ++i) {
+        const uint32_t sbi = in ? sb[i][u] >> (8 * g) : 0u;
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = mfma_fp4_16(b[u][i], a[u][j], acc[i][j], sbi, sa[j][u]);
+      }
+    }
+  }
+  // The upper half of the waves hands its sums to the lower half, whose sums
+  // then meet in a fixed order.
+  if (w >= HALF) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) red[w - HALF][i * MT + j][l] = acc[i][j];
+  }
+  __syncthreads();
+  if (w < HALF) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) red[w][i * MT + j][l] += acc[i][j];
+  }
+  __syncthreads();
+  for (int t = w; t < TILES; t += kBlockWaves) {
+    f32x4 s = red[0][t][l];
+#pragma unroll
+    for (int q = 1; q < HALF; ++q) s += red[q][t][l];
+    const int64_t row = m0 + 16 * (t % MT) + r, col = n0 + 16 * (t / MT) + 4 * g;
+    if (row < M) ep.store_four(row, col, s);
+  }
+}
+
+template <typename O, int MT, int NT, bool QA>
+int block_launch(const char* fn, const uint8_t* A, const uint8_t* As, const O* X, const uint8_t* B, const uint8_t* Bs,
                  int64_t M, int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
-  const int64_t strips = (N + 15) / 16, tiles = strips * ((M + 16 * MS - 1) / (16 * MS));
-  if (!grid_fits(tiles, 64 * kStripWaves)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
-  hipLaunchKernelGGL((k_mxfp4_strip<O, MS, QA>), dim3((unsigned)tiles), dim3(64 * kStripWaves), 0, s, (const uint4*)A,
-                     As, X, (const uint4*)B, Bs, M, N, K, (int)mx_blocks(K), (uint32_t)strips, ep);
+  const int64_t nt = (N + 16 * NT - 1) / (16 * NT), tiles = nt * ((M + 16 * MT - 1) / (16 * MT));
+  if (!grid_fits(tiles, 64 * kBlockWaves)) return fail(TT_ERR_ARG, std::string(fn) + ": m and n too large");
+  hipLaunchKernelGGL((k_mxfp4_block<O, MT, NT, QA>), dim3((unsigned)tiles), dim3(64 * kBlockWaves), 0, s,
+                     (const uint4*)A, As, X, (const uint4*)B, Bs, M, N, K, (int)mx_blocks(K), (uint32_t)nt, ep);
   TT_LAUNCHED(fn, s);
   return ok();
 }
@@ -440,14 +496,22 @@ int tile_launch(const char* fn, const uint8_t* A, const uint8_t* As, const uint8
 template <typename O>
 int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* B, const uint8_t* Bs, int64_t M,
             int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
-  // 32-bit offsets of a tile's rows
-  const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
   auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
-  if (!wide && M > 64 && tiles(256) >= 128) return tile_launch<O, 256, 256, 2, 4>(fn, A, As, B, Bs, M, N, K, ep, s);
-  if (!wide && M > 64) return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
-  if (M <= 16) return strip_launch<O, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
-  if (M <= 32) return strip_launch<O, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
-  return strip_launch<O, 4, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  // Few tiles: the smallest blocks that are not more than two a CU.  Measured
+  // (16 x 16 / 32 x 32 / 128 x 128, us): 1 x 4096 x 4096 4.4 / - / 15.6 (256
+  // blocks), 100 x 1000 x 500 3.5 / 5.2 / 6.1 (441), 64 x 4096 x 4096 12.3 (1024) /
+  // 8.2 / 15.6, 128 x 4096 x 4096 21 / 12.5 (512) / 16.0, 500 x 2000 x 3000 32 / 19.2
+  // (1008) / 13.3.  M <= 16 has nothing to gain from larger ones.
+  if (tiles(16) <= 512 || M <= 16) return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  // the tiles keep the offsets of their rows in 32 bits
+  const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
+  if (wide || tiles(32) <= 512) return block_launch<O, 2, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  // 128 x 128 tiles, two a CU, where one round takes them all.  Measured (128 /
+  // 256, us): 1531 x 4099 x 4096 34.8 / 46.6 (400 small tiles), 2048 x 4096 x 1000
+  // 12.4 / 15.9 (512), 3000 x 3000 x 3000 37.0 / 30.0 (576), 3500 x 3500 x 2000
+  // 35.6 / 28.1 (784).
+  if (tiles(128) <= 512) return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
+  return tile_launch<O, 256, 256, 2, 4>(fn, A, As, B, Bs, M, N, K, ep, s);
 }
 
 // Rows of x quantised at a time; the scratch is of one size, so that graphs may keep its address.
@@ -462,7 +526,7 @@ int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O*
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until the last kernel that reads the buffer is queued
   if (M <= 16 || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
-    return strip_launch<O, 1, true>(fn, nullptr, nullptr, x, W, Ws, M, N, K, all, s);
+    return block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x, W, Ws, M, N, K, all, s);
   for (int64_t r0 = 0; r0 < M; r0 += fit) {
     const int64_t rows = M - r0 < fit ? M - r0 : fit;
     uint8_t* codes = (uint8_t*)ws;
