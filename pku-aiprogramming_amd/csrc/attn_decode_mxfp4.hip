@@ -18,13 +18,13 @@
 //     terms (two for bf16 tensors, 2^-17 off; three for fp32, whose q is split
 //     into three exact terms too), so that no rounding of the weights shows in
 //     the result.
-// The next 32 keys' codes are in flight meanwhile (they are only 4 to 16
-// registers).  The waves of a workgroup meet in LDS at the end, and splits of the
+// The codes of the next step are in flight meanwhile.  The waves of a workgroup meet in LDS at the end, and splits of the
 // keys over workgroups in a second launch.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <cmath>
+#include <limits>
 #include <optional>
 #include <string>
 
@@ -57,11 +57,19 @@ template <int W>
 struct MdPiece {
   uint32_t c[W], s;
 };
-template <int W>
-__device__ __forceinline__ void md_load(MdPiece<W>& p, const uint32_t* codes, const uint8_t* scales, int64_t row,
+// codes and scales: the first row of a step, alike in all lanes; row: this lane's
+// from there.  STREAM: codes that no other workgroup reads are loaded
+// non-temporally (64 x 32 heads x 8192 keys 398 -> 360 us); those that a second
+// tile of query rows reads too are better kept (2 x 8 x 16383 keys, 20 tokens: 20.9
+// against 22.9).
+template <bool STREAM, int W>
+__device__ __forceinline__ void md_load(MdPiece<W>& p, const uint8_t* codes, const uint8_t* scales, uint32_t row,
                                         int g) {
-  __builtin_memcpy(p.c, codes + row * (4 * W) + g * W, 4 * W);
-  p.s = scales[W == 4 ? row * 4 + g : (W == 2 ? row * 2 + (g >> 1) : row)];
+  typedef uint32_t vec __attribute__((ext_vector_type(W)));
+  const vec* from = reinterpret_cast<const vec*>(codes + (row * (16u * W) + (uint32_t)g * (4u * W)));
+  const vec x = STREAM ? __builtin_nontemporal_load(from) : *from;
+  __builtin_memcpy(p.c, &x, 4 * W);
+  p.s = scales[W == 4 ? row * 4u + (uint32_t)g : (W == 2 ? row * 2u + (uint32_t)(g >> 1) : row)];
 }
 __device__ __forceinline__ bf16x8 md_bf16(uint32_t codes, float scale) {
   MxEight<u16> v;
@@ -69,23 +77,46 @@ __device__ __forceinline__ bf16x8 md_bf16(uint32_t codes, float scale) {
   return __builtin_bit_cast(bf16x8, v.w);
 }
 
-// x as a sum of N bf16 terms, each what the earlier ones leave, rounded, or
-// (CUT) cut off: three cut terms hold any fp32 value exactly.
-template <int N, bool CUT>
+// The wave's V tile: [32 keys][D] bf16 in 16-byte chunks, chunk c of row r at
+// chunk c ^ exchange(r), where a row's chunks number D / 8 and 256 / 2 D rows make
+// a line of all banks.  A row write puts one chunk of 16 consecutive rows, a
+// transposed read takes two neighbouring chunks of eight; both spread over the
+// banks.  The chunk enters an address by exclusive or alone, so that one register
+// serves all of them.
+template <int D>
+__device__ __forceinline__ constexpr int md_exchange(int r) {
+  return (r & 15) >> (D == 128 ? 0 : (D == 64 ? 1 : 2));
+}
+
+// x as a sum of N bf16 terms: each what the earlier ones leave, cut off, the last
+// one rounded.  Three hold any fp32 value exactly; of two, the rest is below 2^-17
+// of the value.
+template <int N>
 __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
   float left[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) left[e] = x[e];
 #pragma unroll
-  for (int n = 0; n < N; ++n)
+  for (int n = 0; n < N; ++n) {
+    uint32_t w[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const __bf16 b = CUT ? __builtin_bit_cast(__bf16, (u16)(__float_as_uint(left[e]) >> 16)) : (__bf16)left[e];
-      t[n][e] = b;
-      left[e] -= (float)b;
+    for (int i = 0; i < 4; ++i) {
+      if (n + 1 < N) {
+        const uint32_t lo = __float_as_uint(left[2 * i]), hi = __float_as_uint(left[2 * i + 1]);
+        w[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // the upper halves
+        left[2 * i] -= __uint_as_float(lo & 0xffff0000u);
+        left[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
+      } else {
+        w[i] = pack_bf16x2(left[2 * i], left[2 * i + 1]);
+      }
     }
+    t[n] = __builtin_bit_cast(bf16x8, w);
+  }
 }
 
+__device__ __forceinline__ void lds_st(uint32_t a, const bf16x8& x) {
+  *(__attribute__((address_space(3))) bf16x8*)(uintptr_t)a = x;
+}
 __device__ __forceinline__ void md_load8(const u16* p, float (&f)[8]) {
   u16 x[8];
   __builtin_memcpy(x, p, 16);
@@ -105,49 +136,51 @@ __device__ __forceinline__ float md_lse(float m, float den) {
   return den == 0.f ? -INFINITY : (m + __log2f(den)) * kLn2;
 }
 
+// The maximum is that of the products, the scale sl2 (of log2 e too, above zero:
+// its sign goes into q, and zero is 1e-37, which still hides what is masked)
+// enters the exponent, 2^(sl2 s - sl2 m), one operation a score.
 // Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv,
 // tile = 16 of the head's R query rows.  Each sequence's own length is cut into
 // nsplit spans, so that sequences of any length keep every workgroup busy.
-template <typename T, int D>
-__global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
-    const T* __restrict__ q, const uint32_t* __restrict__ kc, const uint8_t* __restrict__ ks,
-    const uint32_t* __restrict__ vc, const uint8_t* __restrict__ vs, const int* __restrict__ lengths,
-    float* __restrict__ part_o, float2* __restrict__ part_ml, T* __restrict__ o, float* __restrict__ lse, int Hkv,
-    int64_t R, int tokens, int64_t tiles, int cap, int nsplit, float sl2) {
+template <typename T, int D, bool STREAM>
+__global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
+    const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ ks,
+    const uint8_t* __restrict__ vc, const uint8_t* __restrict__ vs, const int* __restrict__ lengths,
+    float* __restrict__ part_o, float2* __restrict__ part_ml, T* __restrict__ o, float* __restrict__ lse,
+    uint32_t Hkv, uint32_t R, uint32_t tokens, uint32_t tiles, int cap, uint32_t nsplit, float sl2, bool negative) {
   constexpr int W = D / 32;                                  // dwords of a lane's piece, and k steps of a key tile
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;  // terms of q and of the weights
   constexpr int ND = D / 16;                                 // 16-row tiles of O^T
-  using Tile = SwzTile<D>;
-  __shared__ __align__(16) u16 s_v[kMdWaves][Tile::kElems(kMdKeys)];
+  __shared__ __align__(256) u16 s_v[kMdWaves][kMdKeys * D];
   __shared__ float s_m[kMdWaves][kMdRows], s_l[kMdWaves][kMdRows];
   static_assert(sizeof(s_v[0]) == kMdRows * D * sizeof(float), "the waves' sums reuse their tiles");
 
   const int l = threadIdx.x & 63, r = l & 15, g = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int split = blockIdx.x % nsplit;
-  const int64_t unit = blockIdx.x / nsplit, head = unit / tiles, row0 = (unit - head * tiles) * kMdRows;
-  const int64_t qrow = head * R + row0;  // the tile's first row of q and o
-  const int nrows = (int)min((int64_t)kMdRows, R - row0);
+  const uint32_t unit = blockIdx.x / nsplit, split = blockIdx.x - unit * nsplit;
+  const uint32_t head = unit / tiles, row0 = (unit - head * tiles) * kMdRows;
+  const int64_t qrow = (int64_t)head * R + row0;  // the tile's first row of q and o
+  const int nrows = (int)min((uint32_t)kMdRows, R - row0);
+
+  float qx[W][8];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) qx[j][e] = 0.f;
+    if (r < nrows) md_load8(q + (qrow + r) * D + g * (8 * W) + 8 * j, qx[j]);
+  }
 
   // Keys that the newest token sees, and that this lane's row sees.
   const int full = lengths[head / Hkv];
-  const int len = min(full, cap);
-  const int t = r < nrows ? (int)((row0 + r) % tokens) : 0;
-  const int seen = r < nrows ? (int)min((int64_t)len, (int64_t)full - (tokens - 1 - t)) : 0;
-  const int all_see = (int)min((int64_t)len, (int64_t)full - (tokens - 1));  // keys that every row sees
+  const int len = min(full, cap), before = (int)tokens - 1;
+  const int t = r < nrows ? (int)((row0 + (uint32_t)r) % tokens) : 0;
+  const int seen = r < nrows ? (int)min((int64_t)len, (int64_t)full - (before - t)) : 0;
+  const int all_see = (int)min((int64_t)len, (int64_t)full - before);  // keys that every row sees
   int kbeg = 0, kend = 0;
   if (len > 0) {
-    const int span = ((len + nsplit - 1) / nsplit + kMdKeys - 1) / kMdKeys * kMdKeys;
-    kbeg = (int)min((int64_t)split * span, (int64_t)len);
-    kend = min(kbeg + span, len);
-  }
-
-  bf16x8 qf[W][NQ];
-#pragma unroll
-  for (int j = 0; j < W; ++j) {
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (r < nrows) md_load8(q + (qrow + r) * D + g * (8 * W) + 8 * j, x);
-    md_terms<NQ, true>(x, qf[j]);
+    const uint32_t span = (((uint32_t)len + nsplit - 1) / nsplit + kMdKeys - 1) / kMdKeys * kMdKeys;
+    kbeg = (int)min((uint64_t)split * span, (uint64_t)len);
+    kend = (int)min((uint32_t)kbeg + span, (uint32_t)len);
   }
 
   f32x4 acc[ND];
@@ -155,23 +188,40 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
   for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
   float m = -INFINITY, lsum = 0.f;
   u16* tile = s_v[w];
-  const int64_t base = head * cap;
+  constexpr uint32_t kRow = 2 * D;  // bytes of a tile row
+  // chunk g W of row r, and columns 4 (r % 4) of row 4 g + r / 4
+  const uint32_t put = lds_addr(tile) + (uint32_t)r * kRow + 16u * (uint32_t)((g * W) ^ md_exchange<D>(r));
+  const int krow = 4 * g + (r >> 2);
+  const uint32_t get = lds_addr(tile) + (uint32_t)krow * kRow + 16u * (uint32_t)(((r & 3) >> 1) ^ md_exchange<D>(krow)) +
+                       8u * (uint32_t)(r & 1);
+  const int64_t base = (int64_t)head * cap;
 
-  MdPiece<W> k[2], v[2];
+  MdPiece<W> k[2], v[2];  // the next step's keys, as loaded
   auto fetch = [&](int j0) {
+    const int64_t at = base + j0;  // the same for the wave: the address of a piece is this and a lane's offset
+    const uint8_t *kp = kc + at * (16 * W), *vp = vc + at * (16 * W), *ksp = ks + at * W, *vsp = vs + at * W;
+    const bool whole = j0 + kMdKeys <= len;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int64_t row = base + min(j0 + 16 * u + r, len - 1);  // keys past the end: the last one, masked below
-      md_load(k[u], kc, ks, row, g);
-      md_load(v[u], vc, vs, row, g);
+      uint32_t row = 16u * u + (uint32_t)r;
+      if (!whole) row = (uint32_t)min((int)row, len - 1 - j0);  // keys past the end: the last one, masked below
+      md_load<STREAM>(k[u], kp, ksp, row, g);
+      md_load<STREAM>(v[u], vp, vsp, row, g);
     }
   };
   int j0 = kbeg + w * kMdKeys;
   if (j0 < kend) fetch(j0);
+  bf16x8 qf[W][NQ];
+#pragma unroll
+  for (int j = 0; j < W; ++j) {
+    if (negative)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qx[j][e] = -qx[j][e];
+    md_terms<NQ>(qx[j], qf[j]);
+  }
   for (; j0 < kend; j0 += kMdWaves * kMdKeys) {
     MdPiece<W> kx[2] = {k[0], k[1]}, vx[2] = {v[0], v[1]};
-    const int next = j0 + kMdWaves * kMdKeys;
-    if (next < kend) fetch(next);
+    if (j0 + kMdWaves * kMdKeys < kend) fetch(j0 + kMdWaves * kMdKeys);
 
     f32x4 s[2];
 #pragma unroll
@@ -185,8 +235,6 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
         for (int n = NQ - 1; n >= 0; --n) s[u] = mfma_bf16_16x16x32(a, qf[j][n], s[u]);
       }
     }
-#pragma unroll
-    for (int u = 0; u < 2; ++u) s[u] *= sl2;
     uint64_t odd[2] = {0, 0};  // lanes whose V block reads as NaN, in a step that some row does not see whole
     const bool edge = j0 + kMdKeys > min(kend, all_see);
     if (edge) {
@@ -216,9 +264,9 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
       for (int i = 0; i < 4; ++i) top = vmax(top, s[u][i]);
     top = max_rows(top);
     const float mn = vmax(m, top);
-    const float mb = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: every weight 0
+    const float mb = mn == -INFINITY ? 0.f : sl2 * mn;  // nothing seen yet: every weight 0
     if (wave_any(mn != m)) {
-      const float a = fast_exp2(m - mb);
+      const float a = fast_exp2(__builtin_fmaf(sl2, m, -mb));
       lsum *= a;
 #pragma unroll
       for (int i = 0; i < ND; ++i) acc[i] *= a;
@@ -227,11 +275,11 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
     float p[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      p[e] = fast_exp2(s[e >> 2][e & 3] - mb);
+      p[e] = fast_exp2(__builtin_fmaf(sl2, s[e >> 2][e & 3], -mb));
       lsum += p[e];
     }
     bf16x8 pf[NP];
-    md_terms<NP, false>(p, pf);
+    md_terms<NP>(p, pf);
 
     // V rows to the wave's tile, 8 values a 16-byte chunk
 #pragma unroll
@@ -239,15 +287,15 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
       const float f = mx_scale(vx[u].s);
 #pragma unroll
       for (int j = 0; j < W; ++j)
-        *reinterpret_cast<bf16x8*>(&tile[Tile::chunk(16 * u + r, g * W + j)]) = md_bf16(vx[u].c[j], f);
+        lds_st((put ^ (16u * j)) + u * 16 * kRow, md_bf16(vx[u].c[j], f));
     }
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 #pragma unroll
     for (int i = 0; i < ND; ++i) {
-      const int col = 16 * i + 4 * (r & 3), krow = 4 * g + (r >> 2);
-      const bf16x8 a = lds_read_tr16x2(&tile[Tile::at4(krow, col)], &tile[Tile::at4(krow + 16, col)]);
+      const uint32_t at = get ^ (32u * i);
+      const bf16x8 a = lds_tr16x2_at(at, at + 16 * kRow);
 #pragma unroll
       for (int n = NP - 1; n >= 0; --n) acc[i] = mfma_bf16_16x16x32(a, pf[n], acc[i]);
     }
@@ -274,7 +322,7 @@ __global__ __launch_bounds__(kMdThreads) void attn_decode_mxfp4_kernel(
   for (int i = 0; i < ND; ++i)
     *reinterpret_cast<f32x4*>(&mine[r * D + 4 * ((4 * i + g) ^ (r & (D / 4 - 1)))]) = acc[i];
   if (g == 0) {
-    s_m[w][r] = m;
+    s_m[w][r] = m == -INFINITY ? m : sl2 * m;
     s_l[w][r] = lsum;
   }
   __syncthreads();
@@ -348,18 +396,51 @@ __global__ __launch_bounds__(256) void attn_decode_mxfp4_merge_kernel(const floa
 }
 
 constexpr size_t kMdWork = size_t(24) << 20;  // the partials' scratch, of one size so that graphs may keep its address
-constexpr int64_t kMdFill = 1024;             // workgroups that fill the chip
+
+// Into how many splits to cut the keys.  A workgroup costs its keys and about
+// kMdFixed more (its queries, the meeting of its waves), a CU's time goes by the
+// workgroups that fall to it, up to per_cu of them at once, of which fewer keep
+// less of memory's latency covered, and splits cost the second launch, about
+// kMdMerge keys.  Measured (d = 128 bf16, 256 CUs, three at once, us): 16 x 8 heads x
+// 16383 keys in 3 / 4 / 5 / 6 splits (1.5, 2, 2.5, 3 a CU) 62 / 55 / 60 / 54, 20 x 8
+// heads in 3 / 4 / 5 68 / 74 / 82, 64 x 32 heads x 8192 keys in 1 / 3 350 / 366.
+constexpr int64_t kMdFixed = 150, kMdMerge = 300;
+inline int64_t md_splits(int64_t units, int64_t keys, int64_t per_cu, int64_t cus, int64_t d, int64_t most) {
+  constexpr int64_t step = kMdWaves * kMdKeys;
+  most = std::min(most, (keys + step - 1) / step);
+  most = std::min(most, std::max<int64_t>(4, 2 * per_cu * cus / units));
+  int64_t best = 1;
+  double least = std::numeric_limits<double>::max();
+  for (int64_t n = 1; n <= most; ++n) {
+    const int64_t here = (units * n + cus - 1) / cus;
+    const int64_t last = here % per_cu, each = ((keys + n - 1) / n + step - 1) / step * step + kMdFixed;
+    auto group = [&](int64_t w) { return w > 0 ? (double)w + 76.8 / (double)d : 0.0; };  // w at once
+    const double cost = (double)each * ((double)(here / per_cu) * group(per_cu) + group(last)) +
+                        (n > 1 ? (double)(kMdMerge + 4 * n) : 0.0);
+    if (cost < least) {
+      least = cost;
+      best = n;
+    }
+  }
+  return best;
+}
 
 template <typename T, int D>
 int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
            const int* lengths, T* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t tokens, int64_t cap,
            float scale, hipStream_t st) {
-  const int64_t R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
   const int64_t rows = B * H * tokens;
-  // Splits: enough workgroups to fill the chip, each with 256 keys or more.
-  int64_t nsplit = (kMdFill + units - 1) / units;
-  nsplit = std::min(nsplit, (cap + 255) / 256);
-  nsplit = std::min(nsplit, (int64_t)(kMdWork / ((size_t)rows * (D + 2) * sizeof(float))));
+  if (rows > 0x7fffffff) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+  const int64_t R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
+  static const int per_cu = [] {
+    int n = 0;
+    const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
+        &n, (const void*)attn_decode_mxfp4_kernel<T, D, true>, kMdThreads, 0);
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e == hipSuccess && n > 0 ? n : 3;
+  }();
+  int64_t nsplit = md_splits(units, std::max<int64_t>(cap, 1), per_cu, device_cu_count(), D,
+                             (int64_t)(kMdWork / ((size_t)rows * (D + 2) * sizeof(float))));
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
   if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsMxfp4Decode, kMdWork, &ws)) nsplit = 1;
@@ -367,9 +448,16 @@ int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, con
     return fail(TT_ERR_ARG, std::string(fn) + ": grid too large");
   float* part_o = (float*)ws;
   float2* part_ml = (float2*)(part_o + rows * nsplit * D);
-  hipLaunchKernelGGL((attn_decode_mxfp4_kernel<T, D>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, st, q,
-                     (const uint32_t*)kc, ks, (const uint32_t*)vc, vs, lengths, part_o, part_ml, o, lse, (int)Hkv, R,
-                     (int)tokens, tiles, (int)cap, (int)nsplit, scale * kLog2e);
+  const float sl2 = std::max(std::fabs(scale * kLog2e), 1e-37f);
+#define TT_MD_LAUNCH(STREAM)                                                                                          \
+  hipLaunchKernelGGL((attn_decode_mxfp4_kernel<T, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, \
+                     st, q, kc, ks, vc, vs, lengths, part_o, part_ml, o, lse, (uint32_t)Hkv, (uint32_t)R,             \
+                     (uint32_t)tokens, (uint32_t)tiles, (int)cap, (uint32_t)nsplit, sl2, scale < 0.f)
+  if (tiles == 1)
+    TT_MD_LAUNCH(true);
+  else
+    TT_MD_LAUNCH(false);
+#undef TT_MD_LAUNCH
   TT_LAUNCHED(fn, st);
   if (nsplit > 1) {
     hipLaunchKernelGGL((attn_decode_mxfp4_merge_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, part_o, part_ml,
