@@ -54,11 +54,30 @@ typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 
+// 16 bytes at any element alignment, non-temporally or not.
+typedef uint32_t mx_word __attribute__((ext_vector_type(4), aligned(2)));
+template <bool NT, typename T>
+__device__ __forceinline__ void mx_load16(void* to, const T* p) {
+  const mx_word* q = reinterpret_cast<const mx_word*>(p);
+  const mx_word x = NT ? __builtin_nontemporal_load(q) : *q;
+  __builtin_memcpy(to, &x, 16);
+}
+template <bool NT, typename T>
+__device__ __forceinline__ void mx_store16(T* p, const void* from) {
+  mx_word x;
+  __builtin_memcpy(&x, from, 16);
+  if constexpr (NT)
+    __builtin_nontemporal_store(x, reinterpret_cast<mx_word*>(p));
+  else
+    *reinterpret_cast<mx_word*>(p) = x;
+}
+
 // Eight consecutive values in registers.
 template <typename T> struct MxEight;
 template <> struct MxEight<u16> {
   uint32_t w[4];
-  __device__ __forceinline__ void load(const u16* p) { __builtin_memcpy(w, p, 16); }
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const u16* p) { mx_load16<NT>(w, p); }
   __device__ __forceinline__ void load_part(const u16* p, int n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -88,7 +107,8 @@ template <> struct MxEight<u16> {
     w[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 2));
     w[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, scale, 3));
   }
-  __device__ __forceinline__ void store(u16* p) const { __builtin_memcpy(p, w, 16); }
+  template <bool NT = false>
+  __device__ __forceinline__ void store(u16* p) const { mx_store16<NT>(p, w); }
   __device__ __forceinline__ void store_part(u16* p, int n) const {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -97,7 +117,11 @@ template <> struct MxEight<u16> {
 };
 template <> struct MxEight<float> {
   float v[8];
-  __device__ __forceinline__ void load(const float* p) { __builtin_memcpy(v, p, 32); }
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const float* p) {
+    mx_load16<NT>(v, p);
+    mx_load16<NT>(v + 4, p + 4);
+  }
   __device__ __forceinline__ void load_part(const float* p, int n) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : 0.f;
@@ -116,17 +140,46 @@ template <> struct MxEight<float> {
     c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[6], v[7], scale, 3);
     return c;
   }
+};
+
+// 16 bytes of values, as a lane of a kernel over whole rows holds them: eight
+// bf16, or four fp32 (with 32 bytes a lane every access would leave out half of
+// each line, which non-temporal stores pay for: 8192 x 4000 read back in 50 us).
+template <typename T> struct MxWord;
+template <> struct MxWord<u16> : MxEight<u16> {
+  typedef uint32_t Codes;
+  static constexpr int N = 8;
+};
+template <> struct MxWord<float> {
+  typedef uint16_t Codes;
+  static constexpr int N = 4;
+  float v[4];
+  template <bool NT = false>
+  __device__ __forceinline__ void load(const float* p) { mx_load16<NT>(v, p); }
+  __device__ __forceinline__ void load_part(const float* p, int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ uint32_t top() const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m >> 23;
+  }
+  __device__ __forceinline__ uint32_t codes(float scale) const {
+    const uint32_t c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, v[0], v[1], scale, 0);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, v[2], v[3], scale, 1);
+  }
   __device__ __forceinline__ void from(uint32_t c, float scale) {
     const f32x2 a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 0);
     const f32x2 b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 1);
-    const f32x2 d = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 2);
-    const f32x2 e = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, scale, 3);
-    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = d.x, v[5] = d.y, v[6] = e.x, v[7] = e.y;
+    v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y;
   }
-  __device__ __forceinline__ void store(float* p) const { __builtin_memcpy(p, v, 32); }
+  template <bool NT = false>
+  __device__ __forceinline__ void store(float* p) const { mx_store16<NT>(p, v); }
   __device__ __forceinline__ void store_part(float* p, int n) const {
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+    for (int i = 0; i < 4; ++i)
       if (i < n) p[i] = v[i];
   }
 };
@@ -137,13 +190,16 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t x) {
   return max(x, (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xf, 0xf, true));  // lanes 2 3 0 1
 }
 
-// The block that a quad holds eight values a lane of: its scale byte, and this
-// lane's four bytes of codes.
+// The block that neighbouring lanes hold a word each of (four or eight of them,
+// all active): its scale byte, and the codes of this lane's word.
 template <typename T>
-__device__ __forceinline__ uint32_t mx_quantize_quad(const MxEight<T>& x, uint32_t* scale_byte) {
-  const uint32_t s = mx_scale_byte(quad_max(x.top()));
+__device__ __forceinline__ typename MxWord<T>::Codes mx_quantize_word(const MxWord<T>& x, uint32_t* scale_byte) {
+  uint32_t e = quad_max(x.top());
+  if constexpr (MxWord<T>::N == 4)  // the other quad of the eight lanes, by their mirror image
+    e = max(e, (uint32_t)__builtin_amdgcn_mov_dpp((int)e, 0x141, 0xf, 0xf, true));
+  const uint32_t s = mx_scale_byte(e);
   *scale_byte = s;
-  return s == 255u ? 0u : x.codes(mx_scale(s));
+  return (typename MxWord<T>::Codes)(s == 255u ? 0u : x.codes(mx_scale(s)));
 }
 
 }  // namespace tt

@@ -3,9 +3,9 @@
 //
 // Each is one pass over the data with next to no arithmetic, so the bytes
 // bound it: 2 (bf16) or 4 (fp32) read or written a value, 17/32 for the codes
-// and scales.  A lane holds eight consecutive values (16 or 32 bytes) and four
-// bytes of their codes, a quad of lanes a block, whose largest exponent takes
-// two quad permutes: every access of a wave is one contiguous run.
+// and scales.  A lane holds 16 bytes of values and their codes, four or eight
+// neighbouring lanes a block, whose largest exponent takes two or three lane
+// permutes: every access of a wave is one contiguous run.
 #include <hip/hip_runtime.h>
 
 #include <string>
@@ -18,7 +18,12 @@ namespace tt {
 namespace {
 
 constexpr int kMxThreads = 256;
-constexpr int kMxUnroll = 4;  // eights a thread, loaded before the first is used
+constexpr int kMxUnroll = 2;  // words a thread, loaded before the first is used
+// Values that fill more than this go by non-temporally: 8192 x 8192 bf16 quantised
+// in 28.1 us instead of 33.8 (6.0 TB/s), read back in 24.3 instead of 33.2 (7.0
+// TB/s).  Smaller ones the next kernel may still find in a cache; 33 MB take 8.3 us
+// either way.
+constexpr int64_t kMxNtBytes = int64_t(64) << 20;
 
 // u / n and u % n, in 32 bits where u fits them.
 __device__ __forceinline__ void mx_divmod(uint64_t u, uint32_t n, uint64_t* q, uint32_t* r) {
@@ -33,55 +38,56 @@ __device__ __forceinline__ void mx_divmod(uint64_t u, uint32_t n, uint64_t* q, u
 
 // Quantises (QUANT) x into codes and scales, or reads them back into x.
 // FLAT: cols is a multiple of 32, so rows follow one another without padding
-// and an eight's number is its place; otherwise rows have nb blocks of their
-// own and end inside the last one.
-template <typename T, bool QUANT, bool FLAT>
-__global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, uint32_t* codes, uint8_t* scales, uint64_t eights,
-                                                           int64_t cols, uint32_t nb) {
+// and a word's number is its place; otherwise rows have nb blocks of their own
+// and end inside the last one.
+template <typename T, bool QUANT, bool FLAT, bool NT>
+__global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, typename MxWord<T>::Codes* codes, uint8_t* scales,
+                                                           uint64_t words, int64_t cols, uint32_t nb) {
+  constexpr int N = MxWord<T>::N, WPB = kMxBlock / N;  // values of a word, words of a block
   const uint64_t step = (uint64_t)gridDim.x * (kMxThreads * kMxUnroll);
-  for (uint64_t base = (uint64_t)blockIdx.x * (kMxThreads * kMxUnroll); base < eights; base += step) {
-    MxEight<T> v[kMxUnroll];
+  for (uint64_t base = (uint64_t)blockIdx.x * (kMxThreads * kMxUnroll); base < words; base += step) {
+    MxWord<T> v[kMxUnroll];
     T* at[kMxUnroll];
-    int n[kMxUnroll];  // values of this eight inside its row
+    int n[kMxUnroll];  // values of this word inside its row
     uint32_t c[kMxUnroll], s[kMxUnroll];
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
       const uint64_t u = base + i * kMxThreads + threadIdx.x;
       n[i] = 0;
-      if (u >= eights) continue;  // whole quads: eights is a multiple of 4
+      if (u >= words) continue;  // whole blocks: words is a multiple of WPB
       if constexpr (FLAT) {
-        at[i] = x + 8 * u;
-        n[i] = 8;
+        at[i] = x + N * u;
+        n[i] = N;
       } else {
         uint64_t row;
         uint32_t blk;
-        mx_divmod(u >> 2, nb, &row, &blk);
-        const int64_t c0 = (int64_t)blk * kMxBlock + 8 * (u & 3);
+        mx_divmod(u / WPB, nb, &row, &blk);
+        const int64_t c0 = (int64_t)blk * kMxBlock + N * (int64_t)(u % WPB);
         at[i] = x + (int64_t)row * cols + c0;
-        n[i] = (int)max((int64_t)0, min((int64_t)8, cols - c0));
+        n[i] = (int)max((int64_t)0, min((int64_t)N, cols - c0));
       }
       if constexpr (QUANT) {
-        if (FLAT || n[i] == 8)
-          v[i].load(at[i]);
+        if (FLAT || n[i] == N)
+          v[i].template load<NT>(at[i]);
         else
           v[i].load_part(at[i], n[i]);
       } else {
         c[i] = codes[u];
-        s[i] = scales[u >> 2];
+        s[i] = scales[u / WPB];
       }
     }
 #pragma unroll
     for (int i = 0; i < kMxUnroll; ++i) {
       const uint64_t u = base + i * kMxThreads + threadIdx.x;
-      if (u >= eights) continue;
+      if (u >= words) continue;
       if constexpr (QUANT) {
         uint32_t sb;
-        codes[u] = mx_quantize_quad(v[i], &sb);
-        if ((u & 3) == 0) scales[u >> 2] = (uint8_t)sb;
+        codes[u] = mx_quantize_word<T>(v[i], &sb);
+        if (u % WPB == 0) scales[u / WPB] = (uint8_t)sb;
       } else {
         v[i].from(c[i], mx_scale(s[i]));
-        if (FLAT || n[i] == 8)
-          v[i].store(at[i]);
+        if (FLAT || n[i] == N)
+          v[i].template store<NT>(at[i]);
         else
           v[i].store_part(at[i], n[i]);
       }
@@ -125,28 +131,27 @@ __global__ __launch_bounds__(kMxThreads) void k_mxfp4_columns(const T* __restric
 // cap, D]: token t of sequence b goes to row lengths[b] - T + t where that
 // lies in [0, cap), and nowhere otherwise.
 template <typename T, int D>
-__global__ __launch_bounds__(kMxThreads) void k_mxfp4_append(const T* __restrict__ k, const T* __restrict__ v,
-                                                             uint32_t* __restrict__ kc, uint8_t* __restrict__ ks,
-                                                             uint32_t* __restrict__ vc, uint8_t* __restrict__ vs,
-                                                             const int* __restrict__ lengths, uint64_t eights,
-                                                             uint32_t Hkv, uint32_t tokens, int64_t cap) {
-  constexpr int E = D / 8;  // eights a row
+__global__ __launch_bounds__(kMxThreads) void k_mxfp4_append(
+    const T* __restrict__ k, const T* __restrict__ v, typename MxWord<T>::Codes* __restrict__ kc,
+    uint8_t* __restrict__ ks, typename MxWord<T>::Codes* __restrict__ vc, uint8_t* __restrict__ vs,
+    const int* __restrict__ lengths, uint64_t words, uint32_t Hkv, uint32_t tokens, int64_t cap) {
+  constexpr int N = MxWord<T>::N, WPB = kMxBlock / N, W = D / N;  // words of a block and of a row
   const T* x = blockIdx.y ? v : k;
-  uint32_t* codes = blockIdx.y ? vc : kc;
+  typename MxWord<T>::Codes* codes = blockIdx.y ? vc : kc;
   uint8_t* scales = blockIdx.y ? vs : ks;
   const uint64_t step = (uint64_t)gridDim.x * kMxThreads;
-  for (uint64_t u = (uint64_t)blockIdx.x * kMxThreads + threadIdx.x; u < eights; u += step) {
+  for (uint64_t u = (uint64_t)blockIdx.x * kMxThreads + threadIdx.x; u < words; u += step) {
     uint64_t head;  // b Hkv + h
     uint32_t t;
-    mx_divmod(u / E, tokens, &head, &t);
-    const int64_t pos = (int64_t)lengths[head / Hkv] - tokens + t;
-    if (pos < 0 || pos >= cap) continue;  // the same for the whole row, so for whole quads
-    MxEight<T> w;
-    w.load(x + 8 * u);
+    mx_divmod(u / W, tokens, &head, &t);
+    const int64_t pos = (int64_t)lengths[(uint32_t)head / Hkv] - tokens + t;
+    if (pos < 0 || pos >= cap) continue;  // the same for the whole row, so for whole blocks
+    MxWord<T> w;
+    w.load(x + N * u);
     uint32_t s;
-    const uint64_t to = ((int64_t)head * cap + pos) * E + u % E;
-    codes[to] = mx_quantize_quad(w, &s);
-    if ((u & 3) == 0) scales[to >> 2] = (uint8_t)s;
+    const uint64_t to = ((int64_t)head * cap + pos) * W + u % W;
+    codes[to] = mx_quantize_word<T>(w, &s);
+    if (u % WPB == 0) scales[to / WPB] = (uint8_t)s;
   }
 }
 
@@ -155,16 +160,26 @@ constexpr int64_t kMxMaxGrid = int64_t(1) << 20;
 template <typename T, bool QUANT>
 int rows_launch(const char* fn, T* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols, hipStream_t s) {
   const int64_t nb = mx_blocks(cols);
-  const uint64_t eights = (uint64_t)(rows * nb) * 4;
+  using Codes = typename MxWord<T>::Codes;
+  const uint64_t words = (uint64_t)(rows * nb) * (kMxBlock / MxWord<T>::N);
   const uint64_t per = kMxThreads * kMxUnroll;
-  const uint64_t want = (eights + per - 1) / per;
+  const uint64_t want = (words + per - 1) / per;
   const dim3 grid((unsigned)(want < (uint64_t)kMxMaxGrid ? want : (uint64_t)kMxMaxGrid)), block(kMxThreads);
-  if (cols % kMxBlock == 0)
-    hipLaunchKernelGGL((k_mxfp4_rows<T, QUANT, true>), grid, block, 0, s, x, (uint32_t*)codes, scales, eights, cols,
-                       (uint32_t)nb);
-  else
-    hipLaunchKernelGGL((k_mxfp4_rows<T, QUANT, false>), grid, block, 0, s, x, (uint32_t*)codes, scales, eights, cols,
-                       (uint32_t)nb);
+#define TT_MX_ROWS(FLAT, NT)                                                                                      \
+  hipLaunchKernelGGL((k_mxfp4_rows<T, QUANT, FLAT, NT>), grid, block, 0, s, x, (Codes*)codes, scales, words, cols, \
+                     (uint32_t)nb)
+  const bool nt = rows * cols * (int64_t)sizeof(T) > kMxNtBytes;
+  if (cols % kMxBlock == 0) {
+    if (nt)
+      TT_MX_ROWS(true, true);
+    else
+      TT_MX_ROWS(true, false);
+  } else if (nt) {
+    TT_MX_ROWS(false, true);
+  } else {
+    TT_MX_ROWS(false, false);
+  }
+#undef TT_MX_ROWS
   TT_LAUNCHED(fn, s);
   return ok();
 }
@@ -183,12 +198,13 @@ int columns_launch(const char* fn, const T* x, uint8_t* codes, uint8_t* scales, 
 template <typename T>
 int append_launch(const char* fn, const T* k, const T* v, uint8_t* kc, uint8_t* ks, uint8_t* vc, uint8_t* vs,
                   const int* lengths, int64_t B, int64_t Hkv, int64_t tokens, int64_t cap, int64_t d, hipStream_t s) {
-  const uint64_t eights = (uint64_t)(B * Hkv * tokens) * (d / 8);
-  const uint64_t want = (eights + kMxThreads - 1) / kMxThreads;
+  using Codes = typename MxWord<T>::Codes;
+  const uint64_t words = (uint64_t)(B * Hkv * tokens) * (d / MxWord<T>::N);
+  const uint64_t want = (words + kMxThreads - 1) / kMxThreads;
   const dim3 grid((unsigned)(want < (uint64_t)kMxMaxGrid ? want : (uint64_t)kMxMaxGrid), 2), block(kMxThreads);
 #define TT_MX_APPEND(D)                                                                                         \
-  hipLaunchKernelGGL((k_mxfp4_append<T, D>), grid, block, 0, s, k, v, (uint32_t*)kc, ks, (uint32_t*)vc, vs, lengths, \
-                     eights, (uint32_t)Hkv, (uint32_t)tokens, cap)
+  hipLaunchKernelGGL((k_mxfp4_append<T, D>), grid, block, 0, s, k, v, (Codes*)kc, ks, (Codes*)vc, vs, lengths, words, \
+                     (uint32_t)Hkv, (uint32_t)tokens, cap)
   switch (d) {
     case 32: TT_MX_APPEND(32); break;
     case 64: TT_MX_APPEND(64); break;
