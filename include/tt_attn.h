@@ -366,7 +366,7 @@ int tt_gemm_mxfp4(int dtype, int64_t m, int64_t n, int64_t k, float alpha, const
  * per-stream library workspace (allocated on first use) and multiplied from
  * there; without it (refused, or under graph capture before a call has left it
  * on the stream) the product quantises them as it reads them, which is slower
- * and gives the same result. */
+ * and gives the same result up to the order of its sums. */
 int tt_fc_forward_mxfp4(int dtype, int64_t batch, int64_t fin, int64_t fout, const void* in, const uint8_t* w_codes,
                         const uint8_t* w_scales, const void* bias, int bias_scalar, void* out, void* stream);
 
@@ -386,12 +386,12 @@ int tt_kv_append_mxfp4(int dtype, const void* k, const void* v, uint8_t* k_codes
  * multiple of Hkv (query head h reads K/V head h / (H / Hkv)), lse [B][H][T]
  * (float, natural log, may be NULL).  Token t sees key j where j < lengths[b] -
  * (T - 1 - t) and j < cap; one that sees none gets o = 0 and lse = -inf.  Rows
- * of the cache that no token sees are not used, whatever they hold.  K and V
- * enter with their 4-bit values, scores, weights and sums in fp32 precision.
- * Few heads split the keys over workgroups and merge their sums through a
- * fixed 24 MiB per-stream library workspace (allocated on first use); without
- * it (refused, or under graph capture before a call has left it on the stream)
- * they run unsplit. */
+ * of the cache that no token sees are not used, whatever they hold.  B H T is
+ * below 2^31 (TT_ERR_ARG otherwise).  K and V enter with their 4-bit values,
+ * scores, weights and sums in fp32 precision.  Few heads split the keys over
+ * workgroups and merge their sums through a fixed 24 MiB per-stream library
+ * workspace (allocated on first use); without it (refused, or under graph
+ * capture before a call has left it on the stream) they run unsplit. */
 int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_codes, const uint8_t* k_scales,
                          const uint8_t* v_codes, const uint8_t* v_scales, const int* lengths, void* o, float* lse,
                          int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t cap, int64_t d, float scale,

@@ -1,4 +1,4 @@
-// Module `myLayer`: the attention entry points, SoftmaxForward with its cross-entropy, FC, convolution and max pooling, bound in the style of
+// Module `myLayer`: the attention entry points, SoftmaxForward with its cross-entropy, FC, convolution, max pooling and the 4-bit layers, bound in the style of
 // Task3/Tinytensor/src/bind_Layer.cpp:10-24 (free functions over TinyTensor
 // references), with float and bf16 overloads.
 #include <pybind11/pybind11.h>
@@ -27,6 +27,27 @@ PYBIND11_MODULE(myLayer, m) {
         py::arg("out"), py::arg("scale"));
   m.def("AttentionDecode", &AttentionDecode<bf16>, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("out"), py::arg("scale"));
+  // values in 4 bits: weights, and a K/V cache with its append and its attention
+  m.def("QuantizeMxfp4", &QuantizeMxfp4<float>, py::arg("input"), py::arg("codes"), py::arg("scales"),
+        py::arg("transposed") = false);
+  m.def("QuantizeMxfp4", &QuantizeMxfp4<bf16>, py::arg("input"), py::arg("codes"), py::arg("scales"),
+        py::arg("transposed") = false);
+  m.def("DequantizeMxfp4", &DequantizeMxfp4<float>, py::arg("codes"), py::arg("scales"), py::arg("output"),
+        py::arg("columns"));
+  m.def("DequantizeMxfp4", &DequantizeMxfp4<bf16>, py::arg("codes"), py::arg("scales"), py::arg("output"),
+        py::arg("columns"));
+  m.def("FcForwardMxfp4", &FcForwardMxfp4<float>, py::arg("input"), py::arg("output"), py::arg("weight_codes"),
+        py::arg("weight_scales"), py::arg("bias"));
+  m.def("FcForwardMxfp4", &FcForwardMxfp4<bf16>, py::arg("input"), py::arg("output"), py::arg("weight_codes"),
+        py::arg("weight_scales"), py::arg("bias"));
+  m.def("KvAppendMxfp4", &KvAppendMxfp4<float>, py::arg("k"), py::arg("v"), py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"));
+  m.def("KvAppendMxfp4", &KvAppendMxfp4<bf16>, py::arg("k"), py::arg("v"), py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"));
+  m.def("AttentionDecodeMxfp4", &AttentionDecodeMxfp4<float>, py::arg("q"), py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"), py::arg("out"), py::arg("scale"));
+  m.def("AttentionDecodeMxfp4", &AttentionDecodeMxfp4<bf16>, py::arg("q"), py::arg("k_codes"), py::arg("k_scales"),
+        py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"), py::arg("out"), py::arg("scale"));
   // the reference binds SoftmaxForward<float> positionally (bind_Layer.cpp:20)
   m.def("SoftmaxForward", &SoftmaxForward<float>, py::arg("input"), py::arg("output"));
   // positional as in the reference (bind_Layer.cpp:12-13), plus bf16 overloads

@@ -1,11 +1,13 @@
 // Module `myTensor`: classes Tensor_float, Tensor_double, Tensor_int (as in
 // Task3/Tinytensor/src/bind_Tensor.cpp:11-53: four constructors, 21 methods
-// and __repr__) plus Tensor_bf16 and a numpy() method.
+// and __repr__) plus Tensor_bf16, Tensor_byte (whose arithmetic methods raise) and
+// a numpy() method.
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
 #include <pybind11/stl.h>
 
 #include <sstream>
+#include <type_traits>
 
 #include "tinytensor.h"
 
@@ -16,8 +18,10 @@ static void bind(py::module_& m, const std::string& category) {
   using Tensor = TinyTensor<T>;
   using Host = typename Tensor::Host;
   const std::string name = "Tensor_" + category;
-  py::class_<Tensor>(m, name.c_str())
-      .def(py::init<const std::vector<int>&, const std::string&>())
+  py::class_<Tensor> c(m, name.c_str());
+  // A row of byte codes is an array before it is a shape; a list stays a shape.
+  if constexpr (std::is_same<T, uint8_t>::value) c.def(py::init<const py::array_t<Host>&, const std::string&>());
+  c.def(py::init<const std::vector<int>&, const std::string&>())
       .def(py::init<const std::vector<int>&, const std::string&, const std::vector<Host>&>())
       .def(py::init<const py::array_t<Host>&, const std::string&>())
       .def(py::init<const Tensor&>())
@@ -56,6 +60,7 @@ PYBIND11_MODULE(myTensor, m) {
   bind<double>(m, "double");
   bind<int>(m, "int");
   bind<bf16>(m, "bf16");
+  bind<uint8_t>(m, "byte");
   m.def("device_count", []() {
     int n = 0;
     tt_device_count(&n);

@@ -253,6 +253,169 @@ void FcForward(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTens
            fn.c_str());
 }
 
+namespace {
+
+constexpr int kMxBlock = 32, kMxBlockBytes = 16;  // values under one scale byte, bytes of their codes
+
+int mx_blocks(int n) { return n / kMxBlock + (n % kMxBlock != 0); }
+
+// The codes' shape that goes with scales of this one.
+std::vector<int> mx_codes_shape(const std::string& fn, std::vector<int> shape) {
+  if (shape.back() > 0x7fffffff / kMxBlockBytes) throw std::invalid_argument(fn + ": too many blocks a row");
+  shape.back() *= kMxBlockBytes;
+  return shape;
+}
+
+// rows of a tensor whose last axis is a row
+int64_t rows_of(const std::vector<int>& shape) {
+  int64_t rows = 1;
+  for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
+  return rows;
+}
+
+void need_mxfp4(const std::string& fn, const std::string& name, const TinyTensor<uint8_t>& codes,
+                const TinyTensor<uint8_t>& scales) {
+  need_gpu(fn, name + "codes", codes.device);
+  need_gpu(fn, name + "scales", scales.device);
+  if (scales.shape.empty() || codes.shape != mx_codes_shape(fn, scales.shape))
+    throw std::invalid_argument(fn + ": " + name + "codes must have the shape of " + name +
+                                "scales with 16 bytes to each");
+}
+
+// Of a cache in 4 bits: B, Hkv, cap, d.
+Dims mx_cache(const std::string& fn, const TinyTensor<uint8_t>& kc, const TinyTensor<uint8_t>& ks,
+              const TinyTensor<uint8_t>& vc, const TinyTensor<uint8_t>& vs, const TinyTensor<int>& lengths) {
+  need_mxfp4(fn, "k_", kc, ks);
+  need_mxfp4(fn, "v_", vc, vs);
+  need_gpu(fn, "lengths", lengths.device);
+  Dims c = dims4(fn, "k_scales", ks);
+  if (vs.shape != ks.shape) throw std::invalid_argument(fn + ": the K and V caches must have the same shape");
+  if (lengths.shape != std::vector<int>{c.B}) throw std::invalid_argument(fn + ": lengths must have shape [B]");
+  if (c.d > 128 / kMxBlock) throw std::invalid_argument(fn + ": head dim must be 32, 64 or 128");
+  c.d *= kMxBlock;
+  return c;
+}
+
+}  // namespace
+
+template <typename T>
+void QuantizeMxfp4(const TinyTensor<T>& input, TinyTensor<uint8_t>& codes, TinyTensor<uint8_t>& scales,
+                   bool transposed) {
+  const std::string fn = "QuantizeMxfp4";
+  need_gpu(fn, "input", input.device);
+  need_gpu(fn, "codes", codes.device);
+  need_gpu(fn, "scales", scales.device);
+  if (input.shape.empty()) throw std::invalid_argument(fn + ": input must have rank >= 1");
+  if (transposed && input.shape.size() != 2)
+    throw std::invalid_argument(fn + ": input must have rank 2 to be transposed");
+  no_alias(fn, {{input.p_data, "input"}}, {{codes.p_data, "codes"}, {scales.p_data, "scales"}});
+  std::vector<int> shape = input.shape;
+  if (transposed) std::swap(shape[0], shape[1]);
+  const int64_t rows = rows_of(shape), cols = shape.back();
+  shape.back() = mx_blocks(shape.back());
+  codes.resize_output(mx_codes_shape(fn, shape));
+  scales.resize_output(shape);
+  tt_check(tt_mxfp4_quantize(dtype_code<T>(), transposed ? 1 : 0, input.p_data, codes.p_data, scales.p_data, rows,
+                             cols, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void DequantizeMxfp4(const TinyTensor<uint8_t>& codes, const TinyTensor<uint8_t>& scales, TinyTensor<T>& output,
+                     int columns) {
+  const std::string fn = "DequantizeMxfp4";
+  need_mxfp4(fn, "", codes, scales);
+  need_gpu(fn, "output", output.device);
+  if (columns < 0 || mx_blocks(columns) != scales.shape.back())
+    throw std::invalid_argument(fn + ": columns must fill the rows' " + std::to_string(scales.shape.back()) +
+                                " blocks of 32 (got " + std::to_string(columns) + ")");
+  no_alias(fn, {{codes.p_data, "codes"}, {scales.p_data, "scales"}}, {{output.p_data, "output"}});
+  std::vector<int> shape = scales.shape;
+  shape.back() = columns;
+  output.resize_output(shape);
+  tt_check(tt_mxfp4_dequantize(dtype_code<T>(), codes.p_data, scales.p_data, output.p_data, rows_of(shape), columns,
+                               nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void FcForwardMxfp4(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<uint8_t>& weight_codes,
+                    const TinyTensor<uint8_t>& weight_scales, const TinyTensor<T>& bias) {
+  const std::string fn = "FcForwardMxfp4";
+  need_gpu(fn, "input", input.device);
+  need_mxfp4(fn, "weight_", weight_codes, weight_scales);
+  need_gpu(fn, "bias", bias.device);
+  need_gpu(fn, "output", output.device);
+  if (input.shape.empty()) throw std::invalid_argument(fn + ": input must have rank >= 1");
+  if (weight_scales.shape.size() != 2)
+    throw std::invalid_argument(fn + ": weight_scales must have rank 2 [fout, ceil(fin / 32)]");
+  const int64_t batch = rows_of(input.shape), fin = input.shape.back(), fout = weight_scales.shape[0];
+  if (weight_scales.shape[1] != mx_blocks((int)fin))
+    throw std::invalid_argument(fn + ": the weight's blocks (" + std::to_string(weight_scales.shape[1]) +
+                                ") must hold the input's last axis (" + std::to_string(fin) + ")");
+  const bool scalar_bias = bias.shape.size() == 1 && bias.shape[0] == 1;
+  if (!scalar_bias && (int64_t)bias.size != fout)
+    throw std::invalid_argument(fn + ": bias must hold fout (" + std::to_string(fout) + ") values or be [1]");
+  no_alias(fn,
+           {{input.p_data, "input"},
+            {weight_codes.p_data, "weight_codes"},
+            {weight_scales.p_data, "weight_scales"},
+            {bias.p_data, "bias"}},
+           {{output.p_data, "output"}});
+  std::vector<int> oshape(input.shape.begin(), input.shape.end() - 1);
+  oshape.push_back((int)fout);
+  output.resize_output(oshape);
+  tt_check(tt_fc_forward_mxfp4(dtype_code<T>(), batch, fin, fout, input.p_data, weight_codes.p_data,
+                               weight_scales.p_data, bias.p_data, scalar_bias ? 1 : 0, output.p_data, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void KvAppendMxfp4(const TinyTensor<T>& k, const TinyTensor<T>& v, TinyTensor<uint8_t>& k_codes,
+                   TinyTensor<uint8_t>& k_scales, TinyTensor<uint8_t>& v_codes, TinyTensor<uint8_t>& v_scales,
+                   const TinyTensor<int>& lengths) {
+  const std::string fn = "KvAppendMxfp4";
+  need_gpu(fn, "k", k.device);
+  need_gpu(fn, "v", v.device);
+  const Dims c = mx_cache(fn, k_codes, k_scales, v_codes, v_scales, lengths), n = dims4(fn, "k", k);
+  if (v.shape != k.shape) throw std::invalid_argument(fn + ": k and v must have the same shape");
+  if (n.B != c.B || n.H != c.H || n.d != c.d)
+    throw std::invalid_argument(fn + ": k and the cache disagree on B, Hkv or d");
+  no_alias(fn, {{k.p_data, "k"}, {v.p_data, "v"}, {lengths.p_data, "lengths"}},
+           {{k_codes.p_data, "k_codes"},
+            {k_scales.p_data, "k_scales"},
+            {v_codes.p_data, "v_codes"},
+            {v_scales.p_data, "v_scales"}});
+  tt_check(tt_kv_append_mxfp4(dtype_code<T>(), k.p_data, v.p_data, k_codes.p_data, k_scales.p_data, v_codes.p_data,
+                              v_scales.p_data, lengths.p_data, c.B, c.H, n.L, c.L, c.d, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void AttentionDecodeMxfp4(const TinyTensor<T>& q, const TinyTensor<uint8_t>& k_codes,
+                          const TinyTensor<uint8_t>& k_scales, const TinyTensor<uint8_t>& v_codes,
+                          const TinyTensor<uint8_t>& v_scales, const TinyTensor<int>& lengths, TinyTensor<T>& out,
+                          float scale) {
+  const std::string fn = "AttentionDecodeMxfp4";
+  need_gpu(fn, "q", q.device);
+  need_gpu(fn, "out", out.device);
+  const Dims c = mx_cache(fn, k_codes, k_scales, v_codes, v_scales, lengths), n = dims4(fn, "q", q);
+  if (n.B != c.B || n.d != c.d) throw std::invalid_argument(fn + ": q and the cache disagree on B or d");
+  no_alias(fn,
+           {{q.p_data, "q"},
+            {k_codes.p_data, "k_codes"},
+            {k_scales.p_data, "k_scales"},
+            {v_codes.p_data, "v_codes"},
+            {v_scales.p_data, "v_scales"},
+            {lengths.p_data, "lengths"}},
+           {{out.p_data, "out"}});
+  out.resize_output(q.shape);
+  tt_check(tt_attn_decode_mxfp4(dtype_code<T>(), q.p_data, k_codes.p_data, k_scales.p_data, v_codes.p_data,
+                                v_scales.p_data, lengths.p_data, out.p_data, nullptr, c.B, n.H, c.H, n.L, c.L, c.d,
+                                scale, nullptr),
+           fn.c_str());
+}
+
 template <typename T>
 void FcBackward(const TinyTensor<T>& input, const TinyTensor<T>& output, const TinyTensor<T>& weight,
                 const TinyTensor<T>& bias, TinyTensor<T>& grad_input, const TinyTensor<T>& grad_output,
@@ -691,6 +854,24 @@ template void AttentionDecode<float>(const TinyTensor<float>&, const TinyTensor<
                                      TinyTensor<float>&, float);
 template void AttentionDecode<bf16>(const TinyTensor<bf16>&, const TinyTensor<bf16>&, const TinyTensor<bf16>&,
                                     TinyTensor<bf16>&, float);
+template void QuantizeMxfp4<float>(const TinyTensor<float>&, TinyTensor<uint8_t>&, TinyTensor<uint8_t>&, bool);
+template void QuantizeMxfp4<bf16>(const TinyTensor<bf16>&, TinyTensor<uint8_t>&, TinyTensor<uint8_t>&, bool);
+template void DequantizeMxfp4<float>(const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&, TinyTensor<float>&, int);
+template void DequantizeMxfp4<bf16>(const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&, TinyTensor<bf16>&, int);
+template void FcForwardMxfp4<float>(const TinyTensor<float>&, TinyTensor<float>&, const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                    const TinyTensor<float>&);
+template void FcForwardMxfp4<bf16>(const TinyTensor<bf16>&, TinyTensor<bf16>&, const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                   const TinyTensor<bf16>&);
+template void KvAppendMxfp4<float>(const TinyTensor<float>&, const TinyTensor<float>&, TinyTensor<uint8_t>&, TinyTensor<uint8_t>&,
+                                   TinyTensor<uint8_t>&, TinyTensor<uint8_t>&, const TinyTensor<int>&);
+template void KvAppendMxfp4<bf16>(const TinyTensor<bf16>&, const TinyTensor<bf16>&, TinyTensor<uint8_t>&, TinyTensor<uint8_t>&,
+                                  TinyTensor<uint8_t>&, TinyTensor<uint8_t>&, const TinyTensor<int>&);
+template void AttentionDecodeMxfp4<float>(const TinyTensor<float>&, const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                          const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                          const TinyTensor<int>&, TinyTensor<float>&, float);
+template void AttentionDecodeMxfp4<bf16>(const TinyTensor<bf16>&, const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                         const TinyTensor<uint8_t>&, const TinyTensor<uint8_t>&,
+                                         const TinyTensor<int>&, TinyTensor<bf16>&, float);
 template void SoftmaxForward<float>(const TinyTensor<float>&, TinyTensor<float>&);
 template void FcForward<float>(const TinyTensor<float>&, TinyTensor<float>&, const TinyTensor<float>&,
                                const TinyTensor<float>&);

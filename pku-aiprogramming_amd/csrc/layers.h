@@ -27,6 +27,40 @@ template <typename T>
 void AttentionDecode(const TinyTensor<T>& q, const TinyTensor<T>& k_cache, const TinyTensor<T>& v_cache,
                      TinyTensor<T>& out, float scale);
 
+// The microscaled 4-bit format (include/tt_attn.h): input [.., n] to codes
+// [.., 16 nb] and scales [.., nb], nb = ceil(n / 32) blocks, and back to output
+// [.., columns], whose width the codes alone do not tell.  transposed: input is
+// rank 2 and its columns become the rows, which takes FcForward's weight
+// [fin, fout] to the [fout, ..] of FcForwardMxfp4.
+template <typename T>
+void QuantizeMxfp4(const TinyTensor<T>& input, TinyTensor<uint8_t>& codes, TinyTensor<uint8_t>& scales,
+                   bool transposed);
+template <typename T>
+void DequantizeMxfp4(const TinyTensor<uint8_t>& codes, const TinyTensor<uint8_t>& scales, TinyTensor<T>& output,
+                     int columns);
+
+// FcForward with a weight in 4 bits: output [.., fout] = quantised(input
+// [.., fin]) weight^T + bias, weight_codes [fout, 16 nb], weight_scales
+// [fout, nb], bias [fout] or [1].
+template <typename T>
+void FcForwardMxfp4(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<uint8_t>& weight_codes,
+                    const TinyTensor<uint8_t>& weight_scales, const TinyTensor<T>& bias);
+
+// A K/V cache in 4 bits, made by the caller: codes [B, Hkv, cap, d / 2] and
+// scales [B, Hkv, cap, d / 32] for K and for V.  lengths [B] counts each
+// sequence's keys, the T new tokens included.  KvAppendMxfp4 quantises k, v
+// [B, Hkv, T, d] into it in place; AttentionDecodeMxfp4 attends q [B, H, T, d]
+// over it, H a multiple of Hkv, token t of T up to its own key.
+template <typename T>
+void KvAppendMxfp4(const TinyTensor<T>& k, const TinyTensor<T>& v, TinyTensor<uint8_t>& k_codes,
+                   TinyTensor<uint8_t>& k_scales, TinyTensor<uint8_t>& v_codes, TinyTensor<uint8_t>& v_scales,
+                   const TinyTensor<int>& lengths);
+template <typename T>
+void AttentionDecodeMxfp4(const TinyTensor<T>& q, const TinyTensor<uint8_t>& k_codes,
+                          const TinyTensor<uint8_t>& k_scales, const TinyTensor<uint8_t>& v_codes,
+                          const TinyTensor<uint8_t>& v_scales, const TinyTensor<int>& lengths, TinyTensor<T>& out,
+                          float scale);
+
 // Row softmax over the last axis (Layers.cu:324-349): output takes input's
 // shape on the "gpu" device (the reference's `output = input`, Layers.cu:333)
 // and holds exp(x - max) / sum exp(x - max) per row.  float, as the

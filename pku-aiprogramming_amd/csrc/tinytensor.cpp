@@ -198,6 +198,17 @@ void TinyTensor<T>::apply(int op, const TinyTensor<T>* a, const TinyTensor<T>* b
   }
 }
 
+// Bytes are not numbers: every arithmetic method ends here.
+template <>
+void TinyTensor<uint8_t>::apply(int, const TinyTensor<uint8_t>*, const TinyTensor<uint8_t>*, double, double,
+                                uint64_t) {
+  throw std::invalid_argument("Tensor_byte has no arithmetic");
+}
+template <>
+TinyTensor<uint8_t>& TinyTensor<uint8_t>::random(uint8_t, uint8_t) {
+  throw std::invalid_argument("Tensor_byte has no arithmetic");
+}
+
 template <typename T>
 TinyTensor<T> TinyTensor<T>::operator+(const TinyTensor<T>& other) const {
   if (shape != other.shape) throw std::invalid_argument("Shape mismatch");
@@ -450,7 +461,7 @@ std::ostream& operator<<(std::ostream& os, const TinyTensor<T>& t) {
   const auto data = t.get_data();
   const size_t row = t.shape.empty() || t.shape.back() == 0 ? 1 : (size_t)t.shape.back();
   for (size_t i = 0; i < data.size(); ++i) {
-    os << data[i] << " ";
+    os << +data[i] << " ";  // + for a byte's number
     if ((i + 1) % row == 0) os << "\n";
   }
   return os;
@@ -460,7 +471,9 @@ template class TinyTensor<int>;
 template class TinyTensor<float>;
 template class TinyTensor<double>;
 template class TinyTensor<bf16>;
+template class TinyTensor<uint8_t>;
 template std::ostream& operator<<(std::ostream&, const TinyTensor<int>&);
 template std::ostream& operator<<(std::ostream&, const TinyTensor<float>&);
 template std::ostream& operator<<(std::ostream&, const TinyTensor<double>&);
 template std::ostream& operator<<(std::ostream&, const TinyTensor<bf16>&);
+template std::ostream& operator<<(std::ostream&, const TinyTensor<uint8_t>&);

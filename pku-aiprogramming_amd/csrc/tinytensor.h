@@ -12,7 +12,8 @@
 // allocator (tt_malloc), work is ordered on one HIP stream and host-visible
 // copies wait for it, every HIP failure raises std::runtime_error, sizes are
 // 64-bit, and a bf16 storage type (TinyTensor<bf16>) is added for the
-// attention path.  numpy() returns the data as an ndarray in one copy.
+// attention path and one of bytes (TinyTensor<uint8_t>) for values in 4 bits,
+// which stores and moves but does no arithmetic.  numpy() returns the data as an ndarray in one copy.
 #pragma once
 
 #include <pybind11/numpy.h>
@@ -79,6 +80,13 @@ template <> struct Dtype<bf16> {
   static constexpr const char* name = "bf16";
   static host to_host(bf16 v) { return bf16_bits_to_float(v.bits); }
   static bf16 from_host(host v) { return bf16{float_to_bf16_bits(v)}; }
+};
+
+template <> struct Dtype<uint8_t> {
+  using host = uint8_t;
+  static constexpr const char* name = "byte";
+  static host to_host(uint8_t v) { return v; }
+  static uint8_t from_host(host v) { return v; }
 };
 
 // Throws std::runtime_error with tt_last_error() when rc != TT_OK
