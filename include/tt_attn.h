@@ -362,9 +362,9 @@ int tt_gemm_mxfp4(int dtype, int64_t m, int64_t n, int64_t k, float alpha, const
 /* The fully connected layer with such a weight: out [batch][fout] =
  * quantised(in [batch][fin]) W^T + bias, W [fout][fin] in 4 bits, the bias
  * (fout values, or one where bias_scalar != 0) added to the fp32 sum.  in,
- * bias and out of `dtype`.  More than 16 rows are quantised into a 32 MiB
- * per-stream library workspace (allocated on first use) and multiplied from
- * there; without it (refused, or under graph capture before a call has left it
+ * bias and out of `dtype`.  All but short or few rows are quantised into a 32
+ * MiB per-stream library workspace (allocated on first use) and multiplied
+ * from there; without it (refused, or under graph capture before a call has left it
  * on the stream) the product quantises them as it reads them, which is slower
  * and gives the same result up to the order of its sums. */
 int tt_fc_forward_mxfp4(int dtype, int64_t batch, int64_t fin, int64_t fout, const void* in, const uint8_t* w_codes,

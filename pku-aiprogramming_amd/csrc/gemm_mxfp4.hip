@@ -138,7 +138,7 @@ __device__ __forceinline__ uint4 quantize_block(const MxEight<T> (&v)[4], uint32
 // flight a wave (their scales as one 16-byte load a row), with no barrier before
 // the end.  QA: A is not quantised yet (X, rows of K values), and each lane
 // quantises the blocks that it would have loaded: one launch for a layer of few
-// rows.
+// or short rows.
 constexpr int kBlockWaves = 8;
 
 // The scales of k steps [st, st + U) of a row, as this lane's half-filled words:
@@ -523,9 +523,17 @@ int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O*
   const MxEpilogue<O> all{out, bias, bias_step, 1.f, 0.f, N};
   const int64_t nb = mx_blocks(K), row_bytes = nb * (kMxBlockBytes + 1);
   const int64_t fit = row_bytes > 0 ? (int64_t)(kMxRowsWork / row_bytes) / 16 * 16 : 0;
+  // One launch, in which every workgroup quantises its 16 rows over again, where
+  // these are short or few, or two launches.  Measured (one / two, us): 256 x 100 x
+  // 784 bf16 5.1 / 6.7, 32 x 4096 x 512 fp32 4.8 / 6.2, 256 x 512 x 2048 bf16 (rows
+  // of 4 KiB) 7.6 / 7.6, fp32 10.8 / 7.4, 16 x 16384 x 1024 (1024 blocks) 9.1 / 8.3;
+  // 1 x 4096 x 4096 bf16 5.3 / 6.1, fp32 (16 KiB) 5.7 / 6.1, 4 x 4096 x 4096 bf16
+  // (32 KiB) 5.8 / 6.3, fp32 7.0 / 6.1, 1 x 4096 x 16384 bf16 11.8 / 10.5.
+  const int64_t row = K * (int64_t)sizeof(O), blocks = ((M + 15) / 16) * ((N + 15) / 16);
+  const bool once = blocks <= 512 && (row <= 4096 || (row <= 16384 && M * row <= 32768));
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until the last kernel that reads the buffer is queued
-  if (M <= 16 || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
+  if (once || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
     return block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x, W, Ws, M, N, K, all, s);
   for (int64_t r0 = 0; r0 < M; r0 += fit) {
     const int64_t rows = M - r0 < fit ? M - r0 : fit;

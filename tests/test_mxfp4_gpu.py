@@ -232,6 +232,23 @@ def test_fc(capi, m, n, k, dtype, scalar_bias):
     assert (np.abs(out.download() - ref) <= product_bound(xv, wv, k, dtype, ref, 1.0, np.abs(bias))).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(1, 50, 4096), (1, 50, 8200), (4, 50, 4100), (5, 50, 4100), (16, 50, 2048), (16, 50, 2049),
+                                   (17, 8200, 40), (530, 240, 100), (600, 240, 100)])
+def test_fc_on_both_sides_of_its_rule(capi, m, n, k, dtype):
+    """Rows of 4, 8 and 16 KiB, 32 KiB of them, and 512 blocks of 16 x 16, from both sides."""
+    rng = np.random.default_rng(m + n + k)
+    x, w, b = normal(rng, (m, k), dtype), normal(rng, (n, k), "f32"), normal(rng, (n,), dtype)
+    wc, ws = held(capi, w)
+    out = capi.DeviceBuffer((m, n), dtype)
+    capi.fc_forward_mxfp4(capi.DeviceBuffer.from_numpy(x, dtype), wc, ws, capi.DeviceBuffer.from_numpy(b, dtype), out)
+    capi.lib().sync()
+    xv, wv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(w), k)
+    ref = xv @ wv.T + b
+    tol = (k + 1) * U * (np.abs(xv) @ np.abs(wv.T) + np.abs(b))
+    assert (np.abs(out.download() - ref) <= tol * (1 + HALF[dtype]) + HALF[dtype] * np.abs(ref)).all()
+
+
 def test_fc_of_no_input_is_the_bias(capi):
     bias = capi.DeviceBuffer.from_numpy(np.arange(5, dtype=np.float32))
     out = capi.DeviceBuffer((40, 5), "f32")
