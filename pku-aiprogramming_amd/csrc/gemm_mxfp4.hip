@@ -44,71 +44,47 @@ struct MxEpilogue {
   int64_t N;
   __device__ __forceinline__ static float get(const float* p) { return *p; }
   __device__ __forceinline__ static float get(const u16* p) { return bf16_to_f32(*p); }
-  __device__ __forceinline__ static void put(float* p, float v) { *p = v; }
-  __device__ __forceinline__ static void put(u16* p, float v) { *p = f32_to_bf16(v); }
+  // four sums as they are stored
+  __device__ __forceinline__ static void round4(float (&o)[4], const float (&v)[4]) { __builtin_memcpy(o, v, 16); }
+  __device__ __forceinline__ static void round4(u16 (&o)[4], const float (&v)[4]) {
+    const uint32_t x[2] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+    __builtin_memcpy(o, x, 8);
+  }
   // bias of columns [col, col + 4), 0 past the last one
   __device__ __forceinline__ void load_bias(int64_t col, float (&b)[4]) const {
 #pragma unroll
     for (int e = 0; e < 4; ++e) b[e] = bias && col + e < N ? get(bias + (col + e) * bias_step) : 0.f;
   }
-  // What half g (l / 32) of a wave holds of a row: v[h], columns [col + 8 h + 4 g, + 4)
-  // without beta C, for both halves' lanes of the same row (every lane calls;
-  // `in`: the row is inside C).  fp32 stores four columns at a time; bf16
-  // changes halves first, so that each lane stores eight.
-  __device__ __forceinline__ void store_pair(bool in, int64_t row, int64_t col, int g, float (&v)[2][4]) const {
-    O* c = C + row * N;
-    if (beta != 0.f && in) {
+  // C[row][col, col + 4), 0 past the last column
+  __device__ __forceinline__ void load_four(int64_t row, int64_t col, float (&v)[4]) const {
+    const O* c = C + row * N + col;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + 8 * h + 4 * g + e < N) v[h][e] += beta * get(c + col + 8 * h + 4 * g + e);
-    }
-    if constexpr (sizeof(O) == 4) {
-      if (!in) return;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int64_t at = col + 8 * h + 4 * g;
-        if (at + 4 <= N) {
-          __builtin_memcpy(c + at, v[h], 16);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (at + e < N) put(c + at + e, v[h][e]);
-        }
-      }
+    for (int e = 0; e < 4; ++e) v[e] = col + e < N ? get(c + e) : 0.f;
+  }
+  // 16 bytes of values to columns from col on of a row inside C.
+  __device__ __forceinline__ void store16(int64_t row, int64_t col, const uint4& x) const {
+    constexpr int E = 16 / (int)sizeof(O);
+    O* c = C + row * N + col;
+    if (col + E <= N) {
+      __builtin_memcpy(c, &x, 16);
     } else {
-      uint32_t x[4];
+      O o[E];
+      __builtin_memcpy(o, &x, 16);
 #pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const auto t = __builtin_amdgcn_permlane32_swap(pack_bf16x2(v[0][2 * p], v[0][2 * p + 1]),
-                                                        pack_bf16x2(v[1][2 * p], v[1][2 * p + 1]), false, false);
-        x[p] = t[0];
-        x[2 + p] = t[1];
-      }
-      if (!in) return;
-      const int64_t at = col + 8 * g;
-      if (at + 8 <= N) {
-        __builtin_memcpy(c + at, x, 16);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (at + e < N) c[at + e] = (u16)(x[e / 2] >> (16 * (e & 1)));
-      }
+      for (int e = 0; e < E; ++e)
+        if (col + e < N) c[e] = o[e];
     }
   }
   // The sums of columns [col, col + 4) of a row inside C, stored at once where all are.
   __device__ __forceinline__ void store_four(int64_t row, int64_t col, const f32x4& acc) const {
     O* c = C + row * N + col;
-    float b[4];
+    float b[4], old[4] = {0.f, 0.f, 0.f, 0.f}, v[4];
     load_bias(col, b);
-    O o[4];
+    if (beta != 0.f) load_four(row, col, old);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float v = alpha * acc[e] + b[e];
-      if (beta != 0.f && col + e < N) v += beta * get(c + e);
-      put(&o[e], v);
-    }
+    for (int e = 0; e < 4; ++e) v[e] = alpha * acc[e] + b[e] + (beta != 0.f ? beta * old[e] : 0.f);
+    O o[4];
+    round4(o, v);
     if (col + 4 <= N) {
       __builtin_memcpy(c, o, sizeof(o));
     } else {
@@ -286,8 +262,8 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
 // the 32 rows of which an operand read takes one chunk spread over all banks.
 // The scales of four stages (16 bytes a row) come the same way, at any
 // alignment: as the two aligned 16-byte words that hold them (a load through
-// registers would wait for every load of the ring, 477 us for 348 at 8192 x 8192
-// x 8224), which the wave that loaded them then lays out by stage.  A wave reads the operands of a k step of 64
+// registers would wait for every load of the ring, a third more time at 8192 x
+// 8192 x 8224), which the wave that loaded them then lays out by stage.  A wave reads the operands of a k step of 64
 // while it multiplies the one before, also across the barrier of the next
 // stage.  Rows past M or N repeat the last one and are not stored.  The matrix
 // unit takes B's rows first, so a lane ends with runs of four consecutive
@@ -461,25 +437,82 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mxfp4_tile(const uint8_t* _
     }
   }
 
+  const int64_t row0 = m0 + wm * (MT * 32), col0 = n0 + wn * (NTL * 32);
+  float alpha = ep.alpha;
+  if (ep.beta != 0.f || ep.bias) {
 #pragma unroll
-  for (int i = 0; i < NTL; ++i)
+    for (int i = 0; i < NTL; ++i)
 #pragma unroll
-    for (int q = 0; q < 4; q += 2) {
-      const int64_t col = n0 + (wn * NTL + i) * 32 + 8 * q;
-      float bias[2][4];
-      ep.load_bias(col + 4 * g, bias[0]);
-      ep.load_bias(col + 8 + 4 * g, bias[1]);
+      for (int q = 0; q < 4; ++q) {
+        const int64_t col = col0 + 32 * i + 8 * q + 4 * g;
+        float bias[4], old[4];
+        ep.load_bias(col, bias);
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const int64_t row = m0 + (wm * MT + j) * 32 + r32;
-        float v[2][4];
+        for (int j = 0; j < MT; ++j) {
+          const int64_t row = row0 + 32 * j + r32;
 #pragma unroll
-        for (int h = 0; h < 2; ++h)
+          for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] = alpha * acc[i][j][4 * q + e] + bias[e];
+          if (ep.beta != 0.f && row < M) {
+            ep.load_four(row, col, old);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) v[h][e] = ep.alpha * acc[i][j][4 * (q + h) + e] + bias[h][e];
-        ep.store_pair(row < M, row, col, g, v);
+            for (int e = 0; e < 4; ++e) acc[i][j][4 * q + e] += ep.beta * old[e];
+          }
+        }
+      }
+    alpha = 1.f;
+  }
+  // C leaves through LDS, so that a store takes whole runs of the wave's columns
+  // (stored as the lanes hold them, 16 bytes a row and half, 8192 x 8192 values took
+  // 56 us, now 13).  A lane's four columns lie in one of a row's 16-byte chunks,
+  // which the row swizzles over the banks.
+  constexpr int ROW = NTL * 32 * (int)sizeof(O), CHUNKS = ROW / 16, UPC = 16 / (4 * (int)sizeof(O));
+  constexpr int MINE = (int)sizeof(s_c) / (WM * WN), JP = MINE / (32 * ROW) < MT ? MINE / (32 * ROW) : MT;
+  constexpr int RPS = 64 / CHUNKS;  // rows of a store
+  static_assert(JP > 0 && MT % JP == 0, "whole tiles a pass");
+  auto chunk_at = [](int row, int c) { return row * ROW + 16 * (c ^ (row / UPC % CHUNKS)); };
+  uint8_t* mine = &s_c[0][0] + w * MINE;
+  const bool whole = m0 + BM <= M && n0 + BN <= N;
+  const int c = l % CHUNKS;
+  __syncthreads();  // nobody reads the ring any more
+#pragma unroll
+  for (int j0 = 0; j0 < MT; j0 += JP) {
+#pragma unroll
+    for (int j = j0; j < j0 + JP; ++j)
+#pragma unroll
+      for (int i = 0; i < NTL; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          float v[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = alpha * acc[i][j][4 * q + e];
+          O o[4];
+          ep.round4(o, v);
+          const int unit = 8 * i + 2 * q + g;
+          __builtin_memcpy(mine + chunk_at(32 * (j - j0) + r32, unit / UPC) + (unit % UPC) * (int)sizeof(o), o,
+                           sizeof(o));
+        }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+    const int64_t first_row = row0 + 32 * j0 + l / CHUNKS, col = col0 + c * (16 / (int)sizeof(O));
+    if (whole) {
+      O* to = ep.C + first_row * N + col;
+#pragma unroll
+      for (int t = 0; t < JP * 32 / RPS; ++t) {
+        __builtin_memcpy(to, mine + chunk_at(t * RPS + l / CHUNKS, c), 16);
+        to += RPS * N;
+      }
+    } else {
+      for (int t = 0; t < JP * 32 / RPS; ++t) {
+        uint4 x;
+        __builtin_memcpy(&x, mine + chunk_at(t * RPS + l / CHUNKS, c), 16);
+        if (first_row + t * RPS < M) ep.store16(first_row + t * RPS, col, x);
       }
     }
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
 }
 
 template <typename O, int BM, int BN, int WM, int WN>
@@ -507,9 +540,9 @@ int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* 
   const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
   if (wide || tiles(32) <= 512) return block_launch<O, 2, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
   // 128 x 128 tiles, two a CU, where one round takes them all.  Measured (128 /
-  // 256, us): 1531 x 4099 x 4096 34.8 / 46.6 (400 small tiles), 2048 x 4096 x 1000
-  // 12.4 / 15.9 (512), 3000 x 3000 x 3000 37.0 / 30.0 (576), 3500 x 3500 x 2000
-  // 35.6 / 28.1 (784).
+  // 256, us): 1531 x 4099 x 4096 25.3 / 32.6 (396 small tiles), 2048 x 4096 x 1000
+  // 10.3 / 13.1 (512), 2600 x 3328 x 2048 20.9 / 19.0 (546), 3500 x 3500 x 2000
+  // 29.6 / 25.1 (784), 8192 x 8192 x 8192 394 / 279.
   if (tiles(128) <= 512) return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
   return tile_launch<O, 256, 256, 2, 4>(fn, A, As, B, Bs, M, N, K, ep, s);
 }
