@@ -95,27 +95,16 @@ struct MxEpilogue {
   }
 };
 
-// The 32 values of one block, quantised in registers: its codes, *s its scale.
-template <typename T>
-__device__ __forceinline__ uint4 quantize_block(const MxEight<T> (&v)[4], uint32_t* s) {
-  uint32_t e = 0;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) e = max(e, v[j].top());
-  *s = mx_scale_byte(e);
-  const float f = mx_scale(*s);
-  if (*s == 255u) return uint4{0, 0, 0, 0};
-  return uint4{v[0].codes(f), v[1].codes(f), v[2].codes(f), v[3].codes(f)};
-}
-
 // Blocks: a workgroup makes 16 MT rows by 16 NT columns of C, its eight waves
 // taking an eighth of the k steps of 128 each and meeting in LDS: for products
 // of few tiles, whose time is the serial chain of one workgroup.  Operands go
 // from global memory to the matrix unit's registers directly, four steps in
 // flight a wave (their scales as one 16-byte load a row), with no barrier before
-// the end.  QA: A is not quantised yet (X, rows of K values), and each lane
-// quantises the blocks that it would have loaded: one launch for a layer of few
-// or short rows.
+// the end.  QA: A is not quantised yet (X, rows of K values), and each wave
+// quantises the 16 rows' k values that it multiplies: one launch for a layer of
+// few or short rows.
 constexpr int kBlockWaves = 8;
+constexpr int kStepK = 128, kStepBytes = kStepK / 2;  // values of a k step, and bytes of their codes
 
 // The scales of k steps [st, st + U) of a row, as this lane's half-filled words:
 // block 4 u + g in byte g of w[u] at least, 0 past the row's nb blocks.
@@ -140,7 +129,10 @@ template <typename O, int MT, int NT, bool QA>
 __global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
     const uint4* __restrict__ A, const uint8_t* __restrict__ As, const O* __restrict__ X, const uint4* __restrict__ B,
     const uint8_t* __restrict__ Bs, int64_t M, int64_t N, int64_t K, int nb, uint32_t ntiles, MxEpilogue<O> ep) {
-  constexpr int TILES = MT * NT, HALF = kBlockWaves / 2, UN = QA && sizeof(O) == 4 ? 2 : 4;
+  static_assert(!QA || MT == 1, "16 rows quantised in place");
+  constexpr int TILES = MT * NT, HALF = kBlockWaves / 2, UN = QA ? MxWord<O>::N / 2 : 4;
+  constexpr int QROW = UN * kStepBytes + 16, QSCALES = 20;  // a row's codes and scales of UN steps, spread over the banks
+  __shared__ __align__(16) uint8_t s_q[QA ? kBlockWaves : 1][16][QA ? QROW : 16], s_qs[QA ? kBlockWaves : 1][16][QSCALES];
   __shared__ __align__(16) f32x4 red[HALF][TILES][64];
   const int l = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r = l & 15, g = l >> 4;
   const int64_t n0 = (int64_t)(blockIdx.x % ntiles) * (16 * NT), m0 = (int64_t)(blockIdx.x / ntiles) * (16 * MT);
@@ -148,7 +140,8 @@ __global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
 #pragma unroll
   for (int i = 0; i < NT; ++i) brow[i] = min(n0 + 16 * i + r, N - 1) * nb;
 #pragma unroll
-  for (int j = 0; j < MT; ++j) arow[j] = min(m0 + 16 * j + r, M - 1) * (QA ? K : (int64_t)nb);
+  for (int j = 0; j < MT; ++j) arow[j] = min(m0 + 16 * j + r, M - 1) * nb;
+  const int rows = (int)min((int64_t)16, M - m0);  // of this workgroup, where it quantises them
   f32x4 acc[NT][MT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -158,7 +151,6 @@ __global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
   for (int st = w * share; st < end; st += UN) {
     uint4 b[UN][NT], a[UN][MT];
     uint32_t sb[NT][UN], sa[MT][UN];
-    MxEight<O> v[QA ? UN : 1][MT][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i) load_step_scales<UN>(sb[i], Bs + brow[i], st, nb, g);
     if constexpr (!QA) {
@@ -174,20 +166,50 @@ __global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
       for (int i = 0; i < NT; ++i) b[u][i] = B[brow[i] + at];
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        if constexpr (QA) {
-          const O* p = X + arow[j] + (int64_t)at * kMxBlock;
-          const int n = (int)min((int64_t)kMxBlock, K - (int64_t)at * kMxBlock);
-          if (n == kMxBlock) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[u][j][q].load(p + 8 * q);
-          } else {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) v[u][j][q].load_part(p + 8 * q, n - 8 * q);
-          }
-        } else {
-          a[u][j] = A[arow[j] + at];
-        }
+        if constexpr (!QA) a[u][j] = A[arow[j] + at];
       }
+    }
+    if constexpr (QA) {
+      // A lane takes a word of each row, as they lie in memory (or of every second
+      // or fourth, where the wave has half or a quarter of UN steps); the operands
+      // come back from the wave's own LDS.  Rows past M hold anything: each stays
+      // in its column of the tile, which is not stored.
+      const int left = end - st, sh = left == 1 ? (UN == 4 ? 2 : 1) : (2 * left <= UN ? 1 : 0);
+      const int word = l & (63 >> sh), first = l >> (6 - sh);
+      MxWord<O> v[16] = {};
+      const int64_t k0 = (int64_t)st * kStepK + word * MxWord<O>::N;
+      const int n = (int)min((int64_t)MxWord<O>::N, min(K, (int64_t)end * kStepK) - k0);  // at most 0: no value
+      const O* p = X + (m0 + first) * K + k0;
+      const int own = rows - first, each = 1 << sh;  // the lane's rows: first + i each
+      if (n == MxWord<O>::N) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i * each < own) v[i].load(p + (i * each) * K);
+      } else if (n > 0) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+          if (i * each < own) v[i].load_part(p + (i * each) * K, n);
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        if (i * each < own) {
+          uint32_t sc;
+          const typename MxWord<O>::Codes c = mx_quantize_word<O>(v[i], &sc);
+          const int m = first + i * each;
+          __builtin_memcpy(&s_q[w][m][word * sizeof(c)], &c, sizeof(c));
+          if (word % (kMxBlock / MxWord<O>::N) == 0) s_qs[w][m][word / (kMxBlock / MxWord<O>::N)] = (uint8_t)sc;
+        }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        __builtin_memcpy(&a[u][0], __builtin_assume_aligned(&s_q[w][r][(4 * u + g) * kMxBlockBytes], 16), 16);
+        sa[0][u] = s_qs[w][r][4 * u + g];
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 #pragma unroll
     for (int u = 0; u < UN; ++u) {
@@ -195,10 +217,7 @@ __global__ __launch_bounds__(64 * kBlockWaves, QA ? 2 : 4) void k_mxfp4_block(
       const bool in = 4 * (st + u) + g < nb;
 #pragma unroll
       for (int j = 0; j < MT; ++j) {
-        if constexpr (QA)
-          a[u][j] = quantize_block(v[u][j], &sa[j][u]);
-        else
-          sa[j][u] >>= 8 * g;
+        if constexpr (!QA) sa[j][u] >>= 8 * g;
         if (!in) {
           a[u][j] = uint4{0, 0, 0, 0};
           sa[j][u] = 0u;
@@ -558,12 +577,12 @@ int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O*
   const int64_t fit = row_bytes > 0 ? (int64_t)(kMxRowsWork / row_bytes) / 16 * 16 : 0;
   // One launch, in which every workgroup quantises its 16 rows over again, where
   // these are short or few, or two launches.  Measured (one / two, us): 256 x 100 x
-  // 784 bf16 5.1 / 6.7, 32 x 4096 x 512 fp32 4.8 / 6.2, 256 x 512 x 2048 bf16 (rows
-  // of 4 KiB) 7.6 / 7.6, fp32 10.8 / 7.4, 16 x 16384 x 1024 (1024 blocks) 9.1 / 8.3;
-  // 1 x 4096 x 4096 bf16 5.3 / 6.1, fp32 (16 KiB) 5.7 / 6.1, 4 x 4096 x 4096 bf16
-  // (32 KiB) 5.8 / 6.3, fp32 7.0 / 6.1, 1 x 4096 x 16384 bf16 11.8 / 10.5.
+  // 784 bf16 4.5 / 6.7, 32 x 4096 x 512 fp32 4.7 / 6.2, 256 x 512 x 2048 bf16 (rows
+  // of 4 KiB) 6.6 / 7.6, fp32 8.0 / 7.4, 16 x 16384 x 1024 (1024 blocks) 9.1 / 8.3;
+  // 1 x 4096 x 4096 bf16 4.4 / 6.1, fp32 5.4 / 6.1, 4 x 4096 x 4096 bf16 (32 KiB) 4.8 /
+  // 6.3, fp32 6.1 / 6.1, 1 x 4096 x 16384 bf16 9.5 / 10.5, fp32 15.0 / 10.3.
   const int64_t row = K * (int64_t)sizeof(O), blocks = ((M + 15) / 16) * ((N + 15) / 16);
-  const bool once = blocks <= 512 && (row <= 4096 || (row <= 16384 && M * row <= 32768));
+  const bool once = blocks <= 512 && (row <= 4096 || M * row <= 32768);
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until the last kernel that reads the buffer is queued
   if (once || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
