@@ -340,7 +340,11 @@ int tt_col_sum(int dtype, const void* x, void* y, int64_t rows, int64_t cols, vo
  * 6.  A block that holds an infinity or a NaN gets scale byte 255 and codes of
  * zero, and every value of such a block reads as NaN.  Only the rounding to
  * the element grid is inexact, so the result is the same everywhere, bit for
- * bit.  A signed zero keeps its sign. */
+ * bit.  A signed zero keeps its sign.
+ *
+ * The layer's and the decode's workspaces have one address a stream, so that
+ * graphs may keep it: graphs captured on one stream share it and must be
+ * replayed in stream order, as eager calls on that stream are. */
 
 /* x [rows][cols] (trans = 0) to codes and scales; with trans = 1, x is stored
  * [cols][rows] and row r of the result takes its column r (a layer's weight

@@ -594,3 +594,61 @@ def test_two_streams_at_once(capi):
         ref = xv @ wv.T
         assert (np.abs(r["y"].download() - ref) <= product_bound(xv, wv, 96, "bf16", ref)).all()
         r["st"].destroy()
+
+
+@pytest.mark.parametrize("warm", [False, True])
+def test_two_graphs_and_two_streams_of_long_rows(capi, warm):
+    """Layers of rows that are quantised into the workspace, beside split
+    attention: two graphs captured on one stream and replayed in turn, with eager
+    calls between and on a second stream at the same time."""
+    from test_capture_gpu import Capture
+
+    m, n, k = 20, 33, 3000  # 6000 bytes a row, 120000 together
+    rng = np.random.default_rng(33)
+    f = capi.DeviceBuffer.from_numpy
+    st, other = capi.Stream(), capi.Stream()
+    jobs = []
+    for i in range(3):
+        c = Cache(capi, rng, 1, 2, 2500, 64, [2400 - i]).upload()
+        q, x, w = normal(rng, (1, 4, 1, 64), "bf16"), normal(rng, (m, k), "bf16"), rng.standard_normal((n, k))
+        wc, ws = held(capi, w)
+        xv, wv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(w), k)
+        jobs.append(dict(c=c, q=q, qb=f(q, "bf16"), xb=f(x, "bf16"), wc=wc, ws=ws, bias=f(np.zeros(n, np.float32), "bf16"),
+                         o=capi.DeviceBuffer(q.shape, "bf16"), y=capi.DeviceBuffer((m, n), "bf16"), xv=xv, wv=wv))
+
+    def call(j, s):
+        capi.attn_decode_mxfp4(j["qb"], *j["c"].dev, j["c"].len, j["o"], None, 0.125, stream=s.handle)
+        capi.fc_forward_mxfp4(j["xb"], j["wc"], j["ws"], j["bias"], j["y"], stream=s.handle)
+
+    def check(j):
+        check_attention(j["c"], j["q"], "bf16", 0.125, j["o"].download(), None)
+        ref = j["xv"] @ j["wv"].T
+        assert (np.abs(j["y"].download() - ref) <= product_bound(j["xv"], j["wv"], k, "bf16", ref)).all()
+
+    capi.lib().call("tt_empty_cache")
+    if warm:
+        call(jobs[0], st)
+        st.sync()
+    graphs = []
+    for j in jobs[:2]:
+        with Capture(capi, st.handle) as g:
+            call(j, st)
+        graphs.append(g)
+    for _ in range(3):
+        for j in jobs:
+            for buf in (j["o"], j["y"]):
+                buf.upload(np.full(buf.shape, 77.0, np.float32))
+        call(jobs[2], other)
+        for g in graphs:
+            g.launch()
+        st.sync()
+        other.sync()
+        for j in jobs:
+            check(j)
+        call(jobs[2], st)  # eager, on the graphs' stream
+        st.sync()
+        check(jobs[2])
+    for g in graphs:
+        g.destroy()
+    st.destroy()
+    other.destroy()
