@@ -266,7 +266,10 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
     const float mn = vmax(m, top);
     const float mb = mn == -INFINITY ? 0.f : sl2 * mn;  // nothing seen yet: every weight 0
     if (wave_any(mn != m)) {
-      const float a = fast_exp2(__builtin_fmaf(sl2, m, -mb));
+      // From the products as they were rounded (no fused multiply and add), so
+      // exactly 1 for a row that keeps its maximum, whatever is beside it.
+#pragma clang fp contract(off)
+      const float a = m == -INFINITY ? 0.f : fast_exp2(sl2 * m - mb);
       lsum *= a;
 #pragma unroll
       for (int i = 0; i < ND; ++i) acc[i] *= a;
@@ -411,7 +414,7 @@ inline int64_t md_splits(int64_t units, int64_t keys, int64_t per_cu, int64_t cu
   most = std::min(most, std::max<int64_t>(4, 2 * per_cu * cus / units));
   int64_t best = 1;
   double least = std::numeric_limits<double>::max();
-  for (int64_t n = 1; n <= most; ++n) {
+  for (int64_t n = 1; n <= most; n += 1 + n / 64) {  // the host's time counts too
     const int64_t here = (units * n + cus - 1) / cus;
     const int64_t last = here % per_cu, each = ((keys + n - 1) / n + step - 1) / step * step + kMdFixed;
     auto group = [&](int64_t w) { return w > 0 ? (double)w + 76.8 / (double)d : 0.0; };  // w at once

@@ -652,3 +652,44 @@ def test_two_graphs_and_two_streams_of_long_rows(capi, warm):
         g.destroy()
     st.destroy()
     other.destroy()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("T", [1, 3])
+def test_a_row_is_the_same_whatever_is_beside_it(capi, T, dtype):
+    """The query rows that share a K / V head are one tile: what the others hold,
+    NaN and rows whose maximum rises with every key included, changes no bit."""
+    from test_capture_gpu import Capture
+
+    H, d, cap = 4, 64, 5000
+    rng = np.random.default_rng(34 + T)
+    c = Cache(capi, rng, 1, 1, cap, d, [cap])
+    rising = np.linspace(0.0, 20.0, cap)[:, None] * np.eye(1, d, 1)  # along one axis, which only some queries have
+    c.kc, c.ks = mx.quantize((mx.dequantize(c.kc, c.ks, d)[0, 0] + rising)[None, None])
+    c.upload()
+    q = normal(rng, (1, H, T, d), dtype)
+    q[:, 0, :, 1] = 0.0
+    q[:, 0, :, 0] = 40.0  # scores far from zero
+    beside = [q.copy() for _ in range(3)]
+    beside[0][:, 1:] = 0.0
+    beside[1][:, 1:] = np.nan
+    beside[2][:, 1:, :, 1] = 8.0
+    for warm in (True, False):  # split over workgroups, and not
+        outs = []
+        for x in beside:
+            b, st = capi.DeviceBuffer.from_numpy(x, dtype), capi.Stream()
+            o, lse = capi.DeviceBuffer(x.shape, dtype), capi.DeviceBuffer(x.shape[:3])
+            if warm:
+                capi.attn_decode_mxfp4(b, *c.dev, c.len, o, lse, 0.125, stream=st.handle)
+            else:
+                with Capture(capi, st.handle) as g:
+                    capi.attn_decode_mxfp4(b, *c.dev, c.len, o, lse, 0.125, stream=st.handle)
+                g.launch()
+                g.destroy()
+            st.sync()
+            outs.append((o.download()[:, 0], lse.download()[:, 0]))
+            if x is beside[1]:
+                assert np.isnan(o.download()[:, 1:]).all()
+            st.destroy()
+        for o, lse in outs[1:]:
+            assert np.array_equal(o, outs[0][0]) and np.array_equal(lse, outs[0][1])
