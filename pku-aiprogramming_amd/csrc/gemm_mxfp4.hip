@@ -52,14 +52,30 @@ struct MxEpilogue {
   }
   // bias of columns [col, col + 4), 0 past the last one
   __device__ __forceinline__ void load_bias(int64_t col, float (&b)[4]) const {
+    O x[4] = {};
+    if (bias && bias_step == 1 && col + 4 <= N) {
+      __builtin_memcpy(x, bias + col, sizeof(x));
+    } else if (bias) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) b[e] = bias && col + e < N ? get(bias + (col + e) * bias_step) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        if (col + e < N) x[e] = bias[(col + e) * bias_step];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) b[e] = get(&x[e]);
   }
   // C[row][col, col + 4), 0 past the last column
   __device__ __forceinline__ void load_four(int64_t row, int64_t col, float (&v)[4]) const {
     const O* c = C + row * N + col;
+    O x[4] = {};
+    if (col + 4 <= N) {
+      __builtin_memcpy(x, c, sizeof(x));
+    } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = col + e < N ? get(c + e) : 0.f;
+      for (int e = 0; e < 4; ++e)
+        if (col + e < N) x[e] = c[e];
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = get(&x[e]);
   }
   // 16 bytes of values to columns from col on of a row inside C.
   __device__ __forceinline__ void store16(int64_t row, int64_t col, const uint4& x) const {
