@@ -693,3 +693,68 @@ def test_a_row_is_the_same_whatever_is_beside_it(capi, T, dtype):
             st.destroy()
         for o, lse in outs[1:]:
             assert np.array_equal(o, outs[0][0]) and np.array_equal(lse, outs[0][1])
+
+
+# ------------------------------------------------------------------ products of many tiles
+
+MANY = [(2900, 3001, 31), (2900, 3001, 96), (2816, 3328, 160), (3001, 2900, 544), (2561, 3500, 1100), (2820, 3329, 4128)]
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_gemm_of_many_tiles(capi, m, n, k, dtype):
+    """More than 512 tiles of 128 x 128: whole and partly filled larger ones, odd
+    numbers of blocks, C at every alignment of its rows, and nothing beside it."""
+    rng = np.random.default_rng(m + n + k)
+    a, b = rng.standard_normal((m, k)), rng.standard_normal((n, k)) * np.ldexp(1.0, rng.integers(-6, 6, (n, 1)))
+    (ac, as_), (bc, bs) = held(capi, a), held(capi, b)
+    av, bv = mx.dequantize(*mx.quantize(a), k), mx.dequantize(*mx.quantize(b), k)
+    ref = av @ bv.T
+    for off in (0, 1):
+        buf = capi.DeviceBuffer.from_numpy(np.full(m * n + 64, 77.0, np.float32), dtype)
+        capi.lib().call("tt_gemm_mxfp4", capi.TT_BF16 if dtype == "bf16" else capi.TT_F32, m, n, k, 1.0, ac.ptr, as_.ptr,
+                        bc.ptr, bs.ptr, 0.0, buf.ptr + (8 + off) * capi.DeviceBuffer.ITEM[dtype], None)
+        capi.lib().sync()
+        got = buf.download()
+        assert (got[:8 + off] == 77.0).all() and (got[8 + off + m * n:] == 77.0).all()
+        got = got[8 + off:8 + off + m * n].reshape(m, n)
+        assert (np.abs(got - ref) <= product_bound(av, bv, k, dtype, ref)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(600, 1101, 200), (2900, 3001, 200), (2816, 3328, 96)])
+def test_tiles_with_old_c_and_with_a_bias(capi, m, n, k, dtype):
+    """128 x 128 and 256 x 256 tiles: alpha and beta; the layer with a bias of each output and of all."""
+    rng = np.random.default_rng(m + n)
+    x, b, c0 = normal(rng, (m, k), dtype), rng.standard_normal((n, k)), normal(rng, (m, n), dtype)
+    (ac, as_), (bc, bs) = held(capi, x), held(capi, b)
+    av, bv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(b), k)
+    ref = av @ bv.T
+    f = capi.DeviceBuffer.from_numpy
+    c = f(c0, dtype)
+    capi.gemm_mxfp4(k, -0.75, ac, as_, bc, bs, 0.5, c)
+    capi.lib().sync()
+    want = -0.75 * ref + 0.5 * c0
+    assert (np.abs(c.download() - want) <= product_bound(av, bv, k, dtype, want, 0.75, np.abs(c0))).all()
+    for size in (n, 1):
+        bias = normal(rng, (size,), dtype)
+        capi.fc_forward_mxfp4(f(x, dtype), bc, bs, f(bias, dtype), c)
+        capi.lib().sync()
+        want = ref + bias
+        assert (np.abs(c.download() - want) <= product_bound(av, bv, k, dtype, want, 1.0, np.abs(bias))).all()
+
+
+def test_nan_blocks_of_many_tiles_reach_their_rows_alone(capi):
+    m, n, k = 2900, 3001, 200
+    rng = np.random.default_rng(35)
+    a, b = rng.standard_normal((m, k)), rng.standard_normal((n, k))
+    a[[0, 300, 2899], [5, 199, 64]] = np.nan
+    b[[1, 1500, 3000], [0, 100, 199]] = np.inf
+    (ac, as_), (bc, bs) = held(capi, a), held(capi, b)
+    c = capi.DeviceBuffer((m, n), "f32")
+    capi.gemm_mxfp4(k, 1.0, ac, as_, bc, bs, 0.0, c)
+    capi.lib().sync()
+    want = np.zeros((m, n), bool)
+    want[[0, 300, 2899]] = True
+    want[:, [1, 1500, 3000]] = True
+    assert np.array_equal(np.isnan(c.download()), want)
