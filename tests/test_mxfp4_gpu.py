@@ -758,3 +758,32 @@ def test_nan_blocks_of_many_tiles_reach_their_rows_alone(capi):
     want[[0, 300, 2899]] = True
     want[:, [1, 1500, 3000]] = True
     assert np.array_equal(np.isnan(c.download()), want)
+
+
+@pytest.mark.parametrize("off", [1, 6, 15])
+@pytest.mark.parametrize("m,n,k", [(5, 40, 1000), (300, 520, 1000), (600, 1101, 1000), (2900, 3001, 544)])
+def test_scales_at_any_address_among_others(capi, m, n, k, off):
+    """Scales in the middle of a buffer whose other bytes read as NaN."""
+    rng = np.random.default_rng(m + off)
+    a, b = rng.standard_normal((m, k)), rng.standard_normal((n, k))
+    (qa, sa), (qb, sb) = mx.quantize(a), mx.quantize(b)
+
+    def among(s):
+        buf = np.full(s.size + 64, 255, np.uint8)
+        buf[off:off + s.size] = s.reshape(-1)
+        return capi.DeviceBuffer.from_numpy(buf, "u8")
+
+    f = capi.DeviceBuffer.from_numpy
+    ac, bc, as_, bs = f(qa, "u8"), f(qb, "u8"), among(sa), among(sb)
+    c = capi.DeviceBuffer((m, n), "f32")
+    capi.lib().call("tt_gemm_mxfp4", capi.TT_F32, m, n, k, 1.0, ac.ptr, as_.ptr + off, bc.ptr, bs.ptr + off, 0.0, c.ptr, None)
+    capi.lib().sync()
+    av, bv = mx.dequantize(qa, sa, k), mx.dequantize(qb, sb, k)
+    ref = av @ bv.T
+    assert (np.abs(c.download() - ref) <= product_bound(av, bv, k, "f32", ref)).all()
+    x, bias = f(a.astype(np.float32)), f(np.zeros(n, np.float32))
+    capi.lib().call("tt_fc_forward_mxfp4", capi.TT_F32, m, k, n, x.ptr, bc.ptr, bs.ptr + off, bias.ptr, 0, c.ptr, None)
+    capi.lib().sync()
+    av = mx.dequantize(*mx.quantize(a.astype(np.float32)), k)
+    ref = av @ bv.T
+    assert (np.abs(c.download() - ref) <= product_bound(av, bv, k, "f32", ref)).all()
