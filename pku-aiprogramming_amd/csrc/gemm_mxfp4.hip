@@ -566,10 +566,11 @@ int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* 
             int64_t N, int64_t K, const MxEpilogue<O>& ep, hipStream_t s) {
   auto tiles = [&](int64_t t) { return ((M + t - 1) / t) * ((N + t - 1) / t); };
   // Few tiles: the smallest blocks that are not more than two a CU.  Measured
-  // (16 x 16 / 32 x 32 / 128 x 128, us): 1 x 4096 x 4096 4.4 / - / 15.6 (256
-  // blocks), 100 x 1000 x 500 3.5 / 5.2 / 6.1 (441), 64 x 4096 x 4096 12.3 (1024) /
-  // 8.2 / 15.6, 128 x 4096 x 4096 21 / 12.5 (512) / 16.0, 500 x 2000 x 3000 32 / 19.2
-  // (1008) / 13.3.  M <= 16 has nothing to gain from larger ones.
+  // (16 x 16 / 32 x 32 / 128 x 128, us): 1 x 4096 x 4096 3.6 / 5.4 / 14.8 (256
+  // blocks), 100 x 1000 x 500 3.5 / 3.6 / 5.5 (441), 64 x 4096 x 4096 11.0 (1024) /
+  // 7.2 / 15.5, 128 x 4096 x 4096 19.9 / 11.4 (512) / 15.0, 600 x 1101 x 1000 12.5 /
+  // 10.3 (665) / 7.4, 500 x 2000 x 3000 24 / 17.1 (1008) / 12.6.  M <= 16 has nothing
+  // to gain from larger ones.
   if (tiles(16) <= 512 || M <= 16) return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
   // the tiles keep the offsets of their rows in 32 bits
   const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
