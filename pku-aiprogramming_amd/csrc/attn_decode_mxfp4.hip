@@ -13,13 +13,16 @@
 //     exactly, with no LDS: the k order of the contraction is free, and q is
 //     laid out to match.  Result: a lane owns one query row and 8 keys.
 //   O^T [D x 16 rows] += V^T P^T: P comes out of S^T in the operand's layout
-//     (the order of the keys is free as well); V's rows are converted to bf16 into the wave's LDS
-//     tile and read back transposed (ds_read_b64_tr_b16).  P is split into bf16
-//     terms (two for bf16 tensors, 2^-17 off; three for fp32, whose q is split
-//     into three exact terms too), so that no rounding of the weights shows in
-//     the result.
-// The codes of the next step are in flight meanwhile.  The waves of a workgroup meet in LDS at the end, and splits of the
-// keys over workgroups in a second launch.
+//     (the order of the keys is free as well); V's rows are converted to bf16
+//     into the wave's LDS tile and read back transposed (ds_read_b64_tr_b16).  P
+//     is split into bf16 terms (two for bf16 tensors, 2^-17 off; three for fp32,
+//     whose q is split into three exact terms too), so that no rounding of the
+//     weights shows in the result.
+// The codes of the next step are in flight meanwhile.  The waves of a workgroup
+// meet in LDS at the end, and splits of the keys over workgroups in a second
+// launch.  Measured: 64 x 32 heads x 8192 keys of 128, bf16, 353 us (6.5 TB/s); 16 x 8
+// heads x 16383 keys 54 us (5.3); 1 x 32 heads x 4097 keys 11.3 us, of which the
+// second launch 2 to 3.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
