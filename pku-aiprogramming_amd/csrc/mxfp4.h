@@ -85,6 +85,11 @@ template <> struct MxEight<u16> {
       w[i] = lo | (hi << 16);
     }
   }
+  // the first n of them and zeros
+  __device__ __forceinline__ void keep(int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = 2 * i + 1 < n ? w[i] : (2 * i < n ? w[i] & 0xffffu : 0u);
+  }
   // the largest exponent field
   __device__ __forceinline__ uint32_t top() const {
     u16x2 m = {0, 0};
@@ -159,6 +164,10 @@ template <> struct MxWord<float> {
   __device__ __forceinline__ void load_part(const float* p, int n) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = i < n ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ void keep(int n) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? v[i] : 0.f;
   }
   __device__ __forceinline__ uint32_t top() const {
     uint32_t m = 0;

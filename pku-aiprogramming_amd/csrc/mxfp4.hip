@@ -42,8 +42,9 @@ __device__ __forceinline__ void mx_divmod(uint64_t u, uint32_t n, uint64_t* q, u
 // and end inside the last one.
 template <typename T, bool QUANT, bool FLAT, bool NT>
 __global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, typename MxWord<T>::Codes* codes, uint8_t* scales,
-                                                           uint64_t words, int64_t cols, uint32_t nb) {
+                                                           uint64_t words, int64_t rows, int64_t cols, uint32_t nb) {
   constexpr int N = MxWord<T>::N, WPB = kMxBlock / N;  // values of a word, words of a block
+  const T* end = x + rows * cols;
   const uint64_t step = (uint64_t)gridDim.x * (kMxThreads * kMxUnroll);
   for (uint64_t base = (uint64_t)blockIdx.x * (kMxThreads * kMxUnroll); base < words; base += step) {
     MxWord<T> v[kMxUnroll];
@@ -67,7 +68,9 @@ __global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, typename MxWord
         n[i] = (int)max((int64_t)0, min((int64_t)N, cols - c0));
       }
       if constexpr (QUANT) {
-        if (FLAT || n[i] == N)
+        // a word past its row's end is loaded whole where the next row's values
+        // follow, which keep() takes out
+        if (FLAT || at[i] + N <= end)
           v[i].template load<NT>(at[i]);
         else
           v[i].load_part(at[i], n[i]);
@@ -81,6 +84,7 @@ __global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, typename MxWord
       const uint64_t u = base + i * kMxThreads + threadIdx.x;
       if (u >= words) continue;
       if constexpr (QUANT) {
+        if (!FLAT && n[i] < N) v[i].keep(n[i]);
         uint32_t sb;
         codes[u] = mx_quantize_word<T>(v[i], &sb);
         if (u % WPB == 0) scales[u / WPB] = (uint8_t)sb;
@@ -179,8 +183,8 @@ int rows_launch(const char* fn, T* x, uint8_t* codes, uint8_t* scales, int64_t r
   const uint64_t want = (words + per - 1) / per;
   const dim3 grid((unsigned)(want < (uint64_t)kMxMaxGrid ? want : (uint64_t)kMxMaxGrid)), block(kMxThreads);
 #define TT_MX_ROWS(FLAT, NT)                                                                                      \
-  hipLaunchKernelGGL((k_mxfp4_rows<T, QUANT, FLAT, NT>), grid, block, 0, s, x, (Codes*)codes, scales, words, cols, \
-                     (uint32_t)nb)
+  hipLaunchKernelGGL((k_mxfp4_rows<T, QUANT, FLAT, NT>), grid, block, 0, s, x, (Codes*)codes, scales, words, rows, \
+                     cols, (uint32_t)nb)
   const bool nt = rows * cols * (int64_t)sizeof(T) > kMxNtBytes;
   if (cols % kMxBlock == 0) {
     if (nt)
