@@ -787,3 +787,17 @@ def test_scales_at_any_address_among_others(capi, m, n, k, off):
     av = mx.dequantize(*mx.quantize(a.astype(np.float32)), k)
     ref = av @ bv.T
     assert (np.abs(c.download() - ref) <= product_bound(av, bv, k, "f32", ref)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("cols", [1, 7, 33, 39, 61, 95, 1023])
+def test_a_rows_end_does_not_take_in_the_next_row(capi, cols, dtype):
+    """Rows behind a row that is NaN, infinite or large from its first value on."""
+    rng = np.random.default_rng(cols)
+    x = normal(rng, (41, cols), dtype)
+    x[1::8] = np.nan
+    x[3::8] = np.inf
+    x[5::8] *= 2.0 ** 60
+    codes, scales = quantized(capi, x, dtype)
+    rc, rs = mx.quantize(x)
+    assert np.array_equal(scales.download(), rs) and np.array_equal(codes.download(), rc)
