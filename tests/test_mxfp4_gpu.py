@@ -801,3 +801,43 @@ def test_a_rows_end_does_not_take_in_the_next_row(capi, cols, dtype):
     codes, scales = quantized(capi, x, dtype)
     rc, rs = mx.quantize(x)
     assert np.array_equal(scales.download(), rs) and np.array_equal(codes.download(), rc)
+
+
+def test_two_host_threads_on_one_stream(capi):
+    """Calls of two threads share the stream's scratch: each call's kernels are queued together."""
+    import threading
+
+    m, n, k = 24, 40, 3000
+    rng = np.random.default_rng(36)
+    f = capi.DeviceBuffer.from_numpy
+    jobs, st = [], capi.Stream()
+    for i in range(2):
+        c = Cache(capi, rng, 1, 2, 2500, 64, [2300 - i]).upload()
+        q, x, w = normal(rng, (1, 4, 1, 64), "bf16"), normal(rng, (m, k), "bf16"), rng.standard_normal((n, k))
+        wc, ws = held(capi, w)
+        xv, wv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(w), k)
+        jobs.append(dict(c=c, q=q, qb=f(q, "bf16"), xb=f(x, "bf16"), wc=wc, ws=ws, bias=f(np.zeros(n, np.float32), "bf16"),
+                         o=[capi.DeviceBuffer(q.shape, "bf16") for _ in range(30)],
+                         y=[capi.DeviceBuffer((m, n), "bf16") for _ in range(30)], xv=xv, wv=wv, error=None))
+
+    def work(j):
+        try:
+            for o, y in zip(j["o"], j["y"]):
+                capi.attn_decode_mxfp4(j["qb"], *j["c"].dev, j["c"].len, o, None, 0.125, stream=st.handle)
+                capi.fc_forward_mxfp4(j["xb"], j["wc"], j["ws"], j["bias"], y, stream=st.handle)
+        except Exception as e:  # reported by the test's own thread
+            j["error"] = e
+
+    threads = [threading.Thread(target=work, args=(j,)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    st.sync()
+    for j in jobs:
+        assert j["error"] is None
+        ref = j["xv"] @ j["wv"].T
+        for o, y in zip(j["o"], j["y"]):
+            check_attention(j["c"], j["q"], "bf16", 0.125, o.download(), None)
+            assert (np.abs(y.download() - ref) <= product_bound(j["xv"], j["wv"], k, "bf16", ref)).all()
+    st.destroy()
