@@ -390,7 +390,9 @@ int tt_kv_append_mxfp4(int dtype, const void* k, const void* v, uint8_t* k_codes
  * multiple of Hkv (query head h reads K/V head h / (H / Hkv)), lse [B][H][T]
  * (float, natural log, may be NULL).  Token t sees key j where j < lengths[b] -
  * (T - 1 - t) and j < cap; one that sees none gets o = 0 and lse = -inf.  Rows
- * of the cache that no token sees are not used, whatever they hold.  B H T is
+ * of the cache that no token sees are not used, whatever they hold.  Values
+ * from 2^128 on (scale bytes 253 and 254) are infinite here too: an infinite or
+ * NaN value of V reaches the tokens that see its key and no others.  B H T is
  * below 2^31 (TT_ERR_ARG otherwise).  K and V enter with their 4-bit values,
  * scores, weights and sums in fp32 precision.  Few heads split the keys over
  * workgroups and merge their sums through a fixed 24 MiB per-stream library

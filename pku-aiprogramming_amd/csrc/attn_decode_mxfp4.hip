@@ -41,6 +41,8 @@ namespace {
 constexpr int kMdThreads = 256, kMdWaves = kMdThreads / 64;
 constexpr int kMdRows = 16;  // query rows of a workgroup
 constexpr int kMdKeys = 32;  // keys of a wave's step
+// From this scale byte on a block may hold infinities (6 2^126 is 2^128 or more) or NaN.
+constexpr uint32_t kMdNotFinite = 253;
 
 __device__ __forceinline__ f32x4 mfma_bf16_16x16x32(const bf16x8& a, const bf16x8& b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
@@ -222,11 +224,8 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
       for (int e = 0; e < 8; ++e) qx[j][e] = -qx[j][e];
     md_terms<NQ>(qx[j], qf[j]);
   }
-  for (; j0 < kend; j0 += kMdWaves * kMdKeys) {
-    MdPiece<W> kx[2] = {k[0], k[1]}, vx[2] = {v[0], v[1]};
-    if (j0 + kMdWaves * kMdKeys < kend) fetch(j0 + kMdWaves * kMdKeys);
-
-    f32x4 s[2];
+  // s[u][i]: key 16 u + 4 g + i of the step, for this lane's row
+  auto scores = [&](const MdPiece<W>(&kx)[2], f32x4(&s)[2]) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
       s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -238,21 +237,34 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
         for (int n = NQ - 1; n >= 0; --n) s[u] = mfma_bf16_16x16x32(a, qf[j][n], s[u]);
       }
     }
-    uint64_t odd[2] = {0, 0};  // lanes whose V block reads as NaN, in a step that some row does not see whole
+  };
+  auto mask = [&](f32x4(&s)[2], int j0) {
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[u][i] = j0 + 16 * u + 4 * g + i < min(seen, kend) ? s[u][i] : -INFINITY;
+  };
+  // A block of V that is taken out of the product: one that holds infinities, and
+  // one of NaN where some row does not see it (the others' every weight makes NaN).
+  auto apart = [](const MdPiece<W>& v, bool edge) { return v.s >= kMdNotFinite && (edge || v.s != 255u); };
+  bool any_apart = false;
+  for (; j0 < kend; j0 += kMdWaves * kMdKeys) {
+    MdPiece<W> kx[2] = {k[0], k[1]}, vx[2] = {v[0], v[1]};
+    if (j0 + kMdWaves * kMdKeys < kend) fetch(j0 + kMdWaves * kMdKeys);
+
+    f32x4 s[2];
+    scores(kx, s);
+    // A weight of zero must not meet an infinity or a NaN, be it a masked key's or
+    // a bf16 term of a weight: V rows that no row sees become zeros, and so do
+    // blocks that may hold either, whose values are added after the loop.
     const bool edge = j0 + kMdKeys > min(kend, all_see);
-    if (edge) {
+    if (edge || wave_any(max(vx[0].s, vx[1].s) >= kMdNotFinite)) {
+      mask(s, j0);
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = j0 + 16 * u + 4 * g + i;
-          s[u][i] = key < min(seen, kend) ? s[u][i] : -INFINITY;
-        }
-        // A weight of zero must not meet a NaN: V rows that no row sees become
-        // zeros, and a block of NaN that only some see is added below.
-        const bool out = j0 + 16 * u + r >= kend;
-        odd[u] = __ballot(!out && vx[u].s == 255u);
-        if (out || vx[u].s == 255u) {
+        const bool out = j0 + 16 * u + r >= kend, odd = apart(vx[u], edge);
+        any_apart |= wave_any(!out && odd);
+        if (out || odd) {
           vx[u].s = 127u;
 #pragma unroll
           for (int j = 0; j < W; ++j) vx[u].c[j] = 0u;
@@ -308,16 +320,36 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
 
+  // Rare: the steps with such blocks once more, for the values of these alone,
+  // under the weights that the final maximum gives.
+  if (any_apart) {
+    const float mb = m == -INFINITY ? 0.f : sl2 * m;
+    for (j0 = kbeg + w * kMdKeys; j0 < kend; j0 += kMdWaves * kMdKeys) {
+      fetch(j0);
+      const bool edge = j0 + kMdKeys > min(kend, all_see);
+      if (!wave_any(apart(v[0], edge) || apart(v[1], edge))) continue;
+      f32x4 s[2];
+      scores(k, s);
+      mask(s, j0);
 #pragma unroll
-    for (int u = 0; u < 2; ++u)
-      for (uint64_t left = odd[u]; left; left &= left - 1) {  // rare: NaN blocks at the border of the mask
-        const int at = __builtin_ctzll(left), blk = W == 4 ? at >> 4 : (W == 2 ? at >> 5 : 0);
-        const bool hit = j0 + 16 * u + (at & 15) < seen;
+      for (int u = 0; u < 2; ++u)
+        for (uint64_t left = __ballot(j0 + 16 * u + r < kend && apart(v[u], edge)); left; left &= left - 1) {
+          const int at = __builtin_ctzll(left), in = at & 15, part = at >> 4, key = j0 + 16 * u + in;
+          float wgt = (in & 2) ? ((in & 1) ? s[u][3] : s[u][2]) : ((in & 1) ? s[u][1] : s[u][0]);
+          wgt = fast_exp2(__builtin_fmaf(sl2, __shfl(wgt, 16 * (in >> 2) + r, 64), -mb));  // from the lane that holds the key's
+          const uint8_t *codes = vc + (base + key) * (16 * W), *scales = vs + (base + key) * W;
 #pragma unroll
-        for (int i = 0; i < ND; ++i)
-          if (hit && i / 2 == blk) acc[i] += f32x4{NAN, NAN, NAN, NAN};
-      }
+          for (int i = 0; i < ND; ++i) {  // this lane's columns 16 i + 4 g and three more, if the piece has them
+            if ((16 * i + 4 * g) / (8 * W) != part || key >= seen) continue;
+            MxWord<float> x;
+            x.from(*reinterpret_cast<const uint16_t*>(codes + 8 * i + 2 * g), mx_scale(scales[i / 2]));
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[i][e] += wgt * x.v[e];
+          }
+        }
+    }
   }
 
   // The waves' sums meet in LDS: [row][D] fp32 over each wave's own tile, chunks

@@ -1,0 +1,88 @@
+"""GPU tests of the 4-bit operators where values, sizes or addresses are at
+their limits.  Bounds as in test_mxfp4_gpu, whose helpers they use; where an
+infinity or a NaN is expected, it is expected exactly there."""
+import numpy as np
+import pytest
+
+from oracle import attn_oracle as orc
+from oracle import mxfp4_oracle as mx
+from test_mxfp4_gpu import HALF, U, Cache, attend, capi, check_attention, held, normal, product_bound  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------------------------------ attention: infinite values
+
+def attention_with_infinities(c, q, dtype, scale, o, lse):
+    """As check_attention, values from 2^128 on being infinite: a row that sees one is infinite in its column."""
+    k, v = c.values()
+    d, n = q.shape[3], c.shape[2]
+    with np.errstate(over="ignore"):
+        k, v = k.astype(np.float32).astype(np.float64), v.astype(np.float32).astype(np.float64)
+    with np.errstate(invalid="ignore"):
+        ro, rl, mag, _ = mx.decode(q, k, v, c.lengths, scale)
+        smax = mx.decode(q, np.where(np.isinf(k), 0.0, k), v, c.lengths, scale)[3]  # infinite keys have no error
+        e = (d + 4) * U * smax
+        tol = (2 * e + (U if dtype == "f32" else 2.0 ** -16) + 2 * (n + 4) * U)[..., None] * mag + HALF[dtype] * np.abs(ro)
+        off = np.abs(o - ro)
+    f = np.isfinite(ro)
+    assert np.array_equal(np.isnan(o), np.isnan(ro))
+    assert np.array_equal(np.isposinf(o), np.isposinf(ro)) and np.array_equal(np.isneginf(o), np.isneginf(ro))
+    assert (off[f] <= tol[f]).all()
+    f = np.isfinite(rl)
+    assert np.array_equal(np.isneginf(lse), np.isneginf(rl))
+    assert (np.abs(lse[f] - rl[f]) <= e[f] + (n + 4) * U + 4 * U * np.abs(rl[f])).all()
+    return ro
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("byte", [253, 254])
+def test_infinite_values_reach_only_the_tokens_that_see_them(capi, byte, d, dtype):
+    """The newest token's V block infinite in some columns and large in others, behind the older tokens' mask."""
+    rng = np.random.default_rng(byte + d)
+    lengths = [37, 3, 64, 700]
+    c = Cache(capi, rng, 4, 2, 700, d, lengths)
+    for b, n in enumerate(lengths):
+        c.vs[b, 0, n - 1, d // 32 - 1] = byte
+        c.vc[b, 0, n - 1, -16:] = rng.permutation(16).astype(np.uint8) * 17  # every code twice
+    q = normal(rng, (4, 4, 3, d), dtype)
+    o, lse = attend(capi, c.upload(), q, dtype, 0.2)
+    ro = attention_with_infinities(c, q, dtype, float(np.float32(0.2)), o, lse)
+    assert np.isfinite(ro[:, :, :2]).all() and np.isinf(ro[:, :2, 2]).any() and (np.abs(ro[:, :2, 2]) > 1e36).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("at", [0, 10, 31, 70, 299])
+def test_an_infinite_value_that_every_token_sees(capi, at, d, dtype):
+    """Weights of exactly one and of any other value; a column is infinite, not NaN, and the others are as before."""
+    rng = np.random.default_rng(at + d)
+    c = Cache(capi, rng, 1, 1, 300, d, [300])
+    c.vs[0, 0, at, 0] = 254
+    c.vc[0, 0, at, :16] = rng.integers(0, 256, 16)
+    c.upload()
+    for q in (np.zeros((1, 3, 1, d), np.float32), normal(rng, (1, 3, 1, d), dtype)):
+        o, lse = attend(capi, c, q, dtype, 0.2)
+        ro = attention_with_infinities(c, q, dtype, float(np.float32(0.2)), o, lse)
+        assert np.isinf(ro).any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_infinite_and_nan_values_in_one_cache(capi, d, dtype):
+    """Blocks of bytes 253 to 255 anywhere, several in a step, some rows' border among them."""
+    rng = np.random.default_rng(d)
+    lengths = [300, 65, 1000]
+    c = Cache(capi, rng, 3, 2, 1000, d, lengths)
+    at = rng.random((3, 2, 1000, d // 32)) < 0.01
+    c.vs[at] = rng.integers(253, 256, int(at.sum()))
+    c.vs[:, :, :30] = 127
+    c.vs[2, :, :, 0] = 127  # columns with none
+    q = normal(rng, (3, 4, 3, d), dtype) * np.float32(0.25)
+    q = orc.bf16_round(q)
+    o, lse = attend(capi, c.upload(), q, dtype, 0.2)
+    ro = attention_with_infinities(c, q, dtype, float(np.float32(0.2)), o, lse)
+    assert np.isnan(ro).any() and np.isfinite(ro).any() and (d == 32 or np.isinf(ro).any())
+
+
