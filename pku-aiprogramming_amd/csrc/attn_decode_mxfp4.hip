@@ -95,8 +95,11 @@ __device__ __forceinline__ constexpr int md_exchange(int r) {
 
 // x as a sum of N bf16 terms: each what the earlier ones leave, cut off, the last
 // one rounded.  Three hold any fp32 value exactly; of two, the rest is below 2^-17
-// of the value.
-template <int N>
+// of the value.  ANY: x may be infinite or NaN, or meet infinities.  A term is then
+// the largest bf16 below the value, so that none but zero's own are zero (1 is
+// 255 / 2^8 + 255 / 2^16 + 1 / 2^16): times an infinity each has x's sign, where
+// 0 inf would be NaN; an infinite x ends in infinite terms, NaN in NaN.
+template <int N, bool ANY = false>
 __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
   float left[8];
 #pragma unroll
@@ -107,7 +110,8 @@ __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (n + 1 < N) {
-        const uint32_t lo = __float_as_uint(left[2 * i]), hi = __float_as_uint(left[2 * i + 1]);
+        uint32_t lo = __float_as_uint(left[2 * i]), hi = __float_as_uint(left[2 * i + 1]);
+        if (ANY) lo -= left[2 * i] != 0.f, hi -= left[2 * i + 1] != 0.f;
         w[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // the upper halves
         left[2 * i] -= __uint_as_float(lo & 0xffff0000u);
         left[2 * i + 1] -= __uint_as_float(hi & 0xffff0000u);
@@ -222,7 +226,7 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
     if (negative)
 #pragma unroll
       for (int e = 0; e < 8; ++e) qx[j][e] = -qx[j][e];
-    md_terms<NQ>(qx[j], qf[j]);
+    md_terms<NQ, true>(qx[j], qf[j]);
   }
   // s[u][i]: key 16 u + 4 g + i of the step, for this lane's row
   auto scores = [&](const MdPiece<W>(&kx)[2], f32x4(&s)[2]) {

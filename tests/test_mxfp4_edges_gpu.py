@@ -86,3 +86,55 @@ def test_infinite_and_nan_values_in_one_cache(capi, d, dtype):
     assert np.isnan(ro).any() and np.isfinite(ro).any() and (d == 32 or np.isinf(ro).any())
 
 
+# ------------------------------------------------------------------ attention: infinite scores
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+def test_infinite_queries(capi, d, dtype):
+    """A query value of -inf: scores of -inf over positive keys leave nothing (o = 0, lse = -inf), and hide positive
+    keys beside others; over a key of zero, or with a score of +inf, the row is NaN.  A NaN query is NaN."""
+    rng = np.random.default_rng(d)
+    c = Cache(capi, rng, 1, 5, 70, d, [70])
+    k = mx.dequantize(c.kc, c.ks, d)
+    k[0, :, :, 0] = 1.5
+    k[0, 1, 20:30, 0] = -1.5
+    k[0, 2, 40, 0] = 0.0
+    c.kc, c.ks = mx.quantize(k)
+    q = normal(rng, (1, 5, 2, d), dtype)
+    q[0, :, 0, 0] = -np.inf
+    q[0, 1, 0, 0] = np.inf
+    q[0, 3, 1, 5] = np.nan
+    q[0, 4, 0, 0] = np.inf
+    if dtype == "f32":  # a NaN of which the upper half alone would be infinite
+        q[0, 3, 1, 5] = np.array(0x7F800001, np.uint32).view(np.float32)
+    o, lse = attend(capi, c.upload(), q, dtype, 0.2)
+    assert (o[0, 0, 0] == 0).all() and np.isneginf(lse[0, 0, 0])
+    for h, t in ((1, 0), (2, 0), (3, 1), (4, 0)):
+        assert np.isnan(o[0, h, t]).all() and np.isnan(lse[0, h, t])
+    keep = np.zeros((1, 5, 2), bool)
+    keep[0, [0, 1, 2, 4], 1] = True
+    q[~keep] = 0.0
+    k, v = c.values()
+    ro, rl, mag, smax = mx.decode(q, k, v, c.lengths, float(np.float32(0.2)))
+    e = (d + 4) * U * smax
+    tol = (2 * e + (U if dtype == "f32" else 2.0 ** -16) + 2 * 74 * U)[..., None] * mag + HALF[dtype] * np.abs(ro)
+    assert (np.abs(o - ro)[keep] <= tol[keep]).all()
+    assert (o[0, 3, 0] == 0).all() and np.isneginf(lse[0, 3, 0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("byte", [253, 254])
+def test_infinite_keys(capi, byte, d, dtype):
+    """Keys of infinite elements under queries of one bf16 term: a score of -inf takes its key out, and no more."""
+    rng = np.random.default_rng(byte + d)
+    c = Cache(capi, rng, 2, 1, 500, d, [500, 90])
+    for b, j in ((0, 3), (0, 450), (1, 88), (1, 89)):
+        c.ks[b, 0, j] = byte
+        c.kc[b, 0, j] = 0x77  # 6 everywhere: infinite
+    q = -np.abs(normal(rng, (2, 3, 2, d), "bf16")) - np.float32(2.0 ** -10)
+    q = orc.bf16_round(q)
+    o, lse = attend(capi, c.upload(), q, dtype, 0.2)
+    attention_with_infinities(c, q, dtype, float(np.float32(0.2)), o, lse)
+
+
