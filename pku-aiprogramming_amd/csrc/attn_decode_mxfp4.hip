@@ -94,11 +94,13 @@ __device__ __forceinline__ constexpr int md_exchange(int r) {
 }
 
 // x as a sum of N bf16 terms: each what the earlier ones leave, cut off, the last
-// one rounded.  Three hold any fp32 value exactly; of two, the rest is below 2^-17
-// of the value.  ANY: x may be infinite or NaN, or meet infinities.  A term is then
-// the largest bf16 below the value, so that none but zero's own are zero (1 is
-// 255 / 2^8 + 255 / 2^16 + 1 / 2^16): times an infinity each has x's sign, where
-// 0 inf would be NaN; an infinite x ends in infinite terms, NaN in NaN.
+// one rounded; three hold any fp32 value exactly.  Of two the first is rounded
+// too: it leaves at most 2^-8 of the value, of which the second is 2^-17 off at
+// most (cut off, it would leave 2^-7, and 2^-16 in the end).  ANY: x may be
+// infinite or NaN, or meet infinities.  A term is then the largest bf16 below the
+// value, so that none but zero's own are zero (1 is 255 / 2^8 + 255 / 2^16 + 1 /
+// 2^16): times an infinity each has x's sign, where 0 inf would be NaN; an
+// infinite x ends in an infinite term, NaN in NaN.
 template <int N, bool ANY = false>
 __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
   float left[8];
@@ -109,7 +111,11 @@ __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
     uint32_t w[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (n + 1 < N) {
+      if (N == 2 && n == 0) {
+        w[i] = pack_bf16x2(left[2 * i], left[2 * i + 1]);
+        left[2 * i] -= __uint_as_float(w[i] << 16);
+        left[2 * i + 1] -= __uint_as_float(w[i] & 0xffff0000u);
+      } else if (n + 1 < N) {
         uint32_t lo = __float_as_uint(left[2 * i]), hi = __float_as_uint(left[2 * i + 1]);
         if (ANY) lo -= left[2 * i] != 0.f, hi -= left[2 * i + 1] != 0.f;
         w[i] = __builtin_amdgcn_perm(hi, lo, 0x07060302u);  // the upper halves

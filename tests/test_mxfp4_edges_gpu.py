@@ -138,3 +138,27 @@ def test_infinite_keys(capi, byte, d, dtype):
     attention_with_infinities(c, q, dtype, float(np.float32(0.2)), o, lse)
 
 
+def test_weights_of_two_terms(capi):
+    """The weights of a bf16 call are off by 2^-17.  Two keys of weight one and values 6 and 6 2^-7 against twelve
+    of weight p = (1 + 2^-7 - x) / 2 and value -1: o = 6 x / 8 and a little, so its store rounds nearly nothing.
+
+    Bound: 2^-17 of 12 p; the store's 2^-8 |o|; of p itself and of the sums, none of which passes 6.1, the score's three
+    exact products and its scale (4 2^-24 0.7), exp2 (2^-23) and 16 additions (2^-24 each): 30 2^-24 6.1, over 2 + 12 p."""
+    H, d = 64, 32
+    k, v = np.zeros((1, 1, 14, d)), np.full((1, 1, 14, d), -1.0)
+    k[:, :, 2:] = 1.0
+    v[:, :, 0], v[:, :, 1] = 6.0, 6.0 * 2.0 ** -7
+    c = Cache(capi, np.random.default_rng(0), 1, 1, 14, d, [14])
+    (c.kc, c.ks), (c.vc, c.vs) = mx.quantize(k), mx.quantize(v)
+    p = 0.5 * (1 + 2.0 ** -7 - 2.0 ** -11 * (np.arange(H) + 0.5) / H)
+    q = np.zeros((1, H, 1, d), np.float32)
+    left = np.log(p)
+    for e in range(3):
+        q[0, :, 0, e] = orc.bf16_round(left.astype(np.float32))
+        left = left - q[0, :, 0, e]
+    o, _ = attend(capi, c.upload(), q, "bf16", 1.0)
+    ro = mx.decode(q, k, v, [14], 1.0)[0]
+    tol = (2.0 ** -17 * 12 * p + 30 * U * 6.1) / (2 + 12 * p)
+    assert (np.abs(o - ro)[0, :, 0] <= tol[:, None] + 2.0 ** -8 * np.abs(ro[0, :, 0])).all()
+
+
