@@ -485,7 +485,10 @@ int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, con
     const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
         &n, (const void*)attn_decode_mxfp4_kernel<T, D, true>, kMdThreads, 0);
     if (e != hipSuccess) (void)hipGetLastError();
-    return e == hipSuccess && n > 0 ? n : 3;
+    // The rule was measured with three at once at d = 128, where registers let a
+    // fourth in; counted, it would take 16 x 8 heads x 16383 keys from 51.5 us to
+    // 52.8 and 16 x 32 / 8 heads of ragged lengths from 46.2 to 47.5.
+    return e != hipSuccess || n < 1 || (D == 128 && n > 3) ? 3 : n;
   }();
   int64_t nsplit = md_splits(units, std::max<int64_t>(cap, 1), per_cu, device_cu_count(), D,
                              (int64_t)(kMdWork / ((size_t)rows * (D + 2) * sizeof(float))));
