@@ -393,7 +393,8 @@ int tt_kv_append_mxfp4(int dtype, const void* k, const void* v, uint8_t* k_codes
  * of the cache that no token sees are not used, whatever they hold.  Values
  * from 2^128 on (scale bytes 253 and 254) are infinite here too: an infinite or
  * NaN value of V reaches the tokens that see its key and no others.  B H T is
- * below 2^31 (TT_ERR_ARG otherwise).  K and V enter with their 4-bit values,
+ * below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an unsplit call,
+ * below 2^24 (TT_ERR_ARG otherwise).  K and V enter with their 4-bit values,
  * scores, weights and sums in fp32, of which the weights of bf16 calls keep 16
  * bits (2^-17 off) where they meet V.  Few heads split the keys over
  * workgroups and merge their sums through a fixed 24 MiB per-stream library

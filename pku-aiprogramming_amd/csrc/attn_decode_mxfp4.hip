@@ -477,9 +477,7 @@ template <typename T, int D>
 int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
            const int* lengths, T* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t tokens, int64_t cap,
            float scale, hipStream_t st) {
-  const int64_t rows = B * H * tokens;
-  if (rows > 0x7fffffff) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
-  const int64_t R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
+  const int64_t rows = B * H * tokens, R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
   static const int per_cu = [] {
     int n = 0;
     const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
@@ -495,8 +493,6 @@ int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, con
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
   if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsMxfp4Decode, kMdWork, &ws)) nsplit = 1;
-  if (!grid_fits(units * nsplit, kMdThreads) || !grid_fits(rows, 256))
-    return fail(TT_ERR_ARG, std::string(fn) + ": grid too large");
   float* part_o = (float*)ws;
   float2* part_ml = (float2*)(part_o + rows * nsplit * D);
   const float sl2 = std::max(std::fabs(scale * kLog2e), 1e-37f);
@@ -548,6 +544,10 @@ extern "C" int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_c
     return fail(TT_ERR_ARG, std::string(fn) + ": H must be a multiple of Hkv");
   if (B == 0 || H == 0 || T == 0) return ok();
   if (H > (int64_t(1) << 24) || B * H > (int64_t(1) << 24)) return fail(TT_ERR_ARG, std::string(fn) + ": too many heads");
+  if (B * H * T > 0x7fffffff) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+  // Splits, and the merge's workgroups of a row each, are few: the scratch holds all of their rows.
+  if (!grid_fits(B * Hkv * ((H / Hkv * T + kMdRows - 1) / kMdRows), kMdThreads))
+    return fail(TT_ERR_ARG, std::string(fn) + ": grid too large");
   if (!q || !o || !lengths || (cap > 0 && (!k_codes || !k_scales || !v_codes || !v_scales)))
     return fail(TT_ERR_ARG, std::string(fn) + ": null pointer");
   if (((uintptr_t)k_codes | (uintptr_t)v_codes) & 15)

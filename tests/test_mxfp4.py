@@ -207,3 +207,20 @@ def test_binding_refusals(capi):
                 (q, kc, ks, kc, ks, n, Fake(q.shape, "f32"), None)):
         with pytest.raises(ValueError):
             capi.attn_decode_mxfp4(*bad, 0.1)
+
+
+def test_attention_size_refusals(capi):
+    """B H T below 2^31, and below 2^24 tiles of 16 rows that share a K / V head."""
+    L = capi.lib()
+
+    def attend(B, H, Hkv, T):
+        return L.lib.tt_attn_decode_mxfp4(capi.TT_BF16, *P[:8], B, H, Hkv, T, 8, 32, 0.1, None)
+
+    assert attend(1, 2, 1, 1 << 30) == capi.TT_ERR_ARG and "too many rows" in L.last_error()
+    assert attend(1 << 24, 1, 1, 1) == capi.TT_ERR_ARG and "grid too large" in L.last_error()
+    assert attend(1 << 22, 4, 4, 1) == capi.TT_ERR_ARG and "grid too large" in L.last_error()
+    assert attend(1 << 23, 1, 1, 17) == capi.TT_ERR_ARG and "grid too large" in L.last_error()
+    a = [None] + P[1:8]
+    for B, H, Hkv, T in (((1 << 24) - 1, 1, 1, 1), (1 << 22, 4, 1, 4), (1, 1, 1, (1 << 28) - 16), (1 << 9, 1 << 9, 1, 1023)):
+        assert L.lib.tt_attn_decode_mxfp4(capi.TT_BF16, *a, B, H, Hkv, T, 8, 32, 0.1, None) == capi.TT_ERR_ARG
+        assert "null pointer" in L.last_error()  # the sizes are taken

@@ -162,3 +162,32 @@ def test_weights_of_two_terms(capi):
     assert (np.abs(o - ro)[0, :, 0] <= tol[:, None] + 2.0 ** -8 * np.abs(ro[0, :, 0])).all()
 
 
+# ------------------------------------------------------------------ attention: sizes and scales
+
+def test_attention_of_more_rows_than_the_merge_could_launch(capi):
+    """2^24 + 40 tokens of one head: the keys are not split, so nothing merges them."""
+    T, d, cap = (1 << 24) + 40, 32, 48
+    rng = np.random.default_rng(41)
+    c = Cache(capi, rng, 1, 1, cap, d, [T]).upload()
+    q, o, lse = capi.DeviceBuffer((1, 1, T, d), "bf16"), capi.DeviceBuffer((1, 1, T, d), "bf16"), capi.DeviceBuffer((1, 1, T))
+    L, some = capi.lib(), normal(rng, (2, 1, 1, 200, d), "bf16")
+    L.call("tt_memset", q.ptr, 0, q.nbytes)
+    head = capi.DeviceBuffer.from_numpy(some, "bf16")
+    places = (0, T - 200)  # the first tokens, which see few keys, and the last
+    for i, t in enumerate(places):
+        L.call("tt_memcpy_d2d", q.ptr + t * 2 * d, head.ptr + i * 400 * d, 400 * d)
+    capi.attn_decode_mxfp4(q, *c.dev, c.len, o, lse, 0.2)
+    L.sync()
+    k, v = c.values()
+    got, gl = capi.DeviceBuffer((2, 1, 1, 200, d), "bf16"), capi.DeviceBuffer((2, 1, 1, 200))
+    for i, t in enumerate(places):
+        L.call("tt_memcpy_d2d", got.ptr + i * 400 * d, o.ptr + t * 2 * d, 400 * d)
+        L.call("tt_memcpy_d2d", gl.ptr + i * 800, lse.ptr + t * 4, 800)
+    L.sync()
+    for i, n in enumerate((200, cap + 200)):  # as the last 200 tokens of so many keys
+        ro, rl, mag, smax = mx.decode(some[i], k, v, [n], float(np.float32(0.2)))
+        e = (d + 4) * U * smax
+        assert (np.abs(got.download()[i] - ro) <= (2 * e + 2.0 ** -16 + 104 * U)[..., None] * mag + HALF["bf16"] * np.abs(ro)).all()
+        assert (np.abs(gl.download()[i] - rl) <= e + 52 * U + 4 * U * np.abs(rl)).all()
+
+
