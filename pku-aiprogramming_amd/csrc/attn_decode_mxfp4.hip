@@ -152,8 +152,9 @@ __device__ __forceinline__ float md_lse(float m, float den) {
 }
 
 // The maximum is that of the products, the scale sl2 (of log2 e too, above zero:
-// its sign goes into q, and zero is 1e-37, which still hides what is masked)
-// enters the exponent, 2^(sl2 s - sl2 m), one operation a score.
+// its sign goes into q, and zero is the smallest fp32, 2^-149, which still hides
+// what is masked and takes no product to more than 2^-21) enters the exponent,
+// 2^(sl2 s - sl2 m), one operation a score.
 // Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv,
 // tile = 16 of the head's R query rows.  Each sequence's own length is cut into
 // nsplit spans, so that sequences of any length keep every workgroup busy.
@@ -495,7 +496,7 @@ int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, con
   if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsMxfp4Decode, kMdWork, &ws)) nsplit = 1;
   float* part_o = (float*)ws;
   float2* part_ml = (float2*)(part_o + rows * nsplit * D);
-  const float sl2 = std::max(std::fabs(scale * kLog2e), 1e-37f);
+  const float sl2 = std::max(std::fabs(scale * kLog2e), std::numeric_limits<float>::denorm_min());
 #define TT_MD_LAUNCH(STREAM)                                                                                          \
   hipLaunchKernelGGL((attn_decode_mxfp4_kernel<T, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, \
                      st, q, kc, ks, vc, vs, lengths, part_o, part_ml, o, lse, (uint32_t)Hkv, (uint32_t)R,             \

@@ -162,7 +162,7 @@ def test_weights_of_two_terms(capi):
     assert (np.abs(o - ro)[0, :, 0] <= tol[:, None] + 2.0 ** -8 * np.abs(ro[0, :, 0])).all()
 
 
-# ------------------------------------------------------------------ attention: sizes and scales
+# ------------------------------------------------------------------ attention: sizes, scales, offsets
 
 def test_attention_of_more_rows_than_the_merge_could_launch(capi):
     """2^24 + 40 tokens of one head: the keys are not split, so nothing merges them."""
@@ -189,5 +189,17 @@ def test_attention_of_more_rows_than_the_merge_could_launch(capi):
         e = (d + 4) * U * smax
         assert (np.abs(got.download()[i] - ro) <= (2 * e + 2.0 ** -16 + 104 * U)[..., None] * mag + HALF["bf16"] * np.abs(ro)).all()
         assert (np.abs(gl.download()[i] - rl) <= e + 52 * U + 4 * U * np.abs(rl)).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [0.0, 1e-38, -1e-38, 1e-41])
+def test_attention_of_no_scale_over_large_scores(capi, scale, dtype):
+    """Products up to 10^38 under a scale of zero, or one that makes them small."""
+    rng = np.random.default_rng(40)
+    c = Cache(capi, rng, 2, 2, 90, 64, [90, 33], std=2.0 ** 122).upload()
+    q = np.zeros((2, 4, 3, 64), np.float32)
+    q[..., 0] = orc.bf16_round(rng.uniform(-1, 1, (2, 4, 3)).astype(np.float32))
+    o, lse = attend(capi, c, q, dtype, scale)
+    check_attention(c, q, dtype, float(np.float32(scale)), o, lse)
 
 
