@@ -203,3 +203,43 @@ def test_attention_of_no_scale_over_large_scores(capi, scale, dtype):
     check_attention(c, q, dtype, float(np.float32(scale)), o, lse)
 
 
+def test_attention_past_32_bit_offsets(capi):
+    """The third sequence's keys begin 4 GiB into the codes and end in three that hold nearly all of the weight: by an
+    offset cut to 32 bits they would be rows of other sequences, which are 1 throughout."""
+    B, cap, d = 3, (1 << 25) + 40, 128
+    L, f = capi.lib(), capi.DeviceBuffer.from_numpy
+    codes = [capi.DeviceBuffer((B, 1, cap, d // 2), "u8") for _ in range(2)]
+    scales = [capi.DeviceBuffer((B, 1, cap, d // 32), "u8") for _ in range(2)]
+    for x in codes + scales:
+        L.call("tt_memset", x.ptr, 0x22 if x in codes else 127, x.nbytes)  # 1.0 everywhere
+    lengths = np.array([cap, 0, cap - 1], np.int32)
+    rng = np.random.default_rng(42)
+    k, v = (normal(rng, (B, 1, 3, d), "bf16") for _ in range(2))
+    dev = (codes[0], scales[0], codes[1], scales[1], f(lengths, "i32"))
+    capi.kv_append_mxfp4(f(k, "bf16"), f(v, "bf16"), *dev)
+    kv, vv = (mx.dequantize(*mx.quantize(x), d) for x in (k, v))
+    # a query that the last sequence's own newest keys answer with scores far above those of the others
+    q = np.zeros((B, 1, 1, d), np.float32)
+    q[0, 0, 0] = orc.bf16_round((kv[0, 0, 1] - 1.0).astype(np.float32))
+    q[2, 0, 0] = orc.bf16_round((kv[2, 0, 0] - 1.0).astype(np.float32))
+    o, lse = capi.DeviceBuffer((B, 1, 1, d), "f32"), capi.DeviceBuffer((B, 1, 1), "f32")
+    capi.attn_decode_mxfp4(f(q), *dev, o, lse, 1.0)
+    L.sync()
+    o, lse = o.download(), lse.download()
+    assert np.array_equal(o[1], np.zeros((1, 1, d))) and np.isneginf(lse[1]).all()
+    for b in (0, 2):
+        n = int(lengths[b]) - 3
+        s = np.append(kv[b, 0] @ q[b, 0, 0].astype(np.float64), q[b, 0, 0].astype(np.float64).sum())
+        w = np.exp(s - s.max()) * np.array([1, 1, 1, n])
+        want = (w[:3] @ vv[b, 0] + w[3]) / w.sum()
+        # More than 0.999 of the weight on the appended keys, so the roundings of a sum of 2^25 weights (2^-24 each of
+        # what they add up to) stay below 2^25 2^-24 0.001; weights below the smallest fp32, 2^-149, may be lost, at
+        # most 2^25 of them.
+        assert w[:3].sum() > 0.999 * w.sum()
+        lost = 2.0 ** (25 - 149) * max(1.0, np.abs(vv[b, 0]).max())
+        assert np.abs(want - 1.0).max() > 0.5  # what keys of other rows would give
+        e = (d + 4) * U * (np.abs(kv[b, 0]) @ np.abs(q[b, 0, 0])).max()
+        assert (np.abs(o[b, 0, 0] - want) <= (2 * e + 2e-3) * (w[:3] @ np.abs(vv[b, 0]) + w[3]) / w.sum() + lost).all()
+        assert abs(lse[b, 0, 0] - s.max() - np.log(w.sum())) <= e + 2e-3
+
+
