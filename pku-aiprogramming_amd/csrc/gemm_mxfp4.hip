@@ -575,7 +575,7 @@ int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* 
   // 7.2 / 15.5, 128 x 4096 x 4096 19.9 / 11.4 (512) / 15.0, 600 x 1101 x 1000 12.5 /
   // 10.3 (665) / 7.4, 500 x 2000 x 3000 24 / 17.1 (1008) / 12.6.  M <= 16 has nothing
   // to gain from larger ones.
-  if (tiles(16) <= 512 || M <= 16) return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  if (tiles(16) <= 512 || (M <= 16 && grid_fits(tiles(16), 64 * kBlockWaves))) return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
   // the tiles keep the offsets of their rows in 32 bits
   const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
   if (wide || tiles(32) <= 512) return block_launch<O, 2, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);

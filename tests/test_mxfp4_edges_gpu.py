@@ -243,3 +243,29 @@ def test_attention_past_32_bit_offsets(capi):
         assert abs(lse[b, 0, 0] - s.max() - np.log(w.sum())) <= e + 2e-3
 
 
+# ------------------------------------------------------------------ products of extreme and narrow shapes
+
+def test_product_of_one_row_by_more_than_2_27(capi):
+    m, n, k = 1, (1 << 27) + 40, 32
+    L = capi.lib()
+    rng = np.random.default_rng(51)
+    a, b = rng.standard_normal((m, k)), rng.standard_normal((64, k))
+    ac, as_ = held(capi, a)
+    bc, bs = capi.mxfp4_buffers((n, k))
+    L.call("tt_memset", bc.ptr, 0x22, bc.nbytes)  # 1.0 everywhere
+    L.call("tt_memset", bs.ptr, 127, bs.nbytes)
+    tc, ts = held(capi, b)
+    L.call("tt_memcpy_d2d", bc.ptr + (n - 64) * 16, tc.ptr, 64 * 16)
+    L.call("tt_memcpy_d2d", bs.ptr + (n - 64), ts.ptr, 64)
+    c = capi.DeviceBuffer((m, n), "bf16")
+    L.call("tt_memset", c.ptr, 0, c.nbytes)
+    capi.gemm_mxfp4(k, 1.0, ac, as_, bc, bs, 0.0, c)
+    L.sync()
+    got = c.download()
+    av, bv = mx.dequantize(*mx.quantize(a), k), mx.dequantize(*mx.quantize(b), k)
+    ref = av @ bv.T
+    assert (np.abs(got[:, -64:] - ref) <= product_bound(av, bv, k, "bf16", ref)).all()
+    one = av.sum()
+    assert (np.abs(got[:, :-64] - one) <= (k + 4) * U * np.abs(av).sum() + 2.0 ** -8 * abs(one)).all()
+
+
