@@ -370,7 +370,8 @@ int tt_gemm_mxfp4(int dtype, int64_t m, int64_t n, int64_t k, float alpha, const
  * MiB per-stream library workspace (allocated on first use) and multiplied
  * from there; without it (refused, or under graph capture before a call has left it
  * on the stream) the product quantises them as it reads them, which is slower
- * and gives the same result up to the order of its sums. */
+ * and gives the same result up to the order of its sums, for up to 2^27 - 16
+ * outputs (fout; TT_ERR_ARG beyond). */
 int tt_fc_forward_mxfp4(int dtype, int64_t batch, int64_t fin, int64_t fout, const void* in, const uint8_t* w_codes,
                         const uint8_t* w_scales, const void* bias, int bias_scalar, void* out, void* stream);
 

@@ -606,8 +606,18 @@ int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O*
   const bool once = blocks <= 512 && (row <= 4096 || M * row <= 32768);
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until the last kernel that reads the buffer is queued
-  if (once || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws))
-    return block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x, W, Ws, M, N, K, all, s);
+  if (once || fit < 16 || !lease.emplace().get_fixed(s, kWsMxfp4Rows, kMxRowsWork, &ws)) {
+    // as many rows a launch as its grid takes
+    const int64_t most = 0xffffffffu / (64 * kBlockWaves) / ((N + 15) / 16) * 16, step = most > 0 ? most : M;
+    for (int64_t r0 = 0; r0 < M; r0 += step) {
+      MxEpilogue<O> ep = all;
+      ep.C = out + r0 * N;
+      const int rc = block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x + r0 * K, W, Ws, M - r0 < step ? M - r0 : step, N, K,
+                                                 ep, s);
+      if (rc) return rc;
+    }
+    return ok();
+  }
   for (int64_t r0 = 0; r0 < M; r0 += fit) {
     const int64_t rows = M - r0 < fit ? M - r0 : fit;
     uint8_t* codes = (uint8_t*)ws;

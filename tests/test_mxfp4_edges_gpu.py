@@ -245,6 +245,35 @@ def test_attention_past_32_bit_offsets(capi):
 
 # ------------------------------------------------------------------ products of extreme and narrow shapes
 
+def test_layer_of_many_blocks_without_its_workspace(capi):
+    """65552 x 32768 outputs are more blocks of 16 x 16 than one launch takes: captured before a call has left the
+    workspace on the stream, the layer quantises its rows as it reads them, in several launches."""
+    from test_capture_gpu import Capture
+
+    m, n, k = 65552, 32768, 32
+    rng = np.random.default_rng(50)
+    f, L = capi.DeviceBuffer.from_numpy, capi.lib()
+    x, w, bias = normal(rng, (m, k), "bf16"), rng.standard_normal((n, k)), normal(rng, (n,), "bf16")
+    wc, ws = held(capi, w)
+    xb, bb, out = f(x, "bf16"), f(bias, "bf16"), capi.DeviceBuffer((m, n), "bf16")
+    L.call("tt_memset", out.ptr, 0, out.nbytes)
+    L.call("tt_empty_cache")
+    st = capi.Stream()
+    with Capture(capi, st.handle) as g:
+        capi.fc_forward_mxfp4(xb, wc, ws, bb, out, stream=st.handle)
+    g.launch()
+    g.destroy()
+    st.destroy()
+    wv = mx.dequantize(*mx.quantize(w), k)
+    rows = capi.DeviceBuffer((48, n), "bf16")
+    for r0 in (0, 32 * 1024, 65504):
+        L.call("tt_memcpy_d2d", rows.ptr, out.ptr + r0 * n * 2, rows.nbytes)
+        L.sync()
+        xv = mx.dequantize(*mx.quantize(x[r0:r0 + 48]), k)
+        ref = xv @ wv.T + bias
+        assert (np.abs(rows.download() - ref) <= product_bound(xv, wv, k, "bf16", ref, 1.0, np.abs(bias))).all()
+
+
 def test_product_of_one_row_by_more_than_2_27(capi):
     m, n, k = 1, (1 << 27) + 40, 32
     L = capi.lib()
