@@ -298,3 +298,91 @@ def test_product_of_one_row_by_more_than_2_27(capi):
     assert (np.abs(got[:, :-64] - one) <= (k + 4) * U * np.abs(av).sum() + 2.0 ** -8 * abs(one)).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(70000, 10, 64), (20000, 10, 784), (9000, 1, 100), (5, 70000, 64), (40000, 17, 33), (8192, 128, 1024)])
+def test_narrow_products(capi, m, n, k, dtype):
+    """Many rows and few columns, as a classifier's last layer has: the product and the layer."""
+    rng = np.random.default_rng(m + n)
+    x, b, bias = normal(rng, (m, k), dtype), rng.standard_normal((n, k)), normal(rng, (n,), dtype)
+    (ac, as_), (bc, bs) = held(capi, x), held(capi, b)
+    f, c = capi.DeviceBuffer.from_numpy, capi.DeviceBuffer((m, n), dtype)
+    capi.gemm_mxfp4(k, 1.0, ac, as_, bc, bs, 0.0, c)
+    capi.lib().sync()
+    av, bv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(b), k)
+    ref = av @ bv.T
+    assert (np.abs(c.download() - ref) <= product_bound(av, bv, k, dtype, ref)).all()
+    capi.fc_forward_mxfp4(f(x, dtype), bc, bs, f(bias, dtype), c)
+    capi.lib().sync()
+    ref += bias
+    assert (np.abs(c.download() - ref) <= product_bound(av, bv, k, dtype, ref, 1.0, np.abs(bias))).all()
+
+
+@pytest.mark.parametrize("m,n", [(600, 1101), (2900, 3001)])
+def test_tiles_of_no_k_are_beta_c(capi, m, n):
+    c0 = normal(np.random.default_rng(52), (m, n), "f32")
+    c = capi.DeviceBuffer.from_numpy(c0)
+    capi.lib().call("tt_gemm_mxfp4", capi.TT_F32, m, n, 0, 1.0, None, None, None, None, 0.5, c.ptr, None)
+    capi.lib().sync()
+    assert np.array_equal(c.download(), c0 * 0.5)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(3, 50, 97), (30, 50, 3000), (600, 1101, 200)])
+def test_layer_at_any_element_alignment(capi, m, n, k, dtype):
+    """in, bias and out one element into their buffers; what lies around out stays."""
+    rng = np.random.default_rng(m)
+    x, w, bias = normal(rng, (m, k), dtype), rng.standard_normal((n, k)), normal(rng, (n,), dtype)
+    wc, ws = held(capi, w)
+    f, e = capi.DeviceBuffer.from_numpy, capi.DeviceBuffer.ITEM[dtype]
+    xb, bb = f(np.concatenate(([9.0], x.ravel())).astype(np.float32), dtype), f(np.append(9.0, bias).astype(np.float32), dtype)
+    out = f(np.full(m * n + 2, 77.0, np.float32), dtype)
+    capi.lib().call("tt_fc_forward_mxfp4", capi.TT_BF16 if dtype == "bf16" else capi.TT_F32, m, k, n, xb.ptr + e, wc.ptr,
+                    ws.ptr, bb.ptr + e, 0, out.ptr + e, None)
+    capi.lib().sync()
+    got = out.download()
+    assert got[0] == got[-1] == 77.0
+    xv, wv = mx.dequantize(*mx.quantize(x), k), mx.dequantize(*mx.quantize(w), k)
+    ref = xv @ wv.T + bias
+    assert (np.abs(got[1:-1].reshape(m, n) - ref) <= product_bound(xv, wv, k, dtype, ref, 1.0, np.abs(bias))).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_at_any_element_alignment(capi, dtype):
+    """q, o and lse one element into their buffers, K and V one cache."""
+    rng = np.random.default_rng(53)
+    B, H, T, d = 2, 4, 2, 64
+    c = Cache(capi, rng, B, 2, 300, d, [300, 41])
+    c.vc, c.vs = c.kc, c.ks
+    c.upload()
+    q = normal(rng, (B, H, T, d), dtype)
+    f, e = capi.DeviceBuffer.from_numpy, capi.DeviceBuffer.ITEM[dtype]
+    qb, o = f(np.append(9.0, q.ravel()).astype(np.float32), dtype), f(np.full(q.size + 2, 77.0, np.float32), dtype)
+    lse = f(np.full(B * H * T + 2, 77.0, np.float32))
+    kc, ks = c.dev[:2]
+    capi.lib().call("tt_attn_decode_mxfp4", capi.TT_BF16 if dtype == "bf16" else capi.TT_F32, qb.ptr + e, kc.ptr, ks.ptr, kc.ptr,
+                    ks.ptr, c.len.ptr, o.ptr + e, lse.ptr + 4, B, H, 2, T, 300, d, 0.125, None)
+    capi.lib().sync()
+    o, lse = o.download(), lse.download()
+    assert o[0] == o[-1] == lse[0] == lse[-1] == 77.0
+    check_attention(c, q, dtype, 0.125, o[1:-1].reshape(q.shape), lse[1:-1].reshape(q.shape[:3]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_calls_repeat_bit_for_bit(capi, dtype):
+    """Split attention and products of every kind of tile, the same in every call."""
+    rng = np.random.default_rng(54)
+    c = Cache(capi, rng, 2, 4, 3000, 128, [3000, 1700]).upload()
+    q = normal(rng, (2, 8, 2, 128), dtype)
+    first = attend(capi, c, q, dtype, 0.1)
+    for _ in range(3):
+        again = attend(capi, c, q, dtype, 0.1)
+        assert np.array_equal(again[0], first[0]) and np.array_equal(again[1], first[1])
+    for m, n, k in ((3, 500, 2000), (300, 300, 1056), (700, 1025, 2049), (2900, 3001, 544)):
+        (ac, as_), (bc, bs) = held(capi, rng.standard_normal((m, k))), held(capi, rng.standard_normal((n, k)))
+        outs = []
+        for _ in range(3):
+            y = capi.DeviceBuffer((m, n), dtype)
+            capi.gemm_mxfp4(k, 1.0, ac, as_, bc, bs, 0.0, y)
+            capi.lib().sync()
+            outs.append(y.download())
+        assert np.array_equal(outs[1], outs[0]) and np.array_equal(outs[2], outs[0])
