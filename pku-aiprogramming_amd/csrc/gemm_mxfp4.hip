@@ -573,17 +573,24 @@ int product(const char* fn, const uint8_t* A, const uint8_t* As, const uint8_t* 
   // (16 x 16 / 32 x 32 / 128 x 128, us): 1 x 4096 x 4096 3.6 / 5.4 / 14.8 (256
   // blocks), 100 x 1000 x 500 3.5 / 3.6 / 5.5 (441), 64 x 4096 x 4096 11.0 (1024) /
   // 7.2 / 15.5, 128 x 4096 x 4096 19.9 / 11.4 (512) / 15.0, 600 x 1101 x 1000 12.5 /
-  // 10.3 (665) / 7.4, 500 x 2000 x 3000 24 / 17.1 (1008) / 12.6.  M <= 16 has nothing
-  // to gain from larger ones.
-  if (tiles(16) <= 512 || (M <= 16 && grid_fits(tiles(16), 64 * kBlockWaves))) return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
+  // 10.3 (665) / 7.4, 500 x 2000 x 3000 24 / 17.1 (1008) / 12.6.  Up to 16 rows stay
+  // with them for their long rows: 1 x 16384 x 16384 24.7 / 36.5 / 50.4, 1 x 128000 x
+  // 4096 46.5 / 47.7 / 50.5; from some 50000 columns on the tiles are the faster
+  // for several rows, 16 x 128000 x 4096 73 / 64 / 53, 10 x 70000 x 784 16.6 / 19.7 /
+  // 11.1.
+  if (tiles(16) <= 512 || (M <= 16 && grid_fits(tiles(16), 64 * kBlockWaves)))
+    return block_launch<O, 1, 1, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
   // the tiles keep the offsets of their rows in 32 bits
   const bool wide = mx_blocks(K) * kMxBlockBytes * 256 > 0xffffffffll;
   if (wide || tiles(32) <= 512) return block_launch<O, 2, 2, false>(fn, A, As, nullptr, B, Bs, M, N, K, ep, s);
-  // 128 x 128 tiles, two a CU, where one round takes them all.  Measured (128 /
-  // 256, us): 1531 x 4099 x 4096 25.3 / 32.6 (396 small tiles), 2048 x 4096 x 1000
-  // 10.3 / 13.1 (512), 2600 x 3328 x 2048 20.9 / 19.0 (546), 3500 x 3500 x 2000
-  // 29.6 / 25.1 (784), 8192 x 8192 x 8192 394 / 279.
-  if (tiles(128) <= 512) return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
+  // 128 x 128 tiles, two a CU, where one round takes them all, and where a larger
+  // one could not be filled on one side.  Measured (128 / 256, us): 1531 x 4099 x
+  // 4096 25.3 / 32.6 (396 small tiles), 2048 x 4096 x 1000 10.3 / 13.1 (512), 2600 x
+  // 3328 x 2048 20.9 / 19.0 (546), 3500 x 3500 x 2000 29.6 / 25.1 (784), 8192 x 8192 x
+  // 8192 394 / 279; 70000 x 10 x 784 13.9 / 25.0, 70000 x 128 x 1024 16.0 / 28.9, 17 x
+  // 70000 x 784 11.7 / 18.3, 128 x 131072 x 1024 22.6 / 35.3.
+  if (tiles(128) <= 512 || M <= 128 || N <= 128)
+    return tile_launch<O, 128, 128, 2, 2>(fn, A, As, B, Bs, M, N, K, ep, s);
   return tile_launch<O, 256, 256, 2, 4>(fn, A, As, B, Bs, M, N, K, ep, s);
 }
 
