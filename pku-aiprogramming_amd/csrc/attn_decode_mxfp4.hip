@@ -27,6 +27,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstring>
 #include <limits>
 #include <optional>
 #include <string>
@@ -349,7 +350,8 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
         for (uint64_t left = __ballot(j0 + 16 * u + r < kend && apart(v[u], edge)); left; left &= left - 1) {
           const int at = __builtin_ctzll(left), in = at & 15, part = at >> 4, key = j0 + 16 * u + in;
           float wgt = (in & 2) ? ((in & 1) ? s[u][3] : s[u][2]) : ((in & 1) ? s[u][1] : s[u][0]);
-          wgt = fast_exp2(__builtin_fmaf(sl2, __shfl(wgt, 16 * (in >> 2) + r, 64), -mb));  // from the lane that holds the key's
+          wgt = __shfl(wgt, 16 * (in >> 2) + r, 64);  // this row's score, from the lane that holds the key's
+          wgt = fast_exp2(__builtin_fmaf(sl2, wgt, -mb));
           const uint8_t *codes = vc + (base + key) * (16 * W), *scales = vs + (base + key) * W;
 #pragma unroll
           for (int i = 0; i < ND; ++i) {  // this lane's columns 16 i + 4 g and three more, if the piece has them
@@ -478,7 +480,8 @@ template <typename T, int D>
 int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, const uint8_t* vc, const uint8_t* vs,
            const int* lengths, T* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t tokens, int64_t cap,
            float scale, hipStream_t st) {
-  const int64_t rows = B * H * tokens, R = H / Hkv * tokens, tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
+  const int64_t rows = B * H * tokens, R = H / Hkv * tokens;
+  const int64_t tiles = (R + kMdRows - 1) / kMdRows, units = B * Hkv * tiles;
   static const int per_cu = [] {
     int n = 0;
     const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
@@ -496,7 +499,11 @@ int launch(const char* fn, const T* q, const uint8_t* kc, const uint8_t* ks, con
   if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsMxfp4Decode, kMdWork, &ws)) nsplit = 1;
   float* part_o = (float*)ws;
   float2* part_ml = (float2*)(part_o + rows * nsplit * D);
-  const float sl2 = std::max(std::fabs(scale * kLog2e), std::numeric_limits<float>::denorm_min());
+  float sl2 = std::fabs(scale * kLog2e);
+  uint32_t bits;  // 1: the smallest fp32, formed as the host's arithmetic may flush it
+  memcpy(&bits, &sl2, sizeof(bits));
+  bits = std::max(bits, 1u);
+  memcpy(&sl2, &bits, sizeof(bits));
 #define TT_MD_LAUNCH(STREAM)                                                                                          \
   hipLaunchKernelGGL((attn_decode_mxfp4_kernel<T, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, \
                      st, q, kc, ks, vc, vs, lengths, part_o, part_ml, o, lse, (uint32_t)Hkv, (uint32_t)R,             \

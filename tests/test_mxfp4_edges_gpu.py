@@ -203,6 +203,21 @@ def test_attention_of_no_scale_over_large_scores(capi, scale, dtype):
     check_attention(c, q, dtype, float(np.float32(scale)), o, lse)
 
 
+@pytest.mark.parametrize("scale", [0.0, 1e-41])
+def test_attention_of_no_scale_where_the_host_flushes_small_values(capi, scale):
+    import torch
+
+    rng = np.random.default_rng(43)
+    c = Cache(capi, rng, 2, 2, 90, 64, [90, 33]).upload()
+    q = normal(rng, (2, 4, 3, 64), "bf16")
+    assert torch.set_flush_denormal(True)
+    try:
+        o, lse = attend(capi, c, q, "bf16", scale)
+    finally:
+        torch.set_flush_denormal(False)
+    check_attention(c, q, "bf16", 0.0, o, lse)  # 10^-41 of scores below 10^3 is nothing
+
+
 def test_attention_past_32_bit_offsets(capi):
     """The third sequence's keys begin 4 GiB into the codes and end in three that hold nearly all of the weight: by an
     offset cut to 32 bits they would be rows of other sequences, which are 1 throughout."""
