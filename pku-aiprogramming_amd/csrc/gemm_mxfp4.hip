@@ -619,8 +619,8 @@ int fc(const char* fn, const O* x, const uint8_t* W, const uint8_t* Ws, const O*
     for (int64_t r0 = 0; r0 < M; r0 += step) {
       MxEpilogue<O> ep = all;
       ep.C = out + r0 * N;
-      const int rc = block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x + r0 * K, W, Ws, M - r0 < step ? M - r0 : step, N, K,
-                                                 ep, s);
+      const int64_t rows = M - r0 < step ? M - r0 : step;
+      const int rc = block_launch<O, 1, 1, true>(fn, nullptr, nullptr, x + r0 * K, W, Ws, rows, N, K, ep, s);
       if (rc) return rc;
     }
     return ok();
