@@ -401,3 +401,19 @@ def test_calls_repeat_bit_for_bit(capi, dtype):
             capi.lib().sync()
             outs.append(y.download())
         assert np.array_equal(outs[1], outs[0]) and np.array_equal(outs[2], outs[0])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(3, 50, 97), (100, 70, 300), (30, 50, 3000), (600, 1101, 200)])
+def test_layer_of_nan_and_infinite_inputs(capi, m, n, k, dtype):
+    """Quantised in the product or before it: such an input makes its own row NaN, and an infinite bias its column infinite."""
+    rng = np.random.default_rng(m + 1)
+    x, w, bias = normal(rng, (m, k), dtype), rng.standard_normal((n, k)), normal(rng, (n,), dtype)
+    x[0, k - 1], x[m - 1, 0], bias[3] = np.nan, -np.inf, np.inf
+    wc, ws = held(capi, w)
+    f, out = capi.DeviceBuffer.from_numpy, capi.DeviceBuffer((m, n), dtype)
+    capi.fc_forward_mxfp4(f(x, dtype), wc, ws, f(bias, dtype), out)
+    capi.lib().sync()
+    got = out.download()
+    assert np.isnan(got[[0, m - 1]]).all() and np.isposinf(got[1:-1, 3]).all()
+    assert np.isfinite(np.delete(got[1:-1], 3, 1)).all()
