@@ -20,9 +20,11 @@
 //     weights shows in the result.
 // The codes of the next step are in flight meanwhile.  The waves of a workgroup
 // meet in LDS at the end, and splits of the keys over workgroups in a second
-// launch.  Measured: 64 x 32 heads x 8192 keys of 128, bf16, 353 us (6.5 TB/s); 16 x 8
-// heads x 16383 keys 54 us (5.3); 1 x 32 heads x 4097 keys 11.3 us, of which the
-// second launch 2 to 3.
+// launch.  Measured: 64 x 32 heads x 8192 keys of 128, bf16, 356 us (6.4 TB/s),
+// fp32 402; 16 x 8 heads x 16383 keys 51.5 us (5.5 TB/s); 1 x 32 heads x 4097 keys
+// 11.0 us, of which the second launch 2 to 3.  A long prompt's tokens are right, but
+// not what this is made for: every 16 rows convert all keys again, and 512 tokens
+// of 32 / 8 heads over 8192 keys take 151 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -65,9 +67,9 @@ struct MdPiece {
 };
 // codes and scales: the first row of a step, alike in all lanes; row: this lane's
 // from there.  STREAM: codes that no other workgroup reads are loaded
-// non-temporally (64 x 32 heads x 8192 keys 398 -> 360 us); those that a second
-// tile of query rows reads too are better kept (2 x 8 x 16383 keys, 20 tokens: 20.9
-// against 22.9).
+// non-temporally (64 x 32 heads x 8192 keys 391 -> 359 us); those that a second
+// tile of query rows reads too are better kept (2 x 8 x 16383 keys, 20 tokens: 18.5
+// against 19.3).
 template <bool STREAM, int W>
 __device__ __forceinline__ void md_load(MdPiece<W>& p, const uint8_t* codes, const uint8_t* scales, uint32_t row,
                                         int g) {
@@ -452,9 +454,9 @@ constexpr size_t kMdWork = size_t(24) << 20;  // the partials' scratch, of one s
 // kMdFixed more (its queries, the meeting of its waves), a CU's time goes by the
 // workgroups that fall to it, up to per_cu of them at once, of which fewer keep
 // less of memory's latency covered, and splits cost the second launch, about
-// kMdMerge keys.  Measured (d = 128 bf16, 256 CUs, three at once, us): 16 x 8 heads x
-// 16383 keys in 3 / 4 / 5 / 6 splits (1.5, 2, 2.5, 3 a CU) 62 / 55 / 60 / 54, 20 x 8
-// heads in 3 / 4 / 5 68 / 74 / 82, 64 x 32 heads x 8192 keys in 1 / 3 350 / 366.
+// kMdMerge keys.  Measured (d = 128 bf16, 256 CUs, us): 16 x 8 heads x 16383 keys
+// in 3 / 4 / 5 / 6 splits (1.5, 2, 2.5, 3 a CU) 58.5 / 51.1 / 57.4 / 52.3, 20 x 8 heads in
+// 3 / 4 / 5 63.9 / 72.2 / 75.0, 64 x 32 heads x 8192 keys in 1 / 3 358 / 358.
 constexpr int64_t kMdFixed = 150, kMdMerge = 300;
 inline int64_t md_splits(int64_t units, int64_t keys, int64_t per_cu, int64_t cus, int64_t d, int64_t most) {
   constexpr int64_t step = kMdWaves * kMdKeys;

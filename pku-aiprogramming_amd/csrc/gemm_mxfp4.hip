@@ -303,10 +303,12 @@ __device__ __forceinline__ const uint8_t* uniform_ptr(const uint8_t* p) {
 // across the barrier of the next stage.  Rows past M or N repeat the last one and
 // are not stored.  The matrix unit takes B's rows first, so a lane ends with runs
 // of four consecutive columns of one row of C.
-// Measured, bf16: 8192 x 8192 x 8192 280 us, 3.9 PFLOP/s (222 us of constant codes:
-// the board's power holds it back), 4096 x 4096 x 4096 40 us, 3.5 PFLOP/s, 2048 x
-// 4096 x 1000 (128 x 128 tiles) 10.3 us, 1.6 PFLOP/s.  Of a stage's cycles the matrix
-// unit needs 1024, the LDS 768 for operand reads and 256 for its fills.
+// Measured, bf16: 8192 x 8192 x 8192 287 to 300 us, 3.7 to 3.8 PFLOP/s, 4096 x 4096 x
+// 4096 41 us, 3.4 PFLOP/s, 2048 x 4096 x 1000 (128 x 128 tiles) 10.5 us, 1.6 PFLOP/s.
+// Of constant codes, which the board's power does not hold back, 8192 x 8192 x 8192
+// takes 224 us where the bare matrix unit would take 117: of a stage's cycles that
+// unit needs 1024, the LDS 768 for operand reads and 256 for its fills, and after
+// each barrier all waves read, load and multiply in step, so these add up in part.
 constexpr int kStageBlocks = 4, kStageBytes = kStageBlocks * kMxBlockBytes, kStages = 4;
 
 template <typename O, int BM, int BN, int WM, int WN>

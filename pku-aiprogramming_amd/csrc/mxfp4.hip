@@ -103,7 +103,9 @@ __global__ __launch_bounds__(kMxThreads) void k_mxfp4_rows(T* x, typename MxWord
 // result takes its column r): a layer's weight [fin, fout], laid out once for
 // the product.  A lane takes one block of one row, 32 loads that are
 // contiguous over the wave; the four waves of a workgroup take neighbouring
-// blocks, so that their 16-byte stores fill whole 64-byte runs.
+// blocks, so that their 16-byte stores fill whole 64-byte runs.  Each load of a
+// wave takes 128 bytes of bf16 or 256 of fp32, which bounds it: 8192 x 8192 in 59 us
+// (2.9 TB/s) or 83 us (3.7), 4096 x 11008 in 37 or 53, once a weight.
 template <typename T>
 __global__ __launch_bounds__(kMxThreads) void k_mxfp4_columns(const T* __restrict__ x, uint4* __restrict__ codes,
                                                               uint8_t* __restrict__ scales, int64_t rows, int64_t cols,
