@@ -349,7 +349,8 @@ int tt_col_sum(int dtype, const void* x, void* y, int64_t rows, int64_t cols, vo
 /* x [rows][cols] (trans = 0) to codes and scales; with trans = 1, x is stored
  * [cols][rows] and row r of the result takes its column r (a layer's weight
  * [fin][fout] to the [fout][fin] that the product takes).  dtype TT_F32 or
- * TT_BF16, x at any element alignment. */
+ * TT_BF16, x at any element alignment.  trans = 1 takes fewer than 2^24 pieces of
+ * 64 rows by 128 columns (TT_ERR_ARG otherwise). */
 int tt_mxfp4_quantize(int dtype, int trans, const void* x, uint8_t* codes, uint8_t* scales, int64_t rows,
                       int64_t cols, void* stream);
 /* The values y [rows][cols] that codes and scales stand for, exact in

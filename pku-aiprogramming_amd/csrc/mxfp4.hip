@@ -207,7 +207,6 @@ template <typename T>
 int columns_launch(const char* fn, const T* x, uint8_t* codes, uint8_t* scales, int64_t rows, int64_t cols,
                    hipStream_t s) {
   const int64_t nb = mx_blocks(cols), row_tiles = (rows + 63) / 64;
-  if (!grid_fits(row_tiles * ((nb + 3) / 4), kMxThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too large");
   hipLaunchKernelGGL(k_mxfp4_columns<T>, dim3((unsigned)(row_tiles * ((nb + 3) / 4))), dim3(kMxThreads), 0, s, x,
                      (uint4*)codes, scales, rows, cols, nb, row_tiles);
   TT_LAUNCHED(fn, s);
@@ -259,6 +258,8 @@ extern "C" int tt_mxfp4_quantize(int dtype, int trans, const void* x, uint8_t* c
   if (rc) return rc;
   if (trans != 0 && trans != 1) return fail(TT_ERR_ARG, std::string(fn) + ": trans must be 0 or 1");
   if (rows == 0 || cols == 0) return ok();
+  if (trans && !grid_fits((rows + 63) / 64 * ((mx_blocks(cols) + 3) / 4), kMxThreads))
+    return fail(TT_ERR_ARG, std::string(fn) + ": too large");
   const size_t nb = (size_t)(rows * mx_blocks(cols)), e = dtype == TT_F32 ? 4 : 2;
   if ((rc = check_no_overlap(fn, {{x, (size_t)rows * cols * e, "x"}},
                              {{codes, nb * kMxBlockBytes, "codes"}, {scales, nb, "scales"}})))

@@ -224,3 +224,15 @@ def test_attention_size_refusals(capi):
     for B, H, Hkv, T in (((1 << 24) - 1, 1, 1, 1), (1 << 22, 4, 1, 4), (1, 1, 1, (1 << 28) - 16), (1 << 9, 1 << 9, 1, 1023)):
         assert L.lib.tt_attn_decode_mxfp4(capi.TT_BF16, *a, B, H, Hkv, T, 8, 32, 0.1, None) == capi.TT_ERR_ARG
         assert "null pointer" in L.last_error()  # the sizes are taken
+
+
+def test_transposed_size_refusals(capi):
+    """Fewer than 2^24 pieces of 64 rows by 128 columns; no such limit for rows as they are stored."""
+    L, F = capi.lib(), capi.TT_F32
+    q = L.lib.tt_mxfp4_quantize
+    overlap = (P[0], P[0], P[1])  # refused once the sizes are taken
+    for rows, cols in ((1, (1 << 31) - 1), (1 << 20, 1 << 17)):
+        assert q(F, 1, *overlap, rows, cols, None) == capi.TT_ERR_ARG and "too large" in L.last_error()
+        assert q(F, 0, *overlap, rows, cols, None) == capi.TT_ERR_ARG and "overlap" in L.last_error()
+    for rows, cols in ((1, (1 << 31) - 128), ((1 << 20) - 64, 1 << 17)):
+        assert q(F, 1, *overlap, rows, cols, None) == capi.TT_ERR_ARG and "overlap" in L.last_error()
