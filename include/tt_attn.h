@@ -398,7 +398,8 @@ int tt_kv_append_mxfp4(int dtype, const void* k, const void* v, uint8_t* k_codes
  * below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an unsplit call,
  * below 2^24 (TT_ERR_ARG otherwise).  K and V enter with their 4-bit values,
  * scores, weights and sums in fp32, of which the weights of bf16 calls keep 16
- * bits (2^-17 off) where they meet V.  Few heads split the keys over
+ * bits (2^-17 off) where they meet V.  The sums are divided last, so values of V
+ * that add up to 2^128 under weights of up to one overflow.  Few heads split the keys over
  * workgroups and merge their sums through a fixed 24 MiB per-stream library
  * workspace (allocated on first use); without it (refused, or under graph
  * capture before a call has left it on the stream) they run unsplit. */
