@@ -161,8 +161,10 @@ __device__ __forceinline__ float md_lse(float m, float den) {
 // Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv,
 // tile = 16 of the head's R query rows.  Each sequence's own length is cut into
 // nsplit spans, so that sequences of any length keep every workgroup busy.
+// Eight workgroups a CU of d = 32 bf16 keep its vector work busy: 64 x 32 heads x
+// 8192 keys 143 us, with seven 147; the others' registers are let be.
 template <typename T, int D, bool STREAM>
-__global__ __launch_bounds__(kMdThreads, 3) void attn_decode_mxfp4_kernel(
+__global__ __launch_bounds__(kMdThreads, sizeof(T) == 2 && D == 32 ? 8 : 3) void attn_decode_mxfp4_kernel(
     const T* __restrict__ q, const uint8_t* __restrict__ kc, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vc, const uint8_t* __restrict__ vs, const int* __restrict__ lengths,
     float* __restrict__ part_o, float2* __restrict__ part_ml, T* __restrict__ o, float* __restrict__ lse,
