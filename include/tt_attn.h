@@ -43,8 +43,8 @@ enum {
   TT_ERR_NOMEM = 4        /* device allocation failed */
 };
 
-/* dtype codes for the generic entry points */
-enum { TT_F32 = 0, TT_F64 = 1, TT_I32 = 2, TT_BF16 = 3 };
+/* dtype codes for the generic entry points; TT_E4M3 (8-bit codes) for caches alone */
+enum { TT_F32 = 0, TT_F64 = 1, TT_I32 = 2, TT_BF16 = 3, TT_E4M3 = 4 };
 
 /* ---------------------------------------------------------------- runtime */
 
@@ -407,6 +407,112 @@ int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_codes, const
                          const uint8_t* v_codes, const uint8_t* v_scales, const int* lengths, void* o, float* lse,
                          int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t cap, int64_t d, float scale,
                          void* stream);
+
+/* ---------------------------------------------------------------- norms of heads, position rotation */
+
+/* What lies between a projection and attention (no counterpart in the
+ * reference): queries and keys normed over each head, rotated by their
+ * positions and laid out as tt_attn_* take them, in one pass.
+ *
+ * q holds B T rows of H heads of d values: head-major [B][H][T][d] (ldq = 0),
+ * or token-major with ldq values from token to token (heads side by side: ldq
+ * is at least H d; q, k and v may be parts of one fused projection).  k and v
+ * have Hkv heads.  Outputs are [B][heads][T][d].  Each of q, k, v may be null
+ * together with its output; v is moved, not changed.
+ *
+ * q_weight, k_weight [d] (float; null: not normed): x / sqrt(mean x^2 + eps)
+ * weight, over each head.  inv_freq [rot / 2] (float; null: not rotated), rot a
+ * multiple of 16 of at most d: at position p, pair i turns by the angle p
+ * inv_freq[i], (a, b) -> (a cos - b sin, a sin + b cos).  Pair i is elements i and
+ * i + rot / 2, or 2 i and 2 i + 1 where interleaved is 1; elements from rot on
+ * stay.  The position is positions[b][t] if given, else lengths[b] - T + t if
+ * lengths are (the T newest of a sequence, as the caches have it), else t; all
+ * of these arrays are on the device.  Angles are formed and reduced in 64
+ * bits, so positions of any size turn by what they say; all else is in fp32 and
+ * rounded once.  x^2 must not overflow.  dtype TT_F32 or TT_BF16; d 32, 64 or
+ * 128; pointers to values are 16-byte aligned and leading dimensions a multiple of
+ * 16 bytes (TT_ERR_ARG otherwise).  B T is below 2^31 - 256. */
+int tt_qkv_norm_rope(int dtype, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv,
+                     const float* q_weight, const float* k_weight, float eps, const float* inv_freq, int64_t rot,
+                     int interleaved, const int* positions, const int* lengths, void* q_out, void* k_out, void* v_out,
+                     int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, void* stream);
+/* Its gradients: dq_out, dk_out, dv_out [B][heads][T][d] to dq, dk, dv, which
+ * lie as q, k and v do (lddq, lddk, lddv; the parts of one fused gradient may lie
+ * between each other's rows), and to the weights' dq_weight, dk_weight [d] (float,
+ * may be null), sums over all rows in a fixed order.  q and k are what the
+ * forward call read, and may be null where they were not normed.  With no rows
+ * the weights' gradients are zero.  These sums meet in a fixed 1 MiB per-stream
+ * library workspace (allocated on first use); without it (refused, or under graph
+ * capture before a call has left it on the stream) a call that asks for them
+ * fails with TT_ERR_NOMEM. */
+int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t ldq, int64_t ldk, const float* q_weight,
+                              const float* k_weight, float eps, const float* inv_freq, int64_t rot, int interleaved,
+                              const int* positions, const int* lengths, const void* dq_out, const void* dk_out,
+                              const void* dv_out, void* dq, void* dk, void* dv, int64_t lddq, int64_t lddk,
+                              int64_t lddv, float* dq_weight, float* dk_weight, int64_t B, int64_t H, int64_t Hkv,
+                              int64_t T, int64_t d, void* stream);
+
+/* ---------------------------------------------------------------- paged K/V cache */
+
+/* A K/V cache in pages of 16, 32, 64 or 128 tokens that sequences need not
+ * reserve: pools k_pages and v_pages [npages][Hkv][page][d], and a table
+ * [B][width] (int, on the device) of each sequence's pages.  Key j of sequence b
+ * is row j % page of page table[b][j / page].  lengths (int, on the device) holds
+ * each sequence's number of keys, the T newest tokens included: token t of them is
+ * key lengths[b] - T + t and sees the keys up to itself, as in the 4-bit cache.
+ * A place of the table that names no page of the pool (a negative number, or one
+ * from npages on) holds no keys: nothing is stored there or read, and its keys are
+ * not seen.  So do keys from width page on.
+ *
+ * The pools hold values of `dtype` (cache = dtype), or 8-bit codes (cache =
+ * TT_E4M3: sign, four exponent bits, three fraction bits, up to 448; 0x7f and
+ * 0xff are NaN) under scale bytes k_scales and v_scales [npages][Hkv], one for each
+ * page and head, that stand for 2^(byte - 127): the smallest power of two, of
+ * 2^-124 to 2^119, that takes the page's largest value to at most 448.  Values
+ * are rounded to nearest, halves to even; infinities and NaN become NaN and do
+ * not count for the scale.  The scales are null for other caches.  Pools are
+ * 16-byte aligned (TT_ERR_ARG otherwise), d is 32, 64 or 128. */
+
+/* Append: the new tokens' k and v, [B][Hkv][T][d] or token-major (ldk, ldv as
+ * above), K normed (k_weight) and rotated (inv_freq) on the way as by
+ * tt_qkv_norm_rope, at its key's place in the sequence unless positions [B][T] say
+ * otherwise.  A token whose key is negative is not stored, so a batch of prompts
+ * padded on the left needs no mask.  Rows that no token goes to stay as they are,
+ * but for 8-bit pages that gain a larger value: their older tokens are rounded
+ * again to the new scale (exactly, save what falls below its smallest steps).  A
+ * page whose first row is among the new ones takes its scale from the new
+ * tokens alone, whatever it held before.  K goes into 8 bits from 64-bit
+ * arithmetic, so that every code is the nearest one.  A page that new tokens go
+ * to belongs to one sequence: calls in which two tokens meet in one row, or two
+ * sequences in one 8-bit page, have no defined result there. */
+int tt_kv_append_paged(int dtype, int cache, const void* k, const void* v, int64_t ldk, int64_t ldv,
+                       const float* k_weight, float eps, const float* inv_freq, int64_t rot, int interleaved,
+                       const int* positions, void* k_pages, void* v_pages, uint8_t* k_scales, uint8_t* v_scales,
+                       const int* table, const int* lengths, int64_t B, int64_t Hkv, int64_t T, int64_t d,
+                       int64_t npages, int64_t page, int64_t width, void* stream);
+/* The cache read back to contiguous k, v [B][Hkv][L][d] of `dtype`: keys 0 to
+ * min(lengths[b], L) - 1 of each sequence, exactly; other rows are left as they
+ * are.  For tt_attn_* over a cached prefix, or to move a sequence. */
+int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
+                       const uint8_t* v_scales, const int* table, const int* lengths, void* k, void* v, int64_t B,
+                       int64_t Hkv, int64_t L, int64_t d, int64_t npages, int64_t page, int64_t width, void* stream);
+/* Attention of the T newest tokens over the cache: q, o [B][H][T][d] of `dtype`
+ * (16-byte aligned), H a multiple of Hkv (query head h reads K/V head h / (H /
+ * Hkv)), lse [B][H][T] (float, natural log, may be NULL).  A token that sees no
+ * key gets o = 0 and lse = -inf.  Rows that no token sees are not used, whatever
+ * they hold; an infinite or NaN value of V reaches the tokens that see its key
+ * and no others.  Scores, weights and sums are in fp32, of which the weights of
+ * bf16 calls keep 16 bits (2^-17 off) where they meet V; the sums are divided
+ * last.  B H T is below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an
+ * unsplit call, below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over
+ * workgroups and merge their sums through a fixed 24 MiB per-stream library
+ * workspace (allocated on first use); without it (refused, or under graph
+ * capture before a call has left it on the stream) they run unsplit.  Graphs
+ * captured on one stream share it and must be replayed in stream order. */
+int tt_attn_decode_paged(int dtype, int cache, const void* q, const void* k_pages, const void* v_pages,
+                         const uint8_t* k_scales, const uint8_t* v_scales, const int* table, const int* lengths,
+                         void* o, float* lse, int64_t B, int64_t H, int64_t Hkv, int64_t T, int64_t d, int64_t npages,
+                         int64_t page, int64_t width, float scale, void* stream);
 
 /* ---------------------------------------------------------------- convolution data movement */
 

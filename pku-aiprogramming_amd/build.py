@@ -30,13 +30,16 @@ OBJ = os.path.join(HERE, "_build")
 INCLUDE = os.path.join(ROOT, "include")
 
 HIP_SOURCES = ["tt_runtime.hip", "attn_fwd.hip", "attn_bwd.hip", "attn_bwd_w64.hip", "attn_decode.hip", "softmax.hip",
-               "gemm.hip", "staging.hip", "conv.hip", "mxfp4.hip", "gemm_mxfp4.hip", "attn_decode_mxfp4.hip"]
+               "gemm.hip", "staging.hip", "conv.hip", "mxfp4.hip", "gemm_mxfp4.hip", "attn_decode_mxfp4.hip",
+               "norm_rope.hip", "kv_paged.hip", "attn_decode_paged.hip"]
 # Per-file extra flags.  attn_bwd_w64.hip keeps its dK / dV accumulators in
 # AGPRs by inline asm and needs its builtin MFMAs (scores) to write VGPRs;
 # attn_decode_mxfp4.hip rescales its accumulators often, and with them in AGPRs
-# moved each of them there and back in every step (72 of 300 vector operations).
+# moved each of them there and back in every step (72 of 300 vector operations);
+# attn_decode_paged.hip likewise.
 HIP_FILE_FLAGS = {"attn_bwd_w64.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
-                  "attn_decode_mxfp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
+                  "attn_decode_mxfp4.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+                  "attn_decode_paged.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]}
 # Host-only C++ linked into libtt_hip.so (the staged transfers' copy loops).
 LIB_HOST_SOURCES = ["host_copy.cpp"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")

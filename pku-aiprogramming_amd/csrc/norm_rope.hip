@@ -1,0 +1,526 @@
+// From a projection's output to the q, k and v that attention takes, and back:
+// queries and keys normed over each head and rotated by their positions, in one
+// pass that also moves token-major rows to [B][H][T][D] (rope.h has the formulas).
+//
+// Each value is read and written once with some ten operations, so the bytes bound
+// it: 2 e a value forward, 3 e backward.  The angles are not stored: a thread keeps
+// one token's N pairs and goes through a run of heads, so that its sines and cosines,
+// formed from 64-bit angles, serve them all.
+//
+// Backward, of y = R (x r w) with r = 1 / sqrt(mean x^2 + eps), n = x r, g = R^T dy:
+//   dw = sum over rows of g n,   dx = r (g w - n mean(g w n)).
+// r is formed again from x, which is read anyway.  A thread sums its rows' g n in
+// registers, a workgroup its threads' in LDS, a second launch the workgroups' in the
+// order of their numbers, so the result does not depend on which ends first.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <optional>
+#include <string>
+
+#include "attn_tiles.h"
+#include "rope.h"
+#include "tt_internal.h"
+
+namespace tt {
+namespace {
+
+constexpr int kNrThreads = 256;
+
+// q, k or v: rows of `heads` heads, token-major with `ld` values a token, or
+// head-major [B][heads][T][D] (ld = 0).
+template <typename T>
+struct NrPart {
+  const T* x;
+  T* y;
+  const float* w;  // null: not normed
+  int64_t ld;
+  int heads;
+};
+
+template <typename T, int D>
+struct NrRow {
+  static constexpr int N = Chunk<T>::N;
+  uint4 a, b;
+  __device__ __forceinline__ void load(const T* row, const Lay<N>& lay) {
+    a = ldg16(row + lay.a);
+    b = ldg16(row + lay.b);
+  }
+  __device__ __forceinline__ void get(float (&f)[2 * N]) const {
+    Chunk<T>::get(a, f);
+    Chunk<T>::get(b, f + N);
+  }
+};
+template <typename T, int N>
+__device__ __forceinline__ void nr_store(T* row, const Lay<N>& lay, const float (&f)[2 * N]) {
+  *reinterpret_cast<uint4*>(row + lay.a) = Chunk<T>::put(f);
+  *reinterpret_cast<uint4*>(row + lay.b) = Chunk<T>::put(f + N);
+}
+template <int N>
+__device__ __forceinline__ void nr_weight(const float* w, const Lay<N>& lay, float (&f)[2 * N]) {
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    f[e] = w ? w[lay.a + e] : 1.f;
+    f[N + e] = w ? w[lay.b + e] : 1.f;
+  }
+}
+template <int N, int LPR>
+__device__ __forceinline__ float nr_scale(const float (&f)[2 * N], float eps) {
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 2 * N; ++e) ss += f[e] * f[e];
+  return __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * (1.f / (2 * N * LPR)) + eps);
+}
+
+// A workgroup: 256 / LPR tokens, heads [first, first + count) of q's, k's and v's in a row.
+template <typename T, int D>
+__global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_kernel(NrPart<T> q, NrPart<T> k, NrPart<T> v, Rope rp,
+                                                                   uint32_t rows, uint32_t tokens, uint32_t chunks,
+                                                                   int count) {
+  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR, UN = 2;
+  const uint32_t tile = blockIdx.x / chunks;
+  const int first = (int)(blockIdx.x - tile * chunks) * count;
+  const uint32_t n = tile * TPB + threadIdx.x / LPR;
+  if (n >= rows) return;  // whole rows of lanes
+  const uint32_t b = n / tokens, t = n - b * tokens;
+  const Lay<N> lay(threadIdx.x % LPR, rp.freq ? rp.rot : 0, rp.inter != 0);
+  float c[N], s[N];
+  if (lay.turns && first < q.heads + k.heads)
+    rope_angles<N>(rp.freq + lay.pair, rope_position(rp, b, t, tokens), c, s);
+
+  int at = first;  // heads of the parts before this one lie behind it
+  auto part = [&](const NrPart<T>& p, bool turn) {
+    const int lo = max(at, 0), hi = min(at + count, p.heads);
+    at -= p.heads;
+    if (lo >= hi) return;
+    const T* x = p.ld ? p.x + (int64_t)n * p.ld : p.x + ((int64_t)b * p.heads * tokens + t) * D;
+    T* y = p.y + ((int64_t)b * p.heads * tokens + t) * D;
+    const int64_t xs = p.ld ? D : (int64_t)tokens * D, ys = (int64_t)tokens * D;
+    float w[2 * N];
+    if (turn) nr_weight<N>(p.w, lay, w);
+    for (int h = lo; h < hi; h += UN) {
+      NrRow<T, D> r[UN];
+#pragma unroll
+      for (int u = 0; u < UN; ++u)
+        if (h + u < hi) r[u].load(x + (h + u) * xs, lay);
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        if (h + u >= hi) break;
+        T* to = y + (h + u) * ys;
+        if (!turn || (!p.w && !lay.turns)) {
+          *reinterpret_cast<uint4*>(to + lay.a) = r[u].a;
+          *reinterpret_cast<uint4*>(to + lay.b) = r[u].b;
+          continue;
+        }
+        float f[2 * N];
+        r[u].get(f);
+        if (p.w) {
+          const float scale = nr_scale<N, LPR>(f, rp.eps);
+#pragma unroll
+          for (int e = 0; e < 2 * N; ++e) f[e] *= scale * w[e];
+        }
+        if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
+        nr_store<T, N>(to, lay, f);
+      }
+    }
+  };
+  part(q, true);
+  part(k, true);
+  part(v, false);
+}
+
+// A part on its way back: its gradient dy is head-major, dx lies as x does.
+template <typename T>
+struct NrBack {
+  const T* x;
+  const T* dy;
+  T* dx;
+  const float* w;
+  int64_t ldx, ld;  // of x and of dx
+  int heads;
+};
+
+// A workgroup: tiles slot, slot + slots, ... of 256 / LPR tokens, a run of heads.
+// part [slots chunks][2][D], or null where no weight's gradient is asked for.
+template <typename T, int D>
+__global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T> q, NrBack<T> k, NrBack<T> v, Rope rp,
+                                                                       uint32_t rows, uint32_t tokens, uint32_t chunks,
+                                                                       uint32_t slots, int count,
+                                                                       float* __restrict__ sums) {
+  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR, UN = 2;
+  const uint32_t slot = blockIdx.x / chunks;
+  const int first = (int)(blockIdx.x - slot * chunks) * count;
+  const uint32_t tiles = (rows + TPB - 1) / TPB;
+  const Lay<N> lay(threadIdx.x % LPR, rp.freq ? rp.rot : 0, rp.inter != 0);
+  float acc[2][2 * N];
+#pragma unroll
+  for (int e = 0; e < 2 * N; ++e) acc[0][e] = acc[1][e] = 0.f;
+
+  for (uint32_t tile = slot; tile < tiles; tile += slots) {
+    const uint32_t n = tile * TPB + threadIdx.x / LPR;
+    if (n >= rows) break;  // whole rows of lanes, and the last tile
+    const uint32_t b = n / tokens, t = n - b * tokens;
+    float c[N], s[N];
+    if (lay.turns && first < q.heads + k.heads) {
+      rope_angles<N>(rp.freq + lay.pair, rope_position(rp, b, t, tokens), c, s);
+#pragma unroll
+      for (int i = 0; i < N; ++i) s[i] = -s[i];
+    }
+    int at = first;
+    auto part = [&](const NrBack<T>& p, bool turn, float (&sum)[2 * N]) {
+      const int lo = max(at, 0), hi = min(at + count, p.heads);
+      at -= p.heads;
+      if (lo >= hi) return;
+      const int64_t base = ((int64_t)b * p.heads * tokens + t) * D, ys = (int64_t)tokens * D;
+      const T* x = p.ldx ? p.x + (int64_t)n * p.ldx : p.x + base;
+      T* dx = p.ld ? p.dx + (int64_t)n * p.ld : p.dx + base;
+      const T* dy = p.dy + base;
+      const int64_t xs = p.ldx ? D : ys, ds = p.ld ? D : ys;
+      float w[2 * N];
+      if (turn) nr_weight<N>(p.w, lay, w);
+      for (int h = lo; h < hi; h += UN) {
+        NrRow<T, D> r[UN], g[UN];
+#pragma unroll
+        for (int u = 0; u < UN; ++u)
+          if (h + u < hi) {
+            g[u].load(dy + (h + u) * ys, lay);
+            if (p.w) r[u].load(x + (h + u) * xs, lay);
+          }
+#pragma unroll
+        for (int u = 0; u < UN; ++u) {
+          if (h + u >= hi) break;
+          T* to = dx + (h + u) * ds;
+          if (!turn || (!p.w && !lay.turns)) {
+            *reinterpret_cast<uint4*>(to + lay.a) = g[u].a;
+            *reinterpret_cast<uint4*>(to + lay.b) = g[u].b;
+            continue;
+          }
+          float f[2 * N];
+          g[u].get(f);
+          if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
+          if (p.w) {
+            float z[2 * N];
+            r[u].get(z);
+            const float scale = nr_scale<N, LPR>(z, rp.eps);
+            float m = 0.f;
+#pragma unroll
+            for (int e = 0; e < 2 * N; ++e) {
+              z[e] *= scale;
+              sum[e] += f[e] * z[e];
+              f[e] *= w[e];
+              m += f[e] * z[e];
+            }
+            m = row_sum<LPR>(m) * (1.f / D);
+#pragma unroll
+            for (int e = 0; e < 2 * N; ++e) f[e] = scale * (f[e] - z[e] * m);
+          }
+          nr_store<T, N>(to, lay, f);
+        }
+      }
+    };
+    part(q, true, acc[0]);
+    part(k, true, acc[1]);
+    part(v, false, acc[1]);
+  }
+  if (!sums) return;
+  __shared__ float s_sum[kNrThreads / 64][2][D];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int e = 0; e < 2 * N; ++e) {
+      float x = acc[i][e];
+#pragma unroll
+      for (int off = LPR; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
+      if ((threadIdx.x & 63) < LPR) s_sum[threadIdx.x >> 6][i][(e < N ? lay.a : lay.b - N) + e] = x;
+    }
+  __syncthreads();
+  for (int i = threadIdx.x; i < 2 * D; i += kNrThreads) {
+    float x = 0.f;
+#pragma unroll
+    for (int w = 0; w < kNrThreads / 64; ++w) x += s_sum[w][0][i];
+    sums[(int64_t)blockIdx.x * (2 * D) + i] = x;
+  }
+}
+
+// dw[i] = the sum of column i of sums [n][2 D], 16 columns a workgroup of 1024 threads.
+constexpr int kNrSumThreads = 1024;
+template <int D>
+__global__ __launch_bounds__(kNrSumThreads) void norm_weight_sum_kernel(const float* __restrict__ sums,
+                                                                        float* __restrict__ dwq,
+                                                                        float* __restrict__ dwk, int n) {
+  constexpr int G = kNrSumThreads / 16;
+  __shared__ float s_sum[G][17];
+  const int col = blockIdx.x * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4;
+  float x = 0.f;
+#pragma unroll 4
+  for (int i = g; i < n; i += G) x += sums[(int64_t)i * (2 * D) + col];
+  s_sum[g][threadIdx.x & 15] = x;
+  __syncthreads();
+  for (int half = G / 2; half > 0; half >>= 1) {
+    if (g < half) s_sum[g][threadIdx.x & 15] += s_sum[g + half][threadIdx.x & 15];
+    __syncthreads();
+  }
+  if (g) return;
+  float* to = col < D ? dwq : dwk;
+  if (to) to[col % D] = s_sum[0][threadIdx.x];
+}
+
+// Workgroups that leave sums behind, and their scratch: of one size, so that graphs may keep its address.
+constexpr int64_t kNrSums = 1024;
+constexpr size_t kNrWork = size_t(kNrSums) * 2 * 128 * sizeof(float);
+
+// How the heads are cut: a workgroup goes through as many as leave some eight
+// workgroups a CU, for the angles that it forms once.
+inline int64_t nr_chunks(int64_t tiles, int64_t heads) {
+  const int64_t want = (8 * (int64_t)device_cu_count() + tiles - 1) / tiles;
+  return std::min(std::max<int64_t>(want, 1), heads);
+}
+
+struct NrShape {
+  int64_t B, H, Hkv, T, d;
+};
+
+template <typename T, int D>
+int forward_launch(const char* fn, NrPart<T> q, NrPart<T> k, NrPart<T> v, const Rope& rp, const NrShape& n,
+                   hipStream_t st) {
+  constexpr int TPB = kNrThreads / (D / (2 * Chunk<T>::N));
+  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = q.heads + k.heads + v.heads;
+  const int64_t count = (heads + nr_chunks(tiles, heads) - 1) / nr_chunks(tiles, heads);
+  const int64_t chunks = (heads + count - 1) / count;
+  if (!grid_fits(tiles * chunks, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+  hipLaunchKernelGGL((qkv_norm_rope_kernel<T, D>), dim3((unsigned)(tiles * chunks)), dim3(kNrThreads), 0, st, q, k, v,
+                     rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)chunks, (int)count);
+  TT_LAUNCHED(fn, st);
+  return ok();
+}
+
+template <typename T, int D>
+int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const Rope& rp, float* dwq, float* dwk,
+                    const NrShape& n, hipStream_t st) {
+  constexpr int TPB = kNrThreads / (D / (2 * Chunk<T>::N));
+  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = q.heads + k.heads + v.heads;
+  float* sums = nullptr;
+  std::optional<WorkspaceLease> lease;  // held until both kernels are queued
+  int64_t parts = 0;
+  if (tiles > 0 && heads > 0) {
+    int64_t chunks = nr_chunks(tiles, heads);
+    if (dwq || dwk) {
+      chunks = std::min(chunks, kNrSums);
+      void* ws = nullptr;
+      if (!lease.emplace().get_fixed(st, kWsNormWeights, kNrWork, &ws))
+        return fail(TT_ERR_NOMEM, std::string(fn) + ": no scratch for the weights' gradients (under graph capture it "
+                                                    "must be there from an earlier call on the stream)");
+      sums = (float*)ws;
+    }
+    const int64_t count = (heads + chunks - 1) / chunks;
+    chunks = (heads + count - 1) / count;
+    const int64_t slots = sums ? std::min(tiles, std::max<int64_t>(1, kNrSums / chunks)) : tiles;
+    parts = slots * chunks;
+    if (!grid_fits(parts, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+    hipLaunchKernelGGL((qkv_norm_rope_bwd_kernel<T, D>), dim3((unsigned)parts), dim3(kNrThreads), 0, st, q, k, v, rp,
+                       (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)chunks, (uint32_t)slots, (int)count, sums);
+    TT_LAUNCHED(fn, st);
+  }
+  if (dwq || dwk) {
+    hipLaunchKernelGGL((norm_weight_sum_kernel<D>), dim3(2 * D / 16), dim3(kNrSumThreads), 0, st, sums, dwq, dwk,
+                       (int)parts);
+    TT_LAUNCHED(fn, st);
+  }
+  return ok();
+}
+
+// A strided or head-major tensor of a call, for the checks.
+struct NrArg {
+  const void* p;
+  int64_t heads, ld;
+  const char* name;
+};
+
+int check_shape(const std::string& f, int dtype, const NrShape& n, const float* freq, int64_t rot, int inter,
+                float eps) {
+  if (dtype != TT_F32 && dtype != TT_BF16) return fail(TT_ERR_ARG, f + ": dtype must be TT_F32 or TT_BF16");
+  if (n.B < 0 || n.H < 0 || n.Hkv < 0 || n.T < 0) return fail(TT_ERR_ARG, f + ": negative dimension");
+  if (n.d != 32 && n.d != 64 && n.d != 128)
+    return fail(TT_ERR_UNSUPPORTED, f + ": head dim must be 32, 64 or 128 (got " + std::to_string(n.d) + ")");
+  if (n.H > (int64_t(1) << 20) || n.Hkv > (int64_t(1) << 20)) return fail(TT_ERR_ARG, f + ": too many heads");
+  if (n.B > 0x7fffffff || n.T > 0x7fffffff || n.B * n.T > 0x7fffffff - 256)
+    return fail(TT_ERR_ARG, f + ": too many tokens");
+  if (freq && (rot < 0 || rot > n.d || rot % 16 != 0))
+    return fail(TT_ERR_ARG, f + ": rot must be a multiple of 16 of at most d");
+  if (inter != 0 && inter != 1) return fail(TT_ERR_ARG, f + ": interleaved must be 0 or 1");
+  if (!(eps >= 0.f)) return fail(TT_ERR_ARG, f + ": eps must not be negative");
+  return TT_OK;
+}
+
+int check_arg(const std::string& f, const NrArg& a, const NrShape& n, size_t e) {
+  if (!a.p) return TT_OK;
+  if ((uintptr_t)a.p & 15) return fail(TT_ERR_ARG, f + ": " + a.name + " must be 16-byte aligned");
+  if (a.ld == 0) return TT_OK;
+  if (a.ld < a.heads * n.d || a.ld > (int64_t(1) << 31) || a.ld * (int64_t)e % 16 != 0)
+    return fail(TT_ERR_ARG, f + ": the leading dimension of " + a.name +
+                                " must hold its heads, in steps of 16 bytes");
+  return TT_OK;
+}
+
+// From its first to behind its last byte.
+ArgSpan span_of(const NrArg& a, const NrShape& n, size_t e) {
+  const int64_t tokens = n.B * n.T;
+  if (!a.p || tokens == 0 || a.heads == 0) return {nullptr, 0, a.name};
+  return {a.p, (size_t)(a.ld ? (tokens - 1) * a.ld + a.heads * n.d : tokens * a.heads * n.d) * e, a.name};
+}
+
+// Strided tensors may lie between each other's rows: parts of one fused matrix.
+bool apart(const NrArg& a, const NrArg& b, const NrShape& n, size_t e) {
+  if (!spans_overlap(span_of(a, n, e), span_of(b, n, e))) return true;
+  if (a.ld == 0 || a.ld != b.ld) return false;
+  const int64_t ld = a.ld * (int64_t)e, wa = a.heads * n.d * (int64_t)e, wb = b.heads * n.d * (int64_t)e;
+  int64_t off = (int64_t)((uintptr_t)b.p - (uintptr_t)a.p) % ld;
+  if (off < 0) off += ld;
+  return off >= wa && off + wb <= ld;
+}
+
+int check_apart(const std::string& f, std::initializer_list<NrArg> inputs, std::initializer_list<ArgSpan> others,
+                std::initializer_list<NrArg> outputs, std::initializer_list<ArgSpan> sums, const NrShape& n, size_t e) {
+  auto clash = [&](const char* a, const char* b) { return fail(TT_ERR_ARG, f + ": " + a + " overlaps " + b); };
+  for (auto o = outputs.begin(); o != outputs.end(); ++o) {
+    const ArgSpan so = span_of(*o, n, e);
+    for (const NrArg& i : inputs)
+      if (spans_overlap(so, span_of(i, n, e))) return clash(o->name, i.name);
+    for (const ArgSpan& i : others)
+      if (spans_overlap(so, i)) return clash(o->name, i.name);
+    for (const ArgSpan& i : sums)
+      if (spans_overlap(so, i)) return clash(o->name, i.name);
+    for (auto p = outputs.begin(); p != o; ++p)
+      if (!apart(*o, *p, n, e)) return clash(o->name, p->name);
+  }
+  for (auto o = sums.begin(); o != sums.end(); ++o) {
+    for (const NrArg& i : inputs)
+      if (spans_overlap(*o, span_of(i, n, e))) return clash(o->name, i.name);
+    for (const ArgSpan& i : others)
+      if (spans_overlap(*o, i)) return clash(o->name, i.name);
+    for (auto p = sums.begin(); p != o; ++p)
+      if (spans_overlap(*o, *p)) return clash(o->name, p->name);
+  }
+  return TT_OK;
+}
+
+#define TT_NR_DIM(T, CALL)                 \
+  switch (n.d) {                           \
+    case 32: { constexpr int D = 32; return CALL; }   \
+    case 64: { constexpr int D = 64; return CALL; }   \
+    default: { constexpr int D = 128; return CALL; }  \
+  }
+
+template <typename T>
+int forward_d(const char* fn, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv,
+              const float* wq, const float* wk, const Rope& rp, void* qo, void* ko, void* vo, const NrShape& n,
+              hipStream_t st) {
+  const int H = q ? (int)n.H : 0, Hk = k ? (int)n.Hkv : 0, Hv = v ? (int)n.Hkv : 0;
+  const NrPart<T> pq{(const T*)q, (T*)qo, wq, ldq, H}, pk{(const T*)k, (T*)ko, wk, ldk, Hk},
+      pv{(const T*)v, (T*)vo, nullptr, ldv, Hv};
+  TT_NR_DIM(T, (forward_launch<T, D>(fn, pq, pk, pv, rp, n, st)))
+}
+
+template <typename T>
+int backward_d(const char* fn, const void* q, const void* k, int64_t ldq, int64_t ldk, const float* wq,
+               const float* wk, const Rope& rp, const void* dqo, const void* dko, const void* dvo, void* dq, void* dk,
+               void* dv, int64_t lddq, int64_t lddk, int64_t lddv, float* dwq, float* dwk, const NrShape& n,
+               hipStream_t st) {
+  const int H = dq ? (int)n.H : 0, Hk = dk ? (int)n.Hkv : 0, Hv = dv ? (int)n.Hkv : 0;
+  const NrBack<T> pq{(const T*)q, (const T*)dqo, (T*)dq, wq, ldq, lddq, H},
+      pk{(const T*)k, (const T*)dko, (T*)dk, wk, ldk, lddk, Hk},
+      pv{nullptr, (const T*)dvo, (T*)dv, nullptr, 0, lddv, Hv};
+  TT_NR_DIM(T, (backward_launch<T, D>(fn, pq, pk, pv, rp, dwq, dwk, n, st)))
+}
+
+}  // namespace
+}  // namespace tt
+
+using namespace tt;
+
+extern "C" int tt_qkv_norm_rope(int dtype, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk,
+                                int64_t ldv, const float* q_weight, const float* k_weight, float eps,
+                                const float* inv_freq, int64_t rot, int interleaved, const int* positions,
+                                const int* lengths, void* q_out, void* k_out, void* v_out, int64_t B, int64_t H,
+                                int64_t Hkv, int64_t T, int64_t d, void* stream) {
+  const char* fn = "tt_qkv_norm_rope";
+  const std::string f(fn);
+  const NrShape n{B, H, Hkv, T, d};
+  int rc = check_shape(f, dtype, n, inv_freq, rot, interleaved, eps);
+  if (rc) return rc;
+  const size_t e = dtype == TT_F32 ? 4 : 2, w = (size_t)d * sizeof(float);
+  const NrArg in[3] = {{q, H, ldq, "q"}, {k, Hkv, ldk, "k"}, {v, Hkv, ldv, "v"}};
+  const NrArg out[3] = {{q_out, H, 0, "q_out"}, {k_out, Hkv, 0, "k_out"}, {v_out, Hkv, 0, "v_out"}};
+  if (B == 0 || T == 0) return ok();
+  for (int i = 0; i < 3; ++i) {
+    if ((in[i].p == nullptr) != (out[i].p == nullptr))
+      return fail(TT_ERR_ARG, f + ": " + in[i].name + " and its output must both be given or both be null");
+    if ((rc = check_arg(f, in[i], n, e)) || (rc = check_arg(f, out[i], n, e))) return rc;
+  }
+  if ((!q || H == 0) && ((!k && !v) || Hkv == 0)) return ok();
+  if ((rc = check_apart(f, {in[0], in[1], in[2]},
+                        {{q_weight, w, "q_weight"},
+                         {k_weight, w, "k_weight"},
+                         {inv_freq, (size_t)(inv_freq ? rot / 2 : 0) * sizeof(float), "inv_freq"},
+                         {positions, (size_t)(B * T) * sizeof(int), "positions"},
+                         {lengths, (size_t)B * sizeof(int), "lengths"}},
+                        {out[0], out[1], out[2]}, {}, n, e)))
+    return rc;
+  if ((rc = ensure_init())) return rc;
+  hipStream_t st = stream_or_default(stream);
+  const Rope rp{inv_freq, positions, lengths, (int)rot, interleaved, eps};
+  return dtype == TT_F32
+             ? forward_d<float>(fn, q, k, v, ldq, ldk, ldv, q_weight, k_weight, rp, q_out, k_out, v_out, n, st)
+             : forward_d<u16>(fn, q, k, v, ldq, ldk, ldv, q_weight, k_weight, rp, q_out, k_out, v_out, n, st);
+}
+
+extern "C" int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t ldq, int64_t ldk,
+                                         const float* q_weight, const float* k_weight, float eps,
+                                         const float* inv_freq, int64_t rot, int interleaved, const int* positions,
+                                         const int* lengths, const void* dq_out, const void* dk_out,
+                                         const void* dv_out, void* dq, void* dk, void* dv, int64_t lddq, int64_t lddk,
+                                         int64_t lddv, float* dq_weight, float* dk_weight, int64_t B, int64_t H,
+                                         int64_t Hkv, int64_t T, int64_t d, void* stream) {
+  const char* fn = "tt_qkv_norm_rope_backward";
+  const std::string f(fn);
+  const NrShape n{B, H, Hkv, T, d};
+  int rc = check_shape(f, dtype, n, inv_freq, rot, interleaved, eps);
+  if (rc) return rc;
+  const size_t e = dtype == TT_F32 ? 4 : 2, w = (size_t)d * sizeof(float);
+  const NrArg x[2] = {{q, H, ldq, "q"}, {k, Hkv, ldk, "k"}};
+  const NrArg dy[3] = {{dq_out, H, 0, "dq_out"}, {dk_out, Hkv, 0, "dk_out"}, {dv_out, Hkv, 0, "dv_out"}};
+  const NrArg dx[3] = {{dq, H, lddq, "dq"}, {dk, Hkv, lddk, "dk"}, {dv, Hkv, lddv, "dv"}};
+  const float* weight[2] = {q_weight, k_weight};
+  float* dw[2] = {dq_weight, dk_weight};
+  const bool some = B > 0 && T > 0;
+  for (int i = 0; i < 3; ++i) {
+    if (some && (dy[i].p == nullptr) != (dx[i].p == nullptr))
+      return fail(TT_ERR_ARG, f + ": " + dx[i].name + " and " + dy[i].name + " must both be given or both be null");
+    if ((rc = check_arg(f, dy[i], n, e)) || (rc = check_arg(f, dx[i], n, e))) return rc;
+    if (i == 2) continue;
+    if (dw[i] && !weight[i])
+      return fail(TT_ERR_ARG, f + ": the gradient of a weight that is not given");
+    if (some && dw[i] && x[i].heads > 0 && !dx[i].p)
+      return fail(TT_ERR_ARG, f + ": a weight's gradient comes with its input's, which is null");
+    if (some && weight[i] && dx[i].p && x[i].heads > 0 && !x[i].p)
+      return fail(TT_ERR_ARG, f + ": " + x[i].name + " is null, but normed");
+    if ((rc = check_arg(f, x[i], n, e))) return rc;
+  }
+  const bool any = some && ((dq && H > 0) || ((dk || dv) && Hkv > 0));
+  if (!any && !dq_weight && !dk_weight) return ok();
+  if ((rc = check_apart(f, {x[0], x[1], dy[0], dy[1], dy[2]},
+                        {{q_weight, w, "q_weight"},
+                         {k_weight, w, "k_weight"},
+                         {inv_freq, (size_t)(inv_freq ? rot / 2 : 0) * sizeof(float), "inv_freq"},
+                         {positions, (size_t)(B * T) * sizeof(int), "positions"},
+                         {lengths, (size_t)B * sizeof(int), "lengths"}},
+                        {dx[0], dx[1], dx[2]}, {{dq_weight, w, "dq_weight"}, {dk_weight, w, "dk_weight"}}, n, e)))
+    return rc;
+  if ((rc = ensure_init())) return rc;
+  hipStream_t st = stream_or_default(stream);
+  const Rope rp{inv_freq, positions, lengths, (int)rot, interleaved, eps};
+  return dtype == TT_F32 ? backward_d<float>(fn, q, k, ldq, ldk, q_weight, k_weight, rp, dq_out, dk_out, dv_out, dq,
+                                             dk, dv, lddq, lddk, lddv, dq_weight, dk_weight, n, st)
+                         : backward_d<u16>(fn, q, k, ldq, ldk, q_weight, k_weight, rp, dq_out, dk_out, dv_out, dq, dk,
+                                           dv, lddq, lddk, lddv, dq_weight, dk_weight, n, st);
+}

@@ -23,7 +23,7 @@ HEADER = os.path.join(os.path.dirname(HERE), "include", "tt_attn.h")
 LIB_PATH = os.environ.get("TT_LIB_PATH") or os.path.join(HERE, "libtt_hip.so")
 
 TT_OK, TT_ERR_ARG, TT_ERR_HIP, TT_ERR_UNSUPPORTED, TT_ERR_NOMEM = range(5)
-TT_F32, TT_F64, TT_I32, TT_BF16 = range(4)
+TT_F32, TT_F64, TT_I32, TT_BF16, TT_E4M3 = range(5)
 
 _p = C.c_void_p
 _i64 = C.c_int64
@@ -88,6 +88,14 @@ _SIGS = {
     "tt_fc_forward_mxfp4": (C.c_int, [C.c_int, _i64, _i64, _i64, _p, _p, _p, _p, C.c_int, _p, _p]),
     "tt_kv_append_mxfp4": (C.c_int, [C.c_int] + [_p] * 7 + [_i64] * 5 + [_p]),
     "tt_attn_decode_mxfp4": (C.c_int, [C.c_int] + [_p] * 8 + [_i64] * 6 + [C.c_float, _p]),
+    "tt_qkv_norm_rope": (C.c_int, [C.c_int] + [_p] * 3 + [_i64] * 3 + [_p] * 2 + [C.c_float, _p, _i64, C.c_int] + [_p] * 5
+                         + [_i64] * 5 + [_p]),
+    "tt_qkv_norm_rope_backward": (C.c_int, [C.c_int] + [_p] * 2 + [_i64] * 2 + [_p] * 2 + [C.c_float, _p, _i64, C.c_int]
+                                  + [_p] * 8 + [_i64] * 3 + [_p] * 2 + [_i64] * 5 + [_p]),
+    "tt_kv_append_paged": (C.c_int, [C.c_int] * 2 + [_p] * 2 + [_i64] * 2 + [_p, C.c_float, _p, _i64, C.c_int] + [_p] * 7
+                           + [_i64] * 7 + [_p]),
+    "tt_kv_gather_paged": (C.c_int, [C.c_int] * 2 + [_p] * 8 + [_i64] * 7 + [_p]),
+    "tt_attn_decode_paged": (C.c_int, [C.c_int] * 2 + [_p] * 9 + [_i64] * 8 + [C.c_float, _p]),
     "tt_col_sum": (C.c_int, [C.c_int, _p, _p, _i64, _i64, _p]),
 }
 
