@@ -469,8 +469,8 @@ int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t l
  * 0xff are NaN) under scale bytes k_scales and v_scales [npages][Hkv], one for each
  * page and head, that stand for 2^(byte - 127): the smallest power of two, of
  * 2^-124 to 2^119, that takes the page's largest value to at most 448.  Values
- * are rounded to nearest, halves to even; infinities and NaN become NaN and do
- * not count for the scale.  The scales are null for other caches.  Pools are
+ * are rounded to nearest, halves to even; infinities and NaN become NaN (of
+ * either code) and do not count for the scale.  The scales are null for other caches.  Pools are
  * 16-byte aligned (TT_ERR_ARG otherwise), d is 32, 64 or 128. */
 
 /* Append: the new tokens' k and v, [B][Hkv][T][d] or token-major (ldk, ldv as

@@ -1,4 +1,4 @@
-// Module `myLayer`: the attention entry points, SoftmaxForward with its cross-entropy, FC, convolution, max pooling and the 4-bit layers, bound in the style of
+// Module `myLayer`: the attention entry points, SoftmaxForward with its cross-entropy, FC, convolution, max pooling, the 4-bit layers, norms and rotation of heads, and the paged cache, bound in the style of
 // Task3/Tinytensor/src/bind_Layer.cpp:10-24 (free functions over TinyTensor
 // references), with float and bf16 overloads.
 #include <pybind11/pybind11.h>
@@ -7,6 +7,44 @@
 #include "layers.h"
 
 namespace py = pybind11;
+
+namespace {
+
+template <typename T>
+void bind_heads(py::module_& m) {
+  m.def("NormRopeForward", &NormRopeForward<T>, py::arg("input"), py::arg("output"), py::arg("weight") = py::none(),
+        py::arg("inv_freq") = py::none(), py::arg("eps") = 1e-6f, py::arg("positions") = py::none(),
+        py::arg("lengths") = py::none(), py::arg("interleaved") = false, py::arg("tokens_first") = false);
+  m.def("NormRopeBackward", &NormRopeBackward<T>, py::arg("input"), py::arg("grad_output"), py::arg("grad_input"),
+        py::arg("weight") = py::none(), py::arg("grad_weight") = py::none(), py::arg("inv_freq") = py::none(),
+        py::arg("eps") = 1e-6f, py::arg("positions") = py::none(), py::arg("lengths") = py::none(),
+        py::arg("interleaved") = false, py::arg("tokens_first") = false);
+  m.def("QkvNormRopeForward", &QkvNormRopeForward<T>, py::arg("qkv"), py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("kv_heads"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(),
+        py::arg("inv_freq") = py::none(), py::arg("eps") = 1e-6f, py::arg("positions") = py::none(),
+        py::arg("lengths") = py::none(), py::arg("interleaved") = false);
+  m.def("QkvNormRopeBackward", &QkvNormRopeBackward<T>, py::arg("qkv"), py::arg("grad_q"), py::arg("grad_k"),
+        py::arg("grad_v"), py::arg("grad_qkv"), py::arg("q_weight") = py::none(), py::arg("k_weight") = py::none(),
+        py::arg("grad_q_weight") = py::none(), py::arg("grad_k_weight") = py::none(),
+        py::arg("inv_freq") = py::none(), py::arg("eps") = 1e-6f, py::arg("positions") = py::none(),
+        py::arg("lengths") = py::none(), py::arg("interleaved") = false);
+}
+
+template <typename T, typename C>
+void bind_paged(py::module_& m) {
+  m.def("KvAppendPaged", &KvAppendPaged<T, C>, py::arg("k"), py::arg("v"), py::arg("k_pages"), py::arg("v_pages"),
+        py::arg("table"), py::arg("lengths"), py::arg("k_weight") = py::none(), py::arg("inv_freq") = py::none(),
+        py::arg("eps") = 1e-6f, py::arg("positions") = py::none(), py::arg("interleaved") = false,
+        py::arg("tokens_first") = false, py::arg("k_scales") = py::none(), py::arg("v_scales") = py::none());
+  m.def("KvGatherPaged", &KvGatherPaged<T, C>, py::arg("k_pages"), py::arg("v_pages"), py::arg("table"),
+        py::arg("lengths"), py::arg("k"), py::arg("v"), py::arg("length"), py::arg("k_scales") = py::none(),
+        py::arg("v_scales") = py::none());
+  m.def("AttentionDecodePaged", &AttentionDecodePaged<T, C>, py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
+        py::arg("table"), py::arg("lengths"), py::arg("out"), py::arg("scale"), py::arg("k_scales") = py::none(),
+        py::arg("v_scales") = py::none());
+}
+
+}  // namespace
 
 PYBIND11_MODULE(myLayer, m) {
   m.doc() = "myLayer: fused attention for MI355X (gfx950)";
@@ -48,6 +86,13 @@ PYBIND11_MODULE(myLayer, m) {
         py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"), py::arg("out"), py::arg("scale"));
   m.def("AttentionDecodeMxfp4", &AttentionDecodeMxfp4<bf16>, py::arg("q"), py::arg("k_codes"), py::arg("k_scales"),
         py::arg("v_codes"), py::arg("v_scales"), py::arg("lengths"), py::arg("out"), py::arg("scale"));
+  // norms of heads with the position rotation, and a K/V cache in pages
+  bind_heads<float>(m);
+  bind_heads<bf16>(m);
+  bind_paged<float, float>(m);
+  bind_paged<bf16, bf16>(m);
+  bind_paged<float, uint8_t>(m);
+  bind_paged<bf16, uint8_t>(m);
   // the reference binds SoftmaxForward<float> positionally (bind_Layer.cpp:20)
   m.def("SoftmaxForward", &SoftmaxForward<float>, py::arg("input"), py::arg("output"));
   // positional as in the reference (bind_Layer.cpp:12-13), plus bf16 overloads

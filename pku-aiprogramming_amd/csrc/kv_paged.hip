@@ -81,14 +81,7 @@ __global__ __launch_bounds__(kPgThreads) void kv_append_kernel(PgNew<T> in, Rope
           float f[2 * N];
           Chunk<T>::get(r[u][0], f);
           Chunk<T>::get(r[u][1], f + N);
-          if (norm) {
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2 * N; ++e) ss += f[e] * f[e];
-            const float scale = __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * (1.f / D) + rp.eps);
-#pragma unroll
-            for (int e = 0; e < 2 * N; ++e) f[e] *= scale * w[e];
-          }
+          if (norm) rope_scale<N>(f, rope_rms<N, LPR>(f, rp.eps), w);
           if (turn) rope_turn<N>(f, c, s, rp.inter != 0);
           r[u][0] = Chunk<T>::put(f);
           r[u][1] = Chunk<T>::put(f + N);
@@ -160,15 +153,10 @@ __global__ __launch_bounds__((PgTile<T, D, PAGE>::THREADS)) void kv_append_e4m3_
 #pragma unroll
       for (int e = 0; e < 2 * N; ++e) g[e] = f[it][e];
       if (norm) {
-        double ss = 0.0;
+        float w[2 * N];
 #pragma unroll
-        for (int e = 0; e < 2 * N; ++e) ss += g[e] * g[e];
-        const double r = 1.0 / __builtin_sqrt(row_sum<LPR>(ss) * (1.0 / D) + (double)rp.eps);
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-          g[e] *= r * (double)in.weight[lay.a + e];
-          g[N + e] *= r * (double)in.weight[lay.b + e];
-        }
+        for (int e = 0; e < N; ++e) w[e] = in.weight[lay.a + e], w[N + e] = in.weight[lay.b + e];
+        rope_scale<N>(g, rope_rms<N, LPR>(g, rp.eps), w);
       }
       if (lay.turns) {
         double c[N], s[N];

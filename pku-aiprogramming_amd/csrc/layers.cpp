@@ -906,3 +906,336 @@ template void MaxPoolingForward<float>(const TinyTensor<float>&, TinyTensor<floa
                                        const std::vector<int>&, int, int, int, int);
 template void MaxPoolingBackward<float>(const TinyTensor<float>&, const TinyTensor<float>&, TinyTensor<float>&,
                                         const std::vector<int>&, const std::vector<int>&, int, int, int, int);
+
+namespace {
+
+template <typename X>
+X* data_of(TinyTensor<X>* t) {
+  return t ? t->p_data : nullptr;
+}
+template <typename X>
+const X* data_of(const TinyTensor<X>* t) {
+  return t ? t->p_data : nullptr;
+}
+
+template <typename X>
+void need_shape(const std::string& fn, const std::string& name, const TinyTensor<X>* t, const std::vector<int>& shape,
+                const char* what) {
+  if (!t) return;
+  need_gpu(fn, name, t->device);
+  if (t->shape != shape) throw std::invalid_argument(fn + ": " + name + " must have shape " + what);
+}
+
+// The arguments that norms and rotations share; returns rot.
+int64_t check_rope(const std::string& fn, const TinyTensor<float>* inv_freq, const TinyTensor<int>* positions,
+                   const TinyTensor<int>* lengths, int B, int tokens) {
+  need_shape(fn, "positions", positions, {B, tokens}, "[B, T]");
+  need_shape(fn, "lengths", lengths, {B}, "[B]");
+  if (!inv_freq) return 0;
+  need_gpu(fn, "inv_freq", inv_freq->device);
+  if (inv_freq->shape.size() != 1) throw std::invalid_argument(fn + ": inv_freq must have rank 1 [rot / 2]");
+  return 2 * (int64_t)inv_freq->shape[0];
+}
+
+// [B, H, L, d] as stored, or [B, L, H, d] read as that.
+Dims heads_of(Dims n, bool tokens_first) {
+  if (tokens_first) std::swap(n.H, n.L);
+  return n;
+}
+
+int fused_heads(const std::string& fn, const Dims& n, int kv_heads) {
+  if (kv_heads < 0 || n.L < 2 * (int64_t)kv_heads)
+    throw std::invalid_argument(fn + ": qkv must have shape [B, T, H + 2 kv_heads, d]");
+  return n.L - 2 * kv_heads;
+}
+
+template <typename T>
+T* part(T* p, int64_t heads, int d) {
+  return p ? p + heads * d : p;
+}
+
+}  // namespace
+
+template <typename T>
+void NormRopeForward(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<float>* weight,
+                     const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                     const TinyTensor<int>* lengths, bool interleaved, bool tokens_first) {
+  const std::string fn = "NormRopeForward";
+  need_gpu(fn, "input", input.device);
+  need_gpu(fn, "output", output.device);
+  const Dims n = heads_of(dims4(fn, "input", input), tokens_first);
+  need_shape(fn, "weight", weight, {n.d}, "[d]");
+  const int64_t rot = check_rope(fn, inv_freq, positions, lengths, n.B, n.L);
+  no_alias(fn, {{input.p_data, "input"}, {data_of(weight), "weight"}, {data_of(inv_freq), "inv_freq"}},
+           {{output.p_data, "output"}});
+  output.resize_output({n.B, n.H, n.L, n.d});
+  if (output.size == 0) return;
+  tt_check(tt_qkv_norm_rope(dtype_code<T>(), input.p_data, nullptr, nullptr, tokens_first ? (int64_t)n.H * n.d : 0, 0,
+                            0, data_of(weight), nullptr, eps, data_of(inv_freq), rot, interleaved, data_of(positions),
+                            data_of(lengths), output.p_data, nullptr, nullptr, n.B, n.H, 0, n.L, n.d, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void NormRopeBackward(const TinyTensor<T>& input, const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input,
+                      const TinyTensor<float>* weight, TinyTensor<float>* grad_weight,
+                      const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                      const TinyTensor<int>* lengths, bool interleaved, bool tokens_first) {
+  const std::string fn = "NormRopeBackward";
+  need_gpu(fn, "input", input.device);
+  need_gpu(fn, "grad_output", grad_output.device);
+  need_gpu(fn, "grad_input", grad_input.device);
+  const Dims n = heads_of(dims4(fn, "input", input), tokens_first);
+  if (grad_output.shape != std::vector<int>{n.B, n.H, n.L, n.d})
+    throw std::invalid_argument(fn + ": grad_output must have shape [B, H, T, d]");
+  need_shape(fn, "weight", weight, {n.d}, "[d]");
+  if (grad_weight) {
+    need_gpu(fn, "grad_weight", grad_weight->device);
+    if (!weight) throw std::invalid_argument(fn + ": grad_weight without a weight");
+  }
+  const int64_t rot = check_rope(fn, inv_freq, positions, lengths, n.B, n.L);
+  no_alias(fn,
+           {{input.p_data, "input"},
+            {grad_output.p_data, "grad_output"},
+            {data_of(weight), "weight"},
+            {data_of(inv_freq), "inv_freq"}},
+           {{grad_input.p_data, "grad_input"}, {data_of(grad_weight), "grad_weight"}});
+  grad_input.resize_output(input.shape);
+  if (grad_weight) grad_weight->resize_output({n.d});
+  const int64_t ld = tokens_first ? (int64_t)n.H * n.d : 0;
+  tt_check(tt_qkv_norm_rope_backward(dtype_code<T>(), input.p_data, nullptr, ld, 0, data_of(weight), nullptr, eps,
+                                     data_of(inv_freq), rot, interleaved, data_of(positions), data_of(lengths),
+                                     grad_output.p_data, nullptr, nullptr, grad_input.p_data, nullptr, nullptr, ld, 0,
+                                     0, data_of(grad_weight), nullptr, n.B, n.H, 0, n.L, n.d, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void QkvNormRopeForward(const TinyTensor<T>& qkv, TinyTensor<T>& q, TinyTensor<T>& k, TinyTensor<T>& v, int kv_heads,
+                        const TinyTensor<float>* q_weight, const TinyTensor<float>* k_weight,
+                        const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                        const TinyTensor<int>* lengths, bool interleaved) {
+  const std::string fn = "QkvNormRopeForward";
+  need_gpu(fn, "qkv", qkv.device);
+  need_gpu(fn, "q", q.device);
+  need_gpu(fn, "k", k.device);
+  need_gpu(fn, "v", v.device);
+  const Dims n = dims4(fn, "qkv", qkv);  // B, T, heads, d
+  const int heads = fused_heads(fn, n, kv_heads);
+  need_shape(fn, "q_weight", q_weight, {n.d}, "[d]");
+  need_shape(fn, "k_weight", k_weight, {n.d}, "[d]");
+  const int64_t rot = check_rope(fn, inv_freq, positions, lengths, n.B, n.H);
+  no_alias(fn,
+           {{qkv.p_data, "qkv"},
+            {data_of(q_weight), "q_weight"},
+            {data_of(k_weight), "k_weight"},
+            {data_of(inv_freq), "inv_freq"}},
+           {{q.p_data, "q"}, {k.p_data, "k"}, {v.p_data, "v"}});
+  q.resize_output({n.B, heads, n.H, n.d});
+  k.resize_output({n.B, kv_heads, n.H, n.d});
+  v.resize_output({n.B, kv_heads, n.H, n.d});
+  if (qkv.size == 0) return;
+  const int64_t ld = (int64_t)n.L * n.d;
+  const bool hq = heads > 0, hk = kv_heads > 0;
+  tt_check(tt_qkv_norm_rope(dtype_code<T>(), hq ? qkv.p_data : nullptr, hk ? part(qkv.p_data, heads, n.d) : nullptr,
+                            hk ? part(qkv.p_data, heads + kv_heads, n.d) : nullptr, ld, ld, ld, data_of(q_weight),
+                            data_of(k_weight), eps, data_of(inv_freq), rot, interleaved, data_of(positions),
+                            data_of(lengths), hq ? q.p_data : nullptr, hk ? k.p_data : nullptr,
+                            hk ? v.p_data : nullptr, n.B, heads, kv_heads, n.H, n.d, nullptr),
+           fn.c_str());
+}
+
+template <typename T>
+void QkvNormRopeBackward(const TinyTensor<T>& qkv, const TinyTensor<T>& grad_q, const TinyTensor<T>& grad_k,
+                         const TinyTensor<T>& grad_v, TinyTensor<T>& grad_qkv, const TinyTensor<float>* q_weight,
+                         const TinyTensor<float>* k_weight, TinyTensor<float>* grad_q_weight,
+                         TinyTensor<float>* grad_k_weight, const TinyTensor<float>* inv_freq, float eps,
+                         const TinyTensor<int>* positions, const TinyTensor<int>* lengths, bool interleaved) {
+  const std::string fn = "QkvNormRopeBackward";
+  need_gpu(fn, "qkv", qkv.device);
+  need_gpu(fn, "grad_q", grad_q.device);
+  need_gpu(fn, "grad_k", grad_k.device);
+  need_gpu(fn, "grad_v", grad_v.device);
+  need_gpu(fn, "grad_qkv", grad_qkv.device);
+  const Dims g = dims4(fn, "grad_k", grad_k), n = dims4(fn, "qkv", qkv);  // n: B, T, heads, d
+  const int kv_heads = g.H, heads = fused_heads(fn, n, kv_heads);
+  if (grad_q.shape != std::vector<int>{n.B, heads, n.H, n.d} ||
+      grad_k.shape != std::vector<int>{n.B, kv_heads, n.H, n.d} || grad_v.shape != grad_k.shape)
+    throw std::invalid_argument(fn + ": grad_q, grad_k and grad_v must be [B, heads, T, d] of qkv's parts");
+  need_shape(fn, "q_weight", q_weight, {n.d}, "[d]");
+  need_shape(fn, "k_weight", k_weight, {n.d}, "[d]");
+  if ((grad_q_weight && !q_weight) || (grad_k_weight && !k_weight))
+    throw std::invalid_argument(fn + ": the gradient of a weight that is not given");
+  if (grad_q_weight) need_gpu(fn, "grad_q_weight", grad_q_weight->device);
+  if (grad_k_weight) need_gpu(fn, "grad_k_weight", grad_k_weight->device);
+  const int64_t rot = check_rope(fn, inv_freq, positions, lengths, n.B, n.H);
+  no_alias(fn,
+           {{qkv.p_data, "qkv"},
+            {grad_q.p_data, "grad_q"},
+            {grad_k.p_data, "grad_k"},
+            {grad_v.p_data, "grad_v"},
+            {data_of(q_weight), "q_weight"},
+            {data_of(k_weight), "k_weight"},
+            {data_of(inv_freq), "inv_freq"}},
+           {{grad_qkv.p_data, "grad_qkv"},
+            {data_of(grad_q_weight), "grad_q_weight"},
+            {data_of(grad_k_weight), "grad_k_weight"}});
+  grad_qkv.resize_output(qkv.shape);
+  if (grad_q_weight) grad_q_weight->resize_output({n.d});
+  if (grad_k_weight) grad_k_weight->resize_output({n.d});
+  const int64_t ld = (int64_t)n.L * n.d;
+  const bool hq = heads > 0, hk = kv_heads > 0;
+  tt_check(tt_qkv_norm_rope_backward(
+               dtype_code<T>(), hq ? qkv.p_data : nullptr, hk ? part(qkv.p_data, heads, n.d) : nullptr, ld, ld,
+               data_of(q_weight), data_of(k_weight), eps, data_of(inv_freq), rot, interleaved, data_of(positions),
+               data_of(lengths), hq ? grad_q.p_data : nullptr, hk ? grad_k.p_data : nullptr,
+               hk ? grad_v.p_data : nullptr, hq ? grad_qkv.p_data : nullptr,
+               hk ? part(grad_qkv.p_data, heads, n.d) : nullptr,
+               hk ? part(grad_qkv.p_data, heads + kv_heads, n.d) : nullptr, ld, ld, ld, data_of(grad_q_weight),
+               data_of(grad_k_weight), n.B, heads, kv_heads, n.H, n.d, nullptr),
+           fn.c_str());
+}
+
+namespace {
+
+template <typename C>
+constexpr int cache_code() {
+  return std::is_same<C, uint8_t>::value ? (int)TT_E4M3 : std::is_same<C, float>::value ? (int)TT_F32 : (int)TT_BF16;
+}
+
+// Of a paged cache: its pools' pages, Hkv, page and d, the table's B and width.
+struct PagedDims {
+  int npages, Hkv, page, d, B, width;
+};
+template <typename C>
+PagedDims paged_cache(const std::string& fn, const TinyTensor<C>& k, const TinyTensor<C>& v,
+                      const TinyTensor<int>& table, const TinyTensor<int>& lengths, const TinyTensor<uint8_t>* ks,
+                      const TinyTensor<uint8_t>* vs) {
+  need_gpu(fn, "k_pages", k.device);
+  need_gpu(fn, "v_pages", v.device);
+  need_gpu(fn, "table", table.device);
+  need_gpu(fn, "lengths", lengths.device);
+  if (k.shape.size() != 4) throw std::invalid_argument(fn + ": k_pages must have rank 4 [pages, Hkv, page, d]");
+  if (v.shape != k.shape) throw std::invalid_argument(fn + ": the K and V pools must have the same shape");
+  if (table.shape.size() != 2) throw std::invalid_argument(fn + ": table must have rank 2 [B, width]");
+  const PagedDims c{k.shape[0], k.shape[1], k.shape[2], k.shape[3], table.shape[0], table.shape[1]};
+  if (lengths.shape != std::vector<int>{c.B}) throw std::invalid_argument(fn + ": lengths must have shape [B]");
+  const bool bytes = std::is_same<C, uint8_t>::value;
+  if (bytes != (ks != nullptr) || bytes != (vs != nullptr))
+    throw std::invalid_argument(fn + ": pools of codes come with k_scales and v_scales, others without");
+  need_shape(fn, "k_scales", ks, {c.npages, c.Hkv}, "[pages, Hkv]");
+  need_shape(fn, "v_scales", vs, {c.npages, c.Hkv}, "[pages, Hkv]");
+  return c;
+}
+
+}  // namespace
+
+template <typename T, typename C>
+void KvAppendPaged(const TinyTensor<T>& k, const TinyTensor<T>& v, TinyTensor<C>& k_pages, TinyTensor<C>& v_pages,
+                   const TinyTensor<int>& table, const TinyTensor<int>& lengths, const TinyTensor<float>* k_weight,
+                   const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions, bool interleaved,
+                   bool tokens_first, TinyTensor<uint8_t>* k_scales, TinyTensor<uint8_t>* v_scales) {
+  const std::string fn = "KvAppendPaged";
+  need_gpu(fn, "k", k.device);
+  need_gpu(fn, "v", v.device);
+  const PagedDims c = paged_cache(fn, k_pages, v_pages, table, lengths, k_scales, v_scales);
+  const Dims n = heads_of(dims4(fn, "k", k), tokens_first);
+  if (v.shape != k.shape) throw std::invalid_argument(fn + ": k and v must have the same shape");
+  if (n.B != c.B || n.H != c.Hkv || n.d != c.d)
+    throw std::invalid_argument(fn + ": k and the cache disagree on B, Hkv or d");
+  need_shape(fn, "k_weight", k_weight, {n.d}, "[d]");
+  const int64_t rot = check_rope(fn, inv_freq, positions, nullptr, n.B, n.L);
+  const int64_t ld = tokens_first ? (int64_t)n.H * n.d : 0;
+  no_alias(fn, {{k.p_data, "k"}, {v.p_data, "v"}, {table.p_data, "table"}, {lengths.p_data, "lengths"}},
+           {{k_pages.p_data, "k_pages"},
+            {v_pages.p_data, "v_pages"},
+            {data_of(k_scales), "k_scales"},
+            {data_of(v_scales), "v_scales"}});
+  tt_check(tt_kv_append_paged(dtype_code<T>(), cache_code<C>(), k.p_data, v.p_data, ld, ld, data_of(k_weight), eps,
+                              data_of(inv_freq), rot, interleaved, data_of(positions), k_pages.p_data, v_pages.p_data,
+                              data_of(k_scales), data_of(v_scales), table.p_data, lengths.p_data, c.B, c.Hkv, n.L, c.d,
+                              c.npages, c.page, c.width, nullptr),
+           fn.c_str());
+}
+
+template <typename T, typename C>
+void KvGatherPaged(const TinyTensor<C>& k_pages, const TinyTensor<C>& v_pages, const TinyTensor<int>& table,
+                   const TinyTensor<int>& lengths, TinyTensor<T>& k, TinyTensor<T>& v, int length,
+                   const TinyTensor<uint8_t>* k_scales, const TinyTensor<uint8_t>* v_scales) {
+  const std::string fn = "KvGatherPaged";
+  const PagedDims c = paged_cache(fn, k_pages, v_pages, table, lengths, k_scales, v_scales);
+  need_gpu(fn, "k", k.device);
+  need_gpu(fn, "v", v.device);
+  if (length < 0) throw std::invalid_argument(fn + ": length must not be negative");
+  no_alias(fn,
+           {{k_pages.p_data, "k_pages"},
+            {v_pages.p_data, "v_pages"},
+            {data_of(k_scales), "k_scales"},
+            {data_of(v_scales), "v_scales"}},
+           {{k.p_data, "k"}, {v.p_data, "v"}});
+  k.resize_output({c.B, c.Hkv, length, c.d});
+  v.resize_output({c.B, c.Hkv, length, c.d});
+  tt_check(tt_kv_gather_paged(dtype_code<T>(), cache_code<C>(), k_pages.p_data, v_pages.p_data, data_of(k_scales),
+                              data_of(v_scales), table.p_data, lengths.p_data, k.p_data, v.p_data, c.B, c.Hkv, length,
+                              c.d, c.npages, c.page, c.width, nullptr),
+           fn.c_str());
+}
+
+template <typename T, typename C>
+void AttentionDecodePaged(const TinyTensor<T>& q, const TinyTensor<C>& k_pages, const TinyTensor<C>& v_pages,
+                          const TinyTensor<int>& table, const TinyTensor<int>& lengths, TinyTensor<T>& out,
+                          float scale, const TinyTensor<uint8_t>* k_scales, const TinyTensor<uint8_t>* v_scales) {
+  const std::string fn = "AttentionDecodePaged";
+  need_gpu(fn, "q", q.device);
+  need_gpu(fn, "out", out.device);
+  const PagedDims c = paged_cache(fn, k_pages, v_pages, table, lengths, k_scales, v_scales);
+  const Dims n = dims4(fn, "q", q);
+  if (n.B != c.B || n.d != c.d) throw std::invalid_argument(fn + ": q and the cache disagree on B or d");
+  no_alias(fn,
+           {{q.p_data, "q"},
+            {k_pages.p_data, "k_pages"},
+            {v_pages.p_data, "v_pages"},
+            {data_of(k_scales), "k_scales"},
+            {data_of(v_scales), "v_scales"}},
+           {{out.p_data, "out"}});
+  out.resize_output(q.shape);
+  tt_check(tt_attn_decode_paged(dtype_code<T>(), cache_code<C>(), q.p_data, k_pages.p_data, v_pages.p_data,
+                                data_of(k_scales), data_of(v_scales), table.p_data, lengths.p_data, out.p_data,
+                                nullptr, c.B, n.H, c.Hkv, n.L, c.d, c.npages, c.page, c.width, scale, nullptr),
+           fn.c_str());
+}
+
+#define TT_HEAD_LAYERS(T)                                                                                            \
+  template void NormRopeForward<T>(const TinyTensor<T>&, TinyTensor<T>&, const TinyTensor<float>*,                  \
+                                   const TinyTensor<float>*, float, const TinyTensor<int>*, const TinyTensor<int>*, \
+                                   bool, bool);                                                                     \
+  template void NormRopeBackward<T>(const TinyTensor<T>&, const TinyTensor<T>&, TinyTensor<T>&,                     \
+                                    const TinyTensor<float>*, TinyTensor<float>*, const TinyTensor<float>*, float,  \
+                                    const TinyTensor<int>*, const TinyTensor<int>*, bool, bool);                    \
+  template void QkvNormRopeForward<T>(const TinyTensor<T>&, TinyTensor<T>&, TinyTensor<T>&, TinyTensor<T>&, int,    \
+                                      const TinyTensor<float>*, const TinyTensor<float>*, const TinyTensor<float>*, \
+                                      float, const TinyTensor<int>*, const TinyTensor<int>*, bool);                 \
+  template void QkvNormRopeBackward<T>(const TinyTensor<T>&, const TinyTensor<T>&, const TinyTensor<T>&,            \
+                                       const TinyTensor<T>&, TinyTensor<T>&, const TinyTensor<float>*,              \
+                                       const TinyTensor<float>*, TinyTensor<float>*, TinyTensor<float>*,            \
+                                       const TinyTensor<float>*, float, const TinyTensor<int>*,                     \
+                                       const TinyTensor<int>*, bool);
+#define TT_PAGED_LAYERS(T, C)                                                                                       \
+  template void KvAppendPaged<T, C>(const TinyTensor<T>&, const TinyTensor<T>&, TinyTensor<C>&, TinyTensor<C>&,     \
+                                    const TinyTensor<int>&, const TinyTensor<int>&, const TinyTensor<float>*,       \
+                                    const TinyTensor<float>*, float, const TinyTensor<int>*, bool, bool,            \
+                                    TinyTensor<uint8_t>*, TinyTensor<uint8_t>*);                                    \
+  template void KvGatherPaged<T, C>(const TinyTensor<C>&, const TinyTensor<C>&, const TinyTensor<int>&,             \
+                                    const TinyTensor<int>&, TinyTensor<T>&, TinyTensor<T>&, int,                    \
+                                    const TinyTensor<uint8_t>*, const TinyTensor<uint8_t>*);                        \
+  template void AttentionDecodePaged<T, C>(const TinyTensor<T>&, const TinyTensor<C>&, const TinyTensor<C>&,        \
+                                           const TinyTensor<int>&, const TinyTensor<int>&, TinyTensor<T>&, float,   \
+                                           const TinyTensor<uint8_t>*, const TinyTensor<uint8_t>*);
+TT_HEAD_LAYERS(float)
+TT_HEAD_LAYERS(bf16)
+TT_PAGED_LAYERS(float, float)
+TT_PAGED_LAYERS(bf16, bf16)
+TT_PAGED_LAYERS(float, uint8_t)
+TT_PAGED_LAYERS(bf16, uint8_t)
+#undef TT_HEAD_LAYERS
+#undef TT_PAGED_LAYERS

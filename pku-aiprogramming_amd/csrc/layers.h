@@ -144,3 +144,54 @@ void MaxPoolingBackward(const TinyTensor<T>& grad_output, const TinyTensor<T>& m
                         const std::vector<int>& input_shape, const std::vector<int>& kernel_shape, int pad_h,
                         int pad_w, int stride_h, int stride_w);
 
+// Heads normed and rotated by their positions (no counterpart in the reference).
+// Optional tensors are null pointers (None): weight [d], no norm without it;
+// inv_freq [rot / 2], no rotation; positions [B, T], or lengths [B] (the T newest
+// tokens of each sequence), else 0 .. T - 1.
+//
+// NormRopeForward: input [B, H, T, d] (tokens_first: [B, T, H, d]) -> output [B, H,
+// T, d].  NormRopeBackward: grad_output [B, H, T, d] -> grad_input in input's
+// layout, and grad_weight [d] (None where there is no weight).
+// QkvNormRopeForward: a fused projection [B, T, H + 2 kv_heads, d] -> q [B, H, T,
+// d], k and v [B, kv_heads, T, d], v unchanged; its backward gives grad_qkv.
+template <typename T>
+void NormRopeForward(const TinyTensor<T>& input, TinyTensor<T>& output, const TinyTensor<float>* weight,
+                     const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                     const TinyTensor<int>* lengths, bool interleaved, bool tokens_first);
+template <typename T>
+void NormRopeBackward(const TinyTensor<T>& input, const TinyTensor<T>& grad_output, TinyTensor<T>& grad_input,
+                      const TinyTensor<float>* weight, TinyTensor<float>* grad_weight,
+                      const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                      const TinyTensor<int>* lengths, bool interleaved, bool tokens_first);
+template <typename T>
+void QkvNormRopeForward(const TinyTensor<T>& qkv, TinyTensor<T>& q, TinyTensor<T>& k, TinyTensor<T>& v, int kv_heads,
+                        const TinyTensor<float>* q_weight, const TinyTensor<float>* k_weight,
+                        const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions,
+                        const TinyTensor<int>* lengths, bool interleaved);
+template <typename T>
+void QkvNormRopeBackward(const TinyTensor<T>& qkv, const TinyTensor<T>& grad_q, const TinyTensor<T>& grad_k,
+                         const TinyTensor<T>& grad_v, TinyTensor<T>& grad_qkv, const TinyTensor<float>* q_weight,
+                         const TinyTensor<float>* k_weight, TinyTensor<float>* grad_q_weight,
+                         TinyTensor<float>* grad_k_weight, const TinyTensor<float>* inv_freq, float eps,
+                         const TinyTensor<int>* positions, const TinyTensor<int>* lengths, bool interleaved);
+
+// A K/V cache in pages (no counterpart in the reference): pools [pages, Hkv, page,
+// d], of the call's type, or Tensor_byte codes with Tensor_byte scales [pages, Hkv];
+// table [B, width] of each sequence's pages, lengths [B] with the T newest tokens
+// counted.  KvAppendPaged: k, v [B, Hkv, T, d] (tokens_first: [B, T, Hkv, d]) into the
+// pools in place, K normed and rotated on the way.  KvGatherPaged: the first
+// `length` keys back to k, v [B, Hkv, length, d]; rows behind a sequence's end are
+// left as they are.  AttentionDecodePaged: q [B, H, T, d] -> out.
+template <typename T, typename C>
+void KvAppendPaged(const TinyTensor<T>& k, const TinyTensor<T>& v, TinyTensor<C>& k_pages, TinyTensor<C>& v_pages,
+                   const TinyTensor<int>& table, const TinyTensor<int>& lengths, const TinyTensor<float>* k_weight,
+                   const TinyTensor<float>* inv_freq, float eps, const TinyTensor<int>* positions, bool interleaved,
+                   bool tokens_first, TinyTensor<uint8_t>* k_scales, TinyTensor<uint8_t>* v_scales);
+template <typename T, typename C>
+void KvGatherPaged(const TinyTensor<C>& k_pages, const TinyTensor<C>& v_pages, const TinyTensor<int>& table,
+                   const TinyTensor<int>& lengths, TinyTensor<T>& k, TinyTensor<T>& v, int length,
+                   const TinyTensor<uint8_t>* k_scales, const TinyTensor<uint8_t>* v_scales);
+template <typename T, typename C>
+void AttentionDecodePaged(const TinyTensor<T>& q, const TinyTensor<C>& k_pages, const TinyTensor<C>& v_pages,
+                          const TinyTensor<int>& table, const TinyTensor<int>& lengths, TinyTensor<T>& out,
+                          float scale, const TinyTensor<uint8_t>* k_scales, const TinyTensor<uint8_t>* v_scales);

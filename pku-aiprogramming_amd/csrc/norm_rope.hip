@@ -64,14 +64,6 @@ __device__ __forceinline__ void nr_weight(const float* w, const Lay<N>& lay, flo
     f[N + e] = w ? w[lay.b + e] : 1.f;
   }
 }
-template <int N, int LPR>
-__device__ __forceinline__ float nr_scale(const float (&f)[2 * N], float eps) {
-  float ss = 0.f;
-#pragma unroll
-  for (int e = 0; e < 2 * N; ++e) ss += f[e] * f[e];
-  return __builtin_amdgcn_rsqf(row_sum<LPR>(ss) * (1.f / (2 * N * LPR)) + eps);
-}
-
 // A workgroup: 256 / LPR tokens, heads [first, first + count) of q's, k's and v's in a row.
 template <typename T, int D>
 __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_kernel(NrPart<T> q, NrPart<T> k, NrPart<T> v, Rope rp,
@@ -114,11 +106,7 @@ __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_kernel(NrPart<T> q, 
         }
         float f[2 * N];
         r[u].get(f);
-        if (p.w) {
-          const float scale = nr_scale<N, LPR>(f, rp.eps);
-#pragma unroll
-          for (int e = 0; e < 2 * N; ++e) f[e] *= scale * w[e];
-        }
+        if (p.w) rope_scale<N>(f, rope_rms<N, LPR>(f, rp.eps), w);
         if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
         nr_store<T, N>(to, lay, f);
       }
@@ -201,7 +189,7 @@ __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T>
           if (p.w) {
             float z[2 * N];
             r[u].get(z);
-            const float scale = nr_scale<N, LPR>(z, rp.eps);
+            const float scale = rope_rms<N, LPR>(z, rp.eps);
             float m = 0.f;
 #pragma unroll
             for (int e = 0; e < 2 * N; ++e) {

@@ -138,26 +138,8 @@ __device__ __forceinline__ int64_t rope_position(const Rope& rp, int64_t b, int6
   return (rp.lengths ? (int64_t)rp.lengths[b] - T : 0) + t;
 }
 
-// A lane's pairs (a side, b side): chunks' elements e of x[0], x[1] as pairs.
-// Pair j of N is (x[0][j], x[1][j]), or INTER: elements 2j and 2j + 1 of both chunks in a row.
-template <int N, typename F>
-__device__ __forceinline__ void rope_turn(F (&x)[2 * N], const F (&c)[N], const F (&s)[N], bool inter) {
-  if (inter) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const F a = x[2 * j], b = x[2 * j + 1];
-      x[2 * j] = a * c[j] - b * s[j];
-      x[2 * j + 1] = a * s[j] + b * c[j];
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const F a = x[j], b = x[N + j];
-      x[j] = a * c[j] - b * s[j];
-      x[N + j] = a * s[j] + b * c[j];
-    }
-  }
-}
+__device__ __forceinline__ float rope_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
+__device__ __forceinline__ double rope_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
 // Sum over the LPR neighbouring lanes that hold a row, the same in each.
 template <int LPR, typename F>
@@ -165,6 +147,51 @@ __device__ __forceinline__ F row_sum(F x) {
 #pragma unroll
   for (int off = 1; off < LPR; off <<= 1) x += __shfl_xor(x, off, 64);
   return x;
+}
+
+// The operations below are spelled out, so that every kernel gives a row the same bits.
+
+// A lane's 2 N values with its pairs turned: pair j is values j and N + j, or INTER
+// 2 j and 2 j + 1.
+template <int N, typename F>
+__device__ __forceinline__ void rope_turn(F (&x)[2 * N], const F (&c)[N], const F (&s)[N], bool inter) {
+#pragma clang fp contract(off)
+  if (inter) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const F a = x[2 * j], b = x[2 * j + 1];
+      x[2 * j] = rope_fma(a, c[j], -(b * s[j]));
+      x[2 * j + 1] = rope_fma(a, s[j], b * c[j]);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const F a = x[j], b = x[N + j];
+      x[j] = rope_fma(a, c[j], -(b * s[j]));
+      x[N + j] = rope_fma(a, s[j], b * c[j]);
+    }
+  }
+}
+
+// 1 / sqrt(mean x^2 + eps) of the row that LPR lanes hold.
+template <int N, int LPR, typename F>
+__device__ __forceinline__ F rope_rms(const F (&x)[2 * N], float eps) {
+#pragma clang fp contract(off)
+  F ss = x[0] * x[0];
+#pragma unroll
+  for (int e = 1; e < 2 * N; ++e) ss = rope_fma(x[e], x[e], ss);
+  ss = rope_fma(row_sum<LPR>(ss), F(1.0 / (2 * N * LPR)), F(eps));
+  if constexpr (sizeof(F) == 8)
+    return 1.0 / __builtin_sqrt(ss);
+  else
+    return __builtin_amdgcn_rsqf(ss);
+}
+// x times that and the weight.
+template <int N, typename F>
+__device__ __forceinline__ void rope_scale(F (&x)[2 * N], F r, const float (&w)[2 * N]) {
+#pragma clang fp contract(off)
+#pragma unroll
+  for (int e = 0; e < 2 * N; ++e) x[e] = x[e] * (r * F(w[e]));
 }
 
 }  // namespace tt

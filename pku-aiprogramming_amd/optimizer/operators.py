@@ -689,6 +689,68 @@ def attention(q, k, v, causal: bool = False, scale: Optional[float] = None, dtyp
     return Attention(causal, scale, dtype)(q, k, v)
 
 
+def rope_frequencies(rot: int, base: float = 10000.0) -> np.ndarray:
+    """base^(-2 i / rot) for the rot / 2 pairs of a rotated head, float32."""
+    return (float(base) ** (-2.0 * np.arange(rot // 2) / rot)).astype(np.float32)
+
+
+class NormRope(TensorOp):
+    """Heads normed and rotated by their positions on the MI355X, as queries and
+    keys go into ``attention``: x [B, H, T, d], or [B, T, H, d] with
+    ``tokens_first`` (a projection's output), to [B, H, T, d].
+
+    With ``norm`` a second input, the weight [d], is a part of the graph:
+    x / sqrt(mean x^2 + eps) * weight over each head.  ``inv_freq`` [rot / 2]
+    turns pair i of a head at position p by p inv_freq[i] (None: no rotation);
+    positions are ``positions`` [B, T], or 0 .. T - 1.  The gradients are those of
+    both inputs."""
+
+    def __init__(self, norm: bool = True, inv_freq=None, positions=None, eps: float = 1e-6, interleaved: bool = False,
+                 tokens_first: bool = False, dtype: str = "float32"):
+        if dtype not in _ATTN_DTYPES:
+            raise ValueError(f"NormRope dtype must be one of {sorted(_ATTN_DTYPES)}, got {dtype!r}")
+        self.norm, self.eps, self.dtype = bool(norm), float(eps), dtype
+        self.interleaved, self.tokens_first = bool(interleaved), bool(tokens_first)
+        self.inv_freq = None if inv_freq is None else np.asarray(inv_freq, np.float32)
+        self.positions = None if positions is None else np.asarray(positions, np.int32)
+
+    def _device(self, arrays):
+        if len(arrays) != (2 if self.norm else 1):
+            raise ValueError(f"NormRope takes {'x and its weight' if self.norm else 'x alone'}")
+        x = _ATTN_DTYPES[self.dtype](np.asarray(arrays[0], np.float32), "gpu")
+        rest = dict(eps=self.eps, interleaved=self.interleaved, tokens_first=self.tokens_first)
+        if self.norm:
+            rest["weight"] = Tensor_float(np.asarray(arrays[1], np.float32), "gpu")
+        if self.inv_freq is not None:
+            rest["inv_freq"] = Tensor_float(self.inv_freq, "gpu")
+        if self.positions is not None:
+            rest["positions"] = Tensor_int(self.positions, "gpu")
+        return x, rest
+
+    def compute(self, *arrays):
+        x, rest = self._device(arrays)
+        out = _ATTN_DTYPES[self.dtype]([1], "gpu")
+        ml.NormRopeForward(x, out, **rest)
+        return out.numpy()
+
+    def gradient(self, out_grad, node):
+        x, rest = self._device([t.realize_cached_data() for t in node.inputs])
+        T = _ATTN_DTYPES[self.dtype]
+        go, gx = T(np.asarray(out_grad.realize_cached_data(), np.float32), "gpu"), T([1], "gpu")
+        if not self.norm:
+            ml.NormRopeBackward(x, go, gx, **rest)
+            return Tensor(gx, requires_grad=False)
+        gw = Tensor_float([1], "gpu")
+        ml.NormRopeBackward(x, go, gx, grad_weight=gw, **rest)
+        return Tensor(gx, requires_grad=False), Tensor(gw, requires_grad=False)
+
+
+def norm_rope(x, weight=None, inv_freq=None, positions=None, eps: float = 1e-6, interleaved: bool = False,
+              tokens_first: bool = False, dtype: str = "float32"):
+    op = NormRope(weight is not None, inv_freq, positions, eps, interleaved, tokens_first, dtype)
+    return op(x) if weight is None else op(x, weight)
+
+
 class AttentionDecode(TensorOp):
     """Single-query decode (forward only): q [B, H, 1, d] against a K/V cache
     [B, H, Lkv, d], no mask; the memory-bound split-KV kernel."""

@@ -378,6 +378,168 @@ def attn_decode_mxfp4(q: DeviceBuffer, k_codes: DeviceBuffer, k_scales: DeviceBu
                stream)
 
 
+# ------------------------------------------------------------------ norms of heads, position rotation
+
+def _ptr(b: Optional[DeviceBuffer], elements: int = 0):
+    return None if b is None else b.ptr + elements * b.ITEM[b.dtype]
+
+
+def _floats(what: str, *bufs: Optional[DeviceBuffer]) -> int:
+    """The dtype code that the float buffers share."""
+    return _mx_dtype(what, *(b for b in bufs if b is not None))
+
+
+def _vector(what: str, name: str, b: Optional[DeviceBuffer], shape, dtype: str):
+    if b is not None and (b.dtype != dtype or tuple(b.shape) != tuple(shape)):
+        raise ValueError(f"{what}: {name} is a {dtype} buffer {tuple(shape)}")
+
+
+def _rope_args(what: str, B: int, T: int, inv_freq, positions, lengths):
+    _vector(what, "positions", positions, (B, T), "i32")
+    _vector(what, "lengths", lengths, (B,), "i32")
+    if inv_freq is not None and (inv_freq.dtype != "f32" or len(inv_freq.shape) != 1):
+        raise ValueError(f"{what}: inv_freq is an f32 buffer [rot / 2]")
+    return _ptr(inv_freq), 2 * inv_freq.shape[0] if inv_freq is not None else 0
+
+
+def norm_rope(x: DeviceBuffer, y: DeviceBuffer, weight: Optional[DeviceBuffer] = None,
+              inv_freq: Optional[DeviceBuffer] = None, eps: float = 1e-6, positions: Optional[DeviceBuffer] = None,
+              lengths: Optional[DeviceBuffer] = None, interleaved: bool = False, tokens_first: bool = False, stream=None):
+    """x [B, H, T, d] (tokens_first: [B, T, H, d]) normed over each head and rotated, to y [B, H, T, d]."""
+    B, H, T, d = y.shape
+    if tuple(x.shape) != ((B, T, H, d) if tokens_first else (B, H, T, d)):
+        raise ValueError("norm_rope: x and y disagree on their shape")
+    _vector("norm_rope", "weight", weight, (d,), "f32")
+    freq, rot = _rope_args("norm_rope", B, T, inv_freq, positions, lengths)
+    lib().call("tt_qkv_norm_rope", _floats("norm_rope", x, y), x.ptr, None, None, H * d if tokens_first else 0, 0, 0,
+               _ptr(weight), None, eps, freq, rot, int(interleaved), _ptr(positions), _ptr(lengths), y.ptr, None, None, B, H, 0,
+               T, d, stream)
+
+
+def norm_rope_backward(x: Optional[DeviceBuffer], dy: DeviceBuffer, dx: DeviceBuffer,
+                       weight: Optional[DeviceBuffer] = None, dweight: Optional[DeviceBuffer] = None,
+                       inv_freq: Optional[DeviceBuffer] = None, eps: float = 1e-6,
+                       positions: Optional[DeviceBuffer] = None, lengths: Optional[DeviceBuffer] = None,
+                       interleaved: bool = False, tokens_first: bool = False, stream=None):
+    """dx in x's layout and dweight [d] for dy [B, H, T, d]; x may be None where no weight is."""
+    B, H, T, d = dy.shape
+    for t in (x, dx):
+        if t is not None and tuple(t.shape) != ((B, T, H, d) if tokens_first else (B, H, T, d)):
+            raise ValueError("norm_rope_backward: x, dx and dy disagree on their shape")
+    _vector("norm_rope_backward", "weight", weight, (d,), "f32")
+    _vector("norm_rope_backward", "dweight", dweight, (d,), "f32")
+    freq, rot = _rope_args("norm_rope_backward", B, T, inv_freq, positions, lengths)
+    ld = H * d if tokens_first else 0
+    lib().call("tt_qkv_norm_rope_backward", _floats("norm_rope_backward", x, dy, dx), _ptr(x), None, ld, 0, _ptr(weight), None,
+               eps, freq, rot, int(interleaved), _ptr(positions), _ptr(lengths), dy.ptr, None, None, dx.ptr, None, None, ld, 0,
+               0, _ptr(dweight), None, B, H, 0, T, d, stream)
+
+
+def _fused(what: str, qkv: DeviceBuffer, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer):
+    (B, H, T, d), Hkv = q.shape, k.shape[1]
+    if tuple(k.shape) != (B, Hkv, T, d) or tuple(v.shape) != (B, Hkv, T, d) or tuple(qkv.shape) != (B, T, H + 2 * Hkv, d):
+        raise ValueError(f"{what}: qkv is [B, T, H + 2 Hkv, d], q [B, H, T, d], k and v [B, Hkv, T, d]")
+    return B, H, Hkv, T, d, (H + 2 * Hkv) * d
+
+
+def qkv_norm_rope(qkv: DeviceBuffer, q: DeviceBuffer, k: DeviceBuffer, v: DeviceBuffer,
+                  q_weight: Optional[DeviceBuffer] = None, k_weight: Optional[DeviceBuffer] = None,
+                  inv_freq: Optional[DeviceBuffer] = None, eps: float = 1e-6, positions: Optional[DeviceBuffer] = None,
+                  lengths: Optional[DeviceBuffer] = None, interleaved: bool = False, stream=None):
+    """A fused projection qkv [B, T, H + 2 Hkv, d] to q, k (normed, rotated) and v, all [B, heads, T, d]."""
+    B, H, Hkv, T, d, ld = _fused("qkv_norm_rope", qkv, q, k, v)
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        _vector("qkv_norm_rope", name, w, (d,), "f32")
+    freq, rot = _rope_args("qkv_norm_rope", B, T, inv_freq, positions, lengths)
+    lib().call("tt_qkv_norm_rope", _floats("qkv_norm_rope", qkv, q, k, v), qkv.ptr, _ptr(qkv, H * d), _ptr(qkv, (H + Hkv) * d),
+               ld, ld, ld, _ptr(q_weight), _ptr(k_weight), eps, freq, rot, int(interleaved), _ptr(positions), _ptr(lengths),
+               q.ptr, k.ptr, v.ptr, B, H, Hkv, T, d, stream)
+
+
+def qkv_norm_rope_backward(qkv: DeviceBuffer, dq: DeviceBuffer, dk: DeviceBuffer, dv: DeviceBuffer, dqkv: DeviceBuffer,
+                           q_weight: Optional[DeviceBuffer] = None, k_weight: Optional[DeviceBuffer] = None,
+                           dq_weight: Optional[DeviceBuffer] = None, dk_weight: Optional[DeviceBuffer] = None,
+                           inv_freq: Optional[DeviceBuffer] = None, eps: float = 1e-6,
+                           positions: Optional[DeviceBuffer] = None, lengths: Optional[DeviceBuffer] = None,
+                           interleaved: bool = False, stream=None):
+    """dqkv [B, T, H + 2 Hkv, d] and the weights' gradients [d] for dq, dk, dv [B, heads, T, d]."""
+    B, H, Hkv, T, d, ld = _fused("qkv_norm_rope_backward", qkv, dq, dk, dv)
+    if tuple(dqkv.shape) != tuple(qkv.shape):
+        raise ValueError("qkv_norm_rope_backward: dqkv has qkv's shape")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight), ("dq_weight", dq_weight), ("dk_weight", dk_weight)):
+        _vector("qkv_norm_rope_backward", name, w, (d,), "f32")
+    freq, rot = _rope_args("qkv_norm_rope_backward", B, T, inv_freq, positions, lengths)
+    lib().call("tt_qkv_norm_rope_backward", _floats("qkv_norm_rope_backward", qkv, dq, dk, dv, dqkv), qkv.ptr,
+               _ptr(qkv, H * d), ld, ld, _ptr(q_weight), _ptr(k_weight), eps, freq, rot, int(interleaved), _ptr(positions),
+               _ptr(lengths), dq.ptr, dk.ptr, dv.ptr, dqkv.ptr, _ptr(dqkv, H * d), _ptr(dqkv, (H + Hkv) * d), ld, ld, ld,
+               _ptr(dq_weight), _ptr(dk_weight), B, H, Hkv, T, d, stream)
+
+
+# ------------------------------------------------------------------ paged cache
+
+def _paged(what: str, k_pages, v_pages, table, lengths, k_scales, v_scales):
+    """(cache code, pool pointers .. lengths, npages, Hkv, page, d, B, width)."""
+    if len(k_pages.shape) != 4 or tuple(v_pages.shape) != tuple(k_pages.shape) or v_pages.dtype != k_pages.dtype:
+        raise ValueError(f"{what}: k_pages and v_pages are [pages, Hkv, page, d] of one dtype")
+    npages, Hkv, page, d = k_pages.shape
+    codes = {"u8": TT_E4M3, "bf16": TT_BF16, "f32": TT_F32}
+    if k_pages.dtype not in codes:
+        raise ValueError(f"{what}: pages are f32, bf16 or u8 buffers")
+    for name, s in (("k_scales", k_scales), ("v_scales", v_scales)):
+        if (s is None) == (k_pages.dtype == "u8"):
+            raise ValueError(f"{what}: u8 pages come with scales, others without")
+        _vector(what, name, s, (npages, Hkv), "u8")
+    if table.dtype != "i32" or len(table.shape) != 2:
+        raise ValueError(f"{what}: table is an i32 buffer [B, width]")
+    B, width = table.shape
+    _vector(what, "lengths", lengths, (B,), "i32")
+    at = (k_pages.ptr, v_pages.ptr, _ptr(k_scales), _ptr(v_scales), table.ptr, lengths.ptr)
+    return codes[k_pages.dtype], at, npages, Hkv, page, d, B, width
+
+
+def kv_append_paged(k: DeviceBuffer, v: DeviceBuffer, k_pages: DeviceBuffer, v_pages: DeviceBuffer, table: DeviceBuffer,
+                    lengths: DeviceBuffer, k_weight: Optional[DeviceBuffer] = None,
+                    inv_freq: Optional[DeviceBuffer] = None, eps: float = 1e-6,
+                    positions: Optional[DeviceBuffer] = None, interleaved: bool = False, tokens_first: bool = False,
+                    k_scales: Optional[DeviceBuffer] = None, v_scales: Optional[DeviceBuffer] = None, stream=None):
+    """New rows k, v [B, Hkv, T, d] (tokens_first: [B, T, Hkv, d]) into the pages; lengths count them already."""
+    code, at, npages, Hkv, page, d, B, width = _paged("kv_append_paged", k_pages, v_pages, table, lengths, k_scales, v_scales)
+    T = k.shape[1 if tokens_first else 2]
+    if tuple(k.shape) != ((B, T, Hkv, d) if tokens_first else (B, Hkv, T, d)) or tuple(v.shape) != tuple(k.shape):
+        raise ValueError("kv_append_paged: k and v are [B, Hkv, T, d] of the cache")
+    _vector("kv_append_paged", "k_weight", k_weight, (d,), "f32")
+    freq, rot = _rope_args("kv_append_paged", B, T, inv_freq, positions, None)
+    ld = Hkv * d if tokens_first else 0
+    lib().call("tt_kv_append_paged", _floats("kv_append_paged", k, v), code, k.ptr, v.ptr, ld, ld, _ptr(k_weight), eps, freq,
+               rot, int(interleaved), _ptr(positions), *at, B, Hkv, T, d, npages, page, width, stream)
+
+
+def kv_gather_paged(k_pages: DeviceBuffer, v_pages: DeviceBuffer, table: DeviceBuffer, lengths: DeviceBuffer, k: DeviceBuffer,
+                    v: DeviceBuffer, k_scales: Optional[DeviceBuffer] = None, v_scales: Optional[DeviceBuffer] = None,
+                    stream=None):
+    """The cache's first L keys back to contiguous k, v [B, Hkv, L, d]; rows behind a sequence's end stay."""
+    code, at, npages, Hkv, page, d, B, width = _paged("kv_gather_paged", k_pages, v_pages, table, lengths, k_scales, v_scales)
+    L = k.shape[2]
+    if tuple(k.shape) != (B, Hkv, L, d) or tuple(v.shape) != tuple(k.shape):
+        raise ValueError("kv_gather_paged: k and v are [B, Hkv, L, d] of the cache")
+    lib().call("tt_kv_gather_paged", _floats("kv_gather_paged", k, v), code, *at, k.ptr, v.ptr, B, Hkv, L, d, npages, page,
+               width, stream)
+
+
+def attn_decode_paged(q: DeviceBuffer, k_pages: DeviceBuffer, v_pages: DeviceBuffer, table: DeviceBuffer,
+                      lengths: DeviceBuffer, o: DeviceBuffer, lse: Optional[DeviceBuffer], scale: float,
+                      k_scales: Optional[DeviceBuffer] = None, v_scales: Optional[DeviceBuffer] = None, stream=None):
+    """Attention of the T newest tokens q [B, H, T, d] over the pages."""
+    code, at, npages, Hkv, page, d, B, width = _paged("attn_decode_paged", k_pages, v_pages, table, lengths, k_scales,
+                                                      v_scales)
+    H, T = q.shape[1], q.shape[2]
+    if tuple(q.shape) != (B, H, T, d) or tuple(o.shape) != tuple(q.shape):
+        raise ValueError("attn_decode_paged: q and o are [B, H, T, d]")
+    _vector("attn_decode_paged", "lse", lse, (B, H, T), "f32")
+    lib().call("tt_attn_decode_paged", _floats("attn_decode_paged", q, o), code, q.ptr, *at, o.ptr, _ptr(lse), B, H, Hkv, T, d,
+               npages, page, width, scale, stream)
+
+
 # ------------------------------------------------------------------ softmax
 
 def softmax_rows(x: DeviceBuffer, y: DeviceBuffer, stream=None):
