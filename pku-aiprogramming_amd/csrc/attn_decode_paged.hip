@@ -5,21 +5,23 @@
 // The bytes of the cache bound it, K and V each read once, so all R = H / Hkv * T
 // query rows that share one K / V head go through the matrix unit as a tile of 16
 // columns.  A wave owns a step of keys at a time (32; 16 of fp32) with a running
-// maximum and sum of its own:
-//   S^T [keys x 16 rows] = K Q^T: a lane's piece of a K row is the operand as it is
-//     loaded (8-bit codes after v_cvt_scalef32_pk_bf16_fp8, exactly): the order of
-//     the contraction is free, and q is laid out to match.  fp32 pools take the fp32
+// maximum and sum of its own, and goes through them without meeting the others:
+//   K and V rows come straight into the wave's own LDS tiles, a load the whole 128
+//     byte lines of neighbouring rows, each tile loaded again as soon as it was read.
+//     (Loaded to registers, in the operand's layout, every line took two requests.)
+//   S^T [keys x 16 rows] = K Q^T: a lane reads its piece of a K row; 8-bit codes
+//     become bf16 by v_cvt_scalef32_pk_bf16_fp8, exactly.  The order of the
+//     contraction is free, and q is laid out to match.  fp32 pools take the fp32
 //     unit.  Result: a lane owns one query row and four keys of each 16.
-//   O^T [D x 16 rows] += V^T P^T: P comes out of S^T in the operand's layout.  V
-//     rows go through the wave's LDS tile and are read back transposed
-//     (ds_read_b64_tr_b16); fp32 needs no transposition, since a lane holds one key
-//     an operand there, and columns may be numbered as they were loaded.  P is
-//     split into bf16 terms (two for bf16 calls, 2^-17 off; three for fp32 calls,
-//     whose q is split into three exact terms too).
+//   O^T [D x 16 rows] += V^T P^T: P comes out of S^T in the operand's layout.  V is
+//     read transposed (ds_read_b64_tr_b16, and _tr_b8 with the conversion behind
+//     it); fp32 needs no transposition, since a lane holds one key an operand there,
+//     and columns may be numbered as they were read.  P is split into bf16 terms
+//     (two for bf16 calls, 2^-17 off; three for fp32 calls, whose q is split into
+//     three exact terms too).
 // A page is 16 keys or a multiple, so a step's 16 keys never straddle two.  The
-// wave holds the next 128 places of its sequence's table in two registers, from
-// which a page's number comes without memory's latency.  K of the next step is
-// loaded once its registers are free, behind the scores, V behind the store to LDS.
+// wave holds the next 128 places of its sequence's table in registers, from
+// which a page's number comes without memory's latency.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -38,67 +40,64 @@
 namespace tt {
 namespace {
 
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+#ifndef PD_LB
+#define PD_LB(C, D) (sizeof(C) == 1 ? (sizeof(T) == 4 && D == 128 ? 3 : 4) : 2)
+#endif
 
 __device__ __forceinline__ f32x4 mfma_f32_16x16x4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// A lane's share of one row of 16, a quarter: DW dwords in pieces of up to 16 bytes
-// that alternate between the four lanes of a row, so that a wave's load takes whole
-// runs of a row.
-template <typename C, int D>
-struct PdRow {
-  static constexpr int DW = D * sizeof(C) / 16, PW = DW < 4 ? DW : 4, NP = DW / PW;
-  uint32_t w[DW];
-  // STREAM: rows that no other workgroup reads are loaded past the caches.
-  template <bool STREAM>
-  __device__ __forceinline__ void load(const C* row, int g) {
-    typedef uint32_t vec __attribute__((ext_vector_type(PW)));
-    const vec* from = reinterpret_cast<const vec*>(row) + g;
-#pragma unroll
-    for (int i = 0; i < NP; ++i) {
-      const vec x = STREAM ? __builtin_nontemporal_load(from + 4 * i) : from[4 * i];
-      __builtin_memcpy(w + PW * i, &x, 4 * PW);
-    }
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+// A wave's tile of rows as they lie in a pool, in 16-byte chunks: chunk c of row r
+// at chunk c ^ exchange(r), so that chunk c of 16 rows, and four rows' neighbouring
+// chunks, spread over the banks.
+template <typename C, int D, int ROWS>
+struct PdTile {
+  static constexpr int ROWB = D * sizeof(C), CPR = ROWB / 16, BYTES = ROWS * ROWB;
+  static constexpr int LOADS = BYTES / 1024, RPL = 64 / CPR;  // loads of a wave, rows of a load
+  __device__ static __forceinline__ constexpr uint32_t exchange(uint32_t r) {
+    return ROWB >= 256 ? r & 15u : (r / (256 / ROWB)) & (CPR - 1);  // the same for rows 16 apart
+  }
+  __device__ static __forceinline__ uint32_t at(uint32_t r, uint32_t chunk) {
+    return r * ROWB + 16u * (chunk ^ exchange(r));
   }
 };
-// The first of the eight values that lane g brings to k step j.
+// The chunk, and the first of the eight codes in it, that lane g brings to k step j.
 template <typename C, int D>
-__device__ __forceinline__ constexpr int pd_first(int j, int g) {
-  if (sizeof(C) == 2) return 8 * (4 * j + g);
-  return PdRow<C, D>::PW == 4 ? 16 * (4 * (j >> 1) + g) + 8 * (j & 1) : 8 * g;
+__device__ __forceinline__ constexpr int pd_chunk(int j, int g) {
+  return sizeof(C) != 1 ? 4 * j + g : D == 32 ? g >> 1 : 4 * (j >> 1) + g;
 }
-template <int D>
-__device__ __forceinline__ bf16x8 pd_operand(const PdRow<u16, D>& x, int j, float) {
-  bf16x8 v;
-  __builtin_memcpy(&v, x.w + 4 * j, 16);
-  return v;
+template <typename C, int D>
+__device__ __forceinline__ constexpr int pd_half(int j, int g) {
+  return sizeof(C) != 1 ? 0 : D == 32 ? 8 * (g & 1) : 8 * (j & 1);
 }
-template <int D>
-__device__ __forceinline__ bf16x8 pd_operand(const PdRow<uint8_t, D>& x, int j, float scale) {
-  const uint32_t lo = x.w[2 * j], hi = x.w[2 * j + 1];
-  const uint32_t w[4] = {__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
-                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
-                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
-                         __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
+// Four codes as two pairs of bf16.
+__device__ __forceinline__ void pd_cvt(uint32_t codes, float scale, uint32_t* w) {
+  w[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
+  w[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true));
+}
+__device__ __forceinline__ bf16x8 pd_cvt8(const u32x2& codes, float lo, float hi) {
+  uint32_t w[4];
+  pd_cvt(codes.x, lo, w);
+  pd_cvt(codes.y, hi, w + 2);
   return __builtin_bit_cast(bf16x8, w);
 }
-// Whether a value may be infinite or NaN.
-template <int D>
-__device__ __forceinline__ bool pd_odd(const PdRow<u16, D>& x, uint32_t) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < PdRow<u16, D>::DW; ++i) any |= (x.w[i] & 0x7f807f80u) + 0x00800080u;
-  return (any & 0x80008000u) != 0;
+// ds_read_b64_tr_b8: within 16 lanes, lane t receives element t % 8 of the 8-byte
+// chunks addressed by lanes 2 e + t / 8, e = 0 .. 7 (checked on the MI355X).
+__device__ __forceinline__ u32x2 lds_tr8_at(uint32_t a) {
+  typedef int i32x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)a));
 }
-template <int D>
-__device__ __forceinline__ bool pd_odd(const PdRow<uint8_t, D>& x, uint32_t byte) {
-  uint32_t any = 0;
-#pragma unroll
-  for (int i = 0; i < PdRow<uint8_t, D>::DW; ++i) any |= (x.w[i] & 0x7f7f7f7fu) + 0x01010101u;
-  return (any & 0x80808080u) != 0 || byte > kE4MaxByte;
+// At most N of the wave's loads are outstanding (they retire in order), and none of
+// its LDS reads: nothing that touches memory moves across either.
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
+__device__ __forceinline__ void wait_reads() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7f800000u) != 0x7f800000u; }
 // The finite values, zeros for the others.
 __device__ __forceinline__ bf16x8 pd_clean(const bf16x8& x) {
@@ -125,30 +124,48 @@ __device__ __forceinline__ void pd_four(const uint8_t* row, int c, float scale, 
 #pragma unroll
   for (int e = 0; e < 4; ++e) x[e] *= scale;
 }
-__device__ __forceinline__ void pd_four(const float* row, int c, float, float (&x)[4]) { __builtin_memcpy(x, row + c, 16); }
 
 // The wave's place in its sequence's table: entries [base, base + 64) and the 64
-// after them, one a lane.  Pages behind the sequence's last are none.
+// after them, one a lane, -1 where the pool has no such page or the sequence ends;
+// of 8-bit pools with their scale bytes, which are loaded 64 pages ahead and their
+// entries 128, so that no step waits for either.  (Loaded in the step, the scales
+// cost it a latency, and all loads before them: 64 x 32 heads x 8192 keys 790 us.)
+template <bool E4>
 struct PdTable {
   const int* row;
-  int count, base, now, next;
+  const uint8_t *ks, *vs;  // of this head
+  int count, pages, hkv, base, id[E4 ? 3 : 2];
+  uint32_t kb[2], vb[2];
   __device__ __forceinline__ int load(int from) const {
     const int at = from + (int)(threadIdx.x & 63);
-    return at < count ? row[at] : -1;
+    const int x = at < count ? row[at] : -1;
+    return x < pages ? x : -1;
   }
-  __device__ __forceinline__ void start(const int* r, int n, int from) {
-    row = r, count = n, base = from;
-    now = load(base);
-    next = load(base + 64);
+  __device__ __forceinline__ void scales(int i) {
+    kb[i] = vb[i] = 127u;
+    if (id[i] >= 0) {
+      kb[i] = ks[(int64_t)id[i] * hkv];
+      vb[i] = vs[(int64_t)id[i] * hkv];
+    }
   }
-  // Page `at`: asked for in order, each at most 64 behind the one before.
-  __device__ __forceinline__ int page(int at) {
+  __device__ __forceinline__ void start(int from) {
+    base = from;
+#pragma unroll
+    for (int i = 0; i < (E4 ? 3 : 2); ++i) id[i] = load(base + 64 * i);
+    if constexpr (E4) scales(0), scales(1);
+  }
+  // The lane that holds place `at`: asked for in order, each at most 64 behind the one before.
+  __device__ __forceinline__ int lane(int at) {
     if (at - base >= 64) {
       base += 64;
-      now = next;
-      next = load(base + 64);
+      id[0] = id[1];
+      if constexpr (E4) {
+        kb[0] = kb[1], vb[0] = vb[1], id[1] = id[2];
+        scales(1);
+      }
+      id[E4 ? 2 : 1] = load(base + (E4 ? 128 : 64));
     }
-    return __builtin_amdgcn_readlane(now, at - base);
+    return at - base;
   }
 };
 
@@ -158,8 +175,8 @@ struct PdTable {
 // Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv, tile =
 // 16 of the head's R query rows.  Each sequence's own length is cut into nsplit
 // spans, so that sequences of any length keep every workgroup busy.
-template <typename T, typename C, int D, bool STREAM>
-__global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
+template <typename T, typename C, int D>
+__global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_kernel(
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, Pages pg, float* __restrict__ part_o, float2* __restrict__ part_ml,
     T* __restrict__ o, float* __restrict__ lse, uint32_t R, uint32_t tokens, uint32_t tiles, uint32_t nsplit,
@@ -170,10 +187,10 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
   constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;  // terms of q and of the weights
   constexpr int ND = D / 16;                                 // 16-row tiles of O^T
   constexpr int VW = F32 ? (D < 64 ? D / 16 : 4) : 4;        // fp32: neighbouring columns of a lane
-  constexpr int VG = F32 ? ND / VW : 1;                      // and groups of them
-  __shared__ __align__(256) u16 s_v[kMdWaves][kMdKeys * D];
+  using Tile = PdTile<C, D, KEYS>;
+  __shared__ __align__(1024) char s_tile[kMdWaves][2][Tile::BYTES];
   __shared__ float s_m[kMdWaves][kMdRows], s_l[kMdWaves][kMdRows];
-  static_assert(sizeof(s_v[0]) == kMdRows * D * sizeof(float), "the waves' sums reuse their tiles");
+  static_assert(sizeof(s_tile[0]) >= kMdRows * D * sizeof(float), "the waves' sums reuse their tiles");
 
   const int l = threadIdx.x & 63, r = l & 15, g = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -196,19 +213,78 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
     kend = (int)min((uint32_t)kbeg + span, (uint32_t)len);
   }
 
+  const int slots = (1 << pg.lp) - 1;
+  const int64_t head_rows = (int64_t)hk << pg.lp, page_rows = (int64_t)pg.hkv << pg.lp;
+  // A step's 16s: their first rows in the pool (the same for the wave), and what is known of them.
+  struct Step {
+    int64_t row[U];
+    bool has[U];
+    uint32_t kb[U], vb[U];
+  };
+  PdTable<E4> table{pg.table + (int64_t)b * pg.width, ks + hk, vs + hk, (len + slots) >> pg.lp,
+                    (int)min(pg.pages, (int64_t)0x7fffffff), (int)pg.hkv};
+  auto look = [&](Step& s, int j0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int key = j0 + 16 * u, at = table.lane(key >> pg.lp);
+      const int id = __builtin_amdgcn_readlane(table.id[0], at);
+      s.has[u] = key < kend && id >= 0;
+      s.row[u] = (s.has[u] ? id : 0) * page_rows + head_rows + (key & slots);
+      if (u > 0 && key >= kend) s.row[u] = s.row[0];  // rows that have been written
+      if constexpr (E4) {
+        s.kb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.kb[0], at);
+        s.vb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.vb[0], at);
+      }
+    }
+  };
+
+  // The step's rows of one pool into a tile.  Rows of a 16 past the sequence's end
+  // are taken from its last: masked below.
+  const uint32_t tile_k = lds_addr(s_tile[w][0]), tile_v = lds_addr(s_tile[w][1]);
+  auto fetch = [&](const Step& s, const C* pool, uint32_t tile, int j0) {
+    const bool whole = j0 + KEYS <= len;
+#pragma unroll
+    for (int n = 0; n < Tile::LOADS; ++n) {
+      const uint32_t row = (uint32_t)(n * Tile::RPL) + (uint32_t)l / Tile::CPR;  // of the tile, and its chunk here
+      const uint32_t chunk = ((uint32_t)l % Tile::CPR) ^ Tile::exchange(row);
+      auto in_half = [&](uint32_t x, int u) { return whole ? x : (uint32_t)min((int)x, max(len - 1 - (j0 + 16 * u), 0)); };
+      if constexpr (Tile::RPL <= 16) {
+        const int u = n * Tile::RPL / 16;
+        glds16(pool + s.row[u] * D, in_half(row - 16u * u, u) * Tile::ROWB + 16u * chunk, tile + 1024u * n);
+      } else {
+        const int u = row >= 16u ? 1 : 0;
+        const int64_t first = u ? s.row[U - 1] : s.row[0];
+        glds16_at(reinterpret_cast<const char*>(pool + first * D) + (in_half(row & 15u, u) * Tile::ROWB + 16u * chunk),
+                  tile + 1024u * n);
+      }
+    }
+  };
+
+  constexpr int kStep = kMdWaves * KEYS;
+  const int jbeg = kbeg + w * KEYS;
+  int j0 = jbeg;
+  Step cur, nxt;
+  if (j0 < kend) {
+    table.start(j0 >> pg.lp);
+    look(cur, j0);
+    fetch(cur, kp, tile_k, j0);
+    fetch(cur, vp, tile_v, j0);
+  }
+
   // q in the layout that K has: lane g's values of each k step
   typename std::conditional<F32, f32x4, bf16x8>::type qf[W][F32 ? 1 : NQ];
 #pragma unroll
   for (int j = 0; j < W; ++j) {
+    const int first = (16 * pd_chunk<C, D>(j, g) + pd_half<C, D>(j, g)) / (int)sizeof(C);
     if constexpr (F32) {
       f32x4 x = {0.f, 0.f, 0.f, 0.f};
-      if (r < nrows) x = *reinterpret_cast<const f32x4*>(q + (qrow + r) * D + 4 * (4 * j + g));
+      if (r < nrows) x = *reinterpret_cast<const f32x4*>(q + (qrow + r) * D + first);
       qf[j][0] = negative ? -x : x;
     } else {
       float x[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) x[e] = 0.f;
-      if (r < nrows) md_load8(q + (qrow + r) * D + pd_first<C, D>(j, g), x);
+      if (r < nrows) md_load8(q + (qrow + r) * D + first, x);
       if (negative)
 #pragma unroll
         for (int e = 0; e < 8; ++e) x[e] = -x[e];
@@ -217,117 +293,74 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
   }
 
   f32x4 acc[ND];
-#pragma unroll
-  for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, lsum = 0.f;
-  u16* tile = s_v[w];
-  constexpr uint32_t kRow = 2 * D;  // bytes of a tile row
-  const uint32_t put = lds_addr(tile) + (uint32_t)r * kRow +
-                       16u * (uint32_t)((E4 && PdRow<C, D>::PW == 4 ? 2 * g : g) ^ md_exchange<D>(r));
-  const int krow = 4 * g + (r >> 2);
-  const uint32_t get = lds_addr(tile) + (uint32_t)krow * kRow + 16u * (uint32_t)(((r & 3) >> 1) ^ md_exchange<D>(krow)) +
-                       8u * (uint32_t)(r & 1);
+  float m, lsum;
+  const uint32_t kread = tile_k + (uint32_t)r * Tile::ROWB;
+  const uint32_t kex = Tile::exchange((uint32_t)r);
+  // rows 4 g + (0 .. 3) of each 16 of V, and a lane's place in its transposed read
+  const int vrow = E4 ? 16 * ((r >> 3) & 1) + 4 * g + ((r >> 1) & 3) : 4 * g + (r >> 2);
+  const uint32_t vread = tile_v + (uint32_t)vrow * Tile::ROWB + 8u * (uint32_t)(r & 1);
+  const uint32_t vex = Tile::exchange((uint32_t)vrow);
 
-  const int slots = (1 << pg.lp) - 1;
-  const int64_t head_rows = (int64_t)hk << pg.lp, page_rows = (int64_t)pg.hkv << pg.lp;
-  // A step's pages: its first row in the pool (the same for the wave), and what is known of it.
-  struct Step {
-    int64_t row[U];
-    bool has[U];
-    uint32_t kb[U], vb[U];
-  };
-  PdTable table;
-  auto look = [&](Step& s, int j0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int key = j0 + 16 * u;
-      int id = table.page(key >> pg.lp);
-      s.has[u] = key < kend && id >= 0 && id < pg.pages;
-      id = s.has[u] ? id : 0;
-      s.row[u] = id * page_rows + head_rows + (key & slots);
-      if constexpr (E4) {
-        s.kb[u] = ks[(int64_t)id * pg.hkv + hk];
-        s.vb[u] = vs[(int64_t)id * pg.hkv + hk];
-      }
-    }
-  };
-  // Rows of a 16 past the sequence's end are taken from its last: masked below.
-  auto row_of = [&](int row, int key) { return key + 16 <= len ? row : min(row, max(len - 1 - key, 0)); };
-
-  typedef typename std::conditional<F32, float, uint32_t>::type word;
-  PdRow<C, D> kr[U];
-  PdRow<C, D> vr[F32 ? 1 : U];
-  float vf[F32 ? 4 : 1][VG][VW];
-  auto fetch_k = [&](const Step& s, int j0) {
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      kr[u].template load<STREAM>(kp + (s.row[u] * D + row_of(r, j0 + 16 * u) * D), g);
-  };
-  auto fetch_v = [&](const Step& s, int j0) {
-    if constexpr (F32) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const C* from = vp + (s.row[0] * D + row_of(4 * g + i, j0) * D + VW * r);
-#pragma unroll
-        for (int k = 0; k < VG; ++k) {
-          typedef float vec __attribute__((ext_vector_type(VW)));
-          const vec* p = reinterpret_cast<const vec*>(from + 16 * VW * k);
-          const vec x = STREAM ? __builtin_nontemporal_load(p) : *p;
-          __builtin_memcpy(vf[i][k], &x, 4 * VW);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u)
-        vr[u].template load<STREAM>(vp + (s.row[u] * D + row_of(r, j0 + 16 * u) * D), g);
-    }
-  };
-
-  constexpr int kStep = kMdWaves * KEYS;
-  int j0 = kbeg + w * KEYS;
-  Step cur, nxt;
-  if (j0 < kend) {
-    const int64_t page = int64_t(1) << pg.lp;
-    table.start(pg.table + (int64_t)b * pg.width, (int)((len + page - 1) >> pg.lp), j0 >> pg.lp);
-    look(cur, j0);
-    fetch_k(cur, j0);
-    fetch_v(cur, j0);
-  }
-  for (; j0 < kend; j0 += kStep) {
-    const bool more = j0 + kStep < kend;
-    if (more) look(nxt, j0 + kStep);
-
-    // s[u][i]: key 16 u + 4 g + i of the step, for this lane's row
-    f32x4 s[U];
+  // s[u][i]: key 16 u + 4 g + i of the step, for this lane's row
+  auto scores = [&](const Step& st, f32x4(&s)[U]) {
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       s[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      u32x4 x = {0, 0, 0, 0};
 #pragma unroll
       for (int j = 0; j < W; ++j) {
+        const uint32_t at = kread + u * 16 * Tile::ROWB + 16u * ((uint32_t)pd_chunk<C, D>(j, g) ^ kex);
         if constexpr (F32) {
-          f32x4 a;
-          __builtin_memcpy(&a, kr[u].w + 4 * j, 16);
+          const f32x4 a = lds_ld<f32x4>(at);
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[u] = mfma_f32_16x16x4(a[e], qf[j][0][e], s[u]);
         } else {
-          const bf16x8 a = pd_operand<D>(kr[u], j, e4_scale(E4 ? cur.kb[u] : 0));
+          bf16x8 a;
+          if constexpr (!E4) {
+            a = lds_ld<bf16x8>(at);
+          } else {
+            const float scale = e4_scale(st.kb[u]);
+            if constexpr (D == 32)
+              a = pd_cvt8(lds_ld<u32x2>(at + 8u * (uint32_t)(g & 1)), scale, scale);
+            else {
+              if (j % 2 == 0) x = lds_ld<u32x4>(at);
+              a = pd_cvt8(j % 2 == 0 ? u32x2{x.x, x.y} : u32x2{x.z, x.w}, scale, scale);
+            }
+          }
 #pragma unroll
           for (int n = NQ - 1; n >= 0; --n) s[u] = mfma_bf16_16x16x32(a, qf[j][n], s[u]);
         }
       }
     }
-    if (more) fetch_k(nxt, j0 + kStep);
-
+  };
+  // whether some row does not see some key of the step
+  auto at_edge = [&](const Step& st, int j0) {
     bool edge = j0 + KEYS > min(kend, all_see);
 #pragma unroll
-    for (int u = 0; u < U; ++u) edge |= !cur.has[u];
-    if (edge) {
+    for (int u = 0; u < U; ++u) edge |= !st.has[u];
+    return edge;
+  };
+  auto mask = [&](const Step& st, f32x4(&s)[U], int j0) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          s[u][i] = cur.has[u] && j0 + 16 * u + 4 * g + i < min(seen, kend) ? s[u][i] : -INFINITY;
+      for (int i = 0; i < 4; ++i)
+        s[u][i] = st.has[u] && j0 + 16 * u + 4 * g + i < min(seen, kend) ? s[u][i] : -INFINITY;
+  };
+
+  // One step: the last one (MORE = false) loads nothing.  CAREFUL: without V's
+  // infinite and NaN values.
+  auto step = [&](auto more, auto careful) {
+    constexpr bool MORE = decltype(more)::value, CAREFUL = decltype(careful)::value;
+    if constexpr (MORE) look(nxt, j0 + kStep);
+    wait_loads<Tile::LOADS>();  // V's may go on
+    f32x4 s[U];
+    scores(cur, s);
+    if constexpr (MORE) {
+      wait_reads();
+      fetch(nxt, kp, tile_k, j0 + kStep);
     }
+    if (at_edge(cur, j0)) mask(cur, s, j0);
 
     float top = -INFINITY;
 #pragma unroll
@@ -354,95 +387,130 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
       lsum += p[e];
     }
 
-    // A weight of zero must not meet an infinity or a NaN, be it a masked key's or a
-    // bf16 term of a weight: such values of V are zeros in the product, and what
-    // the rows that see them get is added apart.
-    bool odd = false;
-    if constexpr (F32) {
-      if (edge)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int k = 0; k < VG; ++k)
-#pragma unroll
-            for (int c = 0; c < VW; ++c) {
-              odd |= !finite(vf[i][k][c]);
-              vf[i][k][c] = finite(vf[i][k][c]) ? vf[i][k][c] : 0.f;
-            }
-    } else {
-#pragma unroll
-      for (int u = 0; u < U; ++u) odd |= pd_odd<D>(vr[u], E4 ? cur.vb[u] : 0);
-    }
-    odd = wave_any(odd);
-
+    wait_loads<MORE ? Tile::LOADS : 0>();  // V is there; the next K may go on
     if constexpr (F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t row = (uint32_t)(4 * g + i);
 #pragma unroll
-        for (int k = 0; k < VG; ++k)
+        for (int k = 0; k < ND / VW; ++k) {
+          float v[VW];
+          if constexpr (VW == 4) {
+            const f32x4 x = lds_ld<f32x4>(tile_v + Tile::at(row, (uint32_t)(16 * k + r)));
+            __builtin_memcpy(v, &x, 16);
+          } else {
+            typedef float f32x2 __attribute__((ext_vector_type(2)));
+            const f32x2 x = lds_ld<f32x2>(tile_v + Tile::at(row, (uint32_t)(r >> 1)) + 8u * (uint32_t)(r & 1));
+            v[0] = x[0], v[1] = x[1];
+          }
 #pragma unroll
-          for (int c = 0; c < VW; ++c) acc[k * VW + c] = mfma_f32_16x16x4(vf[i][k][c], p[i], acc[k * VW + c]);
-      if (more) fetch_v(nxt, j0 + kStep);
+          for (int c = 0; c < VW; ++c) {
+            if (CAREFUL && !finite(v[c])) v[c] = 0.f;
+            acc[k * VW + c] = mfma_f32_16x16x4(v[c], p[i], acc[k * VW + c]);
+          }
+        }
+      }
     } else {
       bf16x8 pf[NP];
       md_terms<NP>(p, pf);
 #pragma unroll
-      for (int u = 0; u < U; ++u)
-#pragma unroll
-        for (int j = 0; j < W; ++j) {
-          bf16x8 x = pd_operand<D>(vr[u], j, e4_scale(E4 ? cur.vb[u] : 0));
-          if (odd) x = pd_clean(x);
-          lds_st((put ^ (16u * (uint32_t)(pd_first<C, D>(j, 0) / 8))) + u * 16 * kRow, x);
-        }
-      if (more) fetch_v(nxt, j0 + kStep);
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-#pragma unroll
       for (int i = 0; i < ND; ++i) {
-        const uint32_t at = get ^ (32u * i);
-        const bf16x8 a = lds_tr16x2_at(at, at + 16 * kRow);
+        bf16x8 a;
+        if constexpr (E4) {
+          const uint32_t at = vread + 16u * ((uint32_t)i ^ vex);
+          a = pd_cvt8(lds_tr8_at(at), e4_scale(cur.vb[0]), e4_scale(cur.vb[U - 1]));
+        } else {
+          const uint32_t at = vread + 16u * ((uint32_t)(2 * i + ((r & 3) >> 1)) ^ vex);
+          a = lds_tr16x2_at(at, at + 16 * Tile::ROWB);
+        }
+        if constexpr (CAREFUL) a = pd_clean(a);
 #pragma unroll
         for (int n = NP - 1; n >= 0; --n) acc[i] = mfma_bf16_16x16x32(a, pf[n], acc[i]);
       }
-      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
-    if (odd) {  // rare
-      for (int kk = 0; kk < KEYS; ++kk) {
-        const int u = U > 1 ? kk >> 4 : 0, in = kk & 15, key = j0 + kk;
-        if (key >= kend || !(u ? cur.has[U - 1] : cur.has[0])) continue;
-        const float a = (in & 2) ? ((in & 1) ? p[3] : p[2]) : ((in & 1) ? p[1] : p[0]);
-        const float z = (in & 2) ? ((in & 1) ? p[4 * U - 1] : p[4 * U - 2]) : ((in & 1) ? p[4 * U - 3] : p[4 * U - 4]);
-        const float wgt = __shfl(u ? z : a, 16 * (in >> 2) + r, 64);  // this row's, from the lane that holds the key's
-        const C* from = vp + ((u ? cur.row[U - 1] : cur.row[0]) + in) * D;
-        const float scale = e4_scale(E4 ? (u ? cur.vb[U - 1] : cur.vb[0]) : 0);
-        if (key >= seen) continue;
+    if constexpr (MORE) {
+      wait_reads();
+      fetch(nxt, vp, tile_v, j0 + kStep);
+    }
+  };
+  auto steps = [&](auto careful) {
 #pragma unroll
-        for (int i = 0; i < ND; ++i)  // columns 16 i + 4 g and three more, in the order that acc has them
-          if constexpr (!F32) {
-            float x[4];
-            pd_four(from, 16 * i + 4 * g, scale, x);
+    for (int i = 0; i < ND; ++i) acc[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    m = -INFINITY, lsum = 0.f;
+    if (j0 >= kend) return;
+    for (; j0 + kStep < kend; j0 += kStep) {
+      step(std::true_type(), careful);
+      cur = nxt;
+    }
+    step(std::false_type(), careful);
+  };
+  steps(std::false_type());
+
+  // A weight of zero must not meet an infinity or a NaN of V, be it a masked key's
+  // or a bf16 term of a weight.  Where one was met, some sum shows it (rare): then
+  // the steps are gone through again without such values, and what the rows that
+  // see their keys get of them is added under the weights of the final maximum.
+  bool odd = false;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (!finite(x[e])) acc[i][e] += wgt * x[e];
-          } else {
+  for (int i = 0; i < ND; ++i)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float x = from[16 * VW * (i / VW) + VW * (4 * g + e) + i % VW];
-              if (!finite(x) && edge) acc[i][e] += wgt * x;
+    for (int e = 0; e < 4; ++e) odd |= !finite(acc[i][e]);
+  if (wave_any(odd && r < nrows)) {
+    auto again = [&](auto&& body) {
+      j0 = jbeg;
+      wait_reads();
+      table.start(j0 >> pg.lp);
+      look(cur, j0);
+      fetch(cur, kp, tile_k, j0);
+      body();
+    };
+    again([&] {
+      fetch(cur, vp, tile_v, j0);
+      steps(std::true_type());
+    });
+    const float mb = m == -INFINITY ? 0.f : sl2 * m;
+    again([&] {
+      for (; j0 < kend; j0 += kStep) {
+        if (j0 != jbeg) {
+          wait_reads();
+          look(cur, j0);
+          fetch(cur, kp, tile_k, j0);
+        }
+        wait_loads<0>();
+        f32x4 s[U];
+        scores(cur, s);
+        if (at_edge(cur, j0)) mask(cur, s, j0);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          for (int in = 0; in < 16 && cur.has[u]; ++in) {
+            const int key = j0 + 16 * u + in;
+            float wgt = (in & 2) ? ((in & 1) ? s[u][3] : s[u][2]) : ((in & 1) ? s[u][1] : s[u][0]);
+            wgt = __shfl(wgt, 16 * (in >> 2) + r, 64);  // this row's score, from the lane that holds the key's
+            wgt = fast_exp2(__builtin_fmaf(sl2, wgt, -mb));
+            if (key >= min(seen, kend)) continue;
+            const C* from = vp + (cur.row[u] + in) * D;
+#pragma unroll
+            for (int i = 0; i < ND; ++i) {  // the columns that acc[i] has here
+              float x[4];
+              if constexpr (F32) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x[e] = from[16 * VW * (i / VW) + VW * (4 * g + e) + i % VW];
+              } else {
+                pd_four(from, 16 * i + 4 * g, e4_scale(E4 ? cur.vb[u] : 0), x);
+              }
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (!finite(x[e])) acc[i][e] += wgt * x[e];
             }
           }
       }
-    }
-    cur = nxt;
+    });
   }
 
   // The waves' sums meet in LDS: [row][D] fp32 over each wave's own tile, chunks
   // of four columns swizzled by the row.
   lsum = sum_rows(lsum);
-  float* mine = reinterpret_cast<float*>(tile);
+  float* mine = reinterpret_cast<float*>(s_tile[w]);
 #pragma unroll
   for (int i = 0; i < ND; ++i) {
     f32x4 x = acc[i];
@@ -474,7 +542,7 @@ __global__ __launch_bounds__(kMdThreads, 3) void attn_decode_paged_kernel(
 #pragma unroll
     for (int i = 0; i < kMdWaves; ++i) {
       const float wgt = fast_exp2(s_m[i][row] - mb);
-      const float* theirs = reinterpret_cast<const float*>(s_v[i]);
+      const float* theirs = reinterpret_cast<const float*>(s_tile[i]);
       den += wgt * s_l[i][row];
       num += wgt * *reinterpret_cast<const f32x4*>(&theirs[row * D + 4 * (d4 ^ (row & (D / 4 - 1)))]);
     }
@@ -534,7 +602,7 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   static const int per_cu = [] {
     int n = 0;
     const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
-        &n, (const void*)attn_decode_paged_kernel<T, C, D, true>, kMdThreads, 0);
+        &n, (const void*)attn_decode_paged_kernel<T, C, D>, kMdThreads, 0);
     if (e != hipSuccess) (void)hipGetLastError();
     return e != hipSuccess || n < 1 ? 3 : n;
   }();
@@ -550,16 +618,9 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   memcpy(&bits, &sl2, sizeof(bits));
   bits = std::max(bits, 1u);
   memcpy(&sl2, &bits, sizeof(bits));
-#define TT_PD_LAUNCH(STREAM)                                                                                         \
-  hipLaunchKernelGGL((attn_decode_paged_kernel<T, C, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), \
-                     0, st, (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml,        \
-                     (T*)a.o, a.lse, (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2,        \
-                     a.scale < 0.f)
-  if (tiles == 1)
-    TT_PD_LAUNCH(true);
-  else
-    TT_PD_LAUNCH(false);
-#undef TT_PD_LAUNCH
+  hipLaunchKernelGGL((attn_decode_paged_kernel<T, C, D>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, st,
+                     (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml, (T*)a.o, a.lse,
+                     (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2, a.scale < 0.f);
   TT_LAUNCHED(fn, st);
   if (nsplit > 1) {
     hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, part_o, part_ml,
