@@ -90,6 +90,25 @@ __device__ __forceinline__ u32x2 lds_tr8_at(uint32_t a) {
   typedef int i32x2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2*)(uintptr_t)a));
 }
+// glds16 and glds16_at (attn_common.h), non-temporal where NT.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <bool NT>
+__device__ __forceinline__ void pd_glds16(const void* sbase, uint32_t voff, uint32_t lds) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+  else
+    glds16(sbase, voff, lds);
+}
+template <bool NT>
+__device__ __forceinline__ void pd_glds16_at(const void* p, uint32_t lds) {
+  if constexpr (NT)
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p), "s"(lds) : "memory", "m0");
+  else
+    glds16_at(p, lds);
+}
+#pragma clang diagnostic pop
+
 // At most N of the wave's loads are outstanding (they retire in order), and none of
 // its LDS reads: nothing that touches memory moves across either.
 template <int N>
@@ -175,7 +194,7 @@ struct PdTable {
 // Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv, tile =
 // 16 of the head's R query rows.  Each sequence's own length is cut into nsplit
 // spans, so that sequences of any length keep every workgroup busy.
-template <typename T, typename C, int D>
+template <typename T, typename C, int D, bool STREAM>
 __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_kernel(
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, Pages pg, float* __restrict__ part_o, float2* __restrict__ part_ml,
@@ -250,11 +269,11 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
       auto in_half = [&](uint32_t x, int u) { return whole ? x : (uint32_t)min((int)x, max(len - 1 - (j0 + 16 * u), 0)); };
       if constexpr (Tile::RPL <= 16) {
         const int u = n * Tile::RPL / 16;
-        glds16(pool + s.row[u] * D, in_half(row - 16u * u, u) * Tile::ROWB + 16u * chunk, tile + 1024u * n);
+        pd_glds16<STREAM>(pool + s.row[u] * D, in_half(row - 16u * u, u) * Tile::ROWB + 16u * chunk, tile + 1024u * n);
       } else {
         const int u = row >= 16u ? 1 : 0;
         const int64_t first = u ? s.row[U - 1] : s.row[0];
-        glds16_at(reinterpret_cast<const char*>(pool + first * D) + (in_half(row & 15u, u) * Tile::ROWB + 16u * chunk),
+        pd_glds16_at<STREAM>(reinterpret_cast<const char*>(pool + first * D) + (in_half(row & 15u, u) * Tile::ROWB + 16u * chunk),
                   tile + 1024u * n);
       }
     }
@@ -602,7 +621,7 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   static const int per_cu = [] {
     int n = 0;
     const hipError_t e = hipOccupancyMaxActiveBlocksPerMultiprocessor(
-        &n, (const void*)attn_decode_paged_kernel<T, C, D>, kMdThreads, 0);
+        &n, (const void*)attn_decode_paged_kernel<T, C, D, true>, kMdThreads, 0);
     if (e != hipSuccess) (void)hipGetLastError();
     return e != hipSuccess || n < 1 ? 3 : n;
   }();
@@ -618,9 +637,16 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   memcpy(&bits, &sl2, sizeof(bits));
   bits = std::max(bits, 1u);
   memcpy(&sl2, &bits, sizeof(bits));
-  hipLaunchKernelGGL((attn_decode_paged_kernel<T, C, D>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), 0, st,
-                     (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml, (T*)a.o, a.lse,
-                     (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2, a.scale < 0.f);
+#define TT_PD_LAUNCH(STREAM)                                                                                         \
+  hipLaunchKernelGGL((attn_decode_paged_kernel<T, C, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), \
+                     0, st, (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml,        \
+                     (T*)a.o, a.lse, (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2,        \
+                     a.scale < 0.f)
+  if (tiles == 1)
+    TT_PD_LAUNCH(true);
+  else
+    TT_PD_LAUNCH(false);
+#undef TT_PD_LAUNCH
   TT_LAUNCHED(fn, st);
   if (nsplit > 1) {
     hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, part_o, part_ml,
