@@ -188,6 +188,16 @@ struct PdTable {
   }
 };
 
+// Two floats to and from where every compute unit sees them, past the caches that only some share.
+__device__ __forceinline__ void pd_put_far(float* p, float a, float b) {
+  const uint64_t x = __float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 pd_get_far(const float* p) {
+  const uint64_t x = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return float2{__uint_as_float((uint32_t)x), __uint_as_float((uint32_t)(x >> 32))};
+}
+
 // The maximum is that of the products, the scale sl2 (of log2 e too, above zero:
 // its sign goes into q, and zero is the smallest fp32, 2^-149) enters the exponent,
 // 2^(sl2 s - sl2 m), one operation a score.
@@ -199,7 +209,7 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, Pages pg, float* __restrict__ part_o, float2* __restrict__ part_ml,
     T* __restrict__ o, float* __restrict__ lse, uint32_t R, uint32_t tokens, uint32_t tiles, uint32_t nsplit,
-    float sl2, bool negative) {
+    float sl2, bool negative, uint32_t* __restrict__ count) {
   constexpr bool F32 = sizeof(C) == 4, E4 = sizeof(C) == 1;  // fp32 pools; 8-bit ones
   constexpr int U = F32 ? 1 : 2, KEYS = 16 * U;              // 16s of keys, and keys, of a step
   constexpr int W = F32 ? D / 16 : D / 32;                   // k steps (fp32: pieces of four) of a key tile
@@ -238,23 +248,32 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
   struct Step {
     int64_t row[U];
     bool has[U];
+    int lane[U];
     uint32_t kb[U], vb[U];
   };
   PdTable<E4> table{pg.table + (int64_t)b * pg.width, ks + hk, vs + hk, (len + slots) >> pg.lp,
                     (int)min(pg.pages, (int64_t)0x7fffffff), (int)pg.hkv};
   auto look = [&](Step& s, int j0) {
+    // A wave's steps begin at even 16s from where its table does: a step's places are in one 64.
+    const int at = table.lane(j0 >> pg.lp);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int key = j0 + 16 * u, at = table.lane(key >> pg.lp);
-      const int id = __builtin_amdgcn_readlane(table.id[0], at);
+      const int key = j0 + 16 * u;
+      s.lane[u] = at + (key >> pg.lp) - (j0 >> pg.lp);
+      const int id = __builtin_amdgcn_readlane(table.id[0], s.lane[u]);
       s.has[u] = key < kend && id >= 0;
       s.row[u] = (s.has[u] ? id : 0) * page_rows + head_rows + (key & slots);
       if (u > 0 && key >= kend) s.row[u] = s.row[0];  // rows that have been written
-      if constexpr (E4) {
-        s.kb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.kb[0], at);
-        s.vb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.vb[0], at);
-      }
     }
+  };
+  // The scales of what look() found last: apart, so that the rows' loads need not wait for them.
+  auto scales = [&](Step& s) {
+    if constexpr (E4)
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        s.kb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.kb[0], s.lane[u]);
+        s.vb[u] = (uint32_t)__builtin_amdgcn_readlane((int)table.vb[0], s.lane[u]);
+      }
   };
 
   // The step's rows of one pool into a tile.  Rows of a 16 past the sequence's end
@@ -288,6 +307,7 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
     look(cur, j0);
     fetch(cur, kp, tile_k, j0);
     fetch(cur, vp, tile_v, j0);
+    scales(cur);
   }
 
   // q in the layout that K has: lane g's values of each k step
@@ -371,7 +391,10 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
   // infinite and NaN values.
   auto step = [&](auto more, auto careful) {
     constexpr bool MORE = decltype(more)::value, CAREFUL = decltype(careful)::value;
-    if constexpr (MORE) look(nxt, j0 + kStep);
+    if constexpr (MORE) {
+      look(nxt, j0 + kStep);
+      scales(nxt);
+    }
     wait_loads<Tile::LOADS>();  // V's may go on
     f32x4 s[U];
     scores(cur, s);
@@ -480,6 +503,7 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
       wait_reads();
       table.start(j0 >> pg.lp);
       look(cur, j0);
+      scales(cur);
       fetch(cur, kp, tile_k, j0);
       body();
     };
@@ -493,6 +517,7 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
         if (j0 != jbeg) {
           wait_reads();
           look(cur, j0);
+          scales(cur);
           fetch(cur, kp, tile_k, j0);
         }
         wait_loads<0>();
@@ -567,17 +592,89 @@ __global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_ker
     }
     if (nsplit > 1) {
       const int64_t at = (qrow + row) * nsplit + split;
-      *reinterpret_cast<f32x4*>(part_o + at * D + 4 * d4) = num;
-      if (d4 == 0) part_ml[at] = float2{top, den};
+      if (count) {
+        pd_put_far(part_o + at * D + 4 * d4, num[0], num[1]);
+        pd_put_far(part_o + at * D + 4 * d4 + 2, num[2], num[3]);
+        if (d4 == 0) pd_put_far(&part_ml[at].x, top, den);
+      } else {
+        *reinterpret_cast<f32x4*>(part_o + at * D + 4 * d4) = num;
+        if (d4 == 0) part_ml[at] = float2{top, den};
+      }
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) md_put(o + (qrow + row) * D + 4 * d4 + e, md_quotient<T>(num[e], den));
       if (d4 == 0 && lse) lse[qrow + row] = md_lse(top, den);
     }
   }
+  if (nsplit == 1 || !count) return;
+
+  // The last workgroup of these rows to get here merges them: a workgroup's sums are
+  // where all others see them once its stores have ended, before it counts itself.
+  wait_loads<0>();
+  __syncthreads();
+  __shared__ uint32_t s_before;
+  if (threadIdx.x == 0) s_before = __hip_atomic_fetch_add(count + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  __syncthreads();
+  if (s_before != nsplit - 1) return;
+  if (threadIdx.x == 0) __hip_atomic_store(count + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
+  // A wave a row: its splits' maxima and sums a lane each, D / 4 lanes to a partial.
+  constexpr int TPR = D / 4, G = 64 / TPR;
+  const int c = l % TPR, gr = l / TPR;
+  for (int row = w; row < nrows; row += kMdWaves) {
+    const int64_t first = (qrow + row) * nsplit;
+    float2 ml = {-INFINITY, 0.f};
+    if ((uint32_t)l < nsplit) ml = pd_get_far(&part_ml[first + l].x);
+    f32x4 sum = {0.f, 0.f, 0.f, 0.f};
+    constexpr int UN = 8;
+    float wgt = 0.f, mx = -INFINITY, den = 0.f;
+    for (uint32_t i0 = 0; i0 < nsplit; i0 += G * UN) {
+      float2 x[UN][2];
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const uint32_t i = min(i0 + u * G + gr, nsplit - 1);
+        const float* po = part_o + (first + i) * D + 4 * c;
+        x[u][0] = pd_get_far(po);
+        x[u][1] = pd_get_far(po + 2);
+      }
+      if (i0 == 0) {  // behind the first partials' loads
+        mx = ml.x;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) mx = vmax(mx, __shfl_xor(mx, off, 64));
+        wgt = fast_exp2(ml.x - (mx == -INFINITY ? 0.f : mx));
+        den = wgt * ml.y;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) den += __shfl_xor(den, off, 64);
+      }
+#pragma unroll
+      for (int u = 0; u < UN; ++u) {
+        const uint32_t i = i0 + u * G + gr;
+        const float a = __shfl(wgt, (int)(i & 63u), 64);
+        if (i < nsplit) sum += a * f32x4{x[u][0].x, x[u][0].y, x[u][1].x, x[u][1].y};
+      }
+    }
+#pragma unroll
+    for (int off = TPR; off < 64; off <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], off, 64);
+    if (gr == 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) md_put(o + (qrow + row) * D + 4 * c + e, md_quotient<T>(sum[e], den));
+      if (c == 0 && lse) lse[qrow + row] = md_lse(mx, den);
+    }
+  }
 }
 
-constexpr size_t kPdWork = size_t(24) << 20;  // the partials' scratch, of one size so that graphs may keep its address
+__global__ __launch_bounds__(256) void pd_zero_kernel(uint32_t* p, int n) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) p[i] = 0u;
+}
+
+// Scratch, of one size so that graphs may keep its address: counts of the units'
+// workgroups, zero between calls, and the partials.
+constexpr int64_t kPdCounts = 16384;
+constexpr size_t kPdPartials = size_t(24) << 20, kPdWork = kPdPartials + kPdCounts * sizeof(uint32_t);
+// The last workgroup of a unit merges its splits where they are short, few, and a
+// wave has one row of them; else a launch of its own does.
+constexpr int64_t kPdMergeSpan = 512, kPdMergeSplits = 40;
 
 // Into how many splits to cut the keys: a workgroup costs its keys and about kPdFixed
 // more, a CU's time goes by the workgroups that fall to it, up to per_cu of them at
@@ -626,11 +723,19 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
     return e != hipSuccess || n < 1 ? 3 : n;
   }();
   int64_t nsplit = pd_splits(units, std::max<int64_t>(cap, 1), per_cu, device_cu_count(),
-                             (int64_t)(kPdWork / ((size_t)rows * (D + 2) * sizeof(float))));
+                             (int64_t)(kPdPartials / ((size_t)rows * (D + 2) * sizeof(float))));
   void* ws = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
-  if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsPagedDecode, kPdWork, &ws)) nsplit = 1;
-  float* part_o = (float*)ws;
+  bool fresh = false;
+  if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsPagedDecode, kPdWork, &ws, &fresh)) nsplit = 1;
+  if (fresh) {
+    hipLaunchKernelGGL(pd_zero_kernel, dim3(16), dim3(256), 0, st, (uint32_t*)ws, (int)kPdCounts);
+    TT_LAUNCHED(fn, st);
+  }
+  const bool fused = nsplit > 1 && nsplit <= kPdMergeSplits && cap <= nsplit * kPdMergeSpan && R <= kMdWaves &&
+                     units <= kPdCounts;
+  uint32_t* count = fused ? (uint32_t*)ws : nullptr;
+  float* part_o = (float*)ws + kPdCounts;
   float2* part_ml = (float2*)(part_o + rows * nsplit * D);
   float sl2 = std::fabs(a.scale * kLog2e);
   uint32_t bits;  // 1: the smallest fp32, formed as the host's arithmetic may flush it
@@ -641,14 +746,14 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   hipLaunchKernelGGL((attn_decode_paged_kernel<T, C, D, STREAM>), dim3((unsigned)(units * nsplit)), dim3(kMdThreads), \
                      0, st, (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml,        \
                      (T*)a.o, a.lse, (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2,        \
-                     a.scale < 0.f)
+                     a.scale < 0.f, count)
   if (tiles == 1)
     TT_PD_LAUNCH(true);
   else
     TT_PD_LAUNCH(false);
 #undef TT_PD_LAUNCH
   TT_LAUNCHED(fn, st);
-  if (nsplit > 1) {
+  if (nsplit > 1 && !fused) {
     hipLaunchKernelGGL((attn_decode_merge_kernel<T, D>), dim3((unsigned)rows), dim3(256), 0, st, part_o, part_ml,
                        (T*)a.o, a.lse, (int)nsplit);
     TT_LAUNCHED(fn, st);

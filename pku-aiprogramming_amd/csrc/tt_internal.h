@@ -66,8 +66,9 @@ class WorkspaceLease {
   bool get_optional(hipStream_t stream, int user, size_t bytes, void** ptr, uint64_t* uses = nullptr);
   // The same for a user whose requests are all of one size: its buffer is never
   // replaced, so a graph may keep the address, and a stream under capture gets
-  // the one that an earlier call left.
-  bool get_fixed(hipStream_t stream, int user, size_t bytes, void** ptr);
+  // the one that an earlier call left.  *fresh (optional): whether it is new, its
+  // contents undefined.
+  bool get_fixed(hipStream_t stream, int user, size_t bytes, void** ptr, bool* fresh = nullptr);
 
  private:
   struct Impl;

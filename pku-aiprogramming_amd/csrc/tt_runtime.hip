@@ -172,8 +172,13 @@ bool WorkspaceLease::get_optional(hipStream_t s, int user, size_t bytes, void** 
   RelaxedCapture relaxed;
   return get(s, user, bytes, ptr, uses) == TT_OK;
 }
-bool WorkspaceLease::get_fixed(hipStream_t s, int user, size_t bytes, void** ptr) {
-  return impl_->lease.get_held(static_cast<void*>(s), user, bytes, ptr) || get_optional(s, user, bytes, ptr);
+bool WorkspaceLease::get_fixed(hipStream_t s, int user, size_t bytes, void** ptr, bool* fresh) {
+  if (fresh) *fresh = false;
+  if (impl_->lease.get_held(static_cast<void*>(s), user, bytes, ptr)) return true;
+  uint64_t uses = 0;
+  if (!get_optional(s, user, bytes, ptr, &uses)) return false;
+  if (fresh) *fresh = uses == 0;
+  return true;
 }
 
 // ---------------------------------------------------------------- elementwise
