@@ -49,8 +49,20 @@ __global__ __launch_bounds__(kPgThreads) void kv_append_kernel(PgNew<T> in, Rope
   if (page < 0 || page >= pg.pages) return;
   const Lay<N> lay(threadIdx.x % LPR, rp.freq ? rp.rot : 0, rp.inter != 0);
   float c[N], s[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) c[i] = s[i] = 0.f;
   if (lay.turns && first < heads)
     rope_angles<N>(rp.freq + lay.pair, rp.positions ? rope_position(rp, b, t, tokens) : pos, c, s);
+  RopeTurn<N> turn;
+  if (first < heads) {
+    float w[2 * N];
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      w[e] = in.weight ? in.weight[lay.a + e] : 1.f;
+      w[N + e] = in.weight ? in.weight[lay.b + e] : 1.f;
+    }
+    turn.set(c, s, w, lay.turns, rp.inter != 0);
+  }
   const int64_t row = ((page * heads) << pg.lp) + (pos & ((1 << pg.lp) - 1));  // of head 0
   for (int side = 0; side < 2; ++side) {
     const int lo = max(first - side * heads, 0), hi = min(first + count - side * heads, heads);
@@ -60,11 +72,7 @@ __global__ __launch_bounds__(kPgThreads) void kv_append_kernel(PgNew<T> in, Rope
     x = ld ? x + (int64_t)n * ld : x + ((int64_t)b * heads * tokens + t) * D;
     T* y = (side ? vp : kp) + row * D;
     const int64_t ys = (int64_t)D << pg.lp;
-    const bool norm = !side && in.weight, turn = !side && lay.turns;
-    float w[2 * N];
-    if (norm)
-#pragma unroll
-      for (int e = 0; e < N; ++e) w[e] = in.weight[lay.a + e], w[N + e] = in.weight[lay.b + e];
+    const bool change = !side && (in.weight || rp.freq);
     for (int h = lo; h < hi; h += UN) {
       uint4 r[UN][2];
 #pragma unroll
@@ -77,12 +85,11 @@ __global__ __launch_bounds__(kPgThreads) void kv_append_kernel(PgNew<T> in, Rope
       for (int u = 0; u < UN; ++u) {
         if (h + u >= hi) break;
         T* to = y + (h + u) * ys;
-        if (norm || turn) {
+        if (change) {
           float f[2 * N];
           Chunk<T>::get(r[u][0], f);
           Chunk<T>::get(r[u][1], f + N);
-          if (norm) rope_scale<N>(f, rope_rms<N, LPR>(f, rp.eps), w);
-          if (turn) rope_turn<N>(f, c, s, rp.inter != 0);
+          turn(f, in.weight ? rope_rms<N, LPR>(f, rp.eps) : 1.f, lay.turns, rp.inter != 0);
           r[u][0] = Chunk<T>::put(f);
           r[u][1] = Chunk<T>::put(f + N);
         }

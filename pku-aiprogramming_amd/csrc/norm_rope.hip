@@ -26,6 +26,7 @@ namespace tt {
 namespace {
 
 constexpr int kNrThreads = 256;
+constexpr int kNrHeads = 4;  // of a workgroup at most
 
 // q, k or v: rows of `heads` heads, token-major with `ld` values a token, or
 // head-major [B][heads][T][D] (ld = 0).
@@ -38,24 +39,35 @@ struct NrPart {
   int heads;
 };
 
-template <typename T, int D>
+template <bool NT>
+__device__ __forceinline__ void nr_st(void* p, const uint4& x) {
+  if constexpr (NT)
+    __builtin_nontemporal_store(u32x4{x.x, x.y, x.z, x.w}, reinterpret_cast<u32x4*>(p));
+  else
+    *reinterpret_cast<uint4*>(p) = x;
+}
+// A lane's two chunks of a row.
+template <typename T, int D, bool NT>
 struct NrRow {
   static constexpr int N = Chunk<T>::N;
   uint4 a, b;
   __device__ __forceinline__ void load(const T* row, const Lay<N>& lay) {
-    a = ldg16(row + lay.a);
-    b = ldg16(row + lay.b);
+    a = NT ? ldg16_stream(row + lay.a) : ldg16(row + lay.a);
+    b = NT ? ldg16_stream(row + lay.b) : ldg16(row + lay.b);
   }
   __device__ __forceinline__ void get(float (&f)[2 * N]) const {
     Chunk<T>::get(a, f);
     Chunk<T>::get(b, f + N);
   }
+  __device__ __forceinline__ void put(const float (&f)[2 * N]) {
+    a = Chunk<T>::put(f);
+    b = Chunk<T>::put(f + N);
+  }
+  __device__ __forceinline__ void store(T* row, const Lay<N>& lay) const {
+    nr_st<NT>(row + lay.a, a);
+    nr_st<NT>(row + lay.b, b);
+  }
 };
-template <typename T, int N>
-__device__ __forceinline__ void nr_store(T* row, const Lay<N>& lay, const float (&f)[2 * N]) {
-  *reinterpret_cast<uint4*>(row + lay.a) = Chunk<T>::put(f);
-  *reinterpret_cast<uint4*>(row + lay.b) = Chunk<T>::put(f + N);
-}
 template <int N>
 __device__ __forceinline__ void nr_weight(const float* w, const Lay<N>& lay, float (&f)[2 * N]) {
 #pragma unroll
@@ -64,57 +76,89 @@ __device__ __forceinline__ void nr_weight(const float* w, const Lay<N>& lay, flo
     f[N + e] = w ? w[lay.b + e] : 1.f;
   }
 }
-// A workgroup: 256 / LPR tokens, heads [first, first + count) of q's, k's and v's in a row.
-template <typename T, int D>
+// Heads [lo, hi), at most HC of them, R rows each: all loaded before the first is
+// used, with `between` meanwhile.  A full chunk has a copy without branches, behind
+// which the compiler would wait for stores too.
+template <int HC, int R, typename Row, typename L, typename M, typename F>
+__device__ __forceinline__ void nr_heads(int lo, int hi, L&& load, M&& between, F&& use) {
+  Row r[HC][R];
+  if (hi - lo == HC) {
+#pragma unroll
+    for (int u = 0; u < HC; ++u) load(r[u], lo + u);
+    between();
+#pragma unroll
+    for (int u = 0; u < HC; ++u) use(r[u], lo + u);
+  } else {
+#pragma unroll
+    for (int u = 0; u < HC; ++u) load(r[u], min(lo + u, hi - 1));
+    between();
+#pragma unroll
+    for (int u = 0; u < HC; ++u)
+      if (lo + u < hi) use(r[u], lo + u);
+  }
+}
+
+// How a launch is cut: chunks of `count` heads of q's, k's and v's, one a workgroup.
+struct NrCut {
+  uint32_t chunks[3], all;
+  int count;
+};
+// The part of chunk `c`, and c's place in it.
+__device__ __forceinline__ int nr_part(const NrCut& cut, uint32_t* c) {
+  int part = 0;
+  if (*c >= cut.chunks[0]) {
+    *c -= cut.chunks[0];
+    part = 1;
+    if (*c >= cut.chunks[1]) {
+      *c -= cut.chunks[1];
+      part = 2;
+    }
+  }
+  return part;
+}
+
+// A workgroup: 256 / LPR tokens, a chunk of the heads of q, k or v.
+template <typename T, int D, int HC>
 __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_kernel(NrPart<T> q, NrPart<T> k, NrPart<T> v, Rope rp,
-                                                                   uint32_t rows, uint32_t tokens, uint32_t chunks,
-                                                                   int count) {
-  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR, UN = 2;
-  const uint32_t tile = blockIdx.x / chunks;
-  const int first = (int)(blockIdx.x - tile * chunks) * count;
+                                                                   uint32_t rows, uint32_t tokens, NrCut cut) {
+  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR;
+  using Row = NrRow<T, D, false>;
+  const uint32_t tile = blockIdx.x / cut.all;
+  uint32_t chunk = blockIdx.x - tile * cut.all;
+  const int part = nr_part(cut, &chunk);
+  const NrPart<T> p = part == 0 ? q : part == 1 ? k : v;
   const uint32_t n = tile * TPB + threadIdx.x / LPR;
   if (n >= rows) return;  // whole rows of lanes
   const uint32_t b = n / tokens, t = n - b * tokens;
-  const Lay<N> lay(threadIdx.x % LPR, rp.freq ? rp.rot : 0, rp.inter != 0);
-  float c[N], s[N];
-  if (lay.turns && first < q.heads + k.heads)
-    rope_angles<N>(rp.freq + lay.pair, rope_position(rp, b, t, tokens), c, s);
-
-  int at = first;  // heads of the parts before this one lie behind it
-  auto part = [&](const NrPart<T>& p, bool turn) {
-    const int lo = max(at, 0), hi = min(at + count, p.heads);
-    at -= p.heads;
-    if (lo >= hi) return;
-    const T* x = p.ld ? p.x + (int64_t)n * p.ld : p.x + ((int64_t)b * p.heads * tokens + t) * D;
-    T* y = p.y + ((int64_t)b * p.heads * tokens + t) * D;
-    const int64_t xs = p.ld ? D : (int64_t)tokens * D, ys = (int64_t)tokens * D;
-    float w[2 * N];
-    if (turn) nr_weight<N>(p.w, lay, w);
-    for (int h = lo; h < hi; h += UN) {
-      NrRow<T, D> r[UN];
+  const int lo = (int)chunk * cut.count, hi = min(lo + cut.count, p.heads);
+  const T* x = p.ld ? p.x + (int64_t)n * p.ld : p.x + ((int64_t)b * p.heads * tokens + t) * D;
+  T* y = p.y + ((int64_t)b * p.heads * tokens + t) * D;
+  const int64_t xs = p.ld ? D : (int64_t)tokens * D, ys = (int64_t)tokens * D;
+  const bool rotate = part < 2 && rp.freq;
+  const Lay<N> lay(threadIdx.x % LPR, rotate ? rp.rot : 0, rp.inter != 0);
+  auto load = [&](Row(&r)[1], int h) { r[0].load(x + h * xs, lay); };
+  if (!rotate && !p.w) {  // moved alone
+    nr_heads<HC, 1, Row>(lo, hi, load, [] {}, [&](const Row(&r)[1], int h) { r[0].store(y + h * ys, lay); });
+    return;
+  }
+  RopeTurn<N> turn;
+  nr_heads<HC, 1, Row>(
+      lo, hi, load,
+      [&] {
+        float c[N], s[N], w[2 * N];
 #pragma unroll
-      for (int u = 0; u < UN; ++u)
-        if (h + u < hi) r[u].load(x + (h + u) * xs, lay);
-#pragma unroll
-      for (int u = 0; u < UN; ++u) {
-        if (h + u >= hi) break;
-        T* to = y + (h + u) * ys;
-        if (!turn || (!p.w && !lay.turns)) {
-          *reinterpret_cast<uint4*>(to + lay.a) = r[u].a;
-          *reinterpret_cast<uint4*>(to + lay.b) = r[u].b;
-          continue;
-        }
+        for (int i = 0; i < N; ++i) c[i] = s[i] = 0.f;
+        nr_weight<N>(p.w, lay, w);
+        if (lay.turns) rope_angles<N>(rp.freq + lay.pair, rope_position(rp, b, t, tokens), c, s);
+        turn.set(c, s, w, lay.turns, rp.inter != 0);
+      },
+      [&](Row(&r)[1], int h) {
         float f[2 * N];
-        r[u].get(f);
-        if (p.w) rope_scale<N>(f, rope_rms<N, LPR>(f, rp.eps), w);
-        if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
-        nr_store<T, N>(to, lay, f);
-      }
-    }
-  };
-  part(q, true);
-  part(k, true);
-  part(v, false);
+        r[0].get(f);
+        turn(f, p.w ? rope_rms<N, LPR>(f, rp.eps) : 1.f, lay.turns, rp.inter != 0);
+        r[0].put(f);
+        r[0].store(y + h * ys, lay);
+      });
 }
 
 // A part on its way back: its gradient dy is head-major, dx lies as x does.
@@ -128,141 +172,150 @@ struct NrBack {
   int heads;
 };
 
-// A workgroup: tiles slot, slot + slots, ... of 256 / LPR tokens, a run of heads.
-// part [slots chunks][2][D], or null where no weight's gradient is asked for.
-template <typename T, int D>
+// A workgroup: tiles slot, slot + slots, ... of 256 / LPR tokens, a chunk of the heads
+// of q, k or v.  sums: [slots][chunks of q][D] and then [slots][chunks of k][D], or null
+// where no weight's gradient is asked for.
+template <typename T, int D, int HC, bool NT>
 __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T> q, NrBack<T> k, NrBack<T> v, Rope rp,
-                                                                       uint32_t rows, uint32_t tokens, uint32_t chunks,
-                                                                       uint32_t slots, int count,
-                                                                       float* __restrict__ sums) {
-  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR, UN = 2;
-  const uint32_t slot = blockIdx.x / chunks;
-  const int first = (int)(blockIdx.x - slot * chunks) * count;
+                                                                       uint32_t rows, uint32_t tokens, uint32_t slots,
+                                                                       NrCut cut, float* __restrict__ sums) {
+  constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR;
+  using Row = NrRow<T, D, NT>;
+  const uint32_t slot = blockIdx.x / cut.all;
+  uint32_t chunk = blockIdx.x - slot * cut.all;
+  const int part = nr_part(cut, &chunk);
+  const NrBack<T> p = part == 0 ? q : part == 1 ? k : v;
   const uint32_t tiles = (rows + TPB - 1) / TPB;
-  const Lay<N> lay(threadIdx.x % LPR, rp.freq ? rp.rot : 0, rp.inter != 0);
-  float acc[2][2 * N];
+  const bool rotate = part < 2 && rp.freq;
+  const Lay<N> lay(threadIdx.x % LPR, rotate ? rp.rot : 0, rp.inter != 0);
+  const int lo = (int)chunk * cut.count, hi = min(lo + cut.count, p.heads);
+  float acc[2 * N], w[2 * N];
 #pragma unroll
-  for (int e = 0; e < 2 * N; ++e) acc[0][e] = acc[1][e] = 0.f;
+  for (int e = 0; e < 2 * N; ++e) acc[e] = 0.f;
+  nr_weight<N>(p.w, lay, w);
 
   for (uint32_t tile = slot; tile < tiles; tile += slots) {
     const uint32_t n = tile * TPB + threadIdx.x / LPR;
     if (n >= rows) break;  // whole rows of lanes, and the last tile
     const uint32_t b = n / tokens, t = n - b * tokens;
+    const int64_t base = ((int64_t)b * p.heads * tokens + t) * D, ys = (int64_t)tokens * D;
+    const T* x = p.ldx ? p.x + (int64_t)n * p.ldx : p.x + base;
+    T* dx = p.ld ? p.dx + (int64_t)n * p.ld : p.dx + base;
+    const T* dy = p.dy + base;
+    const int64_t xs = p.ldx ? D : ys, ds = p.ld ? D : ys;
+    auto load = [&](Row(&r)[1], int h) { r[0].load(dy + h * ys, lay); };
+    if (!rotate && !p.w) {
+      nr_heads<HC, 1, Row>(lo, hi, load, [] {}, [&](const Row(&r)[1], int h) { r[0].store(dx + h * ds, lay); });
+      continue;
+    }
     float c[N], s[N];
-    if (lay.turns && first < q.heads + k.heads) {
+    auto angles = [&] {
+      if (!lay.turns) return;
       rope_angles<N>(rp.freq + lay.pair, rope_position(rp, b, t, tokens), c, s);
 #pragma unroll
       for (int i = 0; i < N; ++i) s[i] = -s[i];
-    }
-    int at = first;
-    auto part = [&](const NrBack<T>& p, bool turn, float (&sum)[2 * N]) {
-      const int lo = max(at, 0), hi = min(at + count, p.heads);
-      at -= p.heads;
-      if (lo >= hi) return;
-      const int64_t base = ((int64_t)b * p.heads * tokens + t) * D, ys = (int64_t)tokens * D;
-      const T* x = p.ldx ? p.x + (int64_t)n * p.ldx : p.x + base;
-      T* dx = p.ld ? p.dx + (int64_t)n * p.ld : p.dx + base;
-      const T* dy = p.dy + base;
-      const int64_t xs = p.ldx ? D : ys, ds = p.ld ? D : ys;
-      float w[2 * N];
-      if (turn) nr_weight<N>(p.w, lay, w);
-      for (int h = lo; h < hi; h += UN) {
-        NrRow<T, D> r[UN], g[UN];
-#pragma unroll
-        for (int u = 0; u < UN; ++u)
-          if (h + u < hi) {
-            g[u].load(dy + (h + u) * ys, lay);
-            if (p.w) r[u].load(x + (h + u) * xs, lay);
-          }
-#pragma unroll
-        for (int u = 0; u < UN; ++u) {
-          if (h + u >= hi) break;
-          T* to = dx + (h + u) * ds;
-          if (!turn || (!p.w && !lay.turns)) {
-            *reinterpret_cast<uint4*>(to + lay.a) = g[u].a;
-            *reinterpret_cast<uint4*>(to + lay.b) = g[u].b;
-            continue;
-          }
-          float f[2 * N];
-          g[u].get(f);
-          if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
-          if (p.w) {
-            float z[2 * N];
-            r[u].get(z);
-            const float scale = rope_rms<N, LPR>(z, rp.eps);
-            float m = 0.f;
-#pragma unroll
-            for (int e = 0; e < 2 * N; ++e) {
-              z[e] *= scale;
-              sum[e] += f[e] * z[e];
-              f[e] *= w[e];
-              m += f[e] * z[e];
-            }
-            m = row_sum<LPR>(m) * (1.f / D);
-#pragma unroll
-            for (int e = 0; e < 2 * N; ++e) f[e] = scale * (f[e] - z[e] * m);
-          }
-          nr_store<T, N>(to, lay, f);
-        }
-      }
     };
-    part(q, true, acc[0]);
-    part(k, true, acc[1]);
-    part(v, false, acc[1]);
-  }
-  if (!sums) return;
-  __shared__ float s_sum[kNrThreads / 64][2][D];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int e = 0; e < 2 * N; ++e) {
-      float x = acc[i][e];
-#pragma unroll
-      for (int off = LPR; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
-      if ((threadIdx.x & 63) < LPR) s_sum[threadIdx.x >> 6][i][(e < N ? lay.a : lay.b - N) + e] = x;
+    if (!p.w) {
+      nr_heads<HC, 1, Row>(lo, hi, load, angles, [&](Row(&r)[1], int h) {
+        float f[2 * N];
+        r[0].get(f);
+        if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
+        r[0].put(f);
+        r[0].store(dx + h * ds, lay);
+      });
+      continue;
     }
-  __syncthreads();
-  for (int i = threadIdx.x; i < 2 * D; i += kNrThreads) {
-    float x = 0.f;
+    nr_heads<HC, 2, Row>(
+        lo, hi,
+        [&](Row(&r)[2], int h) {
+          r[0].load(dy + h * ys, lay);
+          r[1].load(x + h * xs, lay);
+        },
+        angles,
+        [&](Row(&r)[2], int h) {
+          float f[2 * N], z[2 * N], m = 0.f;
+          r[0].get(f);
+          if (lay.turns) rope_turn<N>(f, c, s, rp.inter != 0);
+          r[1].get(z);
+          const float scale = rope_rms<N, LPR>(z, rp.eps);
 #pragma unroll
-    for (int w = 0; w < kNrThreads / 64; ++w) x += s_sum[w][0][i];
-    sums[(int64_t)blockIdx.x * (2 * D) + i] = x;
+          for (int e = 0; e < 2 * N; ++e) {
+            z[e] *= scale;
+            acc[e] += f[e] * z[e];
+            f[e] *= w[e];
+            m += f[e] * z[e];
+          }
+          m = row_sum<LPR>(m) * (1.f / D);
+#pragma unroll
+          for (int e = 0; e < 2 * N; ++e) f[e] = scale * (f[e] - z[e] * m);
+          r[0].put(f);
+          r[0].store(dx + h * ds, lay);
+        });
   }
+  if (!sums || part == 2) return;
+  __shared__ float s_sum[kNrThreads / 64][D];
+#pragma unroll
+  for (int e = 0; e < 2 * N; ++e) {
+    float x = acc[e];
+#pragma unroll
+    for (int off = LPR; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
+    if ((threadIdx.x & 63) < LPR) s_sum[threadIdx.x >> 6][(e < N ? lay.a : lay.b - N) + e] = x;
+  }
+  __syncthreads();
+  if (threadIdx.x >= D) return;
+  float x = 0.f;
+#pragma unroll
+  for (int i = 0; i < kNrThreads / 64; ++i) x += s_sum[i][threadIdx.x];
+  const uint32_t at = part == 0 ? slot * cut.chunks[0] + chunk : slots * cut.chunks[0] + slot * cut.chunks[1] + chunk;
+  sums[(int64_t)at * D + threadIdx.x] = x;
 }
 
-// dw[i] = the sum of column i of sums [n][2 D], 16 columns a workgroup of 1024 threads.
+// Column i of sums [nq][D] to dwq, of the [nk][D] behind them to dwk, 16 columns a
+// workgroup of 1024 threads.
 constexpr int kNrSumThreads = 1024;
 template <int D>
 __global__ __launch_bounds__(kNrSumThreads) void norm_weight_sum_kernel(const float* __restrict__ sums,
                                                                         float* __restrict__ dwq,
-                                                                        float* __restrict__ dwk, int n) {
+                                                                        float* __restrict__ dwk, int nq, int nk) {
   constexpr int G = kNrSumThreads / 16;
   __shared__ float s_sum[G][17];
-  const int col = blockIdx.x * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4;
+  const bool second = blockIdx.x >= D / 16;
+  const int col = (blockIdx.x % (D / 16)) * 16 + (threadIdx.x & 15), g = threadIdx.x >> 4, n = second ? nk : nq;
+  float* to = second ? dwk : dwq;
+  if (!to) return;
+  const float* from = sums + (second ? (int64_t)nq * D : 0) + col;
   float x = 0.f;
 #pragma unroll 4
-  for (int i = g; i < n; i += G) x += sums[(int64_t)i * (2 * D) + col];
+  for (int i = g; i < n; i += G) x += from[(int64_t)i * D];
   s_sum[g][threadIdx.x & 15] = x;
   __syncthreads();
   for (int half = G / 2; half > 0; half >>= 1) {
     if (g < half) s_sum[g][threadIdx.x & 15] += s_sum[g + half][threadIdx.x & 15];
     __syncthreads();
   }
-  if (g) return;
-  float* to = col < D ? dwq : dwk;
-  if (to) to[col % D] = s_sum[0][threadIdx.x];
+  if (g == 0) to[col] = s_sum[0][threadIdx.x];
 }
 
 // Workgroups that leave sums behind, and their scratch: of one size, so that graphs may keep its address.
-constexpr int64_t kNrSums = 1024;
-constexpr size_t kNrWork = size_t(kNrSums) * 2 * 128 * sizeof(float);
+constexpr int64_t kNrSums = 2048;
+constexpr size_t kNrWork = size_t(kNrSums) * 128 * sizeof(float);
 
-// How the heads are cut: a workgroup goes through as many as leave some eight
-// workgroups a CU, for the angles that it forms once.
-inline int64_t nr_chunks(int64_t tiles, int64_t heads) {
-  const int64_t want = (8 * (int64_t)device_cu_count() + tiles - 1) / tiles;
-  return std::min(std::max<int64_t>(want, 1), heads);
+// Four heads a workgroup, for the angles that it forms once and the loads that it has
+// in flight, or one where four would leave fewer than two workgroups a CU.  Measured
+// (bf16, 4 x 4096 tokens of 96 heads of 128, us): forward in ones 211, twos 161, fours
+// 155, eights 160, and 145 to 193 by workgroups that go through 16 or 24 heads in a
+// loop; 3 x 1001 tokens of 20 heads of 64 in fp32, back: 15.3 in ones, 17.9 in fours.
+inline NrCut nr_cut(int64_t tiles, int64_t q, int64_t k, int64_t v) {
+  const int64_t count = tiles * (q + k + v) >= 2 * kNrHeads * (int64_t)device_cu_count() ? kNrHeads : 1;
+  auto cut = [&](int64_t h) { return (uint32_t)((h + count - 1) / count); };
+  NrCut c{{cut(q), cut(k), cut(v)}, 0, (int)count};
+  c.all = c.chunks[0] + c.chunks[1] + c.chunks[2];
+  return c;
 }
+// The backward passes values that fill more than this by the caches: 4 x 4096 tokens
+// of 48 heads, 570 MB, 126 -> 116 us; the forward with its wider spread of writes loses
+// by it (155 -> 183 us), as both do where less is moved.
+constexpr int64_t kNrNtBytes = int64_t(256) << 20;
 
 struct NrShape {
   int64_t B, H, Hkv, T, d;
@@ -272,12 +325,17 @@ template <typename T, int D>
 int forward_launch(const char* fn, NrPart<T> q, NrPart<T> k, NrPart<T> v, const Rope& rp, const NrShape& n,
                    hipStream_t st) {
   constexpr int TPB = kNrThreads / (D / (2 * Chunk<T>::N));
-  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = q.heads + k.heads + v.heads;
-  const int64_t count = (heads + nr_chunks(tiles, heads) - 1) / nr_chunks(tiles, heads);
-  const int64_t chunks = (heads + count - 1) / count;
-  if (!grid_fits(tiles * chunks, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
-  hipLaunchKernelGGL((qkv_norm_rope_kernel<T, D>), dim3((unsigned)(tiles * chunks)), dim3(kNrThreads), 0, st, q, k, v,
-                     rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)chunks, (int)count);
+  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB;
+  const NrCut cut = nr_cut(tiles, q.heads, k.heads, v.heads);
+  if (!grid_fits(tiles * cut.all, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+#define TT_NR_FWD(HC)                                                                                                  \
+  hipLaunchKernelGGL((qkv_norm_rope_kernel<T, D, HC>), dim3((unsigned)(tiles * cut.all)), dim3(kNrThreads), 0, st, q, \
+                     k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, cut)
+  if (cut.count == 1)
+    TT_NR_FWD(1);
+  else
+    TT_NR_FWD(kNrHeads);
+#undef TT_NR_FWD
   TT_LAUNCHED(fn, st);
   return ok();
 }
@@ -286,32 +344,42 @@ template <typename T, int D>
 int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const Rope& rp, float* dwq, float* dwk,
                     const NrShape& n, hipStream_t st) {
   constexpr int TPB = kNrThreads / (D / (2 * Chunk<T>::N));
-  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = q.heads + k.heads + v.heads;
+  const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = (int64_t)q.heads + k.heads + v.heads;
   float* sums = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
-  int64_t parts = 0;
+  int64_t nq = 0, nk = 0;
+  if ((dwq || dwk) && (int64_t)q.heads + k.heads > kNrSums)
+    return fail(TT_ERR_ARG, std::string(fn) + ": too many heads for the weights' gradients");
   if (tiles > 0 && heads > 0) {
-    int64_t chunks = nr_chunks(tiles, heads);
+    NrCut cut = nr_cut(tiles, q.heads, k.heads, v.heads);
+    int64_t slots = tiles;
     if (dwq || dwk) {
-      chunks = std::min(chunks, kNrSums);
+      const int64_t each = (int64_t)cut.chunks[0] + cut.chunks[1];
       void* ws = nullptr;
       if (!lease.emplace().get_fixed(st, kWsNormWeights, kNrWork, &ws))
         return fail(TT_ERR_NOMEM, std::string(fn) + ": no scratch for the weights' gradients (under graph capture it "
                                                     "must be there from an earlier call on the stream)");
       sums = (float*)ws;
+      if (each > 0) slots = std::min(tiles, kNrSums / each);
+      nq = slots * cut.chunks[0];
+      nk = slots * cut.chunks[1];
     }
-    const int64_t count = (heads + chunks - 1) / chunks;
-    chunks = (heads + count - 1) / count;
-    const int64_t slots = sums ? std::min(tiles, std::max<int64_t>(1, kNrSums / chunks)) : tiles;
-    parts = slots * chunks;
-    if (!grid_fits(parts, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
-    hipLaunchKernelGGL((qkv_norm_rope_bwd_kernel<T, D>), dim3((unsigned)parts), dim3(kNrThreads), 0, st, q, k, v, rp,
-                       (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)chunks, (uint32_t)slots, (int)count, sums);
+    if (!grid_fits(slots * cut.all, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
+#define TT_NR_BWD(HC, NT)                                                                                             \
+  hipLaunchKernelGGL((qkv_norm_rope_bwd_kernel<T, D, HC, NT>), dim3((unsigned)(slots * cut.all)), dim3(kNrThreads), 0, \
+                     st, q, k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)slots, cut, sums)
+    if (cut.count == 1)
+      TT_NR_BWD(1, false);
+    else if (n.B * n.T * D * (3 * ((int64_t)q.heads + k.heads) + 2 * v.heads) * (int64_t)sizeof(T) > kNrNtBytes)
+      TT_NR_BWD(kNrHeads, true);
+    else
+      TT_NR_BWD(kNrHeads, false);
+#undef TT_NR_BWD
     TT_LAUNCHED(fn, st);
   }
   if (dwq || dwk) {
     hipLaunchKernelGGL((norm_weight_sum_kernel<D>), dim3(2 * D / 16), dim3(kNrSumThreads), 0, st, sums, dwq, dwk,
-                       (int)parts);
+                       (int)nq, (int)nk);
     TT_LAUNCHED(fn, st);
   }
   return ok();

@@ -46,11 +46,12 @@ template <> struct Chunk<u16> {
 };
 template <> struct Chunk<float> {
   static constexpr int N = 4;
-  __device__ static __forceinline__ void get(const uint4& v, float* f) { __builtin_memcpy(f, &v, 16); }
+  __device__ static __forceinline__ void get(const uint4& v, float* f) {
+    f[0] = __uint_as_float(v.x), f[1] = __uint_as_float(v.y);
+    f[2] = __uint_as_float(v.z), f[3] = __uint_as_float(v.w);
+  }
   __device__ static __forceinline__ uint4 put(const float* f) {
-    uint4 v;
-    __builtin_memcpy(&v, f, 16);
-    return v;
+    return uint4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
   }
 };
 
@@ -72,13 +73,16 @@ struct Lay {
   }
 };
 
-// The angle p f in 64 bits less the nearest multiple of pi / 2, and that multiple
-// modulo 4 (Cody and Waite's reduction: pi / 2 in two parts, each taken off by one
-// fused multiply and add, so what is left is as exact as p f itself).
-__device__ __forceinline__ double rope_reduce(double angle, int* quadrant) {
+// The angle p f in 64 bits less the nearest multiple of pi / 2, and that multiple's
+// number, of which the last two bits count (Cody and Waite's reduction: pi / 2 in two
+// parts, each taken off by one fused multiply and add, so what is left is as exact
+// as p f itself).  Adding 1.5 2^52 rounds to a whole number and leaves it in the last bits.
+__device__ __forceinline__ double rope_reduce(double angle, uint32_t* quadrant) {
+#pragma clang fp contract(off)
   constexpr double kTwoOverPi = 0.63661977236758134308, kHi = 1.57079632679489661923, kLo = 6.12323399573676603587e-17;
-  const double k = __builtin_rint(angle * kTwoOverPi);
-  *quadrant = (int)(k - 4.0 * __builtin_floor(0.25 * k));
+  constexpr double kRound = 6755399441055744.0;
+  const double at = __builtin_fma(angle, kTwoOverPi, kRound), k = at - kRound;
+  *quadrant = (uint32_t)__double_as_longlong(at);
   return __builtin_fma(-k, kLo, __builtin_fma(-k, kHi, angle));
 }
 // sin and cos of r in [-pi / 4, pi / 4] by their series, up to the first term below
@@ -116,6 +120,13 @@ __device__ __forceinline__ void rope_series(F r, F* s, F* c) {
     *c = __builtin_fmaf(v, x, F(1.0));
   }
 }
+// x with its sign changed where the first bit of `by` is set.
+__device__ __forceinline__ float rope_flip(float x, uint32_t by) {
+  return __uint_as_float(__float_as_uint(x) ^ (by & 0x80000000u));
+}
+__device__ __forceinline__ double rope_flip(double x, uint32_t by) {
+  return __longlong_as_double(__double_as_longlong(x) ^ (long long)((uint64_t)(by & 0x80000000u) << 32));
+}
 // cos and sin of position pos times the N frequencies from `freq` on.  The angle
 // is formed and reduced in 64 bits: at position 131072 the product alone, rounded
 // to 32, would be 0.004 off.
@@ -123,13 +134,13 @@ template <int N, typename F>
 __device__ __forceinline__ void rope_angles(const float* freq, int64_t pos, F (&c)[N], F (&s)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    int quadrant;
+    uint32_t quadrant;
     const F r = (F)rope_reduce((double)pos * (double)freq[i], &quadrant);
     F x, y;
     rope_series(r, &x, &y);
-    const F cc = (quadrant & 1) ? x : y, ss = (quadrant & 1) ? y : x;
-    c[i] = (quadrant == 1 || quadrant == 2) ? -cc : cc;
-    s[i] = (quadrant & 2) ? -ss : ss;
+    const F cc = (quadrant & 1u) ? x : y, ss = (quadrant & 1u) ? y : x;
+    c[i] = rope_flip(cc, (quadrant + 1u) << 30);  // negative in quadrants 1 and 2, 2 and 3
+    s[i] = rope_flip(ss, quadrant << 30);
   }
 }
 // The position of token t of sequence b.
@@ -141,11 +152,28 @@ __device__ __forceinline__ int64_t rope_position(const Rope& rp, int64_t b, int6
 __device__ __forceinline__ float rope_fma(float a, float b, float c) { return __builtin_fmaf(a, b, c); }
 __device__ __forceinline__ double rope_fma(double a, double b, double c) { return __builtin_fma(a, b, c); }
 
-// Sum over the LPR neighbouring lanes that hold a row, the same in each.
+// x of the lane that a DPP control names.
+template <int CTRL>
+__device__ __forceinline__ float dpp(float x) {
+  return __uint_as_float((uint32_t)__builtin_amdgcn_mov_dpp((int)__float_as_uint(x), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double x) {
+  const uint64_t u = (uint64_t)__double_as_longlong(x);
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)u, CTRL, 0xf, 0xf, true);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+  return __longlong_as_double((long long)((uint64_t)lo | ((uint64_t)hi << 32)));
+}
+// Sum over the LPR neighbouring lanes that hold a row (2 to 16), the same in each:
+// with lanes 1 0 3 2 and 2 3 0 1 of a quad, then, its lanes being equal, with
+// the mirror images of eight and of 16 lanes.
 template <int LPR, typename F>
 __device__ __forceinline__ F row_sum(F x) {
-#pragma unroll
-  for (int off = 1; off < LPR; off <<= 1) x += __shfl_xor(x, off, 64);
+  static_assert(LPR >= 2 && LPR <= 16, "lanes of a row");
+  x += dpp<0xB1>(x);
+  if constexpr (LPR >= 4) x += dpp<0x4E>(x);
+  if constexpr (LPR >= 8) x += dpp<0x141>(x);
+  if constexpr (LPR >= 16) x += dpp<0x140>(x);
   return x;
 }
 
@@ -172,6 +200,51 @@ __device__ __forceinline__ void rope_turn(F (&x)[2 * N], const F (&c)[N], const 
     }
   }
 }
+
+// A lane's rotation with the weights of its norm in it: pair (a, b) of a row times r
+// becomes (a ca - b cb, a sa + b sb) of that, ca = w_a cos, cb = w_b sin, sa = w_a
+// sin, sb = w_b cos; lanes that turn nothing keep their weights in ca and sb.
+template <int N>
+struct RopeTurn {
+  float ca[N], cb[N], sa[N], sb[N];
+  // w: the weights in the order of the lane's values.
+  __device__ __forceinline__ void set(const float (&c)[N], const float (&s)[N], const float (&w)[2 * N], bool turns,
+                                      bool inter) {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float wa = inter ? w[2 * j] : w[j], wb = inter ? w[2 * j + 1] : w[N + j];
+      ca[j] = turns ? wa * c[j] : wa;
+      sb[j] = turns ? wb * c[j] : wb;
+      cb[j] = wb * s[j];
+      sa[j] = wa * s[j];
+    }
+  }
+  __device__ __forceinline__ void operator()(float (&x)[2 * N], float r, bool turns, bool inter) const {
+#pragma clang fp contract(off)
+    if (inter) {
+      pairs<true>(x, r, turns);
+    } else {
+      pairs<false>(x, r, turns);
+    }
+  }
+  template <bool INTER>
+  __device__ __forceinline__ void pairs(float (&x)[2 * N], float r, bool turns) const {
+#pragma clang fp contract(off)
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      constexpr int A = INTER ? 2 : 1, B = INTER ? 1 : N;
+      const float a = x[A * j] * r, b = x[A * j + B] * r;
+      if (turns) {
+        x[A * j] = rope_fma(a, ca[j], -(b * cb[j]));
+        x[A * j + B] = rope_fma(a, sa[j], b * sb[j]);
+      } else {
+        x[A * j] = a * ca[j];
+        x[A * j + B] = b * sb[j];
+      }
+    }
+  }
+};
 
 // 1 / sqrt(mean x^2 + eps) of the row that LPR lanes hold.
 template <int N, int LPR, typename F>
