@@ -40,10 +40,6 @@
 namespace tt {
 namespace {
 
-#ifndef PD_LB
-#define PD_LB(C, D) (sizeof(C) == 1 ? (sizeof(T) == 4 && D == 128 ? 3 : 4) : 2)
-#endif
-
 __device__ __forceinline__ f32x4 mfma_f32_16x16x4(float a, float b, const f32x4& c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
@@ -144,6 +140,12 @@ __device__ __forceinline__ void pd_four(const uint8_t* row, int c, float scale, 
   for (int e = 0; e < 4; ++e) x[e] *= scale;
 }
 
+// Waves of a SIMD that the registers are held to: what their tiles let onto a CU.
+template <typename T, typename C, int D>
+constexpr int pd_waves() {
+  return sizeof(C) > 1 ? 2 : sizeof(T) == 4 && D == 128 ? 3 : 4;
+}
+
 // The wave's place in its sequence's table: entries [base, base + 64) and the 64
 // after them, one a lane, -1 where the pool has no such page or the sequence ends;
 // of 8-bit pools with their scale bytes, which are loaded 64 pages ahead and their
@@ -205,7 +207,7 @@ __device__ __forceinline__ float2 pd_get_far(const float* p) {
 // 16 of the head's R query rows.  Each sequence's own length is cut into nsplit
 // spans, so that sequences of any length keep every workgroup busy.
 template <typename T, typename C, int D, bool STREAM>
-__global__ __launch_bounds__(kMdThreads, PD_LB(C, D)) void attn_decode_paged_kernel(
+__global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode_paged_kernel(
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, Pages pg, float* __restrict__ part_o, float2* __restrict__ part_ml,
     T* __restrict__ o, float* __restrict__ lse, uint32_t R, uint32_t tokens, uint32_t tiles, uint32_t nsplit,

@@ -48,8 +48,8 @@ __device__ __forceinline__ float e4_scale(uint32_t byte) { return __uint_as_floa
 __device__ __forceinline__ float e4_inverse(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 // x as it goes into a code: infinities become NaN, values past 448 become 448.
 __device__ __forceinline__ float e4_clamp(float x) {
-  return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? __uint_as_float(0x7fc00000u)
-                                                          : __builtin_fminf(__builtin_fmaxf(x, -448.f), 448.f);
+  const float y = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
+  return __builtin_isfpclass(x, 0x207) ? __uint_as_float(0x7fc00000u) : y;  // an infinity or NaN, of one v_cmp_class
 }
 // Four codes of values times `inverse`, nearest, halves to even.
 __device__ __forceinline__ uint32_t e4_codes(const float* x, float inverse) {
