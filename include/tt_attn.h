@@ -429,7 +429,8 @@ int tt_attn_decode_mxfp4(int dtype, const void* q, const uint8_t* k_codes, const
  * lengths are (the T newest of a sequence, as the caches have it), else t; all
  * of these arrays are on the device.  Angles are formed and reduced in 64
  * bits, so positions of any size turn by what they say; all else is in fp32 and
- * rounded once.  x^2 must not overflow.  dtype TT_F32 or TT_BF16; d 32, 64 or
+ * rounded once.  x^2 must not overflow, nor all of a row's fall below 2^-126 where
+ * eps is zero (a row of zeros is 0 / 0 then).  dtype TT_F32 or TT_BF16; d 32, 64 or
  * 128; pointers to values are 16-byte aligned and leading dimensions a multiple of
  * 16 bytes (TT_ERR_ARG otherwise).  B T is below 2^31 - 256. */
 int tt_qkv_norm_rope(int dtype, const void* q, const void* k, const void* v, int64_t ldq, int64_t ldk, int64_t ldv,
@@ -503,7 +504,7 @@ int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_
  * they hold; an infinite or NaN value of V reaches the tokens that see its key
  * and no others.  Scores, weights and sums are in fp32, of which the weights of
  * bf16 calls keep 16 bits (2^-17 off) where they meet V; the sums are divided
- * last.  B H T is below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an
+ * last, so a value of V times the number of keys must stay finite.  B H T is below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an
  * unsplit call, below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over
  * workgroups and merge their sums through a fixed 24 MiB per-stream library
  * workspace (allocated on first use); without it (refused, or under graph

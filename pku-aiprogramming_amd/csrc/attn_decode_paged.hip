@@ -615,10 +615,9 @@ __global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode
   wait_loads<0>();
   __syncthreads();
   __shared__ uint32_t s_before;
-  if (threadIdx.x == 0) s_before = __hip_atomic_fetch_add(count + unit, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (threadIdx.x == 0) s_before = atomicInc(count + unit, nsplit - 1);  // back at zero for the next call
   __syncthreads();
   if (s_before != nsplit - 1) return;
-  if (threadIdx.x == 0) __hip_atomic_store(count + unit, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next call
   // A wave a row: its splits' maxima and sums a lane each, D / 4 lanes to a partial.
   constexpr int TPR = D / 4, G = 64 / TPR;
   const int c = l % TPR, gr = l / TPR;

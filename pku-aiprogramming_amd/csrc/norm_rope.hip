@@ -348,8 +348,6 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
   float* sums = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
   int64_t nq = 0, nk = 0;
-  if ((dwq || dwk) && (int64_t)q.heads + k.heads > kNrSums)
-    return fail(TT_ERR_ARG, std::string(fn) + ": too many heads for the weights' gradients");
   if (tiles > 0 && heads > 0) {
     NrCut cut = nr_cut(tiles, q.heads, k.heads, v.heads);
     int64_t slots = tiles;
@@ -564,6 +562,8 @@ extern "C" int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k
   }
   const bool any = some && ((dq && H > 0) || ((dk || dv) && Hkv > 0));
   if (!any && !dq_weight && !dk_weight) return ok();
+  if ((dq_weight || dk_weight) && (dq ? H : 0) + (dk ? Hkv : 0) > kNrSums)
+    return fail(TT_ERR_ARG, f + ": too many heads for the weights' gradients");
   if ((rc = check_apart(f, {x[0], x[1], dy[0], dy[1], dy[2]},
                         {{q_weight, w, "q_weight"},
                          {k_weight, w, "k_weight"},

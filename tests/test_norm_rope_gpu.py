@@ -245,6 +245,23 @@ def test_no_rows_have_no_gradient(capi, B, H, T):
     assert (dw.download() == 0).all()
 
 
+def test_most_heads(capi):
+    """As many heads as the weights' gradients may have, and more without them."""
+    rng = np.random.default_rng(9)
+    B, T, d, w = 1, 3, 32, normal(rng, (32,), "f32")
+    W, F, pos = capi.DeviceBuffer.from_numpy(w), capi.DeviceBuffer.from_numpy(FREQ[32]), po.positions(B, T)
+    for H, weight in ((2048, True), (5000, False)):
+        x, dy = normal(rng, (B, H, T, d), "bf16"), normal(rng, (B, H, T, d), "bf16")
+        X, Y, out = capi.DeviceBuffer.from_numpy(x, "bf16"), capi.DeviceBuffer.from_numpy(dy, "bf16"), capi.DeviceBuffer(x.shape, "bf16")
+        dw = capi.DeviceBuffer((d,)) if weight else None
+        capi.norm_rope(X, out, W, F, eps=EPS)
+        capi.lib().sync()
+        check_forward(out.download(), x, w, pos, FREQ[32], False, "bf16")
+        capi.norm_rope_backward(X, Y, out, W, dw, F, eps=EPS)
+        capi.lib().sync()
+        check_backward(out.download(), dw.download() if weight else None, x, w, dy, pos, FREQ[32], False, "bf16", B * T * H)
+
+
 def test_captured_and_on_another_stream(capi):
     """A step captured once its scratch is there, replayed on new inputs beside eager calls on two streams."""
     rng = np.random.default_rng(8)

@@ -177,6 +177,11 @@ def test_rotation_gradient_refusals(capi, kw, words):
     refused(capi, rope_back(capi, **kw), ARG, words)
 
 
+def test_heads_of_weight_gradients(capi):
+    big = dict(H=2047, Hkv=2, T=1, B=1, d=32, dq=1 << 26, dqo=1 << 27, q=1 << 28)
+    refused(capi, rope_back(capi, **big), ARG, "too many heads for the weights")
+
+
 CACHE = [(dict(dtype=4), "dtype"), (dict(cache=3), "cache"), (dict(cache=1), "cache"), (dict(B=-1), "negative"),
          (dict(npages=-1), "negative"), (dict(width=-1), "negative"), (dict(width=1 << 27), "too long"),
          (dict(B=1 << 25), "too many heads"), (dict(B=1 << 13, Hkv=1 << 12, **{}), "too many heads"),

@@ -7,6 +7,10 @@ Attention: a score is off by (d + 8) u sum |q| |k| scale, twice over in the weig
 the weights keep 2^-17 (bf16 calls) or 2^-24 of themselves where they meet V; exp2
 and the sums of n keys add 2 (n + 8) u; all of sum p |v|, and the store's half step.
 lse: the scores' bound, (n + 8) u for the sum, and 4 u (|lse| + 1) for the logarithm."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -16,6 +20,7 @@ from test_capture_gpu import Capture
 from test_norm_rope_gpu import EPS, FREQ, HALF, U, normal, pairs
 
 pytestmark = pytest.mark.gpu
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 TERMS = {"f32": 2.0 ** -24, "bf16": 2.0 ** -17}
 KINDS = [("f32", "f32"), ("bf16", "bf16"), ("f32", "u8"), ("bf16", "u8")]
 
@@ -447,6 +452,157 @@ def test_a_pool_past_4_gib(capi, dtype, cache):
     ro, _, mag, score = ref.attend(q, [n], float(np.float32(0.1)))
     rel = 2 * (d + 8) * U * score + TERMS[dtype] + 2 * (n + 8) * U
     assert (np.abs(o.download() - ro) <= rel[..., None] * mag * (1 + HALF[dtype]) + HALF[dtype] * np.abs(ro)).all()
+
+
+# ------------------------------------------------------------------ splits and their merge
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("H,T", [(1, 1), (3, 1), (2, 2)])
+@pytest.mark.parametrize("d,n", [(32, 5117), (64, 1291), (128, 257)])
+def test_splits_of_a_few_rows(capi, d, n, H, T, dtype, cache):
+    """Three to forty splits that their last workgroup merges, call after call: the same bits each time."""
+    rng = np.random.default_rng(d + H)
+    lengths = [n, 1, 0, n // 3]
+    c = filled(capi, dtype, cache, 4, 1, 64, d, lengths, rng)
+    q = normal(rng, (4, H, T, d), dtype)
+    first = c.attend(q, lengths, 0.2)
+    c.check_attention(q, lengths, 0.2, first)
+    for i in range(5):
+        c.attend(normal(rng, (4, H, T, d), dtype), [n - 7 * i, n, 3, 0], 0.1)  # others in between
+        o, lse = c.attend(q, lengths, 0.2, lse=i % 2 == 0)
+        assert np.array_equal(o, first[0]) and (lse is None or np.array_equal(lse, first[1]))
+
+
+@pytest.mark.parametrize("dtype,cache", [("bf16", "bf16"), ("f32", "u8")])
+def test_a_sequence_over_hundreds_of_splits(capi, dtype, cache):
+    rng = np.random.default_rng(21)
+    n, page, d = 200003, 128, 32
+    c = Cache(capi, dtype, cache, 1, 1, page, -(-n // page), d, rng)
+    k, v = (normal(rng, (1, 1, n, d), dtype) for _ in range(2))
+    c.append(k, v, [n])
+    c.adopt()
+    c.check_attention(normal(rng, (1, 2, 3, d), dtype), [n], 0.3)
+
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+def test_many_rows_of_a_head(capi, dtype, cache):
+    """A prompt's chunk: seventeen tiles of query rows, the last one of four, most of whose tokens one sequence lacks."""
+    rng = np.random.default_rng(22)
+    lengths, T = [300, 26], 65
+    c = filled(capi, dtype, cache, 2, 2, 32, 64, lengths, rng)
+    c.check_attention(normal(rng, (2, 8, T, 64), dtype), lengths, 0.125)
+
+
+def test_threads_and_streams(capi):
+    """Four host threads, two to a stream: norms' gradients, appends, reads back and split attention, each as alone."""
+    import threading
+
+    f, d, B, Hkv, page = capi.DeviceBuffer.from_numpy, 64, 2, 2, 32
+    streams, jobs = [capi.Stream(), capi.Stream()], []
+    for i in range(4):
+        rng = np.random.default_rng(30 + i)
+        dtype, cache = KINDS[i]
+        n = 700 + 300 * i
+        c = filled(capi, dtype, cache, B, Hkv, page, d, [n, n // 2], rng, width=80)
+        T = 40 + i
+        x, dy = normal(rng, (B, 4, T, d), dtype), normal(rng, (B, 4, T, d), dtype)
+        k, v, q = (normal(rng, (B, h, 1, d), dtype) for h in (Hkv, Hkv, 4))
+        jobs.append(dict(c=c, st=streams[i % 2].handle, x=f(x, dtype), dy=f(dy, dtype), w=f(normal(rng, (d,), "f32")),
+                         F=f(FREQ[64]), k=f(k, dtype), v=f(v, dtype), q=f(q, dtype), error=None, got=[],
+                         out=lambda shape, t=dtype: capi.DeviceBuffer(shape, t), T=T, L=n))
+
+    def work(j, times):
+        try:
+            c, s = j["c"], dict(stream=j["st"])
+            for _ in range(times):
+                dx, dw, o, lse = j["out"]((B, 4, j["T"], d)), j["out"]((d,), "f32"), j["out"]((B, 4, 1, d)), j["out"]((B, 4, 1), "f32")
+                ko, vo = (j["out"]((B, Hkv, j["L"], d)) for _ in range(2))
+                for b in (ko, vo):
+                    b.zero()
+                capi.lib().sync()
+                capi.norm_rope_backward(j["x"], j["dy"], dx, j["w"], dw, j["F"], eps=EPS, **s)
+                capi.kv_append_paged(j["k"], j["v"], c.dev["k"], c.dev["v"], c.tab, c.lengths, j["w"], j["F"], **c.scales(), **s)
+                capi.attn_decode_paged(j["q"], c.dev["k"], c.dev["v"], c.tab, c.lengths, o, lse, 0.2, **c.scales(), **s)
+                capi.kv_gather_paged(c.dev["k"], c.dev["v"], c.tab, c.lengths, ko, vo, **c.scales(), **s)
+                j["got"].append((dx, dw, o, lse, ko, vo))
+        except Exception as e:  # reported by the test's own thread
+            j["error"] = e
+
+    alone = []
+    for j in jobs:
+        work(j, 1)
+        capi.lib().call("tt_stream_sync", j["st"])
+        assert j["error"] is None
+        alone.append([b.download() for b in j["got"].pop()])
+    threads = [threading.Thread(target=work, args=(j, 12)) for j in jobs]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for st in streams:
+        st.sync()
+    for j, ref in zip(jobs, alone):
+        assert j["error"] is None
+        for got in j["got"]:
+            for a, b in zip(got, ref):
+                assert np.array_equal(a.download(), b)
+
+
+REFUSED = r"""
+import ctypes as C, numpy as np, tt_capi as T
+from oracle import paged_oracle as po
+from test_paged_gpu import Cache, filled, normal
+def in_use():
+    a = C.c_size_t()
+    T.lib().call("tt_mem_stats", C.byref(a), None)
+    return a.value
+class Counted(T.DeviceBuffer):
+    n = 0
+    def __init__(self, *a, **k):
+        Counted.n += 1
+        super().__init__(*a, **k)
+f, T.DeviceBuffer = T.DeviceBuffer, Counted
+rng = np.random.default_rng(1)
+c = filled(T, "f32", "f32", 1, 1, 64, 64, [2000], rng)
+q = normal(rng, (1, 2, 1, 64), "f32")
+o, lse, Q = T.DeviceBuffer(q.shape), T.DeviceBuffer((1, 2, 1)), T.DeviceBuffer.from_numpy(q)
+x, w, dx, dw = (T.DeviceBuffer.from_numpy(np.full(s, 7.0, np.float32)) for s in ((1, 2, 5, 64), (64,), (1, 2, 5, 64), (64,)))
+c.lengths.upload(np.array([2000], np.int32))
+T.lib().sync()
+print("COUNT", Counted.n, flush=True)
+before = in_use()
+T.attn_decode_paged(Q, c.dev["k"], c.dev["v"], c.tab, c.lengths, o, lse, 0.125)
+T.lib().sync()
+if %d:
+    assert in_use() == before, "the scratch was not refused"
+    try:
+        T.norm_rope_backward(x, x, dx, w, dw)
+        print("NOT REFUSED")
+    except T.TTError as e:
+        T.lib().sync()
+        assert e.code == T.TT_ERR_NOMEM and (dx.download() == 7).all() and (dw.download() == 7).all()
+        T.norm_rope_backward(x, x, dx, w, None)  # needs none
+        T.lib().sync()
+        assert not (dx.download() == 7).all()
+        print("REFUSED True")
+c.check_attention(q, [2000], 0.125, (o.download(), lse.download()))
+print("DONE")
+"""
+
+
+def test_refused_scratch(capi):
+    """Without its scratch the attention runs unsplit; weights' gradients are refused before anything is written."""
+    def run(after, refuse):
+        env = dict(os.environ, PYTHONPATH=os.pathsep.join([ROOT, os.path.join(ROOT, "pku-aiprogramming_amd"),
+                                                           os.path.join(ROOT, "tests"), os.environ.get("PYTHONPATH", "")]))
+        if refuse:
+            env["TT_FAIL_ALLOC_AFTER"] = str(after)
+        return subprocess.run([sys.executable, "-c", REFUSED % refuse], env=env, capture_output=True, text=True, timeout=100)
+
+    r = run(0, 0)
+    assert r.returncode == 0 and "DONE" in r.stdout, r.stdout + r.stderr
+    r = run(int(r.stdout.split("COUNT")[1].split()[0]), 1)
+    assert r.returncode == 0 and "REFUSED True" in r.stdout and "DONE" in r.stdout, r.stdout + r.stderr
 
 
 # ------------------------------------------------------------------ together, streams, graphs
