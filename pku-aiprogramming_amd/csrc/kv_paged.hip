@@ -29,7 +29,8 @@ namespace {
 constexpr int kPgThreads = 256;
 // Heads of a workgroup of the 8-bit append, under angles formed once in 64 bits (8 x 4000
 // tokens of 8 heads of 128: 69 -> 57 us); fewer where there would be fewer than four
-// workgroups a CU.
+// workgroups a CU (eight: 8 x 40 tokens 25 -> 24 us with the cache read back, but 4 x 2000 of
+// 16 heads of fp32 48 -> 51).
 constexpr int64_t kPgHeads = 8;
 
 template <typename T>
@@ -120,36 +121,41 @@ __device__ __forceinline__ float cut_odd(double x) {
   return __uint_as_float(bits);
 }
 
-// A workgroup: the new tokens of one page, heads [first, first + heads) of K
-// (blockIdx.y 0) or V (1), one after another, under the angles that it forms once.
+// A workgroup: the new tokens of one page, NEW at most, heads [first, first + heads) of
+// K (blockIdx.y 0) or V (1), one after another, under the angles that it forms once.
+// NEW goes by the call, not by the page: 16 tokens into pages of 64, 56 sequences of 32
+// heads, 44 -> 29 us with the cache read back.
 // Workgroup id = (b * count + i) * groups + group, i = 0 .. count - 1 the pages from
 // the one that the first new token goes to.
-template <typename T, int D, int PAGE>
+template <typename T, int D, int NEW>
 struct PgTile {
-  static constexpr int N = Chunk<T>::N, LPR = D / (2 * N), LANES = PAGE * LPR;
-  static constexpr int THREADS = LANES < 64 ? 64 : LANES > kPgThreads ? kPgThreads : LANES;
+  static constexpr int N = Chunk<T>::N, LPR = D / (2 * N), LANES = NEW * LPR;
+  // 16 values a side of the pairs a thread at most: 8 x 2000 tokens of 16 heads in pages of
+  // 128 take 81 us by 512 threads and 102 by 256; of 64, 256 threads 73 and 512 89.
+  static constexpr int MOST = LANES * N / 16 > kPgThreads ? LANES * N / 16 : kPgThreads;
+  static constexpr int THREADS = LANES < 64 ? 64 : LANES > MOST ? MOST : LANES;
   static constexpr int ITER = (LANES + THREADS - 1) / THREADS, ROWS = THREADS / LPR;  // rows of an iteration
 };
-template <typename T, int D, int PAGE>
-__global__ __launch_bounds__((PgTile<T, D, PAGE>::THREADS)) void kv_append_e4m3_kernel(
+template <typename T, int D, int NEW>
+__global__ __launch_bounds__((PgTile<T, D, NEW>::THREADS)) void kv_append_e4m3_kernel(
     PgNew<T> in, Rope rp, Pages pg, uint8_t* __restrict__ kp, uint8_t* __restrict__ vp, uint8_t* __restrict__ ks,
     uint8_t* __restrict__ vs, uint32_t tokens, uint32_t count, uint32_t groups, uint32_t heads) {
-  using P = PgTile<T, D, PAGE>;
+  using P = PgTile<T, D, NEW>;
   constexpr int N = P::N, LPR = P::LPR, ITER = P::ITER, WAVES = P::THREADS / 64;
   __shared__ uint32_t s_top[2][WAVES];
   const uint32_t group = blockIdx.x % groups, bi = blockIdx.x / groups, b = bi / count, i = bi - b * count;
   const uint32_t h0 = group * heads, h1 = min(h0 + heads, pg.hkv);
   const bool is_v = blockIdx.y != 0;
   const int64_t length = pg.lengths[b], end = paged_end(pg, length), first = max(length - (int64_t)tokens, (int64_t)0);
-  const int64_t j = first / PAGE + i, base = j * PAGE;
+  const int64_t j = (first >> pg.lp) + i, base = j << pg.lp;
   if (base >= end) return;
   const int64_t page = pg.table[b * pg.width + j];
   if (page < 0 || page >= pg.pages) return;
-  const int old = (int)max(first - base, (int64_t)0), fill = (int)min(end - base, (int64_t)PAGE);  // rows [old, fill) are new
+  const int old = (int)max(first - base, (int64_t)0), fill = (int)min(end - base, (int64_t)1 << pg.lp);  // rows [old, fill) are new
   if (old >= fill) return;
   const bool norm = !is_v && in.weight, turns = !is_v && rp.freq;
   const Lay<N> lay(threadIdx.x % LPR, turns ? rp.rot : 0, rp.inter != 0);
-  const int row0 = (int)threadIdx.x / LPR;
+  const int row0 = old + (int)threadIdx.x / LPR;  // and every P::ROWS from there
   const T* x = is_v ? in.v : in.k;
   const int64_t ld = is_v ? in.ldv : in.ldk;
   bool mine[ITER];
@@ -158,7 +164,7 @@ __global__ __launch_bounds__((PgTile<T, D, PAGE>::THREADS)) void kv_append_e4m3_
 #pragma unroll
   for (int it = 0; it < ITER; ++it) {
     const int row = row0 + it * P::ROWS;
-    mine[it] = row >= old && row < fill;
+    mine[it] = row < fill;
     const int64_t t = base + (mine[it] ? row : old) - (length - tokens);
     from[it] = (ld ? x + ((int64_t)b * tokens + t) * ld + h0 * D : x + (((int64_t)b * pg.hkv + h0) * tokens + t) * D);
   }
@@ -234,7 +240,7 @@ __global__ __launch_bounds__((PgTile<T, D, PAGE>::THREADS)) void kv_append_e4m3_
     uint32_t byte = e4_scale_byte(top);
     if (old > 0) byte = max(byte, before);
     const float inverse = byte > 253u ? 0.f : e4_inverse(byte);
-    uint8_t* codes = (is_v ? vp : kp) + (page * pg.hkv + h) * (int64_t)(PAGE * D);
+    uint8_t* codes = (is_v ? vp : kp) + ((page * pg.hkv + h) << pg.lp) * D;
 #pragma unroll
     for (int it = 0; it < ITER; ++it) {
       if (!mine[it]) continue;
@@ -348,12 +354,12 @@ int append_launch(const char* fn, const PgNew<T>& in, const Rope& rp, const Page
   return ok();
 }
 
-template <typename T, int D, int PAGE>
-void append_e4m3_page(const PgNew<T>& in, const Rope& rp, const Pages& pg, uint8_t* kp, uint8_t* vp, uint8_t* ks,
+template <typename T, int D, int NEW>
+void append_e4m3_new(const PgNew<T>& in, const Rope& rp, const Pages& pg, uint8_t* kp, uint8_t* vp, uint8_t* ks,
                       uint8_t* vs, int64_t pages, int64_t tokens, int64_t count, int64_t heads, hipStream_t st) {
   const int64_t groups = (pg.hkv + heads - 1) / heads;
-  hipLaunchKernelGGL((kv_append_e4m3_kernel<T, D, PAGE>), dim3((unsigned)(pages * groups), 2),
-                     dim3(PgTile<T, D, PAGE>::THREADS), 0, st, in, rp, pg, kp, vp, ks, vs, (uint32_t)tokens,
+  hipLaunchKernelGGL((kv_append_e4m3_kernel<T, D, NEW>), dim3((unsigned)(pages * groups), 2),
+                     dim3(PgTile<T, D, NEW>::THREADS), 0, st, in, rp, pg, kp, vp, ks, vs, (uint32_t)tokens,
                      (uint32_t)count, (uint32_t)groups, (uint32_t)heads);
 }
 
@@ -365,13 +371,16 @@ int append_e4m3_launch(const char* fn, const PgNew<T>& in, const Rope& rp, const
     return fail(TT_ERR_ARG, std::string(fn) + ": too many pages of new tokens");
   int64_t heads = std::min<int64_t>(pg.hkv, kPgHeads);
   while (heads > 1 && 2 * pages * ((pg.hkv + heads - 1) / heads) < 4 * (int64_t)device_cu_count()) heads = (heads + 1) / 2;
-#define TT_PG_E4                                                                                              \
-  switch (pg.lp) {                                                                                            \
-    case 4: append_e4m3_page<T, D, 16>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st); break;   \
-    case 5: append_e4m3_page<T, D, 32>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st); break;   \
-    case 6: append_e4m3_page<T, D, 64>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st); break;   \
-    default: append_e4m3_page<T, D, 128>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st); break; \
-  }
+  const int64_t most = std::min(page, tokens);  // new rows of a page
+#define TT_PG_E4                                                                                          \
+  if (most <= 16)                                                                                         \
+    append_e4m3_new<T, D, 16>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st);               \
+  else if (most <= 32)                                                                                    \
+    append_e4m3_new<T, D, 32>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st);               \
+  else if (most <= 64)                                                                                    \
+    append_e4m3_new<T, D, 64>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st);               \
+  else                                                                                                    \
+    append_e4m3_new<T, D, 128>(in, rp, pg, kp, vp, ks, vs, pages, tokens, count, heads, st)
   TT_PG_DIM(TT_PG_E4)
 #undef TT_PG_E4
   TT_LAUNCHED(fn, st);
