@@ -296,17 +296,21 @@ __global__ __launch_bounds__(kNrSumThreads) void norm_weight_sum_kernel(const fl
   if (g == 0) to[col] = s_sum[0][threadIdx.x];
 }
 
-// Workgroups that leave sums behind, and their scratch: of one size, so that graphs may keep its address.
+// Workgroups that leave sums behind, and their scratch: of one size, so that graphs may
+// keep its address.  4 x 4096 tokens of 96 heads 229 us with 1024, 220 with 2048, 219 with
+// 4096, 223 with 8192; 1843 tokens of 160 heads 59, 60, 63, 63.
 constexpr int64_t kNrSums = 2048;
 constexpr size_t kNrWork = size_t(kNrSums) * 128 * sizeof(float);
 
 // Four heads a workgroup, for the angles that it forms once and the loads that it has
-// in flight, or one where four would leave fewer than two workgroups a CU.  Measured
-// (bf16, 4 x 4096 tokens of 96 heads of 128, us): forward in ones 211, twos 161, fours
-// 155, eights 160, and 145 to 193 by workgroups that go through 16 or 24 heads in a
-// loop; 3 x 1001 tokens of 20 heads of 64 in fp32, back: 15.3 in ones, 17.9 in fours.
+// in flight; two, or one, where more would leave fewer than two workgroups a CU.
+// Measured (bf16, 4 x 4096 tokens of 96 heads of 128, us): forward in ones 211, twos 161,
+// fours 155, eights 160, and 145 to 193 by workgroups that go through 16 or 24 heads in a
+// loop; back in twos 226, threes 225, fours 220.  3 x 1001 tokens of 20 heads of 64 in
+// fp32, back: 15.5 in ones, 13.5 in twos, 17.9 in fours.
 inline NrCut nr_cut(int64_t tiles, int64_t q, int64_t k, int64_t v) {
-  const int64_t count = tiles * (q + k + v) >= 2 * kNrHeads * (int64_t)device_cu_count() ? kNrHeads : 1;
+  int64_t count = kNrHeads;
+  while (count > 1 && tiles * (q + k + v) < 2 * count * (int64_t)device_cu_count()) count /= 2;
   auto cut = [&](int64_t h) { return (uint32_t)((h + count - 1) / count); };
   NrCut c{{cut(q), cut(k), cut(v)}, 0, (int)count};
   c.all = c.chunks[0] + c.chunks[1] + c.chunks[2];
@@ -333,6 +337,8 @@ int forward_launch(const char* fn, NrPart<T> q, NrPart<T> k, NrPart<T> v, const 
                      k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, cut)
   if (cut.count == 1)
     TT_NR_FWD(1);
+  else if (cut.count == 2)
+    TT_NR_FWD(2);
   else
     TT_NR_FWD(kNrHeads);
 #undef TT_NR_FWD
@@ -368,6 +374,8 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
                      st, q, k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)slots, cut, sums)
     if (cut.count == 1)
       TT_NR_BWD(1, false);
+    else if (cut.count == 2)
+      TT_NR_BWD(2, false);
     else if (n.B * n.T * D * (3 * ((int64_t)q.heads + k.heads) + 2 * v.heads) * (int64_t)sizeof(T) > kNrNtBytes)
       TT_NR_BWD(kNrHeads, true);
     else
