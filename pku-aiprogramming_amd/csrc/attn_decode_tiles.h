@@ -5,9 +5,7 @@
 
 #include <hip/hip_runtime.h>
 
-#include <algorithm>
 #include <cstdint>
-#include <limits>
 
 #include "attn_common.h"
 
@@ -104,9 +102,9 @@ __device__ __forceinline__ float md_lse(float m, float den) {
 // partials side by side, which meet in LDS.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_decode_merge_kernel(const float* __restrict__ part_o,
-                                                                      const float2* __restrict__ part_ml,
-                                                                      T* __restrict__ o, float* __restrict__ lse,
-                                                                      int nsplit) {
+                                                                const float2* __restrict__ part_ml,
+                                                                T* __restrict__ o, float* __restrict__ lse,
+                                                                int nsplit) {
   constexpr int TPR = D / 4, G = 256 / TPR;
   __shared__ __align__(16) float s_acc[G][D];
   __shared__ float s_w[G];
@@ -141,7 +139,6 @@ __global__ __launch_bounds__(256) void attn_decode_merge_kernel(const float* __r
   md_put(o + row * D + tid, md_quotient<T>(num, den));
   if (tid == 0 && lse) lse[row] = md_lse(mx, den);
 }
-
 
 }  // namespace
 }  // namespace tt

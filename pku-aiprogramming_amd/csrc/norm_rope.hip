@@ -12,6 +12,8 @@
 // r is formed again from x, which is read anyway.  A thread sums its rows' g n in
 // registers, a workgroup its threads' in LDS, a second launch the workgroups' in the
 // order of their numbers, so the result does not depend on which ends first.
+// Measured (MI355X): 4 x 4096 tokens of 32 / 32 heads of 128 in bf16, one fused projection:
+// forward 155 us (805 MB, 5.2 TB/s), back 219 us (1074 MB, 4.9 TB/s); 8 tokens 4 us.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

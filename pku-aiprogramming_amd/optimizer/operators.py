@@ -713,6 +713,10 @@ class NormRope(TensorOp):
         self.interleaved, self.tokens_first = bool(interleaved), bool(tokens_first)
         self.inv_freq = None if inv_freq is None else np.asarray(inv_freq, np.float32)
         self.positions = None if positions is None else np.asarray(positions, np.int32)
+        if self.inv_freq is not None and self.inv_freq.ndim != 1:
+            raise ValueError("NormRope: inv_freq holds one frequency for each pair")
+        if self.positions is not None and self.positions.ndim != 2:
+            raise ValueError("NormRope: positions are [B, T]")
 
     def _device(self, arrays):
         if len(arrays) != (2 if self.norm else 1):

@@ -289,6 +289,15 @@ def test_binding_refusals(capi):
             pytest.fail(f"call {n} was accepted")
 
 
+def test_graph_op_refusals():
+    import operators as ops
+
+    for kw, words in ((dict(positions=np.arange(5)), "positions"), (dict(inv_freq=np.ones((2, 8))), "frequency"),
+                      (dict(dtype="float64"), "dtype")):
+        with pytest.raises(ValueError, match=words):
+            ops.NormRope(**kw)
+
+
 def test_frequencies():
     import operators as ops
 
