@@ -11,12 +11,14 @@
 // bit set where anything was cut off, so that each code is the nearest to the exact
 // value and not to a neighbour of it.
 // Measured (MI355X): 4 x 4001 tokens of 8 heads of 128 in fp32, 166 MB, 34 us (4.9 TB/s),
-// 16 x 16 heads 288 us (5.4 TB/s); 8 x 4000 tokens of bf16 into 8 bits 50 us, bound half by
-// the 64-bit arithmetic, and read back 22 us (5.9 TB/s).
+// 16 x 16 heads 288 us (5.4 TB/s); 8 x 4000 tokens of bf16 into 8 bits 46 us, in which a
+// third of the wave cycles issue vector instructions, with two waves a SIMD (64-bit values in
+// registers), and read back 24 us (5.6 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "attn_tiles.h"
 #include "paged.h"
@@ -102,23 +104,33 @@ __global__ __launch_bounds__(kPgThreads) void kv_append_kernel(PgNew<T> in, Rope
 
 // x in fp32, cut off, the last bit set where anything was: on the same side as x
 // of every number of fewer bits and of every middle between two of them.
-// The digits come by shifts; zeros, what fp32 holds as subnormal, infinities and NaN apart.
 __device__ __forceinline__ float cut_odd(double x) {
-  const uint64_t u = (uint64_t)__double_as_longlong(x);
-  const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u;
-  const uint32_t digits = __builtin_amdgcn_alignbit(hi, lo, 29) + 0x40000000u;  // of an exponent 896 less
-  uint32_t bits = (hi & 0x80000000u) | (digits & 0x7fffffffu) | ((lo & 0x1fffffffu) ? 1u : 0u);
-  if ((hi & 0x7fffffffu) - 0x38100000u >= 0x47f00000u - 0x38100000u) {
-    const float f = (float)x;
-    bits = __float_as_uint(f);
-    if ((bits & 0x7f800000u) != 0x7f800000u) {
-      bits -= __builtin_fabs((double)f) > __builtin_fabs(x) ? 1u : 0u;
-      bits |= (double)__uint_as_float(bits) != x ? 1u : 0u;
-    } else if ((hi & 0x7ff00000u) != 0x7ff00000u) {
-      bits -= 1u;  // past the largest fp32: that
-    }
+  const float f = (float)x;
+  uint32_t bits = __float_as_uint(f);
+  if ((bits & 0x7f800000u) != 0x7f800000u) {
+    bits -= __builtin_fabs((double)f) > __builtin_fabs(x) ? 1u : 0u;
+    bits |= (double)__uint_as_float(bits) != x ? 1u : 0u;
+  } else if (__builtin_isfinite(x)) {
+    bits -= 1u;  // past the largest fp32: that
   }
   return __uint_as_float(bits);
+}
+// M of them.  The digits come by shifts where all are of fp32's normal range: one test
+// for the M, since zeros are rare among values.
+template <int M>
+__device__ __forceinline__ void cut_odd(const double (&x)[M], float (&f)[M]) {
+  uint32_t odd = 0;
+#pragma unroll
+  for (int e = 0; e < M; ++e) {
+    const uint64_t u = (uint64_t)__double_as_longlong(x[e]);
+    const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u;
+    odd = max(odd, (hi << 1) - 2 * 0x38100000u);
+    const uint32_t digits = __builtin_amdgcn_alignbit(hi, lo, 29) + 0x40000000u;  // of an exponent 896 less
+    f[e] = __uint_as_float((hi & 0x80000000u) | (digits & 0x7fffffffu) | min(lo & 0x1fffffffu, 1u));
+  }
+  if (odd >= 2 * (0x47f00000u - 0x38100000u))
+#pragma unroll
+    for (int e = 0; e < M; ++e) f[e] = cut_odd(x[e]);
 }
 
 // A workgroup: the new tokens of one page, NEW at most, heads [first, first + heads) of
@@ -126,7 +138,8 @@ __device__ __forceinline__ float cut_odd(double x) {
 // NEW goes by the call, not by the page: 16 tokens into pages of 64, 56 sequences of 32
 // heads, 44 -> 29 us with the cache read back.
 // Workgroup id = (b * count + i) * groups + group, i = 0 .. count - 1 the pages from
-// the one that the first new token goes to.
+// the one that the first new token goes to.  All of K's come first: ids of K and V in
+// turn, arithmetic beside memory, take longer (8 x 4000 tokens 70 -> 87 us).
 template <typename T, int D, int NEW>
 struct PgTile {
   static constexpr int N = Chunk<T>::N, LPR = D / (2 * N), LANES = NEW * LPR;
@@ -210,8 +223,7 @@ __global__ __launch_bounds__((PgTile<T, D, NEW>::THREADS)) void kv_append_e4m3_k
         for (int e = 0; e < 2 * N; ++e) g[e] = f[it][e];
         if (norm) rope_scale<N>(g, rope_rms<N, LPR>(g, rp.eps), w);
         if (lay.turns) rope_turn<N>(g, c[it], s[it], rp.inter != 0);
-#pragma unroll
-        for (int e = 0; e < 2 * N; ++e) f[it][e] = cut_odd(g[e]);
+        cut_odd(g, f[it]);
       }
       float most = 0.f;  // NaN is passed over, an infinity shows
 #pragma unroll
@@ -241,18 +253,27 @@ __global__ __launch_bounds__((PgTile<T, D, NEW>::THREADS)) void kv_append_e4m3_k
     if (old > 0) byte = max(byte, before);
     const float inverse = byte > 253u ? 0.f : e4_inverse(byte);
     uint8_t* codes = (is_v ? vp : kp) + ((page * pg.hkv + h) << pg.lp) * D;
+    auto store = [&](auto clamp) {
+      constexpr bool CLAMP = decltype(clamp)::value;
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      if (!mine[it]) continue;
-      uint8_t* to = codes + (row0 + it * P::ROWS) * D;
-      if constexpr (N == 8) {
-        *reinterpret_cast<uint2*>(to + lay.a) = uint2{e4_codes(f[it], inverse), e4_codes(f[it] + 4, inverse)};
-        *reinterpret_cast<uint2*>(to + lay.b) = uint2{e4_codes(f[it] + 8, inverse), e4_codes(f[it] + 12, inverse)};
-      } else {
-        *reinterpret_cast<uint32_t*>(to + lay.a) = e4_codes(f[it], inverse);
-        *reinterpret_cast<uint32_t*>(to + lay.b) = e4_codes(f[it] + 4, inverse);
+      for (int it = 0; it < ITER; ++it) {
+        if (!mine[it]) continue;
+        uint8_t* to = codes + (row0 + it * P::ROWS) * D;
+        if constexpr (N == 8) {
+          *reinterpret_cast<uint2*>(to + lay.a) =
+              uint2{e4_codes<CLAMP>(f[it], inverse), e4_codes<CLAMP>(f[it] + 4, inverse)};
+          *reinterpret_cast<uint2*>(to + lay.b) =
+              uint2{e4_codes<CLAMP>(f[it] + 8, inverse), e4_codes<CLAMP>(f[it] + 12, inverse)};
+        } else {
+          *reinterpret_cast<uint32_t*>(to + lay.a) = e4_codes<CLAMP>(f[it], inverse);
+          *reinterpret_cast<uint32_t*>(to + lay.b) = e4_codes<CLAMP>(f[it] + 4, inverse);
+        }
       }
-    }
+    };
+    if (byte < kE4MaxByte)
+      store(std::false_type());
+    else  // the largest scale, past which values are
+      store(std::true_type());
     if (old > 0 && byte != before) {  // past 2^-126 nothing is left of them
       const int down = (int)byte - (int)before;
       const float by = down < 126 ? __uint_as_float((uint32_t)(127 - down) << 23) : 0.f;
@@ -367,7 +388,7 @@ template <typename T>
 int append_e4m3_launch(const char* fn, const PgNew<T>& in, const Rope& rp, const Pages& pg, uint8_t* kp, uint8_t* vp,
                        uint8_t* ks, uint8_t* vs, int64_t B, int64_t tokens, int64_t d, hipStream_t st) {
   const int64_t page = int64_t(1) << pg.lp, count = (tokens + page - 2) / page + 1, pages = B * count;
-  if (pages * pg.hkv > int64_t(0x7fffffff) || !grid_fits(pages * pg.hkv, kPgThreads))
+  if (pages * pg.hkv > int64_t(0x7fffffff) || !grid_fits(pages * pg.hkv, 512))
     return fail(TT_ERR_ARG, std::string(fn) + ": too many pages of new tokens");
   int64_t heads = std::min<int64_t>(pg.hkv, kPgHeads);
   while (heads > 1 && 2 * pages * ((pg.hkv + heads - 1) / heads) < 4 * (int64_t)device_cu_count()) heads = (heads + 1) / 2;

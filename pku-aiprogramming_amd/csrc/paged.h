@@ -51,11 +51,16 @@ __device__ __forceinline__ float e4_clamp(float x) {
   const float y = __builtin_amdgcn_fmed3f(x, -448.f, 448.f);
   return __builtin_isfpclass(x, 0x207) ? __uint_as_float(0x7fc00000u) : y;  // an infinity or NaN, of one v_cmp_class
 }
-// Four codes of values times `inverse`, nearest, halves to even.
+// Four codes of values times `inverse`, nearest, halves to even.  CLAMP false: none is past
+// 448 but infinities, which the conversion makes NaN.
+template <bool CLAMP = true>
 __device__ __forceinline__ uint32_t e4_codes(const float* x, float inverse) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) y[i] = CLAMP ? e4_clamp(x[i] * inverse) : x[i] * inverse;
   uint32_t c = 0;
-  c = __builtin_amdgcn_cvt_pk_fp8_f32(e4_clamp(x[0] * inverse), e4_clamp(x[1] * inverse), c, false);
-  return __builtin_amdgcn_cvt_pk_fp8_f32(e4_clamp(x[2] * inverse), e4_clamp(x[3] * inverse), c, true);
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(y[0], y[1], c, false);
+  return __builtin_amdgcn_cvt_pk_fp8_f32(y[2], y[3], c, true);
 }
 // The values of four codes, not scaled.
 __device__ __forceinline__ void e4_values(uint32_t c, float* x) {
