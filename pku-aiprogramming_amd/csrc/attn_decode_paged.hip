@@ -208,8 +208,12 @@ __device__ __forceinline__ float2 pd_get_far(const float* p) {
 // The maximum is that of the products, the scale sl2 (of log2 e too, above zero:
 // its sign goes into q, and zero is the smallest fp32, 2^-149) enters the exponent,
 // 2^(sl2 s - sl2 m), one operation a score.
-// Workgroup id = (head * tiles + tile) * nsplit + split, head = b Hkv + hkv, tile =
-// 16 of the head's R query rows.  Each sequence's own length is cut into nsplit
+// A workgroup: tile, 16 of the R query rows of head = b Hkv + hkv, and a split of its keys.
+// The tiles of a head's split are eight ids apart (the last, fewer than eight splits of all,
+// as many): on one XCD, whose L2 hands the keys from one to the next.  (Side by side: 3
+// tokens of 3 x 128 / 16 heads x up to 14211 keys 87 us for 65, 8 of 4 x 64 / 8 x 4096 22 for
+// 19.  Two tiles of a wave, for which K and V come to LDS once: 58 in the first, but their
+// registers leave half the waves; over 8 bits 22 for 19, fp32 at d = 64 91 for 76.)  Each sequence's own length is cut into nsplit
 // spans, so that sequences of any length keep every workgroup busy.
 template <typename T, typename C, int D, bool STREAM>
 __global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode_paged_kernel(
@@ -230,8 +234,15 @@ __global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode
 
   const int l = threadIdx.x & 63, r = l & 15, g = l >> 4;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t unit = blockIdx.x / nsplit, split = blockIdx.x - unit * nsplit;
-  const uint32_t head = unit / tiles, row0 = (unit - head * tiles) * kMdRows;
+  uint32_t tile = 0, span = blockIdx.x;  // head * nsplit + split
+  if constexpr (!STREAM) {
+    const uint32_t spans = gridDim.x / tiles, eights = span / (8 * tiles), wide = min(spans - 8 * eights, 8u);
+    span -= eights * 8 * tiles;
+    tile = span / wide;
+    span = 8 * eights + span - tile * wide;
+  }
+  const uint32_t head = span / nsplit, split = span - head * nsplit, unit = head * tiles + tile;
+  const uint32_t row0 = tile * kMdRows;
   const int64_t qrow = (int64_t)head * R + row0;  // the tile's first row of q and o
   const int nrows = (int)min((uint32_t)kMdRows, R - row0);
 
