@@ -548,6 +548,46 @@ def test_threads_and_streams(capi):
                 assert np.array_equal(a.download(), b)
 
 
+def test_graphs_that_share_scratch(capi):
+    """Two graphs of one stream, of other types and numbers of splits, replayed in turn with eager calls between."""
+    rng, st, jobs = np.random.default_rng(40), capi.Stream(), []
+    for dtype, cache, d, n, H, T in (("bf16", "bf16", 64, 5000, 2, 2), ("f32", "u8", 128, 700, 3, 1)):
+        c = filled(capi, dtype, cache, 2, 1, 64, d, [n, n - 90], rng)
+        q, x, dy = (capi.DeviceBuffer((2, H, t, d), dtype) for t in (T, 50, 50))
+        o, lse, dx = capi.DeviceBuffer(q.shape, dtype), capi.DeviceBuffer((2, H, T)), capi.DeviceBuffer(x.shape, dtype)
+        w, dw, F = capi.DeviceBuffer.from_numpy(normal(rng, (d,), "f32")), capi.DeviceBuffer((d,)), capi.DeviceBuffer.from_numpy(FREQ[d])
+
+        def step(c=c, q=q, x=x, dy=dy, o=o, lse=lse, dx=dx, w=w, dw=dw, F=F):
+            capi.attn_decode_paged(q, c.dev["k"], c.dev["v"], c.tab, c.lengths, o, lse, 0.2, stream=st.handle, **c.scales())
+            capi.norm_rope_backward(x, dy, dx, w, dw, F, eps=EPS, stream=st.handle)
+
+        c.lengths.upload(np.array([n, n - 90], np.int32))
+        for b in (q, x, dy):
+            b.fill_normal(1)
+        capi.lib().sync()
+        step()
+        st.sync()
+        with Capture(capi, st.handle, 1) as g:
+            step()
+        jobs.append(dict(step=step, g=g, inputs=(q, x, dy), out=(o, lse, dx, dw), dtype=dtype))
+    for i in range(6):
+        for j in jobs:
+            for b in j["inputs"]:
+                b.upload(normal(rng, b.shape, j["dtype"]))
+        capi.lib().sync()
+        ref = []
+        for j in jobs:
+            j["step"]()
+            st.sync()
+            ref.append([b.download() for b in j["out"]])
+        for j, r in list(zip(jobs, ref))[::1 if i % 2 else -1] * 2:
+            for b in j["out"]:
+                b.zero()
+            capi.lib().sync()
+            j["g"].launch()
+            assert all(np.array_equal(b.download(), a) for b, a in zip(j["out"], r))
+
+
 REFUSED = r"""
 import ctypes as C, numpy as np, tt_capi as T
 from oracle import paged_oracle as po
