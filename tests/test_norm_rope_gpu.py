@@ -215,6 +215,38 @@ def test_strided_rows_between_others(capi):
     assert (got == 7.0).all()
 
 
+@pytest.mark.parametrize("parts", ["q", "k", "v", "kv", "qv"])
+def test_some_of_the_parts(capi, parts):
+    """q, k and v given or not, head-major: what is not given is neither read nor written; frequencies of no pair."""
+    rng = np.random.default_rng(10)
+    B, T, H, Hkv, d = 2, 21, 3, 2, 64
+    heads, w, F = dict(q=H, k=Hkv, v=Hkv), normal(rng, (d,), "f32"), capi.DeviceBuffer.from_numpy(FREQ[32])
+    x = {n: normal(rng, (B, h, T, d), "f32") for n, h in heads.items()}
+    dy = {n: normal(rng, (B, h, T, d), "f32") for n, h in heads.items()}
+    X, DY, W = ({n: capi.DeviceBuffer.from_numpy(a) for n, a in g.items()} for g in (x, dy, dict(q=w, k=w)))
+    out, dx = ({n: capi.DeviceBuffer.from_numpy(np.full(a.shape, 7.0, np.float32)) for n, a in x.items()} for _ in range(2))
+    dw = {n: capi.DeviceBuffer.from_numpy(np.full(d, 7.0, np.float32)) for n in "qk"}
+    ptr = lambda g, n: g[n].ptr if n in parts else None  # noqa: E731
+    for rot in (32, 0):
+        rope = (EPS, F.ptr, rot, 0, None, None)
+        capi.lib().call("tt_qkv_norm_rope", capi.TT_F32, *(ptr(X, n) for n in "qkv"), 0, 0, 0, W["q"].ptr, W["k"].ptr, *rope,
+                        *(ptr(out, n) for n in "qkv"), B, H, Hkv, T, d, None)
+        capi.lib().call("tt_qkv_norm_rope_backward", capi.TT_F32, ptr(X, "q"), ptr(X, "k"), 0, 0, W["q"].ptr, W["k"].ptr, *rope,
+                        *(ptr(DY, n) for n in "qkv"), *(ptr(dx, n) for n in "qkv"), 0, 0, 0, ptr(dw, "q"), ptr(dw, "k"),
+                        B, H, Hkv, T, d, None)
+        capi.lib().sync()
+        pos, freq = po.positions(B, T), FREQ[rot] if rot else None
+        for n in "qkv":
+            if n not in parts:
+                assert (out[n].download() == 7.0).all() and (dx[n].download() == 7.0).all()
+                assert n == "v" or (dw[n].download() == 7.0).all()
+            elif n == "v":
+                assert np.array_equal(out[n].download(), x[n]) and np.array_equal(dx[n].download(), dy[n])
+            else:
+                check_forward(out[n].download(), x[n], w, pos, freq, False, "f32")
+                check_backward(dx[n].download(), dw[n].download(), x[n], w, dy[n], pos, freq, False, "f32", B * T * heads[n])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_sums(capi, dtype):
     """More rows than workgroups that leave sums, of gradients that do not cancel."""
