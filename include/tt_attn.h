@@ -442,8 +442,8 @@ int tt_qkv_norm_rope(int dtype, const void* q, const void* k, const void* v, int
  * between each other's rows), and to the weights' dq_weight, dk_weight [d] (float,
  * may be null), sums over all rows in a fixed order.  q and k are what the
  * forward call read, and may be null where they were not normed.  With no rows
- * the weights' gradients are zero.  These sums meet in a fixed 1 MiB per-stream
- * library workspace (allocated on first use); without it (refused, or under graph
+ * the weights' gradients are zero.  These sums meet in a fixed per-stream library
+ * workspace of about 1 MiB (allocated on first use); without it (refused, or under graph
  * capture before a call has left it on the stream) a call that asks for them
  * fails with TT_ERR_NOMEM, as it does with TT_ERR_ARG for more than 2048 heads. */
 int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t ldq, int64_t ldk, const float* q_weight,
@@ -504,9 +504,9 @@ int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_
  * they hold; an infinite or NaN value of V reaches the tokens that see its key
  * and no others.  Scores, weights and sums are in fp32, of which the weights of
  * bf16 calls keep 16 bits (2^-17 off) where they meet V; the sums are divided
- * last, so a value of V times the number of keys must stay finite.  B H T is below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an
- * unsplit call, below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over
- * workgroups and merge their sums through a fixed 24 MiB per-stream library
+ * last, so a value of V times the number of keys must stay finite.  B H T is
+ * below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an unsplit call,
+ * below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over workgroups and merge their sums through a fixed 24 MiB per-stream library
  * workspace (allocated on first use); without it (refused, or under graph
  * capture before a call has left it on the stream) they run unsplit.  Graphs
  * captured on one stream share it and must be replayed in stream order. */

@@ -213,8 +213,9 @@ __device__ __forceinline__ float2 pd_get_far(const float* p) {
 // as many): on one XCD, whose L2 hands the keys from one to the next.  (Side by side: 3
 // tokens of 3 x 128 / 16 heads x up to 14211 keys 87 us for 65, 8 of 4 x 64 / 8 x 4096 22 for
 // 19.  Two tiles of a wave, for which K and V come to LDS once: 58 in the first, but their
-// registers leave half the waves; over 8 bits 22 for 19, fp32 at d = 64 91 for 76.)  Each sequence's own length is cut into nsplit
-// spans, so that sequences of any length keep every workgroup busy.
+// registers leave half the waves; over 8 bits 22 for 19, fp32 at d = 64 91 for 76.)
+// Each sequence's own length is cut into nsplit spans, so that sequences of any
+// length keep every workgroup busy.
 template <typename T, typename C, int D, bool STREAM>
 __global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode_paged_kernel(
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,

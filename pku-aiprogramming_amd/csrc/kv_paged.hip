@@ -164,7 +164,8 @@ __global__ __launch_bounds__((PgTile<T, D, NEW>::THREADS)) void kv_append_e4m3_k
   if (base >= end) return;
   const int64_t page = pg.table[b * pg.width + j];
   if (page < 0 || page >= pg.pages) return;
-  const int old = (int)max(first - base, (int64_t)0), fill = (int)min(end - base, (int64_t)1 << pg.lp);  // rows [old, fill) are new
+  // rows [old, fill) are new
+  const int old = (int)max(first - base, (int64_t)0), fill = (int)min(end - base, (int64_t)1 << pg.lp);
   if (old >= fill) return;
   const bool norm = !is_v && in.weight, turns = !is_v && rp.freq;
   const Lay<N> lay(threadIdx.x % LPR, turns ? rp.rot : 0, rp.inter != 0);

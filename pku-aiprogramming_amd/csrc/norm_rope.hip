@@ -11,7 +11,8 @@
 //   dw = sum over rows of g n,   dx = r (g w - n mean(g w n)).
 // r is formed again from x, which is read anyway.  A thread sums its rows' g n in
 // registers, a workgroup its threads' in LDS, a second launch the workgroups' in the
-// order of their numbers, so the result does not depend on which ends first.
+// order of their numbers (of a few, the last workgroup to end does), so the result does
+// not depend on which ends first.
 // Measured (MI355X): 4 x 4096 tokens of 32 / 32 heads of 128 in bf16, one fused projection:
 // forward 155 us (805 MB, 5.2 TB/s), back 219 us (1074 MB, 4.9 TB/s); 8 tokens 4 us.
 #include <hip/hip_runtime.h>
@@ -176,11 +177,15 @@ struct NrBack {
 
 // A workgroup: tiles slot, slot + slots, ... of 256 / LPR tokens, a chunk of the heads
 // of q, k or v.  sums: [slots][chunks of q][D] and then [slots][chunks of k][D], or null
-// where no weight's gradient is asked for.
+// where no weight's gradient is asked for.  count (of q, of k; zero between calls): the
+// last workgroup of each adds them up to dwq or dwk.
 template <typename T, int D, int HC, bool NT>
 __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T> q, NrBack<T> k, NrBack<T> v, Rope rp,
                                                                        uint32_t rows, uint32_t tokens, uint32_t slots,
-                                                                       NrCut cut, float* __restrict__ sums) {
+                                                                       NrCut cut, float* __restrict__ sums,
+                                                                       uint32_t* __restrict__ count,
+                                                                       float* __restrict__ dwq,
+                                                                       float* __restrict__ dwk) {
   constexpr int N = Chunk<T>::N, LPR = D / (2 * N), TPB = kNrThreads / LPR;
   using Row = NrRow<T, D, NT>;
   const uint32_t slot = blockIdx.x / cut.all;
@@ -255,7 +260,7 @@ __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T>
         });
   }
   if (!sums || part == 2) return;
-  __shared__ float s_sum[kNrThreads / 64][D];
+  __shared__ float s_sum[kNrThreads / 64 * D < kNrThreads ? kNrThreads / D : kNrThreads / 64][D];
 #pragma unroll
   for (int e = 0; e < 2 * N; ++e) {
     float x = acc[e];
@@ -264,12 +269,47 @@ __global__ __launch_bounds__(kNrThreads) void qkv_norm_rope_bwd_kernel(NrBack<T>
     if ((threadIdx.x & 63) < LPR) s_sum[threadIdx.x >> 6][(e < N ? lay.a : lay.b - N) + e] = x;
   }
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float x = 0.f;
+  const uint32_t nq = slots * cut.chunks[0], nk = slots * cut.chunks[1];
+  const uint32_t at = part == 0 ? slot * cut.chunks[0] + chunk : nq + slot * cut.chunks[1] + chunk;
+  if (threadIdx.x < D) {
+    float x = 0.f;
 #pragma unroll
-  for (int i = 0; i < kNrThreads / 64; ++i) x += s_sum[i][threadIdx.x];
-  const uint32_t at = part == 0 ? slot * cut.chunks[0] + chunk : slots * cut.chunks[0] + slot * cut.chunks[1] + chunk;
-  sums[(int64_t)at * D + threadIdx.x] = x;
+    for (int i = 0; i < kNrThreads / 64; ++i) x += s_sum[i][threadIdx.x];
+    float* to = sums + (int64_t)at * D + threadIdx.x;
+    if (count)  // past the caches that only some compute units share
+      __hip_atomic_store(to, x, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    else
+      *to = x;
+  }
+  if (!count) return;
+  // Stores have ended, and all see them, before the workgroup counts itself.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+  __shared__ uint32_t s_before;
+  const uint32_t n = part == 0 ? nq : nk;
+  if (threadIdx.x == 0) s_before = atomicInc(count + part, n - 1);
+  __syncthreads();
+  float* dw = part == 0 ? dwq : dwk;
+  if (s_before != n - 1 || !dw) return;
+  constexpr uint32_t G = kNrThreads / D;
+  const uint32_t col = threadIdx.x % D, g = threadIdx.x / D;
+  const float* from = sums + (part == 0 ? 0 : (int64_t)nq * D) + col;
+  float x = 0.f;
+  for (uint32_t i0 = g; i0 < n; i0 += 8 * G) {
+    float y[8];
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u)
+      y[u] = __hip_atomic_load(from + (int64_t)min(i0 + u * G, n - 1) * D, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+#pragma unroll
+    for (uint32_t u = 0; u < 8; ++u) x += i0 + u * G < n ? y[u] : 0.f;
+  }
+  float* all = &s_sum[0][0];  // [G][D]
+  all[g * D + col] = x;
+  __syncthreads();
+  if (g > 0) return;
+#pragma unroll
+  for (uint32_t u = 1; u < G; ++u) x += all[u * D + col];
+  dw[col] = x;
 }
 
 // Column i of sums [nq][D] to dwq, of the [nk][D] behind them to dwk, 16 columns a
@@ -302,7 +342,13 @@ __global__ __launch_bounds__(kNrSumThreads) void norm_weight_sum_kernel(const fl
 // keep its address.  4 x 4096 tokens of 96 heads 229 us with 1024, 220 with 2048, 219 with
 // 4096, 223 with 8192; 1843 tokens of 160 heads 59, 60, 63, 63.
 constexpr int64_t kNrSums = 2048;
-constexpr size_t kNrWork = size_t(kNrSums) * 128 * sizeof(float);
+constexpr size_t kNrSumBytes = size_t(kNrSums) * 128 * sizeof(float), kNrWork = kNrSumBytes + 2 * sizeof(uint32_t);
+// So many values of sums, of q and of k, the last workgroup adds up: 23 x 4 tokens of 8 / 1
+// heads of 128 11.9 -> 8.9 us, 2 x 284 of 12 / 3 heads of 64 (6.9 k) 11.9 -> 9.5, in fp32 (13.8
+// k) 11.9 -> 10.3.  More have a launch of their own: 2 x 480 of 4 / 4 heads of 128 (15 k) 11.8
+// so and 12.2 without, 8 x 512 of 8 / 2 heads of 64 (33 k) 11.8 and 20.
+constexpr int64_t kNrFewValues = 12288;
+__global__ void nr_zero_kernel(uint32_t* p) { p[threadIdx.x] = 0u; }
 
 // Four heads a workgroup, for the angles that it forms once and the loads that it has
 // in flight; two, or one, where more would leave fewer than two workgroups a CU.
@@ -354,6 +400,7 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
   constexpr int TPB = kNrThreads / (D / (2 * Chunk<T>::N));
   const int64_t tiles = (n.B * n.T + TPB - 1) / TPB, heads = (int64_t)q.heads + k.heads + v.heads;
   float* sums = nullptr;
+  uint32_t* count = nullptr;
   std::optional<WorkspaceLease> lease;  // held until both kernels are queued
   int64_t nq = 0, nk = 0;
   if (tiles > 0 && heads > 0) {
@@ -362,18 +409,26 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
     if (dwq || dwk) {
       const int64_t each = (int64_t)cut.chunks[0] + cut.chunks[1];
       void* ws = nullptr;
-      if (!lease.emplace().get_fixed(st, kWsNormWeights, kNrWork, &ws))
+      bool fresh = false;
+      if (!lease.emplace().get_fixed(st, kWsNormWeights, kNrWork, &ws, &fresh))
         return fail(TT_ERR_NOMEM, std::string(fn) + ": no scratch for the weights' gradients (under graph capture it "
                                                     "must be there from an earlier call on the stream)");
       sums = (float*)ws;
+      count = (uint32_t*)((char*)ws + kNrSumBytes);
+      if (fresh) {
+        hipLaunchKernelGGL(nr_zero_kernel, dim3(1), dim3(2), 0, st, count);
+        TT_LAUNCHED(fn, st);
+      }
       if (each > 0) slots = std::min(tiles, kNrSums / each);
       nq = slots * cut.chunks[0];
       nk = slots * cut.chunks[1];
+      if (std::max(nq, nk) * D > kNrFewValues || (dwq && nq == 0) || (dwk && nk == 0)) count = nullptr;
     }
     if (!grid_fits(slots * cut.all, kNrThreads)) return fail(TT_ERR_ARG, std::string(fn) + ": too many rows");
 #define TT_NR_BWD(HC, NT)                                                                                             \
   hipLaunchKernelGGL((qkv_norm_rope_bwd_kernel<T, D, HC, NT>), dim3((unsigned)(slots * cut.all)), dim3(kNrThreads), 0, \
-                     st, q, k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)slots, cut, sums)
+                     st, q, k, v, rp, (uint32_t)(n.B * n.T), (uint32_t)n.T, (uint32_t)slots, cut, sums, count,           \
+                     dwq, dwk)
     if (cut.count == 1)
       TT_NR_BWD(1, false);
     else if (cut.count == 2)
@@ -385,7 +440,7 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
 #undef TT_NR_BWD
     TT_LAUNCHED(fn, st);
   }
-  if (dwq || dwk) {
+  if ((dwq || dwk) && !count) {
     hipLaunchKernelGGL((norm_weight_sum_kernel<D>), dim3(2 * D / 16), dim3(kNrSumThreads), 0, st, sums, dwq, dwk,
                        (int)nq, (int)nk);
     TT_LAUNCHED(fn, st);

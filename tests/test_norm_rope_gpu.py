@@ -247,6 +247,35 @@ def test_some_of_the_parts(capi, parts):
                 check_backward(dx[n].download(), dw[n].download(), x[n], w, dy[n], pos, freq, False, "f32", B * T * heads[n])
 
 
+@pytest.mark.parametrize("d", [32, 64, 128])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_few_and_many_sums_in_turn(capi, dtype, d):
+    """Sums that the last workgroup adds up and sums that a launch does, of one weight and of both, call after call."""
+    rng = np.random.default_rng(11)
+    w = capi.DeviceBuffer.from_numpy(1 + normal(rng, (d,), "f32"))
+    jobs = []
+    for B, T, H, Hkv, both in ((1, 1, 1, 1, True), (3, 50, 4, 2, True), (2, 33, 5, 1, False), (2, 700, 6, 2, True)):
+        x, dy = normal(rng, (B, T, H + 2 * Hkv, d), dtype), [normal(rng, (B, h, T, d), dtype) for h in (H, Hkv, Hkv)]
+        jobs.append((B, T, H, Hkv, both, x, dy, capi.DeviceBuffer.from_numpy(x, dtype), [capi.DeviceBuffer.from_numpy(a, dtype) for a in dy]))
+    first = {}
+    for turn in range(4):
+        for i, (B, T, H, Hkv, both, x, dy, X, DY) in enumerate(jobs):
+            dx, dw = capi.DeviceBuffer(x.shape, dtype), [capi.DeviceBuffer((d,)) for _ in range(2)]
+            capi.qkv_norm_rope_backward(X, *DY, dx, w, w, dw[0] if both else None, dw[1], eps=EPS)
+            capi.lib().sync()
+            got = [dx.download(), dw[1].download()] + ([dw[0].download()] if both else [])
+            if turn:
+                assert all(np.array_equal(a, b) for a, b in zip(got, first[i]))
+                continue
+            first[i] = got
+            sides = [np.ascontiguousarray(np.swapaxes(p, 1, 2)) for p in np.split(x, [H, H + Hkv], 2)]
+            back = [np.swapaxes(p, 1, 2) for p in np.split(got[0], [H, H + Hkv], 2)]
+            W, pos = w.download(), po.positions(B, T)
+            check_backward(back[0], got[2] if both else None, sides[0], W, dy[0], pos, None, False, dtype, B * T * H)
+            check_backward(back[1], got[1], sides[1], W, dy[1], pos, None, False, dtype, B * T * Hkv)
+            assert np.array_equal(back[2], dy[2])
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_long_sums(capi, dtype):
     """More rows than workgroups that leave sums, of gradients that do not cancel."""
