@@ -445,7 +445,8 @@ int tt_qkv_norm_rope(int dtype, const void* q, const void* k, const void* v, int
  * the weights' gradients are zero.  These sums meet in a fixed per-stream library
  * workspace of about 1 MiB (allocated on first use); without it (refused, or under graph
  * capture before a call has left it on the stream) a call that asks for them
- * fails with TT_ERR_NOMEM, as it does with TT_ERR_ARG for more than 2048 heads. */
+ * fails with TT_ERR_NOMEM, as it does with TT_ERR_ARG for more than 2048 heads.
+ * Graphs captured on one stream share it and must be replayed in stream order. */
 int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t ldq, int64_t ldk, const float* q_weight,
                               const float* k_weight, float eps, const float* inv_freq, int64_t rot, int interleaved,
                               const int* positions, const int* lengths, const void* dq_out, const void* dk_out,
