@@ -25,8 +25,8 @@
 // which a page's number comes without memory's latency.
 // Measured (MI355X, d = 128): 64 sequences of up to 8192 keys, 32 / 8 heads of bf16, 252 us
 // (6.3 TB/s); 32 / 32 heads over 8 bits, 663 us (6.5 TB/s); one of 4097 keys, 11.4 us, a
-// chain of latencies; 3 tokens of 12 x 20 / 4 heads of fp32 over 8 bits, 34.5 us (4.2 TB/s:
-// three terms of q and of the weights, and the longest sequences last).
+// chain of memory latencies; 3 tokens of 12 x 20 / 4 heads of fp32 over 8 bits, 34.5 us (4.2 TB/s:
+// vector work of three terms of q and of the weights).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -408,6 +408,26 @@ def test_values_that_are_not_finite(capi, d, dtype, cache):
     assert np.array_equal(o[:, :, :3], clean[:, :, :3]) and np.isnan(o[:, :, 3]).all()
 
 
+
+@pytest.mark.parametrize("dtype,cache", KINDS)
+@pytest.mark.parametrize("n,H,T", [(77, 9, 5), (1500, 1, 3), (1500, 9, 5)])
+def test_infinite_values_over_tiles_and_splits(capi, n, H, T, dtype, cache):
+    """One column of a key that the last token alone sees, with several tiles of rows, splits, and splits merged by
+    their last workgroup: the other tokens and columns keep their bits."""
+    rng = np.random.default_rng(n + H)
+    page, d = 32, 64
+    c = filled(capi, dtype, cache, 2, 1, page, d, [n, n], rng)
+    q = normal(rng, (2, H, T, d), dtype)
+    clean, lse = c.attend(q, [n, n - 40], 0.2)
+    host = c.dev["v"].download_bytes() if cache == "u8" else c.dev["v"].download()
+    host[c.table[0, (n - 1) // page], 0, (n - 1) % page, 5] = 127 if cache == "u8" else np.inf
+    c.dev["v"].upload(host)
+    o, again = c.attend(q, [n, n - 40], 0.2)
+    assert np.array_equal(again, lse) and np.array_equal(o[1], clean[1]) and np.array_equal(o[0, :, :-1], clean[0, :, :-1])
+    assert not np.isfinite(o[0, :, -1, 5]).any()
+    assert np.array_equal(np.delete(o[0, :, -1], 5, -1), np.delete(clean[0, :, -1], 5, -1))
+
+
 @pytest.mark.parametrize("dtype,cache", KINDS)
 def test_scores_of_minus_infinity(capi, dtype, cache):
     """A row all of whose keys score -inf has nothing to weigh: o = 0, lse = -inf; one key above it has all the weight."""
