@@ -13,7 +13,7 @@
 // Measured (MI355X): 4 x 4001 tokens of 8 heads of 128 in fp32, 166 MB, 34 us (4.9 TB/s),
 // 16 x 16 heads 288 us (5.4 TB/s); 8 x 4000 tokens of bf16 into 8 bits 46 us, in which a
 // third of the wave cycles issue vector instructions, with two waves a SIMD (64-bit values in
-// registers), and read back 24 us (5.6 TB/s).
+// registers), and read back 23 us (5.9 TB/s).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -290,11 +290,12 @@ __global__ __launch_bounds__((PgTile<T, D, NEW>::THREADS)) void kv_append_e4m3_k
 }
 
 // Rows that fill more than this go by the caches: 8 x 8 heads x 4096 keys of 128 in
-// 8 bits, 134 MB as bf16, 28 -> 22 us.  Smaller ones the next kernel may still find there.
+// 8 bits, 134 MB as bf16, with their append 75 -> 68 us.  Smaller ones the next kernel may still find there.
 constexpr int64_t kPgNtBytes = int64_t(64) << 20;
 // Rows [B][Hkv][L][D] of T from a pool of C, 16 bytes of them a lane and kPgUnroll rows:
-// workgroup id = head * tiles + tile of kPgUnroll 256 / W rows.
-constexpr int kPgUnroll = 4;
+// workgroup id = head * tiles + tile of kPgUnroll 256 / W rows.  Of one, two, four and eight
+// rows a lane 8 x 4000 tokens appended and read back take 69.5, 67.9, 69.8 and 73.0 us.
+constexpr int kPgUnroll = 2;
 template <typename T, typename C, int D, bool NT>
 __global__ __launch_bounds__(kPgThreads) void kv_gather_kernel(const C* __restrict__ kp, const C* __restrict__ vp,
                                                                const uint8_t* __restrict__ ks,
