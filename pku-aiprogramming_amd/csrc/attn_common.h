@@ -234,19 +234,21 @@ __device__ __forceinline__ uint32_t lds_addr(const void* p) {
 // kernels order these loads themselves: a vmcnt wait for the tile (loads
 // retire in order) followed by a workgroup barrier, before any LDS read of
 // that buffer.  M0 is a reserved register that the compiler only sets right
-// before the instructions that read it; each statement sets it itself.
+// before the instructions that read it; each statement sets it itself, and
+// waits the one state that gfx950 needs between a write of M0 and a load that
+// reads it (the compiler adds it to the builtin form, not to inline assembly).
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void glds16(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(voff), "s"(sbase), "s"(lds)
                : "memory", "m0");
 }
 // The same from an address of each lane's own.
 __device__ __forceinline__ void glds16_at(const void* p, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void glds4(const void* sbase, uint32_t voff, uint32_t lds) {
-  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds)
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(voff), "s"(sbase), "s"(lds)
                : "memory", "m0");
 }
 #pragma clang diagnostic pop

@@ -97,14 +97,16 @@ __device__ __forceinline__ u32x2 lds_tr8_at(uint32_t a) {
 template <bool NT>
 __device__ __forceinline__ void pd_glds16(const void* sbase, uint32_t voff, uint32_t lds) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(voff), "s"(sbase), "s"(lds)
+                 : "memory", "m0");
   else
     glds16(sbase, voff, lds);
 }
 template <bool NT>
 __device__ __forceinline__ void pd_glds16_at(const void* p, uint32_t lds) {
   if constexpr (NT)
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(p), "s"(lds)
+                 : "memory", "m0");
   else
     glds16_at(p, lds);
 }
