@@ -755,7 +755,7 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
   if (nsplit < 2 || !lease.emplace().get_fixed(st, kWsPagedDecode, kPdWork, &ws, &fresh)) nsplit = 1;
   if (fresh) {
     hipLaunchKernelGGL(pd_zero_kernel, dim3(16), dim3(256), 0, st, (uint32_t*)ws, (int)kPdCounts);
-    TT_LAUNCHED(fn, st);
+    if (const int rc = lease->cleared(fn, st, kWsPagedDecode)) return rc;
   }
   const bool fused = nsplit > 1 && nsplit <= kPdMergeSplits && cap <= nsplit * kPdMergeSpan && R <= kMdWaves &&
                      units <= kPdCounts;

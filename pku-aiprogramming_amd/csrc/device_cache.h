@@ -259,6 +259,10 @@ class WorkspaceCache {
       if (it == c_.slots_.end() || it->second.bytes < bytes) return false;
       return c_.get_locked(stream, user, bytes, ptr, nullptr) == 0;
     }
+    // Gives the buffer up, for a user whose work that fills a new one could not
+    // be queued: the next call gets a new one, and is told so.  Waits for the
+    // stream; where that fails, the block is not handed out again.
+    void drop(void* stream, int user) { c_.drop_locked(stream, user); }
 
    private:
     WorkspaceCache& c_;
@@ -338,6 +342,12 @@ class WorkspaceCache {
     *ptr = p;
     if (uses) *uses = 0;
     return 0;
+  }
+  void drop_locked(void* stream, int user) {
+    auto it = slots_.find({stream, user});
+    if (it == slots_.end()) return;
+    if (be_.sync(stream) == 0) blocks_.release(it->second.ptr);
+    slots_.erase(it);
   }
 
   Backend& be_;

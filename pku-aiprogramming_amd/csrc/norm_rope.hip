@@ -417,7 +417,7 @@ int backward_launch(const char* fn, NrBack<T> q, NrBack<T> k, NrBack<T> v, const
       count = (uint32_t*)((char*)ws + kNrSumBytes);
       if (fresh) {
         hipLaunchKernelGGL(nr_zero_kernel, dim3(1), dim3(2), 0, st, count);
-        TT_LAUNCHED(fn, st);
+        if (const int rc = lease->cleared(fn, st, kWsNormWeights)) return rc;
       }
       if (each > 0) slots = std::min(tiles, kNrSums / each);
       nq = slots * cut.chunks[0];

@@ -518,8 +518,10 @@ extern "C" int tt_softmax_rows_f32(const float* x, float* y, int64_t rows, int64
         ws.emplace().get_optional(s, kWsSoftmaxPartials, bytes, (void**)&slots, &uses)) {
       const unsigned gen = (unsigned)(uses % 0xffffffffull) + 1;  // 1 .. 2^32 - 1
       if (gen == 1 &&  // a new buffer (or a wrapped count): no word may hold a live generation
-          (rc = tt_elementwise(TT_EW_FILL, TT_F32, slots, nullptr, nullptr, (int64_t)(bytes / 4), 0.0, 0.0, 0, s)))
+          (rc = tt_elementwise(TT_EW_FILL, TT_F32, slots, nullptr, nullptr, (int64_t)(bytes / 4), 0.0, 0.0, 0, s))) {
+        ws->drop(s, kWsSoftmaxPartials);
         return rc;
+      }
       const dim3 grid((unsigned)(rows * nchunk)), blk(kBlock);
       const int n = (int)nchunk;
 #define TT_SPLIT(NE)                                                                                             \

@@ -69,6 +69,10 @@ class WorkspaceLease {
   // the one that an earlier call left.  *fresh (optional): whether it is new, its
   // contents undefined.
   bool get_fixed(hipStream_t stream, int user, size_t bytes, void** ptr, bool* fresh = nullptr);
+  // After the launch that clears such a buffer: its error, with the buffer given up,
+  // so that no later call takes it for cleared.
+  int cleared(const char* what, hipStream_t stream, int user);
+  void drop(hipStream_t stream, int user);
 
  private:
   struct Impl;

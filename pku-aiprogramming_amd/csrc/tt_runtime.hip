@@ -180,6 +180,16 @@ bool WorkspaceLease::get_fixed(hipStream_t s, int user, size_t bytes, void** ptr
   if (fresh) *fresh = uses == 0;
   return true;
 }
+int WorkspaceLease::cleared(const char* what, hipStream_t s, int user) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    drop(s, user);
+    return hip_fail(e, what);
+  }
+  after_launch(s);
+  return TT_OK;
+}
+void WorkspaceLease::drop(hipStream_t s, int user) { impl_->lease.drop(static_cast<void*>(s), user); }
 
 // ---------------------------------------------------------------- elementwise
 __device__ __forceinline__ uint64_t splitmix64(uint64_t x) {
