@@ -1173,8 +1173,13 @@ void KvGatherPaged(const TinyTensor<C>& k_pages, const TinyTensor<C>& v_pages, c
             {data_of(k_scales), "k_scales"},
             {data_of(v_scales), "v_scales"}},
            {{k.p_data, "k"}, {v.p_data, "v"}});
-  k.resize_output({c.B, c.Hkv, length, c.d});
-  v.resize_output({c.B, c.Hkv, length, c.d});
+  for (TinyTensor<T>* t : {&k, &v}) {
+    const std::vector<int> shape{c.B, c.Hkv, length, c.d};
+    if (t->shape == shape) continue;
+    t->resize_output(shape);  // rows that get no key are zeros there, not what the memory held
+    tt_check(tt_elementwise(TT_EW_FILL, dtype_code<T>(), t->p_data, nullptr, nullptr, (int64_t)t->size, 0.0, 0.0, 0, nullptr),
+             fn.c_str());
+  }
   tt_check(tt_kv_gather_paged(dtype_code<T>(), cache_code<C>(), k_pages.p_data, v_pages.p_data, data_of(k_scales),
                               data_of(v_scales), table.p_data, lengths.p_data, k.p_data, v.p_data, c.B, c.Hkv, length,
                               c.d, c.npages, c.page, c.width, nullptr),

@@ -181,7 +181,8 @@ void QkvNormRopeBackward(const TinyTensor<T>& qkv, const TinyTensor<T>& grad_q, 
 // counted.  KvAppendPaged: k, v [B, Hkv, T, d] (tokens_first: [B, T, Hkv, d]) into the
 // pools in place, K normed and rotated on the way.  KvGatherPaged: the first
 // `length` keys back to k, v [B, Hkv, length, d]; rows behind a sequence's end are
-// left as they are.  AttentionDecodePaged: q [B, H, T, d] -> out.
+// left as they are where k and v have that shape, and zeros where they are given it.
+// AttentionDecodePaged: q [B, H, T, d] -> out.
 template <typename T, typename C>
 void KvAppendPaged(const TinyTensor<T>& k, const TinyTensor<T>& v, TinyTensor<C>& k_pages, TinyTensor<C>& v_pages,
                    const TinyTensor<int>& table, const TinyTensor<int>& lengths, const TinyTensor<float>* k_weight,
