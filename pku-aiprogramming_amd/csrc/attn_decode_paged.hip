@@ -147,10 +147,13 @@ __device__ __forceinline__ void pd_four(const uint8_t* row, int c, float scale, 
   for (int e = 0; e < 4; ++e) x[e] *= scale;
 }
 
-// Waves of a SIMD that the registers are held to: what their tiles let onto a CU.
-template <typename T, typename C, int D>
+// Waves of a SIMD that the registers are held to: what their tiles let onto a CU, but
+// for d = 128 over 8 bits, whose four would leave 128 registers: bf16 calls would keep
+// four of their values in memory (64 x 32 heads x 8192 keys 662 us so and 640 with three;
+// 16 x 16 x 1024 14.7 and 14.4, one user's 4097 keys 11.1 both).
+template <typename C, int D>
 constexpr int pd_waves() {
-  return sizeof(C) > 1 ? 2 : sizeof(T) == 4 && D == 128 ? 3 : 4;
+  return sizeof(C) > 1 ? 2 : D == 128 ? 3 : 4;
 }
 
 // The wave's place in its sequence's table: entries [base, base + 64) and the 64
@@ -219,7 +222,7 @@ __device__ __forceinline__ float2 pd_get_far(const float* p) {
 // Each sequence's own length is cut into nsplit spans, so that sequences of any
 // length keep every workgroup busy.
 template <typename T, typename C, int D, bool STREAM>
-__global__ __launch_bounds__(kMdThreads, (pd_waves<T, C, D>())) void attn_decode_paged_kernel(
+__global__ __launch_bounds__(kMdThreads, (pd_waves<C, D>())) void attn_decode_paged_kernel(
     const T* __restrict__ q, const C* __restrict__ kp, const C* __restrict__ vp, const uint8_t* __restrict__ ks,
     const uint8_t* __restrict__ vs, Pages pg, float* __restrict__ part_o, float2* __restrict__ part_ml,
     T* __restrict__ o, float* __restrict__ lse, uint32_t R, uint32_t tokens, uint32_t tiles, uint32_t nsplit,
