@@ -503,8 +503,7 @@ int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_
  * Hkv)), lse [B][H][T] (float, natural log, may be NULL).  A token that sees no
  * key gets o = 0 and lse = -inf.  Rows that no token sees are not used, whatever
  * they hold; an infinite or NaN value of V reaches the tokens that see its key
- * and no others.  Scores, weights and sums are in fp32, of which the weights of
- * bf16 calls keep 16 bits (2^-17 off) where they meet V; the sums are divided
+ * and no others.  Scores, weights and sums are in fp32; the sums are divided
  * last, so a value of V times the number of keys must stay finite.  B H T is
  * below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an unsplit call,
  * below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over workgroups and merge their sums through a fixed 24 MiB per-stream library

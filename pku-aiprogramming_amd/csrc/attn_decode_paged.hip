@@ -17,9 +17,10 @@
 //   O^T [D x 16 rows] += V^T P^T: P comes out of S^T in the operand's layout.  V is
 //     read transposed (ds_read_b64_tr_b16, and _tr_b8 with the conversion behind
 //     it); fp32 needs no transposition, since a lane holds one key an operand there,
-//     and columns may be numbered as they were read.  P is split into bf16 terms
-//     (two for bf16 calls, 2^-17 off; three for fp32 calls, whose q is split into
-//     three exact terms too).
+//     and columns may be numbered as they were read.  P is split into three bf16 terms,
+//     which hold it exactly (two would leave 2^-17 of it and gain what few keys show: 8 x 8
+//     heads x 2048 over 8 bits 12.4 us for 13.0, 64 x 32 x 8192 640 for 642), and so is
+//     the q of fp32 calls.
 // A page is 16 keys or a multiple, so a step's 16 keys never straddle two.  The
 // wave holds the next 128 places of its sequence's table in registers, from
 // which a page's number comes without memory's latency.
@@ -230,7 +231,7 @@ __global__ __launch_bounds__(kMdThreads, (pd_waves<C, D>())) void attn_decode_pa
   constexpr bool F32 = sizeof(C) == 4, E4 = sizeof(C) == 1;  // fp32 pools; 8-bit ones
   constexpr int U = F32 ? 1 : 2, KEYS = 16 * U;              // 16s of keys, and keys, of a step
   constexpr int W = F32 ? D / 16 : D / 32;                   // k steps (fp32: pieces of four) of a key tile
-  constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = sizeof(T) == 4 ? 3 : 2;  // terms of q and of the weights
+  constexpr int NQ = sizeof(T) == 4 ? 3 : 1, NP = 3;         // terms of q and of the weights
   constexpr int ND = D / 16;                                 // 16-row tiles of O^T
   constexpr int VW = F32 ? (D < 64 ? D / 16 : 4) : 4;        // fp32: neighbouring columns of a lane
   using Tile = PdTile<C, D, KEYS>;
