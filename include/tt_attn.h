@@ -470,10 +470,10 @@ int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t l
  * TT_E4M3: sign, four exponent bits, three fraction bits, up to 448; 0x7f and
  * 0xff are NaN) under scale bytes k_scales and v_scales [npages][Hkv], one for each
  * page and head, that stand for 2^(byte - 127): the smallest power of two, of
- * 2^-124 to 2^119, that takes the page's largest value to at most 448.  Values
- * are rounded to nearest, halves to even; infinities and NaN become NaN (of
- * either code) and do not count for the scale.  The scales are null for other caches.  Pools are
- * 16-byte aligned (TT_ERR_ARG otherwise), d is 32, 64 or 128. */
+ * 2^-124 to 2^119, that takes the largest value the page was given to at most 448.
+ * Values are rounded to nearest, halves to even; infinities and NaN become NaN
+ * (of either code) and do not count for the scale.  The scales are null for other
+ * caches.  Pools are 16-byte aligned (TT_ERR_ARG otherwise), d is 32, 64 or 128. */
 
 /* Append: the new tokens' k and v, [B][Hkv][T][d] or token-major (ldk, ldv as
  * above), K normed (k_weight) and rotated (inv_freq) on the way as by
@@ -483,7 +483,8 @@ int tt_qkv_norm_rope_backward(int dtype, const void* q, const void* k, int64_t l
  * but for 8-bit pages that gain a larger value: their older tokens are rounded
  * again to the new scale (exactly, save what falls below its smallest steps).  A
  * page whose first row is among the new ones takes its scale from the new
- * tokens alone, whatever it held before.  K goes into 8 bits from 64-bit
+ * tokens alone, whatever it held before; else a scale never shrinks, not where a
+ * sequence's tokens were taken back either.  K goes into 8 bits from 64-bit
  * arithmetic, so that every code is the nearest one.  A page that new tokens go
  * to belongs to one sequence: calls in which two tokens meet in one row, or two
  * sequences in one 8-bit page, have no defined result there. */
@@ -505,8 +506,9 @@ int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_
  * they hold; an infinite or NaN value of V reaches the tokens that see its key
  * and no others.  Scores, weights and sums are in fp32; the sums are divided
  * last, so a value of V times the number of keys must stay finite.  B H T is
- * below 2^31 and B Hkv ceil(H / Hkv T / 16), the workgroups of an unsplit call,
- * below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys over workgroups and merge their sums through a fixed 24 MiB per-stream library
+ * below 2^31, B H at most 2^24, and B Hkv ceil(H / Hkv T / 16), the workgroups of
+ * an unsplit call, below 2^24 (TT_ERR_ARG otherwise).  Few heads split the keys
+ * over workgroups and merge their sums through a fixed 24 MiB per-stream library
  * workspace (allocated on first use); without it (refused, or under graph
  * capture before a call has left it on the stream) they run unsplit.  Graphs
  * captured on one stream share it and must be replayed in stream order. */

@@ -70,6 +70,20 @@ __device__ __forceinline__ bf16x8 md_bf16(uint32_t codes, float scale) {
   return __builtin_bit_cast(bf16x8, v.w);
 }
 
+// The wave's V tile: [32 keys][D] bf16 in 16-byte chunks, chunk c of row r at
+// chunk c ^ exchange(r), where a row's chunks number D / 8 and 256 / 2 D rows make
+// a line of all banks.  A row write puts one chunk of 16 consecutive rows, a
+// transposed read takes two neighbouring chunks of eight; both spread over the
+// banks.  The chunk enters an address by exclusive or alone, so that one register
+// serves all of them.
+template <int D>
+__device__ __forceinline__ constexpr int md_exchange(int r) {
+  return (r & 15) >> (D == 128 ? 0 : (D == 64 ? 1 : 2));
+}
+__device__ __forceinline__ void lds_st(uint32_t a, const bf16x8& x) {
+  *(__attribute__((address_space(3))) bf16x8*)(uintptr_t)a = x;
+}
+
 // The maximum is that of the products, the scale sl2 (of log2 e too, above zero:
 // its sign goes into q, and zero is the smallest fp32, 2^-149, which still hides
 // what is masked and takes no product to more than 2^-21) enters the exponent,

@@ -24,8 +24,8 @@
 // A page is 16 keys or a multiple, so a step's 16 keys never straddle two.  The
 // wave holds the next 128 places of its sequence's table in registers, from
 // which a page's number comes without memory's latency.
-// Measured (MI355X, d = 128): 64 sequences of up to 8192 keys, 32 / 8 heads of bf16, 252 us
-// (6.3 TB/s); 32 / 32 heads over 8 bits, 663 us (6.5 TB/s); one of 4097 keys, 11.4 us, a
+// Measured (MI355X, d = 128): 64 sequences of up to 8192 keys, 32 / 8 heads of bf16, 255 us
+// (6.3 TB/s); 32 / 32 heads over 8 bits, 647 us (6.6 TB/s); one of 4097 keys, 11.5 us, a
 // chain of memory latencies; 3 tokens of 12 x 20 / 4 heads of fp32 over 8 bits, 34.5 us (4.2 TB/s:
 // vector work of three terms of q and of the weights).
 #include <hip/hip_runtime.h>
@@ -776,8 +776,10 @@ int launch(const char* fn, const PdCall& a, hipStream_t st) {
                      0, st, (const T*)a.q, (const C*)a.kp, (const C*)a.vp, a.ks, a.vs, a.pg, part_o, part_ml,        \
                      (T*)a.o, a.lse, (uint32_t)R, (uint32_t)a.tokens, (uint32_t)tiles, (uint32_t)nsplit, sl2,        \
                      a.scale < 0.f, count)
-  // No second workgroup reads the same keys: past the caches (284 -> 252 us, 725 -> 647 over
-  // 8 bits).  Else they are to be found there.
+  // No second workgroup of a sequence reads the same keys: past the caches (64 x 32 / 8 heads
+  // x 8192 keys 359 -> 316 us, over 8 bits with 32 heads 726 -> 660).  Else they are to be
+  // found there.  Sequences that share pages, which the host does not see, lose by it where
+  // they are many: of one prefix alone 82 -> 98 us and 242 -> 317, 8 of 8 bits 19 both.
   if (tiles == 1)
     TT_PD_LAUNCH(true);
   else

@@ -1,6 +1,6 @@
 // Device-side building blocks that the decodes over quantised and over paged caches
 // share: T newest tokens of a K / V head's query heads as a tile of 16 rows on the
-// matrix unit, a wave's V tile in LDS, and the merge of splits.
+// matrix unit, their bf16 terms, and the merge of splits.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -29,21 +29,11 @@ __device__ __forceinline__ float sum_rows(float x) {
   return sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
-// The wave's V tile: [32 keys][D] bf16 in 16-byte chunks, chunk c of row r at
-// chunk c ^ exchange(r), where a row's chunks number D / 8 and 256 / 2 D rows make
-// a line of all banks.  A row write puts one chunk of 16 consecutive rows, a
-// transposed read takes two neighbouring chunks of eight; both spread over the
-// banks.  The chunk enters an address by exclusive or alone, so that one register
-// serves all of them.
-template <int D>
-__device__ __forceinline__ constexpr int md_exchange(int r) {
-  return (r & 15) >> (D == 128 ? 0 : (D == 64 ? 1 : 2));
-}
-
 // x as a sum of N bf16 terms: each what the earlier ones leave, cut off, the last
-// one rounded; three hold any fp32 value exactly.  Of two the first is rounded
-// too: it leaves at most 2^-8 of the value, of which the second is 2^-17 off at
-// most (cut off, it would leave 2^-7, and 2^-16 in the end).  ANY: x may be
+// one rounded; three hold any fp32 value of 2^-110 and more exactly.  Of two (the
+// 4-bit cache's weights) the first is rounded too: it leaves at most 2^-8 of the
+// value, of which the second is 2^-17 off at most (cut off, it would leave 2^-7,
+// and 2^-16 in the end).  ANY: x may be
 // infinite or NaN, or meet infinities.  A term is then the largest bf16 below the
 // value, so that none but zero's own are zero (1 is 255 / 2^8 + 255 / 2^16 + 1 /
 // 2^16): times an infinity each has x's sign, where 0 inf would be NaN; an
@@ -76,9 +66,6 @@ __device__ __forceinline__ void md_terms(const float (&x)[8], bf16x8 (&t)[N]) {
   }
 }
 
-__device__ __forceinline__ void lds_st(uint32_t a, const bf16x8& x) {
-  *(__attribute__((address_space(3))) bf16x8*)(uintptr_t)a = x;
-}
 __device__ __forceinline__ void md_load8(const u16* p, float (&f)[8]) {
   u16 x[8];
   __builtin_memcpy(x, p, 16);
