@@ -495,7 +495,8 @@ int tt_kv_append_paged(int dtype, int cache, const void* k, const void* v, int64
                        int64_t npages, int64_t page, int64_t width, void* stream);
 /* The cache read back to contiguous k, v [B][Hkv][L][d] of `dtype`: keys 0 to
  * min(lengths[b], L) - 1 of each sequence, exactly; other rows are left as they
- * are.  For tt_attn_* over a cached prefix, or to move a sequence. */
+ * are.  To move a sequence, or for tt_attn_* over a cached prefix (of L keys in
+ * every sequence, Hkv = H). */
 int tt_kv_gather_paged(int dtype, int cache, const void* k_pages, const void* v_pages, const uint8_t* k_scales,
                        const uint8_t* v_scales, const int* table, const int* lengths, void* k, void* v, int64_t B,
                        int64_t Hkv, int64_t L, int64_t d, int64_t npages, int64_t page, int64_t width, void* stream);

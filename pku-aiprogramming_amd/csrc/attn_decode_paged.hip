@@ -18,9 +18,10 @@
 //     read transposed (ds_read_b64_tr_b16, and _tr_b8 with the conversion behind
 //     it); fp32 needs no transposition, since a lane holds one key an operand there,
 //     and columns may be numbered as they were read.  P is split into three bf16 terms,
-//     which hold it exactly (two would leave 2^-17 of it and gain what few keys show: 8 x 8
-//     heads x 2048 over 8 bits 12.4 us for 13.0, 64 x 32 x 8192 640 for 642), and so is
-//     the q of fp32 calls.
+//     which hold it exactly, and so is the q of fp32 calls.  (Two would leave 2^-17 of P
+//     and gain where the bytes do not bound: a chunk of 512 tokens of 32 / 8 heads x 8192
+//     keys 161 us for 178, 8 x 8 heads x 2048 over 8 bits 12.4 for 13.0, but 64 x 32 x
+//     8192 640 for 642.)
 // A page is 16 keys or a multiple, so a step's 16 keys never straddle two.  The
 // wave holds the next 128 places of its sequence's table in registers, from
 // which a page's number comes without memory's latency.
